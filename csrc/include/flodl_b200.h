@@ -92,6 +92,34 @@ int fb_attn_bwd(const void* q, const void* k, const void* v, const void* o, cons
                 int causal, float p_drop, unsigned long long seed, const unsigned long long* seed_dev, int* status,
                 void* stream);
 
+/* ---- rotary positions ------------------------------------------------------------------------ */
+/* Up to three tensors [B, S, heads, D] with a unit inner stride: queries and keys, turned, and values, copied (heads 0: none).
+ * Strides are in elements, {batch, seq, head}. `freqs`: rot / 2 radians per position, fp64. The position of token (b, s) is
+ * positions[b, s] + offset (strides in elements), or s + offset where `positions` is NULL. `norm`: RMS norm of the first two over D with `weight`
+ * (fp32 [D] or NULL) before the turn. `backward`: dy -> y = dx; x is read with `norm` alone, whose weight gradients go to `dw`
+ * (fp32 [D] or NULL) by way of `partial`, fb_rotary_partial_rows() x 2 x D floats. rot <= D, both even; with `norm` D / 64
+ * values have to fit one access (16 bytes where all addresses and halves are so aligned). */
+typedef struct fb_rotary_args {
+  const void* x[3];
+  const void* dy[3];
+  void* y[3];
+  long long x_strides[3][3], dy_strides[3][3], y_strides[3][3];
+  int heads[3];
+  int B, S, D, rot;
+  int dtype;                 /* FLODL_FLOAT32, FLODL_BFLOAT16 or FLODL_FLOAT16 */
+  int interleaved, norm, backward;
+  float amplitude, eps;
+  const double* freqs;
+  const long long* positions;
+  long long pos_strides[2];
+  long long offset;
+  const float* weight[2];
+  float* partial;
+  float* dw[2];
+} fb_rotary_args;
+int fb_rotary(const fb_rotary_args* args, void* stream);
+int fb_rotary_partial_rows(void);
+
 /* ---- normalisation / activation / loss ----------------------------------------------------- */
 int fb_layernorm_fwd(const void* x, const void* residual, const float* gamma, const float* beta, void* y,
                      void* pre_out, float* mean, float* rstd, int rows, int cols, float eps, float p_drop,

@@ -29,3 +29,4 @@ from .core import (  # noqa: F401
     seed_state,
     set_native,
 )
+from .position import qk_norm_rotary, rotary, rotary_frequencies  # noqa: F401

@@ -1,0 +1,230 @@
+"""Rotary positions, and the RMS norm of queries and keys in the same pass (`csrc/kernels/rotary.cu`).
+
+`x` of both operators is what attention takes: a packed projection `[B, S, 3, H, D]`, whose values come back as they were, a pair
+`(q, k)` of `[B, S, H, D]` with head counts of their own, or one such tensor. The result has the same form."""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ..tensor import TensorError
+from .core import FLAGS, _C, _f32, _launched, _plain_call
+
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0, original_length: Optional[int] = None,
+                       device=None) -> torch.Tensor:
+    """Radians per position of the `rotary_dim / 2` pairs of a head, `base^(-2 i / rotary_dim)`, in fp64.
+
+    `scaling` stretches a model's positions by `factor` for contexts longer than it was trained on: `"linear"` slows every pair by it, `"base"` raises
+    the base so that the slowest pair slows by it and the fastest stays, `"wavelength"` slows the pairs that turn less than once in
+    `original_length` positions, leaves those that turn more than 32 times and goes over linearly between."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise TensorError(f"rotary_dim ({rotary_dim}) must be even and at least 2")
+    if not (base > 0 and factor > 0):
+        raise TensorError(f"base ({base}) and factor ({factor}) must be positive")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64)
+    if scaling == "base":
+        if rotary_dim < 4:
+            raise TensorError("scaling \"base\" needs a rotary_dim of at least 4")
+        base = base * factor ** (rotary_dim / (rotary_dim - 2))
+    f = float(base) ** (-i / rotary_dim)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "wavelength":
+        if original_length is None or original_length < 1:
+            raise TensorError("scaling \"wavelength\" needs original_length")
+        turns = original_length * f / (2 * math.pi)
+        kept = ((turns - 1) / 31).clamp(0, 1)
+        f = f / factor * (1 - kept) + f * kept
+    elif scaling not in (None, "base"):
+        raise TensorError(f"scaling must be None, \"linear\", \"base\" or \"wavelength\", not {scaling!r}")
+    return f.to(device) if device is not None else f
+
+
+# ------------------------------------------------------------------------------------------- arguments
+def _parts(x):
+    """The queries and keys in `x`."""
+    if torch.is_tensor(x):
+        return (x[:, :, 0], x[:, :, 1]) if x.dim() == 5 else (x,)
+    return tuple(x)
+
+
+def _check(x, freqs, positions, offset, amplitude):
+    """(tensors given, packed, positions as [B, S] int64 or None), or a TensorError."""
+    given = (x,) if torch.is_tensor(x) else tuple(x)
+    if not given or len(given) > 2 or not all(torch.is_tensor(t) for t in given):
+        raise TensorError("x must be a tensor or a pair of them")
+    lead = given[0]
+    packed = lead.dim() == 5
+    if packed and (len(given) != 1 or lead.shape[2] != 3):
+        raise TensorError(f"a packed projection is [B, S, 3, H, D], not {list(lead.shape)}")
+    for t in given:
+        if not packed and t.dim() != 4:
+            raise TensorError(f"queries and keys are [B, S, H, D], not {list(t.shape)}")
+        if t.shape[:2] != lead.shape[:2] or t.shape[-1] != lead.shape[-1] or t.dtype != lead.dtype or t.device != lead.device:
+            raise TensorError("queries and keys must share batch, length, head dim, type and device")
+        if not t.is_floating_point():
+            raise TensorError(f"queries and keys must be floating point, not {t.dtype}")
+    if freqs is not None:
+        if freqs.dim() != 1 or freqs.dtype != torch.float64 or freqs.device != lead.device:
+            raise TensorError("freqs must be fp64 [rotary_dim / 2] on the device of the rows (rotary_frequencies makes them)")
+        if 2 * freqs.numel() > lead.shape[-1]:
+            raise TensorError(f"{freqs.numel()} pairs do not fit a head of {lead.shape[-1]}")
+    if not math.isfinite(amplitude):
+        raise TensorError(f"amplitude ({amplitude}) must be finite")
+    if int(offset) != offset:
+        raise TensorError(f"offset ({offset}) must be a whole number")
+    if positions is not None:
+        if positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool:
+            raise TensorError(f"positions must be whole numbers, not {positions.dtype}")
+        B, S = lead.shape[:2]
+        if positions.device != lead.device or positions.dim() not in (1, 2) or positions.shape[-1] != S or (positions.dim() == 2 and positions.shape[0] not in (1, B)):
+            raise TensorError(f"positions must be [S] or [B, S] on the device of the rows, not {list(positions.shape)}")
+        positions = positions.to(torch.int64).expand(B, S)
+    return given, packed, positions
+
+
+def _width(t: torch.Tensor, pairs: int) -> int:
+    """Values of an access that the halves of the rotary part and what is behind it allow."""
+    v = 16 // t.element_size()
+    while v > 1 and (pairs % v or (t.shape[-1] - 2 * pairs) % (2 * v)):
+        v //= 2
+    return v
+
+
+def _native(given, pairs: int, norm: bool) -> bool:
+    """Whether the kernel takes these rows. At any size: the plain form is a dozen launches. With the norm a row's items have to fit a warp, also where an
+    address allows narrow accesses only (such rows are copied, `_rows`)."""
+    t = given[0]
+    D = t.shape[-1]
+    return FLAGS.native and t.is_cuda and t.dtype in _TYPES and D % 2 == 0 and (not norm or (D <= 64 * _width(t, pairs) and D <= 768)) and \
+        t.shape[0] * t.shape[1] < 1 << 31 and all(x.shape[-2] < 1 << 15 for x in given)
+
+
+def _rows(t: torch.Tensor, pairs: int, norm: bool = False):
+    """`t` as the kernel can address it: a unit inner stride; with the norm, the accesses that `_native` counted on too."""
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        return t.contiguous()
+    if norm:
+        v = _width(t, pairs)
+        if t.data_ptr() % (v * t.element_size()) or any(s % v for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+            return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _launch(given, grads, freqs, positions, offset, interleaved, amplitude, norm=False, wq=None, wk=None, eps=0.0, want_dw=False):
+    q, k = (*given, None)[:2] if given else (None, None)
+    dq, dk = (*grads, None)[:2] if grads else (None, None)
+    out = _C().rotary(q, k, dq, dk, freqs, positions, offset, interleaved, amplitude, norm, wq, wk, eps, want_dw)
+    _launched(2 if want_dw else 1)
+    return out
+
+
+# ------------------------------------------------------------------------------------------- plain form
+def _turn(x: torch.Tensor, freqs, positions, offset, interleaved, amplitude) -> torch.Tensor:
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    pos = torch.arange(x.shape[1], device=x.device)[None] if positions is None else positions
+    a = (pos + offset).double()[:, :, None, None] * freqs
+    cos, sin = (amplitude * a.cos()).to(wide), (amplitude * a.sin()).to(wide)
+    rot = 2 * freqs.numel()
+    r, rest = x[..., :rot].to(wide), x[..., rot:].to(wide)
+    if interleaved:
+        lo, hi = r[..., 0::2], r[..., 1::2]
+        y = torch.stack((lo * cos - hi * sin, hi * cos + lo * sin), dim=-1).flatten(-2)
+    else:
+        lo, hi = r[..., :rot // 2], r[..., rot // 2:]
+        y = torch.cat((lo * cos - hi * sin, hi * cos + lo * sin), dim=-1)
+    return torch.cat((y, rest), dim=-1)
+
+
+def _formed(x, turned):
+    """Results in the form of `x`."""
+    if torch.is_tensor(x):
+        return torch.stack((turned[0], turned[1], x[:, :, 2]), dim=2) if x.dim() == 5 else turned[0]
+    return tuple(turned)
+
+
+# ------------------------------------------------------------------------------------------------ rotary
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, freqs, positions, cfg, *given):
+        ctx.save_for_backward(freqs, positions)
+        ctx.cfg = cfg
+        return tuple(_launch([_rows(t, 0) for t in given], None, freqs, positions, *cfg))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *dys):
+        return (None, None, None, *_launch(None, [_rows(t, 0) for t in dys], *ctx.saved_tensors, *ctx.cfg))
+
+
+def rotary(x, freqs: torch.Tensor, positions: Optional[torch.Tensor] = None, offset: int = 0, interleaved: bool = False, amplitude: float = 1.0):
+    """Queries and keys with their positions: pair `i` of a head at position `t` turned by `t * freqs[i]` and scaled by `amplitude`.
+
+    `positions` [S] or [B, S] (whole numbers, on the device) or 0, 1, 2, ...; `offset` is added to them. Pair `i` is the values `i` and `i + P` of the head for `P`
+    frequencies, or `2 i` and `2 i + 1` with `interleaved`; what is behind the first `2 P` values stays. Angles are taken in 64 bits."""
+    given, _, positions = _check(x, freqs, positions, offset, amplitude)
+    if not _native(given, freqs.numel(), False):
+        return _formed(x, [_turn(t, freqs, positions, offset, interleaved, amplitude).to(t.dtype) for t in _parts(x)])
+    freqs, cfg = freqs.contiguous(), (int(offset), bool(interleaved), float(amplitude))
+    if _plain_call(*given):
+        out = _launch([_rows(t, 0) for t in given], None, freqs, positions, *cfg)
+    else:
+        out = _RotaryFn.apply(freqs, positions, cfg, *given)
+    return out[0] if torch.is_tensor(x) else tuple(out)
+
+
+# ---------------------------------------------------------------------------------------- norm and rotary
+class _QkNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, freqs, positions, cfg, eps, wq, wk, *given):
+        given = [_rows(t, freqs.numel(), True) for t in given]
+        ctx.cfg, ctx.eps = cfg, eps
+        ctx.save_for_backward(freqs, positions, wq, wk, *given)
+        return tuple(_launch(given, None, freqs, positions, *cfg, True, _f32(wq), _f32(wk), eps))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *dys):
+        freqs, positions, wq, wk, *given = ctx.saved_tensors
+        want = ctx.needs_input_grad[4] or ctx.needs_input_grad[5]
+        out = _launch(given, [_rows(t, freqs.numel(), True) for t in dys], freqs, positions, *ctx.cfg, True, _f32(wq), _f32(wk), ctx.eps, want)
+        n = len(given)
+        dw = [out[n + i].to(w.dtype) if want and w is not None and ctx.needs_input_grad[4 + i] else None for i, w in enumerate((wq, wk))]
+        return (None, None, None, None, *dw, *out[:n])
+
+
+def qk_norm_rotary(x, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, freqs: Optional[torch.Tensor] = None,
+                   positions: Optional[torch.Tensor] = None, offset: int = 0, interleaved: bool = False, amplitude: float = 1.0, eps: float = 1e-6):
+    """Queries and keys normalised per head, `x / sqrt(mean(x^2) + eps) * weight` over the head's values, then turned as `rotary` does (not at all
+    without `freqs`), in one pass. The weights are [D], shared by the heads; None is ones. Statistics are taken in 32 bits."""
+    given, _, positions = _check(x, freqs, positions, offset, amplitude)
+    D = given[0].shape[-1]
+    for w in (q_weight, k_weight):
+        if w is not None and (tuple(w.shape) != (D,) or w.device != given[0].device or not w.is_floating_point()):
+            raise TensorError(f"weights must be [{D}] on the device of the rows")
+    if k_weight is not None and len(_parts(x)) < 2:
+        raise TensorError("k_weight without keys")
+    if not eps >= 0:
+        raise TensorError(f"eps ({eps}) must not be negative")
+    if freqs is None:
+        freqs = torch.empty(0, dtype=torch.float64, device=given[0].device)
+    if not _native(given, freqs.numel(), True):
+        out = []
+        for t, w in zip(_parts(x), (q_weight, k_weight)):
+            n = t if t.dtype == torch.float64 else t.float()
+            n = n * torch.rsqrt(n.square().mean(-1, keepdim=True) + eps)
+            n = n if w is None else n * w.to(n.dtype)
+            out.append((_turn(n, freqs, positions, offset, interleaved, amplitude) if freqs.numel() else n).to(t.dtype))
+        return _formed(x, out)
+    freqs, cfg = freqs.contiguous(), (int(offset), bool(interleaved), float(amplitude))
+    if _plain_call(q_weight, k_weight, *given):
+        out = _launch([_rows(t, freqs.numel(), True) for t in given], None, freqs, positions, *cfg, True, _f32(q_weight), _f32(k_weight), float(eps))
+    else:
+        out = _QkNormFn.apply(freqs, positions, cfg, float(eps), q_weight, k_weight, *given)
+    return out[0] if torch.is_tensor(x) else tuple(out)
