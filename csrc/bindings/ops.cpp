@@ -64,11 +64,15 @@ struct DeviceWords {
   }
 };
 
+}  // namespace
+
 // the status word, shared by every kernel that has bounded waits
 Tensor& status_word(int device) {
   static DeviceWords words;
   return words.get(device);
 }
+
+namespace {
 
 // ------------------------------------------------------------------------------------------ GEMM
 void gemm(const Tensor& a, const Tensor& b, Tensor& out, bool a_mn, bool b_mn, const OptTensor& bias, int epi,
@@ -721,93 +725,13 @@ Tensor attn_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
   return dqkv;
 }
 
-// --------------------------------------------------------------------------- rotary positions
-// q [B, S, H, D] alone, with k [B, S, Hk, D], or packed [B, S, 3, H, D] with its values copied; backward with the same layouts in dq / dk. Returns the
-// results in the layouts given, then dwq and dwk where they are wanted.
-std::vector<Tensor> rotary(const OptTensor& q, const OptTensor& k, const OptTensor& dq, const OptTensor& dk, const Tensor& freqs, const OptTensor& positions,
-                           int64_t offset, bool interleaved, double amplitude, bool norm, const OptTensor& wq, const OptTensor& wk, double eps, bool want_dw) {
-  const bool backward = dq.has_value();
-  const Tensor& lead = backward ? *dq : *q;
-  want_cuda(lead, "x");
-  c10::cuda::CUDAGuard guard(lead.device());
-  const bool packed = lead.dim() == 5;
-  TORCH_CHECK(lead.dim() == 4 || (packed && lead.size(2) == 3), "rotary takes [B, S, H, D] or packed [B, S, 3, H, D]");
-  TORCH_CHECK(freqs.device() == lead.device() && freqs.scalar_type() == at::kDouble && freqs.is_contiguous(), "freqs must be contiguous fp64 on the device of the rows");
-  TORCH_CHECK(!backward || !norm || q.has_value(), "the backward pass of the norm needs its input");
-  fb_rotary_args a = {};
-  a.B = (int)lead.size(0);
-  a.S = (int)lead.size(1);
-  a.D = (int)lead.size(-1);
-  a.rot = (int)freqs.numel() * 2;
-  const auto kind = lead.scalar_type();
-  TORCH_CHECK(kind == at::kFloat || kind == at::kBFloat16 || kind == at::kHalf, "rotary takes fp32, bf16 or fp16");
-  a.dtype = kind == at::kFloat ? FLODL_FLOAT32 : kind == at::kHalf ? FLODL_FLOAT16 : FLODL_BFLOAT16;
-  a.interleaved = interleaved;
-  a.norm = norm;
-  a.backward = backward;
-  a.amplitude = (float)amplitude;
-  a.eps = (float)eps;
-  a.freqs = freqs.data_ptr<double>();
-  a.offset = offset;
-  if (positions.has_value()) {
-    TORCH_CHECK(positions->device() == lead.device() && positions->scalar_type() == at::kLong && positions->dim() == 2 && positions->size(0) == a.B &&
-                positions->size(1) == a.S, "positions must be int64 [B, S]");
-    a.positions = reinterpret_cast<const long long*>(positions->data_ptr<int64_t>());
-    a.pos_strides[0] = positions->stride(0);
-    a.pos_strides[1] = positions->stride(1);
-  }
-  // one segment: rows of `t` as the kernel addresses them (the stride of a dimension of one is never used, whatever it is)
-  const auto slice = [&](const Tensor& t, int seg, const void** at, long long* strides) {
-    TORCH_CHECK(t.device() == lead.device() && t.scalar_type() == kind && t.dim() == lead.dim() && t.size(0) == a.B && t.size(1) == a.S && t.size(-1) == a.D &&
-                (t.stride(-1) == 1 || a.D == 1), "rows of one kind with a unit inner stride");
-    const int64_t h = t.dim() - 2;
-    *at = static_cast<const char*>(t.data_ptr()) + (packed ? seg * t.stride(2) * t.element_size() : 0);
-    strides[0] = t.size(0) == 1 ? 0 : t.stride(0);
-    strides[1] = t.size(1) == 1 ? 0 : t.stride(1);
-    strides[2] = t.size(h) == 1 ? 0 : t.stride(h);
-    if (a.heads[seg] == 0) a.heads[seg] = (int)t.size(h);
-    TORCH_CHECK(a.heads[seg] == t.size(h), "heads differ");
-  };
-  std::vector<Tensor> out;
-  for (int seg = 0; seg < (packed ? 3 : 2); ++seg) {
-    const OptTensor &x = packed || seg == 0 ? q : k, &d = packed || seg == 0 ? dq : dk;
-    if (!packed && seg == 1 && !(backward ? d : x).has_value()) continue;
-    if (x.has_value()) slice(*x, seg, &a.x[seg], a.x_strides[seg]);
-    if (backward) slice(*d, seg, &a.dy[seg], a.dy_strides[seg]);
-    if (!packed || seg == 0) out.push_back(torch::empty((backward ? *d : *x).sizes(), lead.options()));
-    const void* y = nullptr;
-    slice(out.back(), seg, &y, a.y_strides[seg]);
-    a.y[seg] = const_cast<void*>(y);
-  }
-  const OptTensor* weights[2] = {&wq, &wk};
-  for (int i = 0; i < 2; ++i) {
-    if (!weights[i]->has_value()) continue;
-    want_f32(**weights[i], "weight");
-    TORCH_CHECK((*weights[i])->device() == lead.device() && (*weights[i])->numel() == a.D, "weight must be [D] on the device of the rows");
-    a.weight[i] = (*weights[i])->data_ptr<float>();
-  }
-  Tensor partial;
-  if (norm && backward) {
-    const auto f32 = lead.options().dtype(torch::kFloat);
-    partial = torch::empty({fb_rotary_partial_rows(), 2, a.D}, f32);
-    a.partial = partial.data_ptr<float>();
-    if (want_dw) {
-      for (int i = 0; i < 2; ++i) {
-        out.push_back(lead.numel() == 0 ? torch::zeros({a.D}, f32) : torch::empty({a.D}, f32));
-        a.dw[i] = out.back().data_ptr<float>();
-      }
-    }
-  }
-  check(fb_rotary(&a, stream_of(lead)), "fb_rotary");
-  return out;
-}
-
 }  // namespace
 
 void bind_comm(py::module_& m);     // comm.cpp
 void bind_runtime(py::module_& m);  // runtime.cpp
 void bind_graph_exec(py::module_& m);  // graph_exec.cpp
 void bind_cpu_avg(py::module_& m);     // cpu_avg.cpp
+void bind_attention_ops(py::module_& m);  // attention_ops.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "flodl_b200 native kernels (sm_100a) and runtime";
@@ -864,9 +788,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("p_drop") = 0.0, py::arg("seed") = 0, py::arg("seed_dev") = py::none());
   m.def("attn_bwd", &attn_bwd, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("o"), py::arg("d_o"), py::arg("lse"), py::arg("mask"),
         py::arg("scale"), py::arg("causal"), py::arg("p_drop") = 0.0, py::arg("seed") = 0, py::arg("seed_dev") = py::none());
-  m.def("rotary", &rotary, py::arg("q"), py::arg("k"), py::arg("dq"), py::arg("dk"), py::arg("freqs"), py::arg("positions"), py::arg("offset"),
-        py::arg("interleaved"), py::arg("amplitude"), py::arg("norm") = false, py::arg("wq") = py::none(), py::arg("wk") = py::none(), py::arg("eps") = 0.0,
-        py::arg("want_dw") = false);
+  bind_attention_ops(m);
   bind_comm(m);
   bind_runtime(m);
   bind_graph_exec(m);

@@ -120,6 +120,28 @@ typedef struct fb_rotary_args {
 int fb_rotary(const fb_rotary_args* args, void* stream);
 int fb_rotary_partial_rows(void);
 
+/* ---- attention over another sequence ------------------------------------------------------------ */
+/* q, o, d_o, dq: bf16 [B, Sq, H, D], k, v, dk, dv: bf16 [B, Sk, Hk, D] with a unit inner stride, the others in elements {batch, seq, head} (multiples of 8, not 0 where the
+ * dimension is more than one; 16-byte aligned bases). D is 64 or 128; Hk divides H, query head h reads key head h / (H / Hk). dk and dv share dk_strides.
+ * mask: [B, Sk] with a unit inner stride, one byte a key (mask_bool; 0: the key is absent) or fp32 addends (-inf: absent). stats: fp32 [B, H, Sq, 2] in an order of the
+ * kernels' own, written by the forward pass (or NULL) and read by the backward pass. workspace: fb_cross_workspace floats. */
+typedef struct fb_cross_args {
+  const void *q, *k, *v, *d_o;
+  void *o, *dq, *dk, *dv;
+  long long q_strides[3], k_strides[3], v_strides[3], o_strides[3], do_strides[3], dq_strides[3], dk_strides[3];
+  int B, H, Hk, Sq, Sk, D;
+  const void* mask;
+  long long mask_stride;     /* of the batch; 0: one row for all */
+  int mask_bool;
+  float scale;
+  float* stats;
+  float* workspace;
+  int* status;
+} fb_cross_args;
+long long fb_cross_workspace(const fb_cross_args* args, int backward);
+int fb_cross_attn_fwd(const fb_cross_args* args, void* stream);
+int fb_cross_attn_bwd(const fb_cross_args* args, void* stream);
+
 /* ---- normalisation / activation / loss ----------------------------------------------------- */
 int fb_layernorm_fwd(const void* x, const void* residual, const float* gamma, const float* beta, void* y,
                      void* pre_out, float* mean, float* rstd, int rows, int cols, float eps, float p_drop,

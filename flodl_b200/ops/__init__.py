@@ -29,4 +29,5 @@ from .core import (  # noqa: F401
     seed_state,
     set_native,
 )
+from .cross import cross_attention  # noqa: F401
 from .position import qk_norm_rotary, rotary, rotary_frequencies  # noqa: F401

@@ -1,0 +1,72 @@
+"""Attention over another sequence (`csrc/kernels/cross_attn.cu`)."""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from ..tensor import TensorError
+from .core import FLAGS, _C, _launched
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """softmax(q k^T * scale + mask) v for queries [B, Sq, H, D] over keys and values [B, Sk, Hk, D] of any other length; returns [B, Sq, H, D].
+
+    `Hk` divides `H`: query head `h` reads key head `h // (H / Hk)`, whose gradient is the sum over them. `scale` is 1 / sqrt(D) unless given. `mask` is of keys, [B, Sk],
+    [1, Sk] or [B, 1, 1, Sk]: bool, True for the keys that take part, or floating point, added to the scores. A key at False or -inf is absent, whatever its key and
+    value hold, and gets no gradient; a query without any key gets zeros. bf16 heads of 64 and 128 on a GPU run on the kernel, at any size, others as plain
+    products in 32 bits (64 for fp64)."""
+    if FLAGS.native and torch.is_tensor(q) and q.is_cuda and q.dim() == 4:
+        o = _C().cross_attention(q, k, v, mask, float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1] or 1))
+        if o is not None:
+            _launched()
+            return o
+    return _plain(q, k, v, mask, scale)
+
+
+def _plain(q, k, v, mask, scale):
+    if not all(torch.is_tensor(t) and t.dim() == 4 for t in (q, k, v)):
+        raise TensorError("queries, keys and values are [B, S, H, D]")
+    B, Sq, H, D = q.shape
+    Sk, Hk = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise TensorError(f"keys {list(k.shape)} and values {list(v.shape)} must be [{B}, Sk, Hk, {D}]")
+    if H == 0 or Hk == 0 or H % Hk:
+        raise TensorError(f"{Hk} key heads do not divide {H} query heads")
+    if not q.is_floating_point() or len({(t.dtype, t.device) for t in (q, k, v)}) != 1:
+        raise TensorError("queries, keys and values must be floating point, of one type and on one device")
+    if D == 0:
+        raise TensorError("heads of no values")
+    scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
+    if not math.isfinite(scale):
+        raise TensorError(f"scale ({scale}) must be finite")
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    qh = q.to(wide).transpose(1, 2).reshape(B, Hk, H // Hk * Sq, D)
+    kh, vh = (t.to(wide).transpose(1, 2) for t in (k, v))
+    add = absent = None
+    if mask is not None:
+        m = mask
+        if m.device != q.device or not (m.dtype == torch.bool or m.is_floating_point()):
+            raise TensorError("mask must be bool or floating point on the device of the rows")
+        if m.dim() == 4 and m.shape[1] == 1 and m.shape[2] == 1:
+            m = m[:, 0, 0]
+        if m.dim() != 2 or m.shape[1] != Sk or m.shape[0] not in (1, B):
+            raise TensorError(f"mask must be of keys, [{B}, {Sk}], not {list(mask.shape)}")
+        absent = ~m if m.dtype == torch.bool else m == float("-inf")
+        if m.dtype != torch.bool:
+            add = m.to(wide).masked_fill(absent, 0.0)[:, None, None]
+        kh, vh = (t.masked_fill(absent[:, None, :, None], 0.0) for t in (kh, vh))
+    s = (qh @ kh.transpose(-1, -2)) * scale
+    if add is not None:
+        s = s + add
+    if absent is not None:
+        s = s.masked_fill(absent[:, None, None], float("-inf"))
+    if Sk == 0:
+        p = s
+    else:
+        top = s.detach().amax(-1, keepdim=True)
+        p = torch.exp(s - top.masked_fill(top == float("-inf"), 0.0))
+        total = p.sum(-1, keepdim=True)
+        p = p / torch.where(total == 0, torch.ones_like(total), total)
+    return (p @ vh).reshape(B, H, Sq, D).transpose(1, 2).to(q.dtype)

@@ -8,12 +8,9 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ..tensor import TensorError
-from .core import FLAGS, _C, _f32, _launched, _plain_call
-
-_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+from .core import FLAGS, _C, _launched
 
 
 def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0, original_length: Optional[int] = None,
@@ -55,7 +52,7 @@ def _parts(x):
 
 
 def _check(x, freqs, positions, offset, amplitude):
-    """(tensors given, packed, positions as [B, S] int64 or None), or a TensorError."""
+    """(tensors given, positions as [B, S] int64 or None), or a TensorError."""
     given = (x,) if torch.is_tensor(x) else tuple(x)
     if not given or len(given) > 2 or not all(torch.is_tensor(t) for t in given):
         raise TensorError("x must be a tensor or a pair of them")
@@ -86,43 +83,23 @@ def _check(x, freqs, positions, offset, amplitude):
         if positions.device != lead.device or positions.dim() not in (1, 2) or positions.shape[-1] != S or (positions.dim() == 2 and positions.shape[0] not in (1, B)):
             raise TensorError(f"positions must be [S] or [B, S] on the device of the rows, not {list(positions.shape)}")
         positions = positions.to(torch.int64).expand(B, S)
-    return given, packed, positions
+    return given, positions
 
 
-def _width(t: torch.Tensor, pairs: int) -> int:
-    """Values of an access that the halves of the rotary part and what is behind it allow."""
-    v = 16 // t.element_size()
-    while v > 1 and (pairs % v or (t.shape[-1] - 2 * pairs) % (2 * v)):
-        v //= 2
-    return v
-
-
-def _native(given, pairs: int, norm: bool) -> bool:
-    """Whether the kernel takes these rows. At any size: the plain form is a dozen launches. With the norm a row's items have to fit a warp, also where an
-    address allows narrow accesses only (such rows are copied, `_rows`)."""
-    t = given[0]
-    D = t.shape[-1]
-    return FLAGS.native and t.is_cuda and t.dtype in _TYPES and D % 2 == 0 and (not norm or (D <= 64 * _width(t, pairs) and D <= 768)) and \
-        t.shape[0] * t.shape[1] < 1 << 31 and all(x.shape[-2] < 1 << 15 for x in given)
-
-
-def _rows(t: torch.Tensor, pairs: int, norm: bool = False):
-    """`t` as the kernel can address it: a unit inner stride; with the norm, the accesses that `_native` counted on too."""
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
-        return t.contiguous()
-    if norm:
-        v = _width(t, pairs)
-        if t.data_ptr() % (v * t.element_size()) or any(s % v for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
-            return t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
-def _launch(given, grads, freqs, positions, offset, interleaved, amplitude, norm=False, wq=None, wk=None, eps=0.0, want_dw=False):
-    q, k = (*given, None)[:2] if given else (None, None)
-    dq, dk = (*grads, None)[:2] if grads else (None, None)
-    out = _C().rotary(q, k, dq, dk, freqs, positions, offset, interleaved, amplitude, norm, wq, wk, eps, want_dw)
-    _launched(2 if want_dw else 1)
-    return out
+def _native(x, freqs, positions, offset, interleaved, amplitude, norm=False, wq=None, wk=None, eps=0.0):
+    """The kernel's results, or None for a call that it does not take: another device or type, or arguments that the checks explain. At any size: the
+    plain form is a dozen launches."""
+    pair = isinstance(x, (tuple, list))
+    if pair and len(x) not in (1, 2):
+        return None
+    q, k = (x if len(x) == 2 else (x[0], None)) if pair else (x, None)
+    if not (FLAGS.native and torch.is_tensor(q) and q.is_cuda and (k is None or torch.is_tensor(k)) and type(offset) is int):
+        return None
+    out = _C().turn(q, k, freqs, positions, offset, interleaved, amplitude, norm, wq, wk, eps)
+    if out is None:
+        return None
+    _launched()
+    return tuple(out) if pair else out[0]
 
 
 # ------------------------------------------------------------------------------------------- plain form
@@ -150,60 +127,30 @@ def _formed(x, turned):
 
 
 # ------------------------------------------------------------------------------------------------ rotary
-class _RotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, freqs, positions, cfg, *given):
-        ctx.save_for_backward(freqs, positions)
-        ctx.cfg = cfg
-        return tuple(_launch([_rows(t, 0) for t in given], None, freqs, positions, *cfg))
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *dys):
-        return (None, None, None, *_launch(None, [_rows(t, 0) for t in dys], *ctx.saved_tensors, *ctx.cfg))
-
-
 def rotary(x, freqs: torch.Tensor, positions: Optional[torch.Tensor] = None, offset: int = 0, interleaved: bool = False, amplitude: float = 1.0):
     """Queries and keys with their positions: pair `i` of a head at position `t` turned by `t * freqs[i]` and scaled by `amplitude`.
 
     `positions` [S] or [B, S] (whole numbers, on the device) or 0, 1, 2, ...; `offset` is added to them. Pair `i` is the values `i` and `i + P` of the head for `P`
     frequencies, or `2 i` and `2 i + 1` with `interleaved`; what is behind the first `2 P` values stays. Angles are taken in 64 bits."""
-    given, _, positions = _check(x, freqs, positions, offset, amplitude)
-    if not _native(given, freqs.numel(), False):
-        return _formed(x, [_turn(t, freqs, positions, offset, interleaved, amplitude).to(t.dtype) for t in _parts(x)])
-    freqs, cfg = freqs.contiguous(), (int(offset), bool(interleaved), float(amplitude))
-    if _plain_call(*given):
-        out = _launch([_rows(t, 0) for t in given], None, freqs, positions, *cfg)
-    else:
-        out = _RotaryFn.apply(freqs, positions, cfg, *given)
-    return out[0] if torch.is_tensor(x) else tuple(out)
+    out = _native(x, freqs, positions, offset, interleaved, amplitude)
+    if out is not None:
+        return out
+    _, positions = _check(x, freqs, positions, offset, amplitude)
+    return _formed(x, [_turn(t, freqs, positions, offset, interleaved, amplitude).to(t.dtype) for t in _parts(x)])
 
 
 # ---------------------------------------------------------------------------------------- norm and rotary
-class _QkNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, freqs, positions, cfg, eps, wq, wk, *given):
-        given = [_rows(t, freqs.numel(), True) for t in given]
-        ctx.cfg, ctx.eps = cfg, eps
-        ctx.save_for_backward(freqs, positions, wq, wk, *given)
-        return tuple(_launch(given, None, freqs, positions, *cfg, True, _f32(wq), _f32(wk), eps))
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *dys):
-        freqs, positions, wq, wk, *given = ctx.saved_tensors
-        want = ctx.needs_input_grad[4] or ctx.needs_input_grad[5]
-        out = _launch(given, [_rows(t, freqs.numel(), True) for t in dys], freqs, positions, *ctx.cfg, True, _f32(wq), _f32(wk), ctx.eps, want)
-        n = len(given)
-        dw = [out[n + i].to(w.dtype) if want and w is not None and ctx.needs_input_grad[4 + i] else None for i, w in enumerate((wq, wk))]
-        return (None, None, None, None, *dw, *out[:n])
-
-
 def qk_norm_rotary(x, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, freqs: Optional[torch.Tensor] = None,
                    positions: Optional[torch.Tensor] = None, offset: int = 0, interleaved: bool = False, amplitude: float = 1.0, eps: float = 1e-6):
     """Queries and keys normalised per head, `x / sqrt(mean(x^2) + eps) * weight` over the head's values, then turned as `rotary` does (not at all
     without `freqs`), in one pass. The weights are [D], shared by the heads; None is ones. Statistics are taken in 32 bits."""
-    given, _, positions = _check(x, freqs, positions, offset, amplitude)
+    if freqs is None:
+        lead = x if torch.is_tensor(x) else x[0]
+        freqs = torch.empty(0, dtype=torch.float64, device=lead.device)
+    out = _native(x, freqs, positions, offset, interleaved, amplitude, True, q_weight, k_weight, eps)
+    if out is not None:
+        return out
+    given, positions = _check(x, freqs, positions, offset, amplitude)
     D = given[0].shape[-1]
     for w in (q_weight, k_weight):
         if w is not None and (tuple(w.shape) != (D,) or w.device != given[0].device or not w.is_floating_point()):
@@ -212,19 +159,10 @@ def qk_norm_rotary(x, q_weight: Optional[torch.Tensor] = None, k_weight: Optiona
         raise TensorError("k_weight without keys")
     if not eps >= 0:
         raise TensorError(f"eps ({eps}) must not be negative")
-    if freqs is None:
-        freqs = torch.empty(0, dtype=torch.float64, device=given[0].device)
-    if not _native(given, freqs.numel(), True):
-        out = []
-        for t, w in zip(_parts(x), (q_weight, k_weight)):
-            n = t if t.dtype == torch.float64 else t.float()
-            n = n * torch.rsqrt(n.square().mean(-1, keepdim=True) + eps)
-            n = n if w is None else n * w.to(n.dtype)
-            out.append((_turn(n, freqs, positions, offset, interleaved, amplitude) if freqs.numel() else n).to(t.dtype))
-        return _formed(x, out)
-    freqs, cfg = freqs.contiguous(), (int(offset), bool(interleaved), float(amplitude))
-    if _plain_call(q_weight, k_weight, *given):
-        out = _launch([_rows(t, freqs.numel(), True) for t in given], None, freqs, positions, *cfg, True, _f32(q_weight), _f32(k_weight), float(eps))
-    else:
-        out = _QkNormFn.apply(freqs, positions, cfg, float(eps), q_weight, k_weight, *given)
-    return out[0] if torch.is_tensor(x) else tuple(out)
+    out = []
+    for t, w in zip(_parts(x), (q_weight, k_weight)):
+        n = t if t.dtype == torch.float64 else t.float()
+        n = n * torch.rsqrt(n.square().mean(-1, keepdim=True) + eps)
+        n = n if w is None else n * w.to(n.dtype)
+        out.append((_turn(n, freqs, positions, offset, interleaved, amplitude) if freqs.numel() else n).to(t.dtype))
+    return _formed(x, out)

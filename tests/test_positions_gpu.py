@@ -10,6 +10,16 @@ from flodl_b200 import ops
 
 pytestmark = pytest.mark.gpu
 
+@pytest.fixture(autouse=True)
+def kernels_only(monkeypatch):
+    """No call of these tests is answered by the plain form unnoticed."""
+    from flodl_b200.ops import position
+
+    def refuse(*a):
+        raise AssertionError("the plain form was taken")
+    monkeypatch.setattr(position, "_turn", refuse)
+
+
 U = 2.0 ** -24
 EPS = 1e-6
 
