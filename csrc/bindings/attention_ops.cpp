@@ -276,7 +276,7 @@ Tensor launch_cross(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, 
   a.o = o.data_ptr();
   strides_of(o, a.o_strides);
   if (stats) {
-    *stats = at::empty({q.size(0), q.size(2), q.size(1), 2}, at::TensorOptions().dtype(at::kFloat).device(q.device()));
+    *stats = at::empty({q.size(0) * (q.size(2) * q.size(1) + 1)}, at::TensorOptions().dtype(at::kFloat).device(q.device()));
     a.stats = stats->data_ptr<float>();
   }
   const Tensor space = space_for(a, false, q);

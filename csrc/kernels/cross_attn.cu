@@ -8,8 +8,7 @@
 // Masks are of keys. Blocks of 128 keys none of which takes part are left out; blocks all of which do, with nothing added, take the short path; the rest go by a table
 // of {scale, addend} for each key. A key at -inf is absent: its score is replaced whatever it is, and where it meets a product as a row of the streamed operand that row
 // is zeroed in shared memory, so infinities and NaN behind a mask reach nothing. An addend beyond 2^100 takes the score's place, as it would in 64 bits.
-// Otherwise the row's maximum is taken from the addend first, so that a mask common to a row's keys costs its scores no bits; for the same reason the maximum and the
-// logarithm of the sum are saved apart for the backward pass.
+// Addends are taken relative to the batch row's largest, so that a mask common to a row's keys costs its scores no bits.
 //
 // Statistics, sums and products are fp32; P and dS are rounded to bf16 once, as operands of the tensor cores.
 #include <cuda.h>
@@ -31,6 +30,7 @@ struct CrossParams {
   int B, Hq, Hk, R, Sk;             // Hq = H / pack rows of heads; R = Sq * pack rows each
   int pack_log2, per_kv;            // log2 of pack; rows of heads that share a key head
   const void* mask;                 // [B, Sk]: one byte a key (0: absent), or fp32 addends; null: none
+  float* base;                      // [B] of addends: the batch row's largest, which the forward pass leaves for the backward pass (null: nobody wants it)
   long long mask_stride;
   int mask_bool;
   float scale;
@@ -80,17 +80,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// What the mask says of a key: {scale, addend}, both in units of log2.
-__device__ __forceinline__ float2 key_entry(const CrossParams& p, int b, int kv) {
-  const float sc = p.scale * kLog2e;
-  if (kv >= p.Sk) return make_float2(0.f, -INFINITY);
-  if (!p.mask) return make_float2(sc, 0.f);
+// The addend of a key in units of log2, held at the largest finite values; -inf: the key is absent.
+__device__ __forceinline__ float key_addend(const CrossParams& p, int b, int kv) {
+  if (kv >= p.Sk) return -INFINITY;
+  if (!p.mask) return 0.f;
   const long long at = b * p.mask_stride + kv;
-  if (p.mask_bool) return static_cast<const uint8_t*>(p.mask)[at] ? make_float2(sc, 0.f) : make_float2(0.f, -INFINITY);
+  if (p.mask_bool) return static_cast<const uint8_t*>(p.mask)[at] ? 0.f : -INFINITY;
   const float a = static_cast<const float*>(p.mask)[at];
-  if (a == -INFINITY) return make_float2(0.f, -INFINITY);
-  if (fabsf(a) < kHuge) return make_float2(sc, a * kLog2e);
-  return make_float2(0.f, isinf(a) || isnan(a) ? a : fminf(fmaxf(a * kLog2e, -3.402823466e38f), 3.402823466e38f));
+  return isinf(a) || isnan(a) ? a : fminf(fmaxf(a * kLog2e, -3.402823466e38f), 3.402823466e38f);
+}
+// What the mask says of a key: {scale, addend beyond `base`}. An addend beyond 2^100 leaves nothing of the score.
+__device__ __forceinline__ float2 key_entry(const CrossParams& p, int b, int kv, float base) {
+  const float a = key_addend(p, b, kv);
+  return make_float2(fabsf(a) < kHuge ? p.scale * kLog2e : 0.f, a - base);
 }
 // Of a block of 128 keys, by a whole warp: 0 nothing takes part, 1 by the table, 2 all of it with nothing added.
 __device__ __forceinline__ int block_state(const CrossParams& p, int b, int blk, int lane) {
@@ -118,6 +120,27 @@ __device__ __forceinline__ int block_state(const CrossParams& p, int b, int blk,
 }
 __device__ __forceinline__ int block_state_unmasked(const CrossParams& p, int blk) { return (blk + 1) * kKeys <= p.Sk && !p.table ? 2 : 1; }
 
+// A thread's row of scores in TMEM, kChunks x 32 columns: each with its key's scale and addend, an absent key's at -inf whatever it was. In place and in a loop: in the
+// registers of the common path it would cost that one spills.
+template <int kChunks>
+__device__ __forceinline__ void apply_table(uint32_t scores, const float2* tb) {
+#pragma unroll 1
+  for (int c = 0; c < 2 * kChunks; ++c) {
+    uint32_t v[16];
+    tmem_ld16(scores + 16 * c, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) {
+      asm volatile("" : "+r"(v[i]), "+r"(v[i + 1]));
+      const float4 k2 = *reinterpret_cast<const float4*>(tb + 16 * c + i);
+      v[i] = __float_as_uint(k2.y == -INFINITY ? -INFINITY : fmaf(__uint_as_float(v[i]), k2.x, k2.y));
+      v[i + 1] = __float_as_uint(k2.w == -INFINITY ? -INFINITY : fmaf(__uint_as_float(v[i + 1]), k2.z, k2.w));
+    }
+    tmem_st16(scores + 16 * c, v);
+  }
+  tmem_st_wait();
+}
+
 // Zeroes row `row` of a tile of `rows` rows.
 template <int kD>
 __device__ __forceinline__ void zero_row(uint32_t tile, int rows, int row) {
@@ -139,6 +162,7 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t base, int bytes, int lbo) {
 // One CTA per 128 rows of a row of heads, and per part of the keys where there are few such tiles; two CTAs an SM, so that one's products run under the other's
 // exponentials. Four softmax warps (a thread is a row), one that issues products, one that loads. P goes to the second product through TMEM.
 constexpr int kFwdThreads = 192;
+constexpr float kSlack = 8.f;       // the accumulator is scaled anew once a row's maximum has grown by 2^8: most blocks' maxima grow a little in some row of a warp
 
 template <int kD>
 struct Fwd {
@@ -149,6 +173,7 @@ struct Fwd {
   static constexpr int V = K + kStages * kTile;
   static constexpr int TAB = V + kStages * kTile;        // 2 x 128 x {scale, addend}
   static constexpr int BARS = TAB + 2 * 128 * 8;
+  static constexpr int BASE = BARS + 160;                // 6 floats: the warps' largest addends
   static constexpr int STATE = BARS + 256;               // a byte for each of the item's blocks
   static constexpr int bytes(int blocks) { return STATE + (blocks + 15) / 16 * 16 + 1024; }
   // Columns of TMEM. With 128 values a head P takes the place of the scores, which it is made from.
@@ -158,7 +183,7 @@ struct Fwd {
 struct FwdOut {
   __nv_bfloat16* o;
   long long osb, oss, osh;
-  float2* stats;               // [B, Hq, R] {maximum, log2 of the sum}, in units of log2; null: not wanted
+  float* stats;                // [B, Hq, R] log2 of the sum of the exponentials, relative to the mask's base; null: not wanted
   float* part_o;               // parts > 1: [parts][B, Hq, R][D] sums relative to the part's maximum
   float2* part_ml;             // ... {maximum, sum}
   int parts, blocks_per_part, n_tiles;
@@ -224,7 +249,21 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const int s = p.mask ? block_state(p, b, j0 + j, lane) : block_state_unmasked(p, j0 + j);
     if (lane == 0) state[j] = static_cast<uint8_t>(s);
   }
+  float* bases = reinterpret_cast<float*>(smem + L::BASE);
+  const bool addends = p.mask && !p.mask_bool;
+  if (addends) {
+    float a = -INFINITY;
+    for (int kv = threadIdx.x; kv < p.Sk; kv += kFwdThreads) a = fmaxf(a, key_addend(p, b, kv));
+    a = warp_max(a);
+    if (lane == 0) bases[warp] = a;
+  }
   __syncthreads();
+  float base = 0.f;
+  if (addends) {
+    base = max3(max3(bases[0], bases[1], bases[2]), bases[3], fmaxf(bases[4], bases[5]));
+    if (isinf(base)) base = 0.f;       // no key takes part
+    if (p.base && threadIdx.x == 0) p.base[b] = base;       // every CTA of the batch row the same
+  }
   const uint32_t sQ = smem_u32(smem + L::Q), sK = smem_u32(smem + L::K), sV = smem_u32(smem + L::V);
 
   if (warp == 5) {
@@ -311,7 +350,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       float2* tb = tab + (it & 1) * 128;
       if (kind == 1) {
         for (int e = t; e < kKeys; e += warps * 32) {
-          const float2 k = key_entry(p, b, (j0 + j) * kKeys + e);
+          const float2 k = key_entry(p, b, (j0 + j) * kKeys + e, base);
           tb[e] = k;
           if (p.mask && k.y == -INFINITY && ok) {        // an absent key's values meet a probability of zero
             ok = mbar_wait(&v_full[it % L::kStages], (it / L::kStages) & 1, abort_flag, p.status, kStatusWaitFull);
@@ -324,6 +363,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       ok = __all_sync(0xffffffffu, ok && mbar_wait(s_full, it & 1, abort_flag, p.status, kStatusWaitAccum));
       if (ok) {
         tc_fence_after_sync();
+        if (kind != 2) apply_table<4>(tmem + L::S + lanes, tb);        // from here on all blocks are alike
         uint32_t s[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(tmem + L::S + lanes + 32 * c, s[c]);
@@ -336,32 +376,20 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           tc_fence_before_sync();
           arrive_warp(s_free, lane);
         }
+        const float mul = kind == 2 ? sc : 1.f, below = kind == 2 ? base : 0.f;        // a key with nothing added is `base` below the largest
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (kind == 2) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) mx[c] = max3(mx[c], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-#pragma unroll
-          for (int c = 0; c < 4; ++c) mx[c] *= sc;
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float4 k2 = *reinterpret_cast<const float4*>(tb + 32 * c + i);
-              // an absent key's score becomes 0, whatever it is; its addend does the rest
-              if (k2.y == -INFINITY) s[c][i] = 0u;
-              if (k2.w == -INFINITY) s[c][i + 1] = 0u;
-              mx[c] = max3(mx[c], fmaf(__uint_as_float(s[c][i]), k2.x, k2.y), fmaf(__uint_as_float(s[c][i + 1]), k2.z, k2.w));
-            }
-        }
-        const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+          for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+        const float m_new = fmaxf(m, fmaf(mul, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), -below));
         if (it > 0) {        // P may be overwritten, O touched
           ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum));
           tc_fence_after_sync();
-          if (ok && __any_sync(0xffffffffu, m_new > m)) {
+          // (m is -inf where no key has been seen: its sums are zeros, and stay so whatever they are scaled by)
+          if (ok && __any_sync(0xffffffffu, m_new > m + kSlack)) {
             const float alpha = m_new == -INFINITY ? 1.f : ex2_approx(m - m_new);
+            m = m_new;
             l *= alpha;
 #pragma unroll 1
             for (int c = 0; c < kD; c += 16) {
@@ -375,24 +403,16 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           }
         }
         if (ok) {
-          m = m_new;
-          const float neg_m = m == -INFINITY ? 0.f : -m;
+          if (it == 0) m = m_new;
+          const float neg_m = m == -INFINITY ? 0.f : -m - below;
           F2 sum[2] = {f2_splat(0.f), f2_splat(0.f)};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             uint32_t pk[16];
 #pragma unroll
             for (int i = 0; i < 32; i += 2) {
-              const F2 s2 = f2_make(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-              F2 x;
-              if (kind == 2) {
-                x = f2_fma(s2, f2_splat(sc), f2_splat(neg_m));
-              } else {
-                const float4 k2 = *reinterpret_cast<const float4*>(tb + 32 * c + i);
-                x = f2_fma(s2, f2_make(k2.x, k2.z), f2_add(f2_make(k2.y, k2.w), f2_splat(neg_m)));
-              }
               float lo, hi;
-              f2_get(x, lo, hi);
+              f2_get(f2_fma(f2_make(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), f2_splat(mul), f2_splat(neg_m)), lo, hi);
               lo = ex2_approx(lo);
               hi = ex2_approx(hi);
               sum[(i >> 1) & 1] = f2_add(sum[(i >> 1) & 1], f2_make(lo, hi));
@@ -422,7 +442,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const long long pat = static_cast<long long>(part) * p.B * p.Hq * p.R + at;
         if (split) out.part_ml[pat] = make_float2(m, l);
         // a row that no key takes part in: +inf, which makes every probability 2^-inf = 0
-        else if (out.stats) out.stats[at] = l == 0.f ? make_float2(INFINITY, 0.f) : make_float2(m, log2f(l));
+        else if (out.stats) out.stats[at] = l == 0.f ? INFINITY : m + log2f(l);
       }
       float* po = split ? out.part_o + (static_cast<long long>(part) * p.B * p.Hq * p.R + at) * kD : nullptr;
 #pragma unroll
@@ -493,7 +513,7 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const CrossParams p, co
     const long long bh = row / p.R;
     __nv_bfloat16* dst = out_row(p, out.o, out.osb, out.oss, out.osh, static_cast<int>(bh / p.Hq), static_cast<int>(bh % p.Hq), r) + c;
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
-    if (out.stats && c == 0) out.stats[row] = l == 0.f ? make_float2(INFINITY, 0.f) : make_float2(m, log2f(l));
+    if (out.stats && c == 0) out.stats[row] = l == 0.f ? INFINITY : m + log2f(l);
   }
 }
 
@@ -513,15 +533,15 @@ struct Bwd {
   static constexpr int kFixed = 128 * kD * 2, kStream = 64 * kD * 2;
   static constexpr int F0 = 0, F1 = kFixed;
   static constexpr int RING = 2 * kFixed;                          // kStages x {A, B}
-  static constexpr int TAB = RING + kStages * 2 * kStream;         // kStages x 4 x 64 floats
-  static constexpr int BARS = TAB + kStages * 1024;
+  static constexpr int TAB = RING + kStages * 2 * kStream;         // kStages x 128 floats
+  static constexpr int BARS = TAB + kStages * 512;
   static constexpr int TOTAL = BARS + 256;
   static constexpr uint32_t S = 0, DP = 128, ACC0 = 256, ACC1 = 256 + kD;       // S and dP: 2 x 64 columns each
 };
 static_assert(Bwd<128>::TOTAL + 1024 <= 227 * 1024, "shared memory budget");
 
 struct BwdOut {
-  const float2* stats;             // of the forward pass
+  const float* stats;              // of the forward pass
   const float* D;                  // [B, Hq, R]
   const uint8_t* state;            // [B, blocks] of a mask; null without one
   __nv_bfloat16 *dq, *dk, *dv;
@@ -531,6 +551,54 @@ struct BwdOut {
   int row_tiles, key_blocks;       // items of a row of heads, of a key head
   int key_items;                   // the first of all
 };
+
+// 64 columns of a thread's scores and dP in TMEM become P (for keys only) and dS, as bf16 in the first half of their columns:
+// P = 2^(mul s - l), dS = P (dP - D), with l and D of the thread's row, or, where the columns are rows, of the table {-l[64], -D[64]}.
+template <bool kKeys>
+__device__ __forceinline__ void p_and_ds(uint32_t tS, uint32_t tDP, float mul, const float* tb, float neg_l, float neg_d) {
+  uint32_t s[2][32], d[2][32];
+  tmem_ld32(tS, s[0]);
+  tmem_ld32(tS + 32, s[1]);
+  tmem_ld32(tDP, d[0]);
+  tmem_ld32(tDP + 32, d[1]);
+  tmem_ld_wait();
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int e = 0; e < 32; ++e) asm volatile("" : "+r"(s[c][e]), "+r"(d[c][e]));
+  const F2 mul2 = f2_splat(mul);
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    uint32_t pk[16], dk[16];
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+      F2 nl[2] = {f2_splat(neg_l), f2_splat(neg_l)}, nd[2] = {f2_splat(neg_d), f2_splat(neg_d)};
+      if (kKeys) {
+        const float4 x = *reinterpret_cast<const float4*>(tb + 32 * c + e), y = *reinterpret_cast<const float4*>(tb + 64 + 32 * c + e);
+        nl[0] = f2_make(x.x, x.y);
+        nl[1] = f2_make(x.z, x.w);
+        nd[0] = f2_make(y.x, y.y);
+        nd[1] = f2_make(y.z, y.w);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int at = e + 2 * k;
+        float lo, hi;
+        f2_get(f2_fma(f2_make(__uint_as_float(s[c][at]), __uint_as_float(s[c][at + 1])), mul2, nl[k]), lo, hi);
+        const F2 pr = f2_make(ex2_approx(lo), ex2_approx(hi));
+        const F2 ds = f2_mul(pr, f2_add(f2_make(__uint_as_float(d[c][at]), __uint_as_float(d[c][at + 1])), nd[k]));
+        if (kKeys) {
+          f2_get(pr, lo, hi);
+          pk[at >> 1] = pack2(lo, hi);
+        }
+        f2_get(ds, lo, hi);
+        dk[at >> 1] = pack2(lo, hi);
+      }
+    }
+    if (kKeys) tmem_st16(tS + 16 * c, pk);
+    tmem_st16(tDP + 16 * c, dk);
+  }
+}
 
 template <int kD>
 __global__ void __launch_bounds__(kBwdThreads, 1)
@@ -590,6 +658,7 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   pdl_entry();
   const uint32_t sF0 = smem_u32(smem + L::F0), sF1 = smem_u32(smem + L::F1), ring = smem_u32(smem + L::RING);
   const int key_state = keys ? state_of(tile) : fixed_kind;
+  const float mask_base = p.base ? __ldg(p.base + b) : 0.f;
   if (key_state == 0) i1 = i0;                // no key of the block takes part
   const auto live = [&](int i) { return keys || state_of(i >> 1) != 0; };
 
@@ -634,34 +703,27 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     for (int i = i0; i < i1; ++i) {
       if (!live(i)) continue;
       const int st = it % L::kStages;
-      float* tb = tab + st * 256;
-      float2 v[2];
-      float d[2];
+      float* tb = tab + st * 128;
+      float2 v[2];        // rows: -statistic, -D; keys: their entries
       if (keys) {
         const long long base = (static_cast<long long>(b) * p.Hq + h * p.per_kv + i / row_steps) * p.R;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = (i % row_steps) * 64 + e * 32 + lane;
-          v[e] = make_float2(INFINITY, 0.f);
-          d[e] = 0.f;
-          if (r < p.R) {
-            v[e] = __ldg(out.stats + base + r);
-            d[e] = __ldcg(out.D + base + r);
-          }
+          v[e] = make_float2(-INFINITY, 0.f);
+          if (r < p.R) v[e] = make_float2(-__ldg(out.stats + base + r) - (key_state == 2 ? mask_base : 0.f), -__ldcg(out.D + base + r));
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) v[e] = state_of(i >> 1) == 1 ? key_entry(p, b, i * 64 + e * 32 + lane) : make_float2(0.f, 0.f);
+        for (int e = 0; e < 2; ++e) v[e] = state_of(i >> 1) == 1 ? key_entry(p, b, i * 64 + e * 32 + lane, mask_base) : make_float2(0.f, 0.f);
       }
       if (!warp_wait(&empty[st], ((it / L::kStages) & 1) ^ 1, abort_flag, p.status, kStatusWaitEmpty)) break;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int at = e * 32 + lane;
         if (keys) {
-          tb[at] = -(v[e].x + v[e].y);
-          tb[64 + at] = -d[e];
-          tb[128 + at] = -v[e].x;
-          tb[192 + at] = -v[e].y;
+          tb[at] = v[e].x;
+          tb[64 + at] = v[e].y;
         } else {
           reinterpret_cast<float2*>(tb)[at] = v[e];
         }
@@ -720,17 +782,13 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t tS = tmem + L::S + w * 64 + lanes, tDP = tmem + L::DP + w * 64 + lanes;
     // of the row: an entry of the mask, or statistics
-    float sc = p.scale * kLog2e, add = 0.f, neg_m = 0.f, neg_l = 0.f, neg_d = 0.f;
-    bool absent = false;
+    float2 entry = make_float2(0.f, 0.f);
+    float neg_l = 0.f, neg_d = 0.f;
     if (keys) {
-      const float2 k = key_entry(p, b, tile * 128 + t);
-      absent = k.y == -INFINITY;
-      if (!absent) { sc = k.x; add = k.y; }
+      if (key_state == 1) entry = key_entry(p, b, tile * 128 + t, mask_base);
     } else if (tile * 128 + t < p.R) {
       const long long at = (static_cast<long long>(b) * p.Hq + h) * p.R + tile * 128 + t;
-      const float2 s = __ldg(out.stats + at);
-      neg_m = -s.x;
-      neg_l = -s.y;
+      neg_l = -__ldg(out.stats + at);
       neg_d = -__ldcg(out.D + at);
     }
     bool ok = true;
@@ -739,75 +797,42 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (!live(i)) continue;
       if ((it & 1) != w) { ++it; continue; }
       const int st = it % L::kStages;
-      const float* tb = tab + st * 256;
+      const float* tb = tab + st * 128;
       const int kind = keys ? key_state : state_of(i >> 1);
       ok = __all_sync(0xffffffffu, mbar_wait(&tab_full[st], (it / L::kStages) & 1, abort_flag, p.status, kStatusWaitFull) &&
                                        mbar_wait(&s_full[w], (it >> 1) & 1, abort_flag, p.status, kStatusWaitAccum));
       if (!ok) break;
       tc_fence_after_sync();
-      uint32_t s[2][32], d[2][32];
-      tmem_ld32(tS, s[0]);
-      tmem_ld32(tS + 32, s[1]);
-      tmem_ld32(tDP, d[0]);
-      tmem_ld32(tDP + 32, d[1]);
-      tmem_ld_wait();
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int e = 0; e < 32; ++e) asm volatile("" : "+r"(s[c][e]), "+r"(d[c][e]));
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t pk[16], dk[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          F2 off[2], nd[2], s2[2];
+      const float mul = kind == 2 ? p.scale * kLog2e : 1.f;
+      if (kind != 2) {
+        // the scores with their keys' scales and addends, as in the forward pass; nothing of an absent key's dP is left either
+        if (!keys) apply_table<2>(tS, reinterpret_cast<const float2*>(tb));
+#pragma unroll 1
+        for (int c = 0; c < 64; c += 16) {
+          uint32_t v[16];
           if (keys) {
-            const float4 x = *reinterpret_cast<const float4*>(tb + 64 + 32 * c + e);
-            nd[0] = f2_make(x.x, x.y);
-            nd[1] = f2_make(x.z, x.w);
-            if (kind == 2) {
-              const float4 y = *reinterpret_cast<const float4*>(tb + 32 * c + e);
-              off[0] = f2_make(y.x, y.y);
-              off[1] = f2_make(y.z, y.w);
-            } else {
-              const float4 y = *reinterpret_cast<const float4*>(tb + 128 + 32 * c + e), z = *reinterpret_cast<const float4*>(tb + 192 + 32 * c + e);
-              off[0] = f2_add(f2_add(f2_make(y.x, y.y), f2_splat(add)), f2_make(z.x, z.y));
-              off[1] = f2_add(f2_add(f2_make(y.z, y.w), f2_splat(add)), f2_make(z.z, z.w));
-            }
-            s2[0] = s2[1] = f2_splat(sc);
-          } else {
-            nd[0] = nd[1] = f2_splat(neg_d);
-            if (kind == 2) {
-              off[0] = off[1] = f2_splat(neg_m + neg_l);
-              s2[0] = s2[1] = f2_splat(sc);
-            } else {
+            tmem_ld16(tS + c, v);
+            tmem_ld_wait();
 #pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const float4 x = *reinterpret_cast<const float4*>(tb + 2 * (32 * c + e + 2 * k));
-                s2[k] = f2_make(x.x, x.z);
-                off[k] = f2_add(f2_add(f2_make(x.y, x.w), f2_splat(neg_m)), f2_splat(neg_l));
-                if (x.y == -INFINITY) s[c][e + 2 * k] = d[c][e + 2 * k] = 0u;        // absent: nothing of it is left
-                if (x.w == -INFINITY) s[c][e + 2 * k + 1] = d[c][e + 2 * k + 1] = 0u;
-              }
+            for (int e = 0; e < 16; ++e) {
+              asm volatile("" : "+r"(v[e]));
+              v[e] = __float_as_uint(entry.y == -INFINITY ? -INFINITY : fmaf(__uint_as_float(v[e]), entry.x, entry.y));
             }
+            tmem_st16(tS + c, v);
           }
+          tmem_ld16(tDP + c, v);
+          tmem_ld_wait();
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int at = e + 2 * k;
-            float lo, hi;
-            f2_get(f2_fma(f2_make(__uint_as_float(s[c][at]), __uint_as_float(s[c][at + 1])), s2[k], off[k]), lo, hi);
-            const F2 pr = f2_make(ex2_approx(lo), ex2_approx(hi));
-            const F2 ds = f2_mul(pr, f2_add(f2_make(__uint_as_float(d[c][at]), __uint_as_float(d[c][at + 1])), nd[k]));
-            f2_get(pr, lo, hi);
-            pk[at >> 1] = pack2(lo, hi);
-            f2_get(ds, lo, hi);
-            dk[at >> 1] = pack2(lo, hi);
-            if (keys && kind != 2 && absent) pk[at >> 1] = dk[at >> 1] = 0u;
+          for (int e = 0; e < 16; ++e) {
+            asm volatile("" : "+r"(v[e]));
+            if ((keys ? entry.y : reinterpret_cast<const float2*>(tb)[c + e].y) == -INFINITY) v[e] = 0u;
           }
+          tmem_st16(tDP + c, v);
         }
-        if (keys) tmem_st16(tS + 16 * c, pk);
-        tmem_st16(tDP + 16 * c, dk);
+        tmem_st_wait();
       }
+      if (keys) p_and_ds<true>(tS, tDP, mul, tb, 0.f, 0.f);
+      else p_and_ds<false>(tS, tDP, mul, tb, kind == 2 ? neg_l - mask_base : neg_l, neg_d);
       if (!keys && kind == 1 && p.mask && t < 64) {        // an absent key's K meets a dS of zero; S and dP have been read from it
         if (reinterpret_cast<const float2*>(tb)[t].y == -INFINITY) zero_row<kD>(ring + st * 2 * L::kStream, 64, t);
         fence_proxy_async_smem();
@@ -946,6 +971,7 @@ bool make_cross(const fb_cross_args& a, CrossParams& p, int& pack) {
   p.mask = a.mask;
   p.mask_stride = a.mask_stride;
   p.mask_bool = a.mask_bool;
+  p.base = a.mask && !a.mask_bool && a.stats ? a.stats + static_cast<long long>(a.B) * a.H * a.Sq : nullptr;
   p.scale = a.scale;
   p.table = !(a.scale > 0.f);
   p.status = a.status;
@@ -992,7 +1018,7 @@ int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   out.osb = a.o_strides[0];
   out.oss = a.o_strides[1];
   out.osh = a.o_strides[2];
-  out.stats = reinterpret_cast<float2*>(a.stats);
+  out.stats = a.stats;
   out.parts = fwd_parts(p);
   out.blocks_per_part = ceil_div(ceil_div(p.Sk, kKeys), out.parts);
   out.n_tiles = ceil_div(p.R, 128);
@@ -1050,7 +1076,7 @@ int cross_bwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   if (!a.workspace || !a.stats) return -3;
   float* D = a.workspace + space.D;
   uint8_t* state = p.mask ? reinterpret_cast<uint8_t*>(a.workspace + space.state) : nullptr;
-  out.stats = reinterpret_cast<const float2*>(a.stats);
+  out.stats = a.stats;
   out.D = D;
   out.state = state;
   out.part_q = a.workspace + space.part_q;
