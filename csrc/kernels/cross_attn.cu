@@ -38,8 +38,8 @@ struct CrossParams {
   int* status;
 };
 
-// 5-D tensor map over [B, S, H, D] bf16 as (D, pack, S, H / pack, B), one 64-wide panel of `rows` rows a box.
-int make_tmap_rows(CUtensorMap* out, const void* base, int D, int pack, long long S, long long Hq, long long B, long long sb, long long ss, long long sh, int rows) {
+// 5-D tensor map over [B, S, H, D] bf16 as (D, pack, S, H / pack, B), one 64-wide panel of 128 rows a box.
+int make_tmap_rows(CUtensorMap* out, const void* base, int D, int pack, long long S, long long Hq, long long B, long long sb, long long ss, long long sh) {
   static EncodeTiledFn fn = nullptr;
   if (!fn) {
     void* ptr = nullptr;
@@ -52,7 +52,7 @@ int make_tmap_rows(CUtensorMap* out, const void* base, int D, int pack, long lon
   const auto legal = [&](long long stride, long long n) { return static_cast<cuuint64_t>(n > 1 ? stride * 2 : 2 * D); };
   cuuint64_t dims[5] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(pack), static_cast<cuuint64_t>(S), static_cast<cuuint64_t>(Hq), static_cast<cuuint64_t>(B)};
   cuuint64_t strides[4] = {legal(sh, pack), legal(ss, S), legal(sh * pack, Hq), legal(sb, B)};
-  cuuint32_t box[5] = {64, static_cast<cuuint32_t>(pack), static_cast<cuuint32_t>(rows / pack), 1, 1};
+  cuuint32_t box[5] = {64, static_cast<cuuint32_t>(pack), static_cast<cuuint32_t>(128 / pack), 1, 1};
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -153,6 +153,12 @@ __device__ __forceinline__ void zero_row(uint32_t tile, int rows, int row) {
 // Waits, whatever the block's state, until the copies counted by `bar` have landed: shared memory may not be left while one is on its way to it.
 __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
   for (uint32_t it = 0; it < (1u << 20) && !mbar_test(bar, parity); ++it) __nanosleep(20);
+}
+
+// A whole warp's wait. Most find the phase already over, and a plain test says so in a quarter of the time (26 cycles against 98 of the waiting loop).
+__device__ __forceinline__ bool warp_ready(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
+  return warp_wait(bar, parity, abort_flag, status, code);
 }
 
 __device__ __forceinline__ uint64_t k_desc(uint32_t base, int bytes) { return desc_of(smem_desc_lo(base, 16) + (bytes >> 4), smem_desc_hi(1024)); }
@@ -278,14 +284,14 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (!state[j]) continue;
       const int st = it % L::kStages;
       const uint32_t ph = ((it / L::kStages) & 1) ^ 1;
-      if (!warp_wait(&k_empty[st], ph, abort_flag, p.status, kStatusWaitEmpty)) break;
+      if (!warp_ready(&k_empty[st], ph, abort_flag, p.status, kStatusWaitEmpty)) break;
       if (elect_one()) {
         mbar_expect_tx(&k_full[st], L::kTile);
         load_tile<kD>(sK + st * L::kTile, &tmK, &k_full[st], 128, (j0 + j) * kKeys, hk, b);
       }
       __syncwarp();
       ++ks;
-      if (!warp_wait(&v_empty[st], ph, abort_flag, p.status, kStatusWaitEmpty)) break;
+      if (!warp_ready(&v_empty[st], ph, abort_flag, p.status, kStatusWaitEmpty)) break;
       if (elect_one()) {
         mbar_expect_tx(&v_full[st], L::kTile);
         load_tile<kD>(sV + st * L::kTile, &tmV, &v_full[st], 128, (j0 + j) * kKeys, hk, b);
@@ -304,7 +310,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     for (int j = 0; j < n_blocks; ++j) n += state[j] != 0;
     auto scores = [&](int it) {
       const int st = it % L::kStages;
-      if (!warp_wait(&k_full[st], (it / L::kStages) & 1, abort_flag, p.status, kStatusWaitFull)) return false;
+      if (!warp_ready(&k_full[st], (it / L::kStages) & 1, abort_flag, p.status, kStatusWaitFull)) return false;
       tc_fence_after_sync();
       if (elect_one()) {
 #pragma unroll
@@ -316,14 +322,14 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       __syncwarp();
       return true;
     };
-    bool ok = n > 0 && warp_wait(q_full, 0, abort_flag, p.status, kStatusWaitFull) && scores(0);
+    bool ok = n > 0 && warp_ready(q_full, 0, abort_flag, p.status, kStatusWaitFull) && scores(0);
     for (int it = 0; it < n && ok; ++it) {
       if (kD == 64 && it + 1 < n) {        // P has a place of its own: the next scores may come under this block's exponentials
-        ok = warp_wait(s_free, it & 1, abort_flag, p.status, kStatusWaitEpi) && scores(it + 1);
+        ok = warp_ready(s_free, it & 1, abort_flag, p.status, kStatusWaitEpi) && scores(it + 1);
         if (!ok) break;
       }
       const int st = it % L::kStages;
-      ok = warp_wait(p_ready, it & 1, abort_flag, p.status, kStatusWaitEpi) && warp_wait(&v_full[st], (it / L::kStages) & 1, abort_flag, p.status, kStatusWaitFull);
+      ok = warp_ready(p_ready, it & 1, abort_flag, p.status, kStatusWaitEpi) && warp_ready(&v_full[st], (it / L::kStages) & 1, abort_flag, p.status, kStatusWaitFull);
       if (!ok) break;
       tc_fence_after_sync();
       if (elect_one()) {
@@ -333,7 +339,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         umma_commit(&v_empty[st]);
       }
       __syncwarp();
-      if (kD != 64 && it + 1 < n) ok = warp_wait(pv_done, it & 1, abort_flag, p.status, kStatusWaitAccum) && scores(it + 1);
+      if (kD != 64 && it + 1 < n) ok = warp_ready(pv_done, it & 1, abort_flag, p.status, kStatusWaitAccum) && scores(it + 1);
     }
   } else if (warp < warps) {
     // ------------------------------------------------------------------ softmax: a thread is a row
@@ -357,10 +363,11 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (ok) zero_row<kD>(sV + (it % L::kStages) * L::kTile, 128, e);
           }
         }
+        ok = __all_sync(0xffffffffu, ok);
         fence_proxy_async_smem();
         asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
       }
-      ok = __all_sync(0xffffffffu, ok && mbar_wait(s_full, it & 1, abort_flag, p.status, kStatusWaitAccum));
+      ok = ok && warp_ready(s_full, it & 1, abort_flag, p.status, kStatusWaitAccum);
       if (ok) {
         tc_fence_after_sync();
         if (kind != 2) apply_table<4>(tmem + L::S + lanes, tb);        // from here on all blocks are alike
@@ -384,7 +391,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
         const float m_new = fmaxf(m, fmaf(mul, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), -below));
         if (it > 0) {        // P may be overwritten, O touched
-          ok = __all_sync(0xffffffffu, mbar_wait(pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum));
+          ok = warp_ready(pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);
           tc_fence_after_sync();
           // (m is -inf where no key has been seen: its sums are zeros, and stay so whatever they are scaled by)
           if (ok && __any_sync(0xffffffffu, m_new > m + kSlack)) {
@@ -518,25 +525,34 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const CrossParams p, co
 }
 
 // ==================================================================================== backward
-// Two kinds of work item, in one launch. Both keep a tile of 128 rows of two tensors in shared memory and stream tiles of 64 rows of the other two:
+// Two kinds of work item, in one launch. Both keep a tile of 128 rows of two tensors in shared memory and stream tiles of 128 rows of the other two:
 //   keys:  K, V stay; Q, dO stream.   S^T = K Q^T, dP^T = V dO^T;   dV += P^T dO,  dK += dS^T Q
 //   rows:  Q, dO stay; K, V stream.   S = Q K^T,   dP = dO V^T;     dQ += dS K
-// Scores are so worked out twice, but P and dS reach their products in TMEM, never through shared memory, and every gradient is summed by one CTA in the order of the
-// tiles: two calls give the same bits, with no atomics and no pass over a scratch. Scores and dP of a tile go to one of two TMEM buffers, whose warpgroup (a
-// thread is a row of the tile that stays) turns them into P and dS in place while the tensor cores work for the other. Where there are few items, the streamed
-// tiles are cut into parts, whose fp32 sums are added in their order by a second launch.
-constexpr int kBwdThreads = 32 * 11;        // 2 x 4 softmax warps, one that issues products, one that loads, one that fills tables
+// Scores are so worked out twice, but P and dS reach their products in TMEM, in the place of the scores and the dP that they are made from, and never through shared memory,
+// and every gradient is summed by one CTA in the order of the tiles: two calls give the same bits, with no atomics and no pass over a scratch. Sixteen softmax
+// warps: a thread is a row of the tile that stays and 32 of the streamed tile's columns. (With eight, 64 columns each, a warp's exponentials alone took 1050 cycles where the
+// unit needs 512: two warps a scheduler do not hide the latencies.) Products of one CTA run in the order in which they are issued, so that what overwrites a place may be
+// issued right behind what reads it: S(j+1) behind dV(j) (ahead of time, where there is a second buffer), dP(j+1) behind dK(j) or dQ(j).
+// Tiles of 128 columns, not two of 64: with both operands in shared memory a product of 128 x 64 x 16 takes the 64 cycles of one of 128 x 128 x 16.
+// Where there are few items, the streamed tiles are cut into parts, whose fp32 sums are added in their order by a second launch.
+constexpr int kBwdSoftmaxWarps = 16;
+constexpr int kBwdThreads = 32 * (kBwdSoftmaxWarps + 3);        // ... one that issues products, one that loads, one that fills tables
 
 template <int kD>
 struct Bwd {
-  static constexpr int kStages = 4;
-  static constexpr int kFixed = 128 * kD * 2, kStream = 64 * kD * 2;
-  static constexpr int F0 = 0, F1 = kFixed;
-  static constexpr int RING = 2 * kFixed;                          // kStages x {A, B}
-  static constexpr int TAB = RING + kStages * 2 * kStream;         // kStages x 128 floats
-  static constexpr int BARS = TAB + kStages * 512;
+  // Streamed tiles that are there at a time: of Q or K (A), of dO or V (B). A block of V has done its work with dP, Q, K and dO are read again by the products behind.
+  static constexpr int stages_a(bool keys) { return kD == 64 ? 3 : keys ? 2 : 3; }
+  static constexpr int stages_b(bool keys) { return kD == 64 ? 3 : keys ? 2 : 1; }
+  static constexpr int kTile = 128 * kD * 2;
+  static constexpr int F0 = 0, F1 = kTile;
+  static constexpr int RING = 2 * kTile;                           // A's tiles, then B's
+  static constexpr int TAB = RING + (kD == 64 ? 6 : 4) * kTile;    // 3 x 256 floats
+  static constexpr int BARS = TAB + 3 * 1024;
   static constexpr int TOTAL = BARS + 256;
-  static constexpr uint32_t S = 0, DP = 128, ACC0 = 256, ACC1 = 256 + kD;       // S and dP: 2 x 64 columns each
+  // Columns of TMEM: one more buffer of scores where the accumulators leave room for it.
+  static constexpr uint32_t S = 0, DP = 128, ACC0 = 256, ACC1 = 256 + kD;
+  static constexpr uint32_t S2_KEYS = 384, S2_ROWS = kD == 64 ? 384 : 256;
+  static constexpr bool kTwoForKeys = kD == 64;
 };
 static_assert(Bwd<128>::TOTAL + 1024 <= 227 * 1024, "shared memory budget");
 
@@ -552,73 +568,347 @@ struct BwdOut {
   int key_items;                   // the first of all
 };
 
-// 64 columns of a thread's scores and dP in TMEM become P (for keys only) and dS, as bf16 in the first half of their columns:
-// P = 2^(mul s - l), dS = P (dP - D), with l and D of the thread's row, or, where the columns are rows, of the table {-l[64], -D[64]}.
+// P of 32 columns of a thread's scores, as fp32 in `pr` and, for keys, as bf16 in TMEM: P = 2^(mul s - l), with l of the thread's row or, where the columns are rows, -l of `tb`.
 template <bool kKeys>
-__device__ __forceinline__ void p_and_ds(uint32_t tS, uint32_t tDP, float mul, const float* tb, float neg_l, float neg_d) {
-  uint32_t s[2][32], d[2][32];
-  tmem_ld32(tS, s[0]);
-  tmem_ld32(tS + 32, s[1]);
-  tmem_ld32(tDP, d[0]);
-  tmem_ld32(tDP + 32, d[1]);
-  tmem_ld_wait();
-#pragma unroll
-  for (int c = 0; c < 2; ++c)
-#pragma unroll
-    for (int e = 0; e < 32; ++e) asm volatile("" : "+r"(s[c][e]), "+r"(d[c][e]));
+__device__ __forceinline__ void make_p(uint32_t tS, float mul, const float* tb, float neg_l, uint32_t (&pr)[32]) {
+  tmem_ld32_sync(tS, pr);
   const F2 mul2 = f2_splat(mul);
+  uint32_t pk[16];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    uint32_t pk[16], dk[16];
+  for (int e = 0; e < 32; e += 4) {
+    F2 nl[2] = {f2_splat(neg_l), f2_splat(neg_l)};
+    if (kKeys) {
+      const float4 x = *reinterpret_cast<const float4*>(tb + e);
+      nl[0] = f2_make(x.x, x.y);
+      nl[1] = f2_make(x.z, x.w);
+    }
 #pragma unroll
-    for (int e = 0; e < 32; e += 4) {
-      F2 nl[2] = {f2_splat(neg_l), f2_splat(neg_l)}, nd[2] = {f2_splat(neg_d), f2_splat(neg_d)};
+    for (int k = 0; k < 2; ++k) {
+      const int at = e + 2 * k;
+      float lo, hi;
+      f2_get(f2_fma(f2_make(__uint_as_float(pr[at]), __uint_as_float(pr[at + 1])), mul2, nl[k]), lo, hi);
+      lo = ex2_approx(lo);
+      hi = ex2_approx(hi);
+      pr[at] = __float_as_uint(lo);
+      pr[at + 1] = __float_as_uint(hi);
+      if (kKeys) pk[at >> 1] = pack2(lo, hi);
+    }
+  }
+  if (kKeys) tmem_st16(tS, pk);
+}
+// dS = P (dP - D) of the same columns, as bf16 in TMEM.
+template <bool kKeys>
+__device__ __forceinline__ void make_ds(uint32_t tDP, const float* tb, float neg_d, const uint32_t (&pr)[32]) {
+  uint32_t d[32], dk[16];
+  tmem_ld32_sync(tDP, d);
+#pragma unroll
+  for (int e = 0; e < 32; e += 4) {
+    F2 nd[2] = {f2_splat(neg_d), f2_splat(neg_d)};
+    if (kKeys) {
+      const float4 y = *reinterpret_cast<const float4*>(tb + e);
+      nd[0] = f2_make(y.x, y.y);
+      nd[1] = f2_make(y.z, y.w);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int at = e + 2 * k;
+      float lo, hi;
+      f2_get(f2_mul(f2_make(__uint_as_float(pr[at]), __uint_as_float(pr[at + 1])), f2_add(f2_make(__uint_as_float(d[at]), __uint_as_float(d[at + 1])), nd[k])), lo, hi);
+      dk[at >> 1] = pack2(lo, hi);
+    }
+  }
+  tmem_st16(tDP, dk);
+}
+
+struct BwdBars {
+  uint64_t f_full;
+  uint64_t a_full[3], a_empty[3];     // a streamed tile of Q or K has landed; every product that reads it has retired
+  uint64_t b_full[3], b_empty[3];     // ... of dO or V
+  uint64_t tab_full[3];               // A's table is written
+  uint64_t s_full[2], dp_full;        // scores and dP are in TMEM
+  uint64_t p_ready, ds_ready;         // ... and P and dS in their place
+  uint64_t acc_done;                  // every product has retired
+  uint32_t tmem_slot;
+  int abort_flag;
+};
+
+template <int kD, bool kKeys>
+__device__ __forceinline__ void bwd_products(BwdBars& bar, int* status, uint32_t tmem, uint32_t smem, int n) {
+  using L = Bwd<kD>;
+  volatile int* abort_flag = &bar.abort_flag;
+  constexpr bool kTwo = !kKeys || L::kTwoForKeys;
+  constexpr int kA = L::stages_a(kKeys), kB = L::stages_b(kKeys);
+  const uint32_t idesc_s = make_idesc_bf16(128, 128, 0, 0), idesc_acc = make_idesc_bf16(128, kD, 0, 1);
+  const auto s_at = [&](int it) { return tmem + (kTwo && (it & 1) ? (kKeys ? L::S2_KEYS : L::S2_ROWS) : L::S); };
+  const auto a_at = [&](int it) { return smem + L::RING + it % kA * L::kTile; };
+  const auto b_at = [&](int it) { return smem + L::RING + (kA + it % kB) * L::kTile; };
+  const auto scores = [&](int it) {
+    if (!warp_ready(&bar.a_full[it % kA], (it / kA) & 1, abort_flag, status, kStatusWaitFull)) return false;
+    tc_fence_after_sync();
+    if (elect_one()) {
+#pragma unroll
+      for (int k = 0; k < kD / 16; ++k)
+        umma_bf16<1>(s_at(it), k_desc(smem + L::F0, (k >> 2) * 16384 + (k & 3) * 32), k_desc(a_at(it), (k >> 2) * 16384 + (k & 3) * 32), idesc_s, k > 0);
+      umma_commit(&bar.s_full[kTwo ? it & 1 : 0]);
+    }
+    __syncwarp();
+    return true;
+  };
+  const auto dp = [&](int it) {
+    if (!warp_ready(&bar.b_full[it % kB], (it / kB) & 1, abort_flag, status, kStatusWaitFull)) return false;
+    tc_fence_after_sync();
+    if (elect_one()) {
+#pragma unroll
+      for (int k = 0; k < kD / 16; ++k)
+        umma_bf16<1>(tmem + L::DP, k_desc(smem + L::F1, (k >> 2) * 16384 + (k & 3) * 32), k_desc(b_at(it), (k >> 2) * 16384 + (k & 3) * 32), idesc_s, k > 0);
+      umma_commit(&bar.dp_full);
+      if (!kKeys) umma_commit(&bar.b_empty[it % kB]);
+    }
+    __syncwarp();
+    return true;
+  };
+  // acc += (the 128 columns, each 32 left as bf16 in the first half of their place) x (the 128 rows of a streamed tile)
+  const auto accumulate = [&](uint32_t acc, uint32_t from, uint32_t tile, int it, uint64_t* ready, uint64_t* empty) {
+    if (!warp_ready(ready, it & 1, abort_flag, status, kStatusWaitEpi)) return false;
+    tc_fence_after_sync();
+    if (elect_one()) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) umma_bf16_ts(tmem + acc, from + (k >> 1) * 32 + (k & 1) * 8, mn_desc(tile, k * 2048, 16384), idesc_acc, it > 0 || k > 0);
+      umma_commit(empty);
+    }
+    __syncwarp();
+    return true;
+  };
+  bool ok = n > 0 && warp_ready(&bar.f_full, 0, abort_flag, status, kStatusWaitFull) && scores(0) && dp(0);
+  for (int it = 0; it < n && ok; ++it) {
+    const bool more = it + 1 < n;
+    if (kTwo && more) ok = scores(it + 1);
+    if (kKeys) {
+      ok = ok && accumulate(L::ACC0, s_at(it), b_at(it), it, &bar.p_ready, &bar.b_empty[it % kB]);
+      if (!kTwo && more) ok = ok && scores(it + 1);
+    }
+    ok = ok && accumulate(L::ACC1, tmem + L::DP, a_at(it), it, &bar.ds_ready, &bar.a_empty[it % kA]);
+    if (more) ok = ok && dp(it + 1);
+  }
+  if (ok && elect_one()) umma_commit(&bar.acc_done);
+  __syncwarp();
+}
+
+// What the roles of a work item share.
+struct BwdItem {
+  int tile, h, b;              // the 128 keys or rows that stay; a key head or a row of heads
+  int i0, i1;                  // the streamed tiles: rows of the key head's rows of heads one after the other, or blocks of keys
+  int key_state;               // of the keys that stay
+  float mask_base;
+  const uint8_t* state;        // of the batch row's blocks; null without a mask
+};
+template <bool kKeys>
+__device__ __forceinline__ int kind_of(const CrossParams& p, const BwdItem& x, int i) {
+  return kKeys ? x.key_state : x.state ? __ldg(x.state + i) : block_state_unmasked(p, i);
+}
+// A place in a ring of kN stages, and the parity of its turn.
+template <int kN>
+struct Ring {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ void next() {
+    if (++stage == kN) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+};
+
+template <int kD, bool kKeys>
+__device__ __forceinline__ void bwd_loads(BwdBars& bar, const CrossParams& p, const BwdItem& x, uint32_t smem, int row_tiles, const void* f0, const void* f1, const void* a, const void* b) {
+  using L = Bwd<kD>;
+  constexpr int kA = L::stages_a(kKeys), kB = L::stages_b(kKeys);
+  volatile int* abort_flag = &bar.abort_flag;
+  if (elect_one()) {
+    const int at = kKeys ? x.tile * 128 : (x.tile * 128) >> p.pack_log2;
+    mbar_expect_tx(&bar.f_full, 2 * L::kTile);
+    load_tile<kD>(smem + L::F0, f0, &bar.f_full, 128, at, x.h, x.b);
+    load_tile<kD>(smem + L::F1, f1, &bar.f_full, 128, at, x.h, x.b);
+  }
+  __syncwarp();
+  Ring<kA> ra;
+  Ring<kB> rb;
+  int as = 0, bs = 0;
+  int head = kKeys ? x.h * p.per_kv + x.i0 / row_tiles : x.h / p.per_kv, row = kKeys ? x.i0 % row_tiles : 0;
+  for (int i = x.i0; i < x.i1; ++i) {
+    if (!kind_of<kKeys>(p, x, i)) continue;
+    const int seq = kKeys ? (row * 128) >> p.pack_log2 : i * 128;
+    if (!warp_ready(&bar.a_empty[ra.stage], ra.parity ^ 1, abort_flag, p.status, kStatusWaitEmpty)) break;
+    if (elect_one()) {
+      mbar_expect_tx(&bar.a_full[ra.stage], L::kTile);
+      load_tile<kD>(smem + L::RING + ra.stage * L::kTile, a, &bar.a_full[ra.stage], 128, seq, head, x.b);
+    }
+    __syncwarp();
+    ++as;
+    if (!warp_ready(&bar.b_empty[rb.stage], rb.parity ^ 1, abort_flag, p.status, kStatusWaitEmpty)) break;
+    if (elect_one()) {
+      mbar_expect_tx(&bar.b_full[rb.stage], L::kTile);
+      load_tile<kD>(smem + L::RING + (kA + rb.stage) * L::kTile, b, &bar.b_full[rb.stage], 128, seq, head, x.b);
+    }
+    __syncwarp();
+    ++bs;
+    ra.next();
+    rb.next();
+    if (kKeys && ++row == row_tiles) {
+      row = 0;
+      ++head;
+    }
+  }
+  drain(&bar.f_full, 0);
+  for (int u = max(0, as - kA); u < as; ++u) drain(&bar.a_full[u % kA], (u / kA) & 1);
+  for (int u = max(0, bs - kB); u < bs; ++u) drain(&bar.b_full[u % kB], (u / kB) & 1);
+}
+
+// The table of a streamed tile: {-l[128], -D[128]} of its rows, or its keys' entries.
+template <int kD, bool kKeys>
+__device__ __forceinline__ void bwd_tables(BwdBars& bar, const CrossParams& p, const BwdItem& x, float* tab, const float* stats, const float* D, int row_tiles, int lane) {
+  Ring<Bwd<kD>::stages_a(kKeys)> ra;
+  int head = kKeys ? x.h * p.per_kv + x.i0 / row_tiles : 0, row = kKeys ? x.i0 % row_tiles : 0;
+  for (int i = x.i0; i < x.i1; ++i) {
+    const int kind = kind_of<kKeys>(p, x, i);
+    if (!kind) continue;
+    float* tb = tab + ra.stage * 256;
+    float2 v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
       if (kKeys) {
-        const float4 x = *reinterpret_cast<const float4*>(tb + 32 * c + e), y = *reinterpret_cast<const float4*>(tb + 64 + 32 * c + e);
-        nl[0] = f2_make(x.x, x.y);
-        nl[1] = f2_make(x.z, x.w);
-        nd[0] = f2_make(y.x, y.y);
-        nd[1] = f2_make(y.z, y.w);
-      }
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int at = e + 2 * k;
-        float lo, hi;
-        f2_get(f2_fma(f2_make(__uint_as_float(s[c][at]), __uint_as_float(s[c][at + 1])), mul2, nl[k]), lo, hi);
-        const F2 pr = f2_make(ex2_approx(lo), ex2_approx(hi));
-        const F2 ds = f2_mul(pr, f2_add(f2_make(__uint_as_float(d[c][at]), __uint_as_float(d[c][at + 1])), nd[k]));
-        if (kKeys) {
-          f2_get(pr, lo, hi);
-          pk[at >> 1] = pack2(lo, hi);
-        }
-        f2_get(ds, lo, hi);
-        dk[at >> 1] = pack2(lo, hi);
+        const int r = row * 128 + e * 32 + lane;
+        const long long at = (static_cast<long long>(x.b) * p.Hq + head) * p.R + r;
+        v[e] = make_float2(-INFINITY, 0.f);
+        if (r < p.R) v[e] = make_float2(-__ldg(stats + at) - (x.key_state == 2 ? x.mask_base : 0.f), -__ldcg(D + at));
+      } else {
+        v[e] = kind == 1 ? key_entry(p, x.b, i * 128 + e * 32 + lane, x.mask_base) : make_float2(0.f, 0.f);
       }
     }
-    if (kKeys) tmem_st16(tS + 16 * c, pk);
-    tmem_st16(tDP + 16 * c, dk);
+    if (!warp_ready(&bar.a_empty[ra.stage], ra.parity ^ 1, &bar.abort_flag, p.status, kStatusWaitEmpty)) break;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int at = e * 32 + lane;
+      if (kKeys) {
+        tb[at] = v[e].x;
+        tb[128 + at] = v[e].y;
+      } else if (kind == 1) {
+        reinterpret_cast<float2*>(tb)[at] = v[e];
+      }
+    }
+    arrive_warp(&bar.tab_full[ra.stage], lane);
+    ra.next();
+    if (kKeys && ++row == row_tiles) {
+      row = 0;
+      ++head;
+    }
   }
+}
+
+// A tile whose keys go by a table: the scores with their keys' scales and addends, as in the forward pass, in place.
+template <bool kKeys>
+__device__ __noinline__ void masked_scores(uint32_t tS, float2 entry, const float2* tb) {
+  if (!kKeys) return apply_table<1>(tS, tb);
+#pragma unroll 1
+  for (int c = 0; c < 32; c += 16) {
+    uint32_t v[16];
+    tmem_ld16(tS + c, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      asm volatile("" : "+r"(v[e]));
+      v[e] = __float_as_uint(entry.y == -INFINITY ? -INFINITY : fmaf(__uint_as_float(v[e]), entry.x, entry.y));
+    }
+    tmem_st16(tS + c, v);
+  }
+  tmem_st_wait();
+}
+// ... and nothing is left of an absent key's dP.
+template <bool kKeys>
+__device__ __noinline__ void masked_dp(uint32_t tDP, float2 entry, const float2* tb) {
+#pragma unroll 1
+  for (int c = 0; c < 32; c += 16) {
+    uint32_t v[16];
+    tmem_ld16(tDP + c, v);
+    tmem_ld_wait();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      asm volatile("" : "+r"(v[e]));
+      if ((kKeys ? entry.y : tb[c + e].y) == -INFINITY) v[e] = 0u;
+    }
+    tmem_st16(tDP + c, v);
+  }
+  tmem_st_wait();
+}
+
+// P and dS, tile by tile; returns the number of tiles, or -1 after a wait that gave up.
+template <int kD, bool kKeys>
+__device__ __forceinline__ int bwd_softmax(BwdBars& bar, const CrossParams& p, const BwdItem& x, uint32_t tmem, uint32_t smem, const float* tab, const float* stats, const float* D, int warp,
+                                           int lane) {
+  using L = Bwd<kD>;
+  constexpr bool kTwo = !kKeys || L::kTwoForKeys;
+  const int w = warp >> 2, quarter = warp & 3, t = quarter * 32 + lane;
+  const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + w * 32;
+  volatile int* abort_flag = &bar.abort_flag;
+  // of the row: an entry of the mask, or statistics
+  float2 entry = make_float2(0.f, 0.f);
+  float neg_l = 0.f, neg_d = 0.f;
+  if (kKeys) {
+    if (x.key_state == 1) entry = key_entry(p, x.b, x.tile * 128 + t, x.mask_base);
+  } else if (x.tile * 128 + t < p.R) {
+    const long long row = (static_cast<long long>(x.b) * p.Hq + x.h) * p.R + x.tile * 128 + t;
+    neg_l = -__ldg(stats + row);
+    neg_d = -__ldcg(D + row);
+  }
+  Ring<L::stages_a(kKeys)> ra;
+  Ring<kTwo ? 2 : 1> rs;
+  int it = 0;
+  for (int i = x.i0; i < x.i1; ++i) {
+    const int kind = kind_of<kKeys>(p, x, i);
+    if (!kind) continue;
+    const float* tb = tab + ra.stage * 256 + (kKeys ? w * 32 : w * 64);
+    const uint32_t tS = at + (rs.stage ? (kKeys ? L::S2_KEYS : L::S2_ROWS) : L::S), tDP = at + L::DP;
+    if (kKeys || kind != 2)
+      if (!warp_ready(&bar.tab_full[ra.stage], ra.parity, abort_flag, p.status, kStatusWaitFull)) return -1;
+    if (!warp_ready(&bar.s_full[rs.stage], rs.parity, abort_flag, p.status, kStatusWaitAccum)) return -1;
+    tc_fence_after_sync();
+    if (kind != 2) masked_scores<kKeys>(tS, entry, reinterpret_cast<const float2*>(tb));
+    uint32_t pr[32];
+    make_p<kKeys>(tS, kind == 2 ? p.scale * kLog2e : 1.f, tb, kind == 2 ? neg_l - x.mask_base : neg_l, pr);
+    if (kKeys) {
+      tmem_st_wait();
+      tc_fence_before_sync();
+      arrive_warp(&bar.p_ready, lane);
+    }
+    if (!warp_ready(&bar.dp_full, it & 1, abort_flag, p.status, kStatusWaitAccum)) return -1;
+    tc_fence_after_sync();
+    if (kind != 2) {
+      masked_dp<kKeys>(tDP, entry, reinterpret_cast<const float2*>(tb));
+      if (!kKeys && p.mask) {        // nor of an absent key's K, which its dS of zero meets: S and dP have been read from it
+        if (w == 0 && reinterpret_cast<const float2*>(tb)[t].y == -INFINITY) zero_row<kD>(smem + L::RING + ra.stage * L::kTile, 128, t);
+        fence_proxy_async_smem();
+      }
+    }
+    make_ds<kKeys>(tDP, tb + 128, neg_d, pr);
+    tmem_st_wait();
+    tc_fence_before_sync();
+    arrive_warp(&bar.ds_ready, lane);
+    ++it;
+    ra.next();
+    rs.next();
+  }
+  return it;
 }
 
 template <int kD>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
-                 const __grid_constant__ CUtensorMap tmQs, const __grid_constant__ CUtensorMap tmKs, const __grid_constant__ CUtensorMap tmVs,
-                 const __grid_constant__ CUtensorMap tmDOs, const CrossParams p, const BwdOut out) {
+                 const CrossParams p, const BwdOut out) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using L = Bwd<kD>;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
-  uint64_t* f_full = bars;
-  uint64_t* full = bars + 1;                 // [kStages] a streamed pair of tiles has landed
-  uint64_t* empty = full + L::kStages;       // [kStages] ... and every product that reads them has retired
-  uint64_t* tab_full = empty + L::kStages;   // [kStages] its table is written
-  uint64_t* s_full = tab_full + L::kStages;  // [2] S and dP are in TMEM
-  uint64_t* ds_ready = s_full + 2;           // [2] ... and P and dS in their place
-  uint64_t* prod = ds_ready + 2;             // [2] ... and read
-  uint64_t* acc_done = prod + 2;             // every product has retired
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_done + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert(sizeof(BwdBars) <= 256, "barriers");
+  BwdBars& bar = *reinterpret_cast<BwdBars*>(smem + L::BARS);
   float* tab = reinterpret_cast<float*>(smem + L::TAB);
 
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
@@ -627,257 +917,99 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const int parts = keys ? out.parts_k : out.parts_q, per = keys ? out.key_blocks : out.row_tiles, heads = keys ? p.Hk : p.Hq;
   const int part = lin % parts;
   lin /= parts;
-  const int tile = lin % per;
+  BwdItem x;
+  x.tile = lin % per;
   lin /= per;
-  const int h = lin % heads, b = lin / heads;
-  const int nblk = (p.Sk + kKeys - 1) / kKeys;
-  const uint8_t* state_b = out.state ? out.state + static_cast<long long>(b) * nblk : nullptr;
-  const auto state_of = [&](int blk) -> int { return state_b ? __ldg(state_b + blk) : block_state_unmasked(p, blk); };
-  // the streamed tiles: rows of the key head's rows of heads one after the other, or keys
-  const int row_steps = (p.R + 63) / 64, n_all = keys ? p.per_kv * row_steps : (p.Sk + 63) / 64;
-  const int per_part = (n_all + parts - 1) / parts, i0 = part * per_part;
-  int i1 = min(n_all, i0 + per_part);
-  const int fixed_kind = keys ? 0 : 2;
+  x.h = lin % heads;
+  x.b = lin / heads;
+  x.state = out.state ? out.state + static_cast<long long>(x.b) * out.key_blocks : nullptr;
+  const int n_all = keys ? p.per_kv * out.row_tiles : out.key_blocks, per_part = (n_all + parts - 1) / parts;
+  x.i0 = part * per_part;
+  x.i1 = min(n_all, x.i0 + per_part);
 
   if (threadIdx.x == 0) {
-    mbar_init(f_full, 1);
-    for (int s = 0; s < L::kStages; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); mbar_init(&tab_full[s], 1); }
-    for (int s = 0; s < 2; ++s) { mbar_init(&s_full[s], 1); mbar_init(&ds_ready[s], 4); mbar_init(&prod[s], 1); }
-    mbar_init(acc_done, 1);
-    *abort_flag = 0;
+    mbar_init(&bar.f_full, 1);
+    for (int s = 0; s < 3; ++s) {
+      mbar_init(&bar.a_full[s], 1);
+      mbar_init(&bar.a_empty[s], 1);
+      mbar_init(&bar.b_full[s], 1);
+      mbar_init(&bar.b_empty[s], 1);
+      mbar_init(&bar.tab_full[s], 1);
+    }
+    mbar_init(&bar.s_full[0], 1);
+    mbar_init(&bar.s_full[1], 1);
+    mbar_init(&bar.dp_full, 1);
+    mbar_init(&bar.p_ready, kBwdSoftmaxWarps);
+    mbar_init(&bar.ds_ready, kBwdSoftmaxWarps);
+    mbar_init(&bar.acc_done, 1);
+    bar.abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == 8) {
-    tmem_alloc<1>(tmem_slot, 512);
+  if (warp == kBwdSoftmaxWarps) {
+    tmem_alloc<1>(&bar.tmem_slot, 512);
     tmem_relinquish<1>();
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = bar.tmem_slot;
   pdl_entry();
-  const uint32_t sF0 = smem_u32(smem + L::F0), sF1 = smem_u32(smem + L::F1), ring = smem_u32(smem + L::RING);
-  const int key_state = keys ? state_of(tile) : fixed_kind;
-  const float mask_base = p.base ? __ldg(p.base + b) : 0.f;
-  if (key_state == 0) i1 = i0;                // no key of the block takes part
-  const auto live = [&](int i) { return keys || state_of(i >> 1) != 0; };
+  const uint32_t base = smem_u32(smem);
+  x.key_state = !keys ? 0 : x.state ? __ldg(x.state + x.tile) : block_state_unmasked(p, x.tile);
+  x.mask_base = p.base ? __ldg(p.base + x.b) : 0.f;
+  if (keys && x.key_state == 0) x.i1 = x.i0;                // no key of the block takes part
 
-  if (warp == 9) {
-    // ------------------------------------------------------------------ loads
-    if (elect_one()) {
-      mbar_expect_tx(f_full, 2 * L::kFixed);
-      if (keys) {
-        load_tile<kD>(sF0, &tmK, f_full, 128, tile * 128, h, b);
-        load_tile<kD>(sF1, &tmV, f_full, 128, tile * 128, h, b);
-      } else {
-        load_tile<kD>(sF0, &tmQ, f_full, 128, (tile * 128) >> p.pack_log2, h, b);
-        load_tile<kD>(sF1, &tmDO, f_full, 128, (tile * 128) >> p.pack_log2, h, b);
-      }
-    }
-    __syncwarp();
-    int it = 0;
-    for (int i = i0; i < i1; ++i) {
-      if (!live(i)) continue;
-      const int st = it % L::kStages;
-      if (!warp_wait(&empty[st], ((it / L::kStages) & 1) ^ 1, abort_flag, p.status, kStatusWaitEmpty)) break;
-      if (elect_one()) {
-        const uint32_t dst = ring + st * 2 * L::kStream;
-        mbar_expect_tx(&full[st], 2 * L::kStream);
-        if (keys) {
-          const int hq = h * p.per_kv + i / row_steps, seq = ((i % row_steps) * 64) >> p.pack_log2;
-          load_tile<kD>(dst, &tmQs, &full[st], 64, seq, hq, b);
-          load_tile<kD>(dst + L::kStream, &tmDOs, &full[st], 64, seq, hq, b);
-        } else {
-          load_tile<kD>(dst, &tmKs, &full[st], 64, i * 64, h / p.per_kv, b);
-          load_tile<kD>(dst + L::kStream, &tmVs, &full[st], 64, i * 64, h / p.per_kv, b);
-        }
-      }
-      __syncwarp();
-      ++it;
-    }
-    drain(f_full, 0);
-    for (int u = max(0, it - L::kStages); u < it; ++u) drain(&full[u % L::kStages], (u / L::kStages) & 1);
-  } else if (warp == 10) {
-    // ------------------------------------------------------------------ tables of the streamed rows: statistics of rows, entries of keys
-    int it = 0;
-    for (int i = i0; i < i1; ++i) {
-      if (!live(i)) continue;
-      const int st = it % L::kStages;
-      float* tb = tab + st * 128;
-      float2 v[2];        // rows: -statistic, -D; keys: their entries
-      if (keys) {
-        const long long base = (static_cast<long long>(b) * p.Hq + h * p.per_kv + i / row_steps) * p.R;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = (i % row_steps) * 64 + e * 32 + lane;
-          v[e] = make_float2(-INFINITY, 0.f);
-          if (r < p.R) v[e] = make_float2(-__ldg(out.stats + base + r) - (key_state == 2 ? mask_base : 0.f), -__ldcg(out.D + base + r));
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) v[e] = state_of(i >> 1) == 1 ? key_entry(p, b, i * 64 + e * 32 + lane, mask_base) : make_float2(0.f, 0.f);
-      }
-      if (!warp_wait(&empty[st], ((it / L::kStages) & 1) ^ 1, abort_flag, p.status, kStatusWaitEmpty)) break;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int at = e * 32 + lane;
-        if (keys) {
-          tb[at] = v[e].x;
-          tb[64 + at] = v[e].y;
-        } else {
-          reinterpret_cast<float2*>(tb)[at] = v[e];
-        }
-      }
-      arrive_warp(&tab_full[st], lane);
-      ++it;
-    }
-  } else if (warp == 8) {
-    // ------------------------------------------------------------------ products
-    const uint32_t idesc_s = make_idesc_bf16(128, 64, 0, 0), idesc_acc = make_idesc_bf16(128, kD, 0, 1);
-    int n = 0;
-    for (int i = i0; i < i1; ++i) n += live(i);
-    auto scores = [&](int it) {
-      const int st = it % L::kStages, w = it & 1;
-      const uint32_t a = ring + st * 2 * L::kStream;
-      if (!warp_wait(&full[st], (it / L::kStages) & 1, abort_flag, p.status, kStatusWaitFull)) return false;
-      tc_fence_after_sync();
-      if (elect_one()) {
-#pragma unroll
-        for (int k = 0; k < kD / 16; ++k)
-          umma_bf16<1>(tmem + L::S + w * 64, k_desc(sF0, (k >> 2) * 16384 + (k & 3) * 32), k_desc(a, (k >> 2) * 8192 + (k & 3) * 32), idesc_s, k > 0);
-#pragma unroll
-        for (int k = 0; k < kD / 16; ++k)
-          umma_bf16<1>(tmem + L::DP + w * 64, k_desc(sF1, (k >> 2) * 16384 + (k & 3) * 32), k_desc(a + L::kStream, (k >> 2) * 8192 + (k & 3) * 32), idesc_s, k > 0);
-        umma_commit(&s_full[w]);
-      }
-      __syncwarp();
-      return true;
-    };
-    bool ok = n > 0 && warp_wait(f_full, 0, abort_flag, p.status, kStatusWaitFull) && scores(0) && (n < 2 || scores(1));
-    for (int it = 0; it < n && ok; ++it) {
-      const int st = it % L::kStages, w = it & 1;
-      const uint32_t a = ring + st * 2 * L::kStream;
-      ok = warp_wait(&ds_ready[w], (it >> 1) & 1, abort_flag, p.status, kStatusWaitEpi);
-      if (!ok) break;
-      tc_fence_after_sync();
-      if (elect_one()) {
-        if (keys) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16_ts(tmem + L::ACC0, tmem + L::S + w * 64 + k * 8, mn_desc(a + L::kStream, k * 2048, 8192), idesc_acc, it > 0 || k > 0);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) umma_bf16_ts(tmem + L::ACC1, tmem + L::DP + w * 64 + k * 8, mn_desc(a, k * 2048, 8192), idesc_acc, it > 0 || k > 0);
-        umma_commit(&prod[w]);
-        umma_commit(&empty[st]);
-      }
-      __syncwarp();
-      // the next scores of this buffer overwrite what these products read
-      if (it + 2 < n) ok = warp_wait(&prod[w], (it >> 1) & 1, abort_flag, p.status, kStatusWaitAccum) && scores(it + 2);
-    }
-    if (ok && elect_one()) umma_commit(acc_done);
-    __syncwarp();
-  } else {
-    // ------------------------------------------------------------------ P and dS: a thread is a row of the tile that stays, a warpgroup takes every other streamed tile
-    const int w = warp >> 2, quarter = warp & 3, t = quarter * 32 + lane;
-    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t tS = tmem + L::S + w * 64 + lanes, tDP = tmem + L::DP + w * 64 + lanes;
-    // of the row: an entry of the mask, or statistics
-    float2 entry = make_float2(0.f, 0.f);
-    float neg_l = 0.f, neg_d = 0.f;
+  if (warp == kBwdSoftmaxWarps + 1) {
+    if (keys) bwd_loads<kD, true>(bar, p, x, base, out.row_tiles, &tmK, &tmV, &tmQ, &tmDO);
+    else bwd_loads<kD, false>(bar, p, x, base, out.row_tiles, &tmQ, &tmDO, &tmK, &tmV);
+  } else if (warp == kBwdSoftmaxWarps + 2) {
+    if (keys) bwd_tables<kD, true>(bar, p, x, tab, out.stats, out.D, out.row_tiles, lane);
+    else bwd_tables<kD, false>(bar, p, x, tab, out.stats, out.D, out.row_tiles, lane);
+  } else if (warp == kBwdSoftmaxWarps) {
+    int n = x.i1 - x.i0;
     if (keys) {
-      if (key_state == 1) entry = key_entry(p, b, tile * 128 + t, mask_base);
-    } else if (tile * 128 + t < p.R) {
-      const long long at = (static_cast<long long>(b) * p.Hq + h) * p.R + tile * 128 + t;
-      neg_l = -__ldg(out.stats + at);
-      neg_d = -__ldcg(out.D + at);
+      bwd_products<kD, true>(bar, p.status, tmem, base, n);
+    } else {
+      for (int i = x.i0; i < x.i1; ++i) n -= kind_of<false>(p, x, i) == 0;
+      bwd_products<kD, false>(bar, p.status, tmem, base, n);
     }
-    bool ok = true;
-    int it = 0;
-    for (int i = i0; i < i1; ++i) {
-      if (!live(i)) continue;
-      if ((it & 1) != w) { ++it; continue; }
-      const int st = it % L::kStages;
-      const float* tb = tab + st * 128;
-      const int kind = keys ? key_state : state_of(i >> 1);
-      ok = __all_sync(0xffffffffu, mbar_wait(&tab_full[st], (it / L::kStages) & 1, abort_flag, p.status, kStatusWaitFull) &&
-                                       mbar_wait(&s_full[w], (it >> 1) & 1, abort_flag, p.status, kStatusWaitAccum));
-      if (!ok) break;
+  } else {
+    const int n = keys ? bwd_softmax<kD, true>(bar, p, x, tmem, base, tab, out.stats, out.D, warp, lane) : bwd_softmax<kD, false>(bar, p, x, tmem, base, tab, out.stats, out.D, warp, lane);
+    if (n == 0 || (n > 0 && warp_ready(&bar.acc_done, 0, &bar.abort_flag, p.status, kStatusWaitAccum))) {
       tc_fence_after_sync();
-      const float mul = kind == 2 ? p.scale * kLog2e : 1.f;
-      if (kind != 2) {
-        // the scores with their keys' scales and addends, as in the forward pass; nothing of an absent key's dP is left either
-        if (!keys) apply_table<2>(tS, reinterpret_cast<const float2*>(tb));
-#pragma unroll 1
-        for (int c = 0; c < 64; c += 16) {
-          uint32_t v[16];
-          if (keys) {
-            tmem_ld16(tS + c, v);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              asm volatile("" : "+r"(v[e]));
-              v[e] = __float_as_uint(entry.y == -INFINITY ? -INFINITY : fmaf(__uint_as_float(v[e]), entry.x, entry.y));
-            }
-            tmem_st16(tS + c, v);
-          }
-          tmem_ld16(tDP + c, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            asm volatile("" : "+r"(v[e]));
-            if ((keys ? entry.y : reinterpret_cast<const float2*>(tb)[c + e].y) == -INFINITY) v[e] = 0u;
-          }
-          tmem_st16(tDP + c, v);
-        }
-        tmem_st_wait();
-      }
-      if (keys) p_and_ds<true>(tS, tDP, mul, tb, 0.f, 0.f);
-      else p_and_ds<false>(tS, tDP, mul, tb, kind == 2 ? neg_l - mask_base : neg_l, neg_d);
-      if (!keys && kind == 1 && p.mask && t < 64) {        // an absent key's K meets a dS of zero; S and dP have been read from it
-        if (reinterpret_cast<const float2*>(tb)[t].y == -INFINITY) zero_row<kD>(ring + st * 2 * L::kStream, 64, t);
-        fence_proxy_async_smem();
-      }
-      tmem_st_wait();
-      tc_fence_before_sync();
-      arrive_warp(&ds_ready[w], lane);
-      ++it;
-    }
-    // ---- out; `it` counts the tiles of both warpgroups
-    if (it > 0) ok = __all_sync(0xffffffffu, ok && mbar_wait(acc_done, 0, abort_flag, p.status, kStatusWaitAccum));
-    if (ok) {
-      tc_fence_after_sync();
-      const int r = tile * 128 + t;
-      // keys: the first warpgroup writes dK, the second dV; rows: half of dQ's columns each
-      const bool inside = keys ? r < p.Sk : r < p.R;
-      const int c0 = keys ? 0 : w * (kD / 2), c1 = keys ? kD : c0 + kD / 2;
-      const uint32_t acc = tmem + (keys && w == 1 ? L::ACC0 : L::ACC1) + lanes;
-      const float mul = keys && w == 1 ? 1.f : p.scale;
-      const long long line = keys ? (static_cast<long long>(b) * p.Hk + h) * p.Sk + r : (static_cast<long long>(b) * p.Hq + h) * p.R + r;
+      // keys: half of the warps write dK, the others dV; rows: all of them dQ
+      const int w = warp >> 2, quarter = warp & 3, r = x.tile * 128 + quarter * 32 + lane;
+      const bool inside = keys ? r < p.Sk : r < p.R, is_v = keys && w >= 2;
+      const int step = keys ? kD / 2 : kD / 4, c0 = (keys ? w & 1 : w) * step, c1 = c0 + step;
+      const uint32_t acc = tmem + (is_v ? L::ACC0 : L::ACC1) + (static_cast<uint32_t>(quarter * 32) << 16);
+      const float mul = is_v ? 1.f : p.scale;
+      const long long line = keys ? (static_cast<long long>(x.b) * p.Hk + x.h) * p.Sk + r : (static_cast<long long>(x.b) * p.Hq + x.h) * p.R + r;
       const long long lines = keys ? static_cast<long long>(p.B) * p.Hk * p.Sk : static_cast<long long>(p.B) * p.Hq * p.R;
       float* part_at = nullptr;
       __nv_bfloat16* at = nullptr;
-      if (parts > 1) part_at = (keys ? (w == 1 ? out.part_v : out.part_k) : out.part_q) + (part * lines + line) * kD;
-      else if (keys) at = (w == 1 ? out.dv : out.dk) + b * out.ksb + r * out.kss + h * out.ksh;
-      else at = out_row(p, out.dq, out.qsb, out.qss, out.qsh, b, h, r);
+      if (parts > 1) part_at = (keys ? (is_v ? out.part_v : out.part_k) : out.part_q) + (part * lines + line) * kD;
+      else if (keys) at = (is_v ? out.dv : out.dk) + x.b * out.ksb + r * out.kss + x.h * out.ksh;
+      else at = out_row(p, out.dq, out.qsb, out.qss, out.qsh, x.b, x.h, r);
 #pragma unroll 1
-      for (int c = c0; c < c1; c += 32) {
-        uint32_t v[32];
-        if (it > 0) {
-          tmem_ld32_sync(acc + c, v);
-        } else {
+      for (int c = c0; c < c1; c += 16) {
+        uint32_t v[16];
+        if (n > 0) {
+          tmem_ld16(acc + c, v);
+          tmem_ld_wait();
+        }
+        float f[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = 0u;
+        for (int e = 0; e < 16; ++e) {
+          if (n > 0) asm volatile("" : "+r"(v[e]));
+          f[e] = n > 0 ? __uint_as_float(v[e]) * mul : 0.f;
         }
         if (inside) {
-          float f[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(v[e]) * mul;
           if (parts > 1) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(part_at + c + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+            for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(part_at + c + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) *reinterpret_cast<uint4*>(at + c + e) = pack8(f + e);
+            for (int e = 0; e < 16; e += 8) *reinterpret_cast<uint4*>(at + c + e) = pack8(f + e);
           }
         }
       }
@@ -885,7 +1017,7 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == kBwdSoftmaxWarps) {
     tc_fence_after_sync();
     tmem_dealloc<1>(tmem, 512);
   }
@@ -996,10 +1128,10 @@ int fwd_parts(const CrossParams& p) {
 
 // Parts of an item's streamed tiles in the backward pass: an item longer than its share of all the work holds up the launch's end.
 void bwd_parts(const CrossParams& p, int& parts_q, int& parts_k) {
-  const long long n_q = ceil_div(p.Sk, 64), n_k = static_cast<long long>(p.per_kv) * ceil_div(p.R, 64);
+  const long long n_q = ceil_div(p.Sk, 128), n_k = static_cast<long long>(p.per_kv) * ceil_div(p.R, 128);
   const long long items_q = static_cast<long long>(ceil_div(p.R, 128)) * p.Hq * p.B, items_k = static_cast<long long>(ceil_div(p.Sk, 128)) * p.Hk * p.B;
   const long long share = (n_q * items_q + n_k * items_k) / sm_count();
-  const long long least = share > 8 ? share : 8;
+  const long long least = share > 4 ? share : 4;
   parts_q = n_q > least ? ceil_div(n_q, least) : 1;
   parts_k = n_k > least ? ceil_div(n_k, least) : 1;
   parts_q = ceil_div(n_q, ceil_div(n_q, parts_q));
@@ -1009,9 +1141,9 @@ void bwd_parts(const CrossParams& p, int& parts_q, int& parts_k) {
 template <int kD>
 int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream_t stream) {
   CUtensorMap tq, tk, tv;
-  int e = make_tmap_rows(&tq, a.q, kD, pack, a.Sq, p.Hq, a.B, a.q_strides[0], a.q_strides[1], a.q_strides[2], 128);
-  if (!e) e = make_tmap_rows(&tk, a.k, kD, 1, a.Sk, a.Hk, a.B, a.k_strides[0], a.k_strides[1], a.k_strides[2], 128);
-  if (!e) e = make_tmap_rows(&tv, a.v, kD, 1, a.Sk, a.Hk, a.B, a.v_strides[0], a.v_strides[1], a.v_strides[2], 128);
+  int e = make_tmap_rows(&tq, a.q, kD, pack, a.Sq, p.Hq, a.B, a.q_strides[0], a.q_strides[1], a.q_strides[2]);
+  if (!e) e = make_tmap_rows(&tk, a.k, kD, 1, a.Sk, a.Hk, a.B, a.k_strides[0], a.k_strides[1], a.k_strides[2]);
+  if (!e) e = make_tmap_rows(&tv, a.v, kD, 1, a.Sk, a.Hk, a.B, a.v_strides[0], a.v_strides[1], a.v_strides[2]);
   if (e) return e;
   FwdOut out = {};
   out.o = static_cast<__nv_bfloat16*>(a.o);
@@ -1060,15 +1192,11 @@ BwdSpace bwd_space(const CrossParams& p, int D, int parts_q, int parts_k) {
 
 template <int kD>
 int cross_bwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream_t stream) {
-  CUtensorMap maps[8];
-  int e = 0;
-  for (int i = 0; i < 2 && !e; ++i) {
-    const int rows = i ? 64 : 128;
-    e = make_tmap_rows(&maps[4 * i], a.q, kD, pack, a.Sq, p.Hq, a.B, a.q_strides[0], a.q_strides[1], a.q_strides[2], rows);
-    if (!e) e = make_tmap_rows(&maps[4 * i + 1], a.k, kD, 1, a.Sk, a.Hk, a.B, a.k_strides[0], a.k_strides[1], a.k_strides[2], rows);
-    if (!e) e = make_tmap_rows(&maps[4 * i + 2], a.v, kD, 1, a.Sk, a.Hk, a.B, a.v_strides[0], a.v_strides[1], a.v_strides[2], rows);
-    if (!e) e = make_tmap_rows(&maps[4 * i + 3], a.d_o, kD, pack, a.Sq, p.Hq, a.B, a.do_strides[0], a.do_strides[1], a.do_strides[2], rows);
-  }
+  CUtensorMap tq, tk, tv, tdo;
+  int e = make_tmap_rows(&tq, a.q, kD, pack, a.Sq, p.Hq, a.B, a.q_strides[0], a.q_strides[1], a.q_strides[2]);
+  if (!e) e = make_tmap_rows(&tk, a.k, kD, 1, a.Sk, a.Hk, a.B, a.k_strides[0], a.k_strides[1], a.k_strides[2]);
+  if (!e) e = make_tmap_rows(&tv, a.v, kD, 1, a.Sk, a.Hk, a.B, a.v_strides[0], a.v_strides[1], a.v_strides[2]);
+  if (!e) e = make_tmap_rows(&tdo, a.d_o, kD, pack, a.Sq, p.Hq, a.B, a.do_strides[0], a.do_strides[1], a.do_strides[2]);
   if (e) return e;
   BwdOut out = {};
   bwd_parts(p, out.parts_q, out.parts_k);
@@ -1101,8 +1229,8 @@ int cross_bwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
              a.o_strides[2], static_cast<const __nv_bfloat16*>(a.d_o), a.do_strides[0], a.do_strides[1], a.do_strides[2], D, state, row_blocks);
   constexpr int smem = Bwd<kD>::TOTAL + 1024;
   if (const cudaError_t err = allow_smem<cross_bwd_kernel<kD>>(smem)) return static_cast<int>(err);
-  if (const cudaError_t err = launch_pdl(cross_bwd_kernel<kD>, dim3(static_cast<unsigned>(items)), dim3(kBwdThreads), static_cast<size_t>(smem), stream, maps[0], maps[1], maps[2], maps[3],
-                                         maps[4], maps[5], maps[6], maps[7], p, out))
+  if (const cudaError_t err = launch_pdl(cross_bwd_kernel<kD>, dim3(static_cast<unsigned>(items)), dim3(kBwdThreads), static_cast<size_t>(smem), stream, tq, tk, tv, tdo,
+                                         p, out))
     return static_cast<int>(err);
   if (out.parts_q > 1 || out.parts_k > 1) {
     const long long sum_rows = (out.parts_q > 1 ? rows : 0) + (out.parts_k > 1 ? 2ll * p.B * p.Hk * p.Sk : 0), blocks = (sum_rows * (kD / 4) + 255) / 256;
