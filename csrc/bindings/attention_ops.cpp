@@ -268,7 +268,7 @@ Tensor space_for(fb_cross_args& a, bool backward, const Tensor& like) {
   return t;
 }
 
-Tensor launch_cross(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& mask, double scale, Tensor* stats) {
+Tensor launch_cross(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& mask, double scale, Tensor* stats, Tensor* info) {
   const Tensor q = mapped(q_in), k = mapped(k_in), v = mapped(v_in);
   c10::cuda::CUDAGuard guard(q.device());
   Tensor o = at::empty(q.sizes(), at::TensorOptions().dtype(at::kBFloat16).device(q.device()));
@@ -276,8 +276,12 @@ Tensor launch_cross(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, 
   a.o = o.data_ptr();
   strides_of(o, a.o_strides);
   if (stats) {
-    *stats = at::empty({q.size(0) * (q.size(2) * q.size(1) + 1)}, at::TensorOptions().dtype(at::kFloat).device(q.device()));
+    *stats = at::empty({q.size(0) * q.size(2) * q.size(1)}, at::TensorOptions().dtype(at::kFloat).device(q.device()));
     a.stats = stats->data_ptr<float>();
+  }
+  if (mask.defined()) {
+    *info = at::empty({fb_cross_mask_info(&a)}, at::TensorOptions().dtype(at::kInt).device(q.device()));
+    a.mask_info = info->data_ptr<int>();
   }
   const Tensor space = space_for(a, false, q);
   check(fb_cross_attn_fwd(&a, stream_of(q)), "fb_cross_attn_fwd");
@@ -287,8 +291,8 @@ Tensor launch_cross(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, 
 struct CrossFn : public torch::autograd::Function<CrossFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask_in, double scale) {
     const Tensor mask = value(mask_in);
-    Tensor stats, o = launch_cross(q, k, v, mask, scale, &stats);
-    ctx->save_for_backward({q, k, v, mask, o, stats});
+    Tensor stats, info, o = launch_cross(q, k, v, mask, scale, &stats, &info);
+    ctx->save_for_backward({q, k, v, mask, o, stats, info});
     ctx->saved_data["scale"] = scale;
     return o;
   }
@@ -311,6 +315,7 @@ struct CrossFn : public torch::autograd::Function<CrossFn> {
     a.dv = dv.data_ptr();
     strides_of(dk, a.dk_strides);
     a.stats = stats.data_ptr<float>();
+    if (mask.defined()) a.mask_info = saved[6].data_ptr<int>();
     const Tensor space = space_for(a, true, q);
     check(fb_cross_attn_bwd(&a, stream_of(q)), "fb_cross_attn_bwd");
     return {dq, dk, dv, Tensor(), Tensor()};
@@ -336,7 +341,8 @@ std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Te
     if (Sk > 1 && mask.stride(1) != 1) mask = mask.contiguous();
   }
   if (records({&q, &k, &v})) return CrossFn::apply(q, k, v, given(mask), scale);
-  return launch_cross(q, k, v, mask, scale, nullptr);
+  Tensor info;
+  return launch_cross(q, k, v, mask, scale, nullptr, &info);
 }
 
 }  // namespace

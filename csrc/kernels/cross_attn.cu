@@ -5,10 +5,16 @@
 // Rows. The query heads of a key head lie side by side in memory, so a tile's rows are (query, head) pairs of a power of two `pack` of them, head fastest, which one 5-D
 // tensor map gives; what is left of the group is heads of their own. One key head's K and V are so read once for all of them, and few queries fill a tile better.
 //
-// Masks are of keys. Blocks of 128 keys none of which takes part are left out; blocks all of which do, with nothing added, take the short path; the rest go by a table
-// of {scale, addend} for each key. A key at -inf is absent: its score is replaced whatever it is, and where it meets a product as a row of the streamed operand that row
-// is zeroed in shared memory, so infinities and NaN behind a mask reach nothing. An addend beyond 2^100 takes the score's place, as it would in 64 bits.
-// Addends are taken relative to the batch row's largest, so that a mask common to a row's keys costs its scores no bits.
+// Masks are of keys. A first, small launch lists each batch row's live blocks of 128 keys: those all of whose keys take part, with nothing added, take the short path, the rest
+// go by a table of {scale, addend} for each key, and blocks without a key are left out. A key at -inf is absent: its score is replaced whatever it is, and where
+// it meets a product as a row of the streamed operand that row is zeroed in shared memory, so infinities and NaN behind a mask reach nothing. An addend beyond
+// 2^100 takes the score's place, as it would in 64 bits. Addends are taken relative to the batch row's largest, so that a mask common to a row's keys costs its
+// scores no bits.
+//
+// Work. A unit is a tile of 128 rows that stays with 128 of what streams past it. As many CTAs as fit the GPU take whole tiles as long as there is one for each of them, side by
+// side, so that they stream the same heads out of L2 (with one stretch of all units for each CTA, as long heads of 128 took 287 us against 241). What is left, less
+// than a tile each, is cut into equal stretches of units: no last wave, and few queries over many keys fill the GPU as well. A tile that a stretch's border cuts leaves
+// fp32 sums behind, which a small second launch adds up in the order of the stretches (two calls give the same bits).
 //
 // Statistics, sums and products are fp32; P and dS are rounded to bf16 once, as operands of the tensor cores.
 #include <cuda.h>
@@ -22,19 +28,22 @@
 namespace fb {
 namespace {
 
-constexpr int kKeys = 128;          // keys of a mask block
-constexpr int kMaxBlocks = 4096;    // mask blocks of one work item
+constexpr int kKeys = 128;                  // keys of a block
 constexpr float kHuge = 1.2676506e30f;      // 2^100
 
 struct CrossParams {
   int B, Hq, Hk, R, Sk;             // Hq = H / pack rows of heads; R = Sq * pack rows each
   int pack_log2, per_kv;            // log2 of pack; rows of heads that share a key head
+  int row_tiles, key_blocks;        // of a row of heads; of a key head
   const void* mask;                 // [B, Sk]: one byte a key (0: absent), or fp32 addends; null: none
-  float* base;                      // [B] of addends: the batch row's largest, which the forward pass leaves for the backward pass (null: nobody wants it)
   long long mask_stride;
   int mask_bool;
   float scale;
   int table;                        // 1: every block by the table (the short path wants a positive scale)
+  // what the mask comes to (null without one): live blocks of a batch row, its largest addend, and [B, key_blocks] of block << 1 | goes by the table, those without a key last
+  int* live_count;
+  float* base;
+  int* live;
   int* status;
 };
 
@@ -99,26 +108,267 @@ __device__ __forceinline__ int block_state(const CrossParams& p, int b, int blk,
   bool any = false, all = true;
 #pragma unroll
   for (int i = 0; i < kKeys / 32; ++i) {
-    const int kv = blk * kKeys + i * 32 + lane;
-    bool in = kv < p.Sk, plain = in;
-    if (in && p.mask) {
-      const long long at = b * p.mask_stride + kv;
-      if (p.mask_bool) {
-        in = plain = static_cast<const uint8_t*>(p.mask)[at] != 0;
-      } else {
-        const float a = static_cast<const float*>(p.mask)[at];
-        in = a != -INFINITY;
-        plain = a == 0.f;
-      }
-    }
-    any |= in;
-    all &= plain;
+    const float a = key_addend(p, b, blk * kKeys + i * 32 + lane);
+    any |= a != -INFINITY;
+    all &= a == 0.f;
   }
   any = __any_sync(0xffffffffu, any);
   all = __all_sync(0xffffffffu, all);
   return !any ? 0 : all && !p.table ? 2 : 1;
 }
-__device__ __forceinline__ int block_state_unmasked(const CrossParams& p, int blk) { return (blk + 1) * kKeys <= p.Sk && !p.table ? 2 : 1; }
+
+// One block a batch row: its live blocks in their order, then the others, and its largest addend.
+__global__ void __launch_bounds__(256) cross_live_kernel(const CrossParams p) {
+  __shared__ int state[256], warp_live[8];
+  __shared__ float largest[8];
+  pdl_entry();
+  const int b = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int* live = p.live + static_cast<long long>(b) * p.key_blocks;
+  int n_live = 0, n_dead = 0;
+  for (int first = 0; first < p.key_blocks; first += 256) {
+    const int n = min(256, p.key_blocks - first);
+#pragma unroll 4
+    for (int j = warp; j < n; j += 8) {
+      const int s = block_state(p, b, first + j, lane);
+      if (lane == 0) state[j] = s;
+    }
+    __syncthreads();
+    const int s = static_cast<int>(threadIdx.x) < n ? state[threadIdx.x] : 0;
+    const unsigned bits = __ballot_sync(0xffffffffu, s != 0);
+    if (lane == 0) warp_live[warp] = __popc(bits);
+    __syncthreads();
+    int before = __popc(bits & ((1u << lane) - 1)), total = 0;
+    for (int k = 0; k < 8; ++k) {
+      if (k < warp) before += warp_live[k];
+      total += warp_live[k];
+    }
+    if (static_cast<int>(threadIdx.x) < n) {
+      const int at = s ? n_live + before : p.key_blocks - 1 - (n_dead + static_cast<int>(threadIdx.x) - before);
+      live[at] = (first + static_cast<int>(threadIdx.x)) << 1 | (s == 1);
+    }
+    n_live += total;
+    n_dead += n - total;
+    __syncthreads();
+  }
+  float a = -INFINITY;
+  if (!p.mask_bool)
+    for (int kv = threadIdx.x; kv < p.Sk; kv += 256) a = fmaxf(a, key_addend(p, b, kv));
+  a = warp_max(a);
+  if (lane == 0) largest[warp] = a;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < 8; ++k) a = fmaxf(a, largest[k]);
+    p.base[b] = isinf(a) ? 0.f : a;
+    p.live_count[b] = n_live;
+  }
+}
+
+// What an earlier kernel of the stream wrote is read with plain loads or past L1. A read-only load (ld.global.nc) may answer from a line that was in L1 before the earlier
+// kernel wrote it: with programmatic launches that happened about once in 10^4 calls.
+// Live blocks of the batch rows: null without a mask, a copy in shared memory of up to kCounts, p.live_count otherwise.
+constexpr int kCounts = 512;
+__device__ __forceinline__ int live_of(const CrossParams& p, const int* counts, int b) { return counts ? *reinterpret_cast<const volatile int*>(counts + b) : p.key_blocks; }
+__device__ __forceinline__ const int* counts_of(const CrossParams& p, int* copy) {
+  if (!p.live_count || p.B > kCounts) return p.live_count;
+  for (int b = threadIdx.x; b < p.B; b += blockDim.x) copy[b] = __ldcg(p.live_count + b);
+  return copy;
+}
+// Live block i of a batch row: {block, whether it goes by the table}.
+__device__ __forceinline__ int2 live_block(const CrossParams& p, int b, int i) {
+  if (p.live) {
+    const int v = __ldcg(p.live + static_cast<long long>(b) * p.key_blocks + i);
+    return make_int2(v >> 1, v & 1);
+  }
+  return make_int2(i, p.table || (i + 1) * kKeys > p.Sk);
+}
+
+// Waits, whatever the block's state, until the copies counted by `bar` have landed: shared memory may not be left while one is on its way to it.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+  for (uint32_t it = 0; it < (1u << 20) && !mbar_test(bar, parity); ++it) __nanosleep(20);
+}
+
+// A whole warp's wait. Most find the phase already over, and a plain test says so in a quarter of the time (26 cycles against 98 of the waiting loop).
+__device__ __forceinline__ bool warp_ready(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
+  return warp_wait(bar, parity, abort_flag, status, code);
+}
+
+// A place in a ring of kN stages, and the parity of its turn.
+template <int kN>
+struct Ring {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ void next() {
+    if (++stage == kN) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+};
+
+// ---- who does what. Tiles go batch row by batch row.
+struct Place {
+  int b, tile, i;
+};
+struct Run {
+  int b, tile, i0, i1, n;        // a tile's units [i0, i1) of n
+};
+// kKeyTiles: a tile is a live block of a key head, and the rows of its rows of heads stream past it; otherwise it is 128 rows of a row of heads, and live blocks do.
+template <bool kKeyTiles>
+__device__ __forceinline__ int tiles_of(const CrossParams& p, const int* counts, int b) {
+  const int n = live_of(p, counts, b);
+  return kKeyTiles ? p.Hk * n : n ? p.Hq * p.row_tiles : 0;
+}
+template <bool kKeyTiles>
+__device__ __forceinline__ int length_of(const CrossParams& p, const int* counts, int b) { return kKeyTiles ? p.per_kv * p.row_tiles : live_of(p, counts, b); }
+
+// A CTA's share: tiles `first`, `first` + CTAs, ... , `waves` of them, then the stretch [begin, end).
+struct Share {
+  int waves;
+  Place begin, end;
+};
+// The batch row in which `u` falls, counted in what `of` gives each, from batch row `b` on; u is left as what remains of it there. By a whole warp.
+template <typename Of>
+__device__ __forceinline__ int row_of(const CrossParams& p, int b, unsigned& u, int lane, Of of) {
+  for (; b < p.B; b += 32) {
+    const unsigned mine = b + lane < p.B ? of(b + lane) : 0;
+    unsigned upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, u < upto);
+    if (past) {
+      const int k = __ffs(past) - 1;
+      u -= __shfl_sync(0xffffffffu, upto - mine, k);
+      return b + k;
+    }
+    u -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return p.B;
+}
+// By a whole warp.
+template <bool kKeyTiles>
+__device__ __forceinline__ Share share_of(const CrossParams& p, const int* counts, int cta, int ctas, bool whole, int lane) {
+  const auto tiles = [&](int b) { return static_cast<unsigned>(tiles_of<kKeyTiles>(p, counts, b)); };
+  const auto units = [&](int b) { return tiles(b) * static_cast<unsigned>(length_of<kKeyTiles>(p, counts, b)); };
+  unsigned total, tile, rest;
+  int b0;
+  if (!counts) {
+    const unsigned per_b = tiles(0);
+    total = p.B * per_b;
+    tile = total / ctas * ctas;
+    b0 = tile / per_b;
+    rest = (total - tile) * static_cast<unsigned>(length_of<kKeyTiles>(p, counts, 0));        // (less than a tile for each CTA: 32 bits hold the units)
+    tile -= b0 * per_b;
+  } else {
+    total = 0;
+    for (int b = lane; b < p.B; b += 32) total += tiles(b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    tile = total / ctas * ctas;
+    b0 = row_of(p, 0, tile, lane, tiles);
+    rest = 0;
+    for (int b = b0 + lane; b < p.B; b += 32) rest += units(b);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+    if (b0 < p.B) rest -= tile * length_of<kKeyTiles>(p, counts, b0);
+  }
+  // the place that is so many units behind the start of tile (b0, tile), or at the next start of a tile from there
+  const auto border = [&](int k) -> Place {
+    unsigned u = static_cast<unsigned>(static_cast<unsigned long long>(rest) * k / ctas);
+    int b = b0;
+    if (b >= p.B) return {p.B, 0, 0};
+    u += tile * length_of<kKeyTiles>(p, counts, b);
+    if (!counts) {
+      const unsigned per_b = units(0), n = u / per_b;
+      b += n;
+      u -= n * per_b;
+    } else {
+      b = row_of(p, b, u, lane, units);
+    }
+    if (b >= p.B) return {p.B, 0, 0};
+    const unsigned len = length_of<kKeyTiles>(p, counts, b);
+    Place at = {b, static_cast<int>(u / len), static_cast<int>(u % len)};
+    if (whole && at.i > 0) {
+      at.i = 0;
+      if (++at.tile == static_cast<int>(tiles(b))) {
+        at.tile = 0;
+        do ++at.b;
+        while (at.b < p.B && live_of(p, counts, at.b) == 0);
+      }
+    }
+    return at;
+  };
+  return {static_cast<int>(total / ctas), border(cta), border(cta + 1)};
+}
+// The runs of a share, one after the other.
+template <bool kKeyTiles>
+struct Walk {
+  const int* counts;
+  Place at;
+  int waves, tile, b = 0, step;
+  __device__ Walk(const int* counts, const Share& s, int first, int ctas) : counts(counts), at(s.begin), waves(s.waves), tile(first), step(ctas) {}
+  __device__ bool next(const CrossParams& p, const Place& end, Run& r) {
+    if (waves > 0) {
+      if (!counts) {
+        const int n = tiles_of<kKeyTiles>(p, counts, 0), k = tile / n;
+        b += k;
+        tile -= k * n;
+      } else {
+        for (int n; tile >= (n = tiles_of<kKeyTiles>(p, counts, b)); ++b) tile -= n;
+      }
+      const int n = length_of<kKeyTiles>(p, counts, b);
+      r = {b, tile, 0, n, n};
+      tile += step;
+      --waves;
+      return true;
+    }
+    if (at.b > end.b || (at.b == end.b && (at.tile > end.tile || (at.tile == end.tile && at.i >= end.i)))) return false;
+    const int n = length_of<kKeyTiles>(p, counts, at.b);
+    r = {at.b, at.tile, at.i, at.b == end.b && at.tile == end.tile ? end.i : n, n};
+    at.i = 0;
+    if (++at.tile == tiles_of<kKeyTiles>(p, counts, at.b)) {
+      at.tile = 0;
+      do ++at.b;
+      while (at.b < p.B && live_of(p, counts, at.b) == 0);
+    }
+    return true;
+  }
+};
+// A run as the warp that loads works it out and hands it to the others, two ahead at most: what the others would keep in registers through their loops, or divide for, they
+// read from here when they need it.
+struct Task {
+  int valid, b, h;              // h: of the row of heads, or the key head
+  int at;                       // the tile: which 128 rows, or block of keys
+  int i0, i1, whole, slot, ends, tile;
+  int masked;                   // keys that stay: whether they go by a table
+  float base;                   // of the mask
+};
+template <bool kKeyTiles>
+__device__ __forceinline__ Task task_of(const CrossParams& p, const int* counts, const Run& r) {
+  const int per = kKeyTiles ? live_of(p, counts, r.b) : p.row_tiles, h = r.tile / per, tile = r.tile - h * per;
+  const int2 at = kKeyTiles ? live_block(p, r.b, tile) : make_int2(tile, 0);
+  const bool whole = r.i0 == 0 && r.i1 == r.n;
+  return {1, r.b, h, at.x, r.i0, r.i1, whole, r.i0 > 0 ? 0 : 1, r.i1 == r.n, r.tile, at.y, p.base ? __ldcg(p.base + r.b) : 0.f};
+}
+struct TaskRing {
+  uint64_t full[2], empty[2];
+  Task task[2];
+};
+// By the whole loading warp; false after a wait that gave up.
+__device__ __forceinline__ bool hand_out(TaskRing& ring, int slot, uint32_t parity, const Task& t, volatile int* abort_flag, int* status, int lane) {
+  if (!warp_ready(&ring.empty[slot], parity ^ 1, abort_flag, status, kStatusWaitEmpty)) return false;
+  if (lane == 0) ring.task[slot] = t;
+  arrive_warp(&ring.full[slot], lane);
+  return true;
+}
+
+// What a CTA leaves of tiles that its stretch does not hold whole: slot 0 for one that another began, slot 1 for one that it began itself.
+struct Left {
+  int used, ends, b, tile;       // ends: with this the tile is complete
+};
 
 // A thread's row of scores in TMEM, kChunks x 32 columns: each with its key's scale and addend, an absent key's at -inf whatever it was. In place and in a loop: in the
 // registers of the common path it would cost that one spills.
@@ -150,25 +400,33 @@ __device__ __forceinline__ void zero_row(uint32_t tile, int rows, int row) {
     for (int g = 0; g < 8; ++g) st_shared_v4(tile + c * rows * 128 + row * 128 + g * 16, make_uint4(0u, 0u, 0u, 0u));
 }
 
-// Waits, whatever the block's state, until the copies counted by `bar` have landed: shared memory may not be left while one is on its way to it.
-__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
-  for (uint32_t it = 0; it < (1u << 20) && !mbar_test(bar, parity); ++it) __nanosleep(20);
-}
-
-// A whole warp's wait. Most find the phase already over, and a plain test says so in a quarter of the time (26 cycles against 98 of the waiting loop).
-__device__ __forceinline__ bool warp_ready(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
-  if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
-  return warp_wait(bar, parity, abort_flag, status, code);
-}
-
 __device__ __forceinline__ uint64_t k_desc(uint32_t base, int bytes) { return desc_of(smem_desc_lo(base, 16) + (bytes >> 4), smem_desc_hi(1024)); }
 __device__ __forceinline__ uint64_t mn_desc(uint32_t base, int bytes, int lbo) { return desc_of(smem_desc_lo(base, lbo) + (bytes >> 4), smem_desc_hi(1024)); }
 
+__device__ __forceinline__ __nv_bfloat16* out_row(const CrossParams& p, __nv_bfloat16* base, long long sb, long long ss, long long sh, int b, int h, int r) {
+  const int g = r & ((1 << p.pack_log2) - 1);
+  return base + b * sb + (r >> p.pack_log2) * ss + ((static_cast<long long>(h) << p.pack_log2) + g) * sh;
+}
 // ===================================================================================== forward
-// One CTA per 128 rows of a row of heads, and per part of the keys where there are few such tiles; two CTAs an SM, so that one's products run under the other's
-// exponentials. Four softmax warps (a thread is a row), one that issues products, one that loads. P goes to the second product through TMEM.
+// Two CTAs an SM, so that one's products run under the other's exponentials. Four softmax warps (a thread is a row and all of a block's keys: with two warps to a row, which
+// have to agree on its maximum, 8 x 12 x 1024 x 4096 took 206 us against 176), one that issues products, one that loads. P goes to the second product through TMEM.
 constexpr int kFwdThreads = 192;
 constexpr float kSlack = 8.f;       // the accumulator is scaled anew once a row's maximum has grown by 2^8: most blocks' maxima grow a little in some row of a warp
+
+__device__ __forceinline__ bool all_of_128(bool mine) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 2, 128, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t"
+      "}\n"
+      : "=r"(all)
+      : "r"(static_cast<uint32_t>(mine))
+      : "memory");
+  return all != 0;
+}
 
 template <int kD>
 struct Fwd {
@@ -179,26 +437,33 @@ struct Fwd {
   static constexpr int V = K + kStages * kTile;
   static constexpr int TAB = V + kStages * kTile;        // 2 x 128 x {scale, addend}
   static constexpr int BARS = TAB + 2 * 128 * 8;
-  static constexpr int BASE = BARS + 160;                // 6 floats: the warps' largest addends
-  static constexpr int STATE = BARS + 256;               // a byte for each of the item's blocks
-  static constexpr int bytes(int blocks) { return STATE + (blocks + 15) / 16 * 16 + 1024; }
-  // Columns of TMEM. With 128 values a head P takes the place of the scores, which it is made from.
+  static constexpr int COUNTS = BARS + 512;
+  static constexpr int TOTAL = COUNTS + kCounts * 4;
+  // Columns of TMEM. With 128 values a head P takes the place of the scores that it is made from.
   static constexpr uint32_t S = 0, P = kD == 64 ? 128 : 0, O = kD == 64 ? 192 : 128;
+};
+struct FwdBars {
+  uint64_t q_full, q_empty;
+  uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+  uint64_t s_full;             // the scores of a block are in TMEM
+  uint64_t s_free;             // ... and in the softmax warps' registers
+  uint64_t p_ready;            // the probabilities are in TMEM and O has been rescaled where it had to be
+  uint64_t pv_done;            // P V has been added to O
+  TaskRing tasks;
+  Left left[2];
+  uint32_t tmem_slot;
+  int abort_flag;
 };
 
 struct FwdOut {
   __nv_bfloat16* o;
   long long osb, oss, osh;
   float* stats;                // [B, Hq, R] log2 of the sum of the exponentials, relative to the mask's base; null: not wanted
-  float* part_o;               // parts > 1: [parts][B, Hq, R][D] sums relative to the part's maximum
-  float2* part_ml;             // ... {maximum, sum}
-  int parts, blocks_per_part, n_tiles;
+  Left* left;                  // [CTAs][2]
+  float* part_o;               // [CTAs][2][128][D] sums relative to the part's maximum
+  float2* part_ml;             // ... [128] {maximum, sum}
+  int whole;                   // stretches begin and end with tiles
 };
-
-__device__ __forceinline__ __nv_bfloat16* out_row(const CrossParams& p, __nv_bfloat16* base, long long sb, long long ss, long long sh, int b, int h, int r) {
-  const int g = r & ((1 << p.pack_log2) - 1);
-  return base + b * sb + (r >> p.pack_log2) * ss + ((static_cast<long long>(h) << p.pack_log2) + g) * sh;
-}
 
 template <int kD>
 __global__ void __launch_bounds__(kFwdThreads, 2)
@@ -206,171 +471,189 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using L = Fwd<kD>;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
-  uint64_t* q_full = bars;
-  uint64_t* k_full = bars + 1;     // [kStages]
-  uint64_t* k_empty = bars + 3;
-  uint64_t* v_full = bars + 5;
-  uint64_t* v_empty = bars + 7;
-  uint64_t* s_full = bars + 9;     // the scores of a block are in TMEM
-  uint64_t* s_free = bars + 10;    // ... and in the softmax warps' registers
-  uint64_t* p_ready = bars + 11;   // the probabilities are in TMEM and O has been rescaled where it had to be
-  uint64_t* pv_done = bars + 12;   // P V has been added to O
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  constexpr int kS = L::kStages;
+  static_assert(sizeof(FwdBars) <= 512, "barriers");
+  FwdBars& bar = *reinterpret_cast<FwdBars*>(smem + L::BARS);
+  volatile int* abort_flag = &bar.abort_flag;
   float2* tab = reinterpret_cast<float2*>(smem + L::TAB);
-  uint8_t* state = smem + L::STATE;
-
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  int lin = blockIdx.x;
-  const int part = lin % out.parts;
-  lin /= out.parts;
-  const int tile = lin % out.n_tiles;
-  lin /= out.n_tiles;
-  const int h = lin % p.Hq, b = lin / p.Hq, hk = h / p.per_kv;
-  const int row0 = tile * 128, rows = min(128, p.R - row0);
-  const int j0 = part * out.blocks_per_part, n_blocks = min(out.blocks_per_part, (p.Sk + kKeys - 1) / kKeys - j0);
-  const int warps = (rows + 31) >> 5;        // softmax warps that have rows
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 1);
-    for (int i = 0; i < L::kStages; ++i) { mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
-    mbar_init(s_full, 1);
-    mbar_init(s_free, warps);
-    mbar_init(p_ready, warps);
-    mbar_init(pv_done, 1);
-    *abort_flag = 0;
+    mbar_init(&bar.q_full, 1);
+    mbar_init(&bar.q_empty, 4);
+    for (int i = 0; i < 2; ++i) { mbar_init(&bar.k_full[i], 1); mbar_init(&bar.k_empty[i], 1); mbar_init(&bar.v_full[i], 1); mbar_init(&bar.v_empty[i], 1); }
+    mbar_init(&bar.s_full, 1);
+    mbar_init(&bar.s_free, 4);
+    mbar_init(&bar.p_ready, 4);
+    mbar_init(&bar.pv_done, 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(&bar.tasks.full[i], 1); mbar_init(&bar.tasks.empty[i], 5); }
+    bar.left[0] = bar.left[1] = Left{0, 0, 0, 0};
+    bar.abort_flag = 0;
     mbar_fence_init();
   }
   if (warp == 4) {
-    tmem_alloc<1>(tmem_slot, 256);
+    tmem_alloc<1>(&bar.tmem_slot, 256);
     tmem_relinquish<1>();
+  }
+  if (warp == 5 && elect_one()) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
   }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = bar.tmem_slot;
   pdl_entry();       // behind the allocation: the next kernel's may not come before it
-  for (int j = warp; j < n_blocks; j += kFwdThreads / 32) {
-    const int s = p.mask ? block_state(p, b, j0 + j, lane) : block_state_unmasked(p, j0 + j);
-    if (lane == 0) state[j] = static_cast<uint8_t>(s);
-  }
-  float* bases = reinterpret_cast<float*>(smem + L::BASE);
-  const bool addends = p.mask && !p.mask_bool;
-  if (addends) {
-    float a = -INFINITY;
-    for (int kv = threadIdx.x; kv < p.Sk; kv += kFwdThreads) a = fmaxf(a, key_addend(p, b, kv));
-    a = warp_max(a);
-    if (lane == 0) bases[warp] = a;
-  }
-  __syncthreads();
-  float base = 0.f;
-  if (addends) {
-    base = max3(max3(bases[0], bases[1], bases[2]), bases[3], fmaxf(bases[4], bases[5]));
-    if (isinf(base)) base = 0.f;       // no key takes part
-    if (p.base && threadIdx.x == 0) p.base[b] = base;       // every CTA of the batch row the same
-  }
+  const int* counts = counts_of(p, reinterpret_cast<int*>(smem + L::COUNTS));
+  if (counts) __syncthreads();
   const uint32_t sQ = smem_u32(smem + L::Q), sK = smem_u32(smem + L::K), sV = smem_u32(smem + L::V);
 
   if (warp == 5) {
     // ------------------------------------------------------------------ loads
-    if (elect_one()) {
-      mbar_expect_tx(q_full, L::kTile);
-      load_tile<kD>(sQ, &tmQ, q_full, 128, row0 >> p.pack_log2, h, b);
-    }
-    __syncwarp();
-    int it = 0, ks = 0, vs = 0;
-    for (int j = 0; j < n_blocks; ++j) {
-      if (!state[j]) continue;
-      const int st = it % L::kStages;
-      const uint32_t ph = ((it / L::kStages) & 1) ^ 1;
-      if (!warp_ready(&k_empty[st], ph, abort_flag, p.status, kStatusWaitEmpty)) break;
+    const Share share = share_of<false>(p, counts, blockIdx.x, gridDim.x, out.whole, lane);
+    Walk<false> walk(counts, share, blockIdx.x, gridDim.x);
+    const Place end = share.end;
+    Run r;
+    Ring<2> rt;
+    Ring<kS> ring;
+    int runs = 0, ks = 0, vs = 0;
+    bool ok = true;
+    while (ok) {
+      Task task = {};
+      if (walk.next(p, end, r)) task = task_of<false>(p, counts, r);
+      ok = hand_out(bar.tasks, rt.stage, rt.parity, task, abort_flag, p.status, lane);
+      rt.next();
+      if (!ok || !task.valid) break;
+      const int hk = task.h / p.per_kv;
+      ok = warp_ready(&bar.q_empty, (runs & 1) ^ 1, abort_flag, p.status, kStatusWaitEmpty);
+      if (!ok) break;
       if (elect_one()) {
-        mbar_expect_tx(&k_full[st], L::kTile);
-        load_tile<kD>(sK + st * L::kTile, &tmK, &k_full[st], 128, (j0 + j) * kKeys, hk, b);
+        mbar_expect_tx(&bar.q_full, L::kTile);
+        load_tile<kD>(sQ, &tmQ, &bar.q_full, 128, (task.at * 128) >> p.pack_log2, task.h, r.b);
       }
       __syncwarp();
-      ++ks;
-      if (!warp_ready(&v_empty[st], ph, abort_flag, p.status, kStatusWaitEmpty)) break;
-      if (elect_one()) {
-        mbar_expect_tx(&v_full[st], L::kTile);
-        load_tile<kD>(sV + st * L::kTile, &tmV, &v_full[st], 128, (j0 + j) * kKeys, hk, b);
+      ++runs;
+      int2 next = live_block(p, r.b, r.i0);
+      for (int i = r.i0; i < r.i1; ++i) {
+        const int key0 = next.x * kKeys;
+        if (i + 1 < r.i1) next = live_block(p, r.b, i + 1);
+        ok = warp_ready(&bar.k_empty[ring.stage], ring.parity ^ 1, abort_flag, p.status, kStatusWaitEmpty);
+        if (!ok) break;
+        if (elect_one()) {
+          mbar_expect_tx(&bar.k_full[ring.stage], L::kTile);
+          load_tile<kD>(sK + ring.stage * L::kTile, &tmK, &bar.k_full[ring.stage], 128, key0, hk, r.b);
+        }
+        __syncwarp();
+        ++ks;
+        ok = warp_ready(&bar.v_empty[ring.stage], ring.parity ^ 1, abort_flag, p.status, kStatusWaitEmpty);
+        if (!ok) break;
+        if (elect_one()) {
+          mbar_expect_tx(&bar.v_full[ring.stage], L::kTile);
+          load_tile<kD>(sV + ring.stage * L::kTile, &tmV, &bar.v_full[ring.stage], 128, key0, hk, r.b);
+        }
+        __syncwarp();
+        ++vs;
+        ring.next();
       }
-      __syncwarp();
-      ++vs;
-      ++it;
     }
-    drain(q_full, 0);
-    for (int u = max(0, ks - L::kStages); u < ks; ++u) drain(&k_full[u % L::kStages], (u / L::kStages) & 1);
-    for (int u = max(0, vs - L::kStages); u < vs; ++u) drain(&v_full[u % L::kStages], (u / L::kStages) & 1);
+    if (runs > 0) drain(&bar.q_full, (runs - 1) & 1);
+    for (int u = max(0, ks - kS); u < ks; ++u) drain(&bar.k_full[u % kS], (u / kS) & 1);
+    for (int u = max(0, vs - kS); u < vs; ++u) drain(&bar.v_full[u % kS], (u / kS) & 1);
   } else if (warp == 4) {
     // ------------------------------------------------------------------ products
     const uint32_t idesc_s = make_idesc_bf16(128, 128, 0, 0), idesc_o = make_idesc_bf16(128, kD, 0, 1);
-    int n = 0;
-    for (int j = 0; j < n_blocks; ++j) n += state[j] != 0;
-    auto scores = [&](int it) {
-      const int st = it % L::kStages;
-      if (!warp_ready(&k_full[st], (it / L::kStages) & 1, abort_flag, p.status, kStatusWaitFull)) return false;
+    Ring<2> rt;
+    Ring<kS> rk, rv;
+    int it = 0, runs = 0;
+    bool ok = true;
+    const auto scores = [&]() {
+      if (!warp_ready(&bar.k_full[rk.stage], rk.parity, abort_flag, p.status, kStatusWaitFull)) return false;
       tc_fence_after_sync();
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < kD / 16; ++k)
-          umma_bf16<1>(tmem + L::S, k_desc(sQ, (k >> 2) * 16384 + (k & 3) * 32), k_desc(sK + st * L::kTile, (k >> 2) * 16384 + (k & 3) * 32), idesc_s, k > 0);
-        umma_commit(s_full);
-        umma_commit(&k_empty[st]);
+          umma_bf16<1>(tmem + L::S, k_desc(sQ, (k >> 2) * 16384 + (k & 3) * 32), k_desc(sK + rk.stage * L::kTile, (k >> 2) * 16384 + (k & 3) * 32), idesc_s, k > 0);
+        umma_commit(&bar.s_full);
+        umma_commit(&bar.k_empty[rk.stage]);
       }
       __syncwarp();
+      rk.next();
       return true;
     };
-    bool ok = n > 0 && warp_ready(q_full, 0, abort_flag, p.status, kStatusWaitFull) && scores(0);
-    for (int it = 0; it < n && ok; ++it) {
-      if (kD == 64 && it + 1 < n) {        // P has a place of its own: the next scores may come under this block's exponentials
-        ok = warp_ready(s_free, it & 1, abort_flag, p.status, kStatusWaitEpi) && scores(it + 1);
+    while (ok && warp_ready(&bar.tasks.full[rt.stage], rt.parity, abort_flag, p.status, kStatusWaitFull) && bar.tasks.task[rt.stage].valid) {
+      const int n = bar.tasks.task[rt.stage].i1 - bar.tasks.task[rt.stage].i0;
+      arrive_warp(&bar.tasks.empty[rt.stage], lane);
+      rt.next();
+      ok = warp_ready(&bar.q_full, runs & 1, abort_flag, p.status, kStatusWaitFull) && scores();
+      ++runs;
+      for (int i = 0; i < n && ok; ++i, ++it) {
+        // Where P has a place of its own the next scores may come under this block's exponentials, otherwise right behind the product that reads P: a CTA's products
+        // run in the order in which they are issued.
+        if (kD == 64 && i + 1 < n) {
+          ok = warp_ready(&bar.s_free, it & 1, abort_flag, p.status, kStatusWaitEpi) && scores();
+          if (!ok) break;
+        }
+        ok = warp_ready(&bar.p_ready, it & 1, abort_flag, p.status, kStatusWaitEpi) && warp_ready(&bar.v_full[rv.stage], rv.parity, abort_flag, p.status, kStatusWaitFull);
         if (!ok) break;
-      }
-      const int st = it % L::kStages;
-      ok = warp_ready(p_ready, it & 1, abort_flag, p.status, kStatusWaitEpi) && warp_ready(&v_full[st], (it / L::kStages) & 1, abort_flag, p.status, kStatusWaitFull);
-      if (!ok) break;
-      tc_fence_after_sync();
-      if (elect_one()) {
+        tc_fence_after_sync();
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < 128 / 16; ++k) umma_bf16_ts(tmem + L::O, tmem + L::P + k * 8, mn_desc(sV + st * L::kTile, k * 2048, 16384), idesc_o, it > 0 || k > 0);
-        umma_commit(pv_done);
-        umma_commit(&v_empty[st]);
+          for (int k = 0; k < 128 / 16; ++k) umma_bf16_ts(tmem + L::O, tmem + L::P + k * 8, mn_desc(sV + rv.stage * L::kTile, k * 2048, 16384), idesc_o, i > 0 || k > 0);
+          umma_commit(&bar.pv_done);
+          umma_commit(&bar.v_empty[rv.stage]);
+        }
+        __syncwarp();
+        rv.next();
+        if (kD != 64 && i + 1 < n) ok = scores();
       }
-      __syncwarp();
-      if (kD != 64 && it + 1 < n) ok = warp_ready(pv_done, it & 1, abort_flag, p.status, kStatusWaitAccum) && scores(it + 1);
     }
-  } else if (warp < warps) {
+  } else {
     // ------------------------------------------------------------------ softmax: a thread is a row
-    const int t = threadIdx.x, r = row0 + t;
+    const int t = threadIdx.x;
     const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
     const float sc = p.scale * kLog2e;
-    float m = -INFINITY, l = 0.f;       // the maximum the accumulator is relative to, and the sum
-    bool ok = true;
+    Ring<2> rt;
+    Ring<kS> rv;
     int it = 0;
-    // After a wait that gave up the loop runs out without work, so that no warp is missed at the barriers.
-    for (int j = 0; j < n_blocks; ++j) {
-      const int kind = state[j];
-      if (!kind) continue;
-      float2* tb = tab + (it & 1) * 128;
-      if (kind == 1) {
-        for (int e = t; e < kKeys; e += warps * 32) {
-          const float2 k = key_entry(p, b, (j0 + j) * kKeys + e, base);
-          tb[e] = k;
+    bool ok = true;
+    // After a wait that gave up the loop over a run's blocks runs out without work, and the four warps go on to the next run or leave together, so that none is missed at
+    // the barriers.
+    while (all_of_128(warp_ready(&bar.tasks.full[rt.stage], rt.parity, abort_flag, p.status, kStatusWaitFull))) {
+      const volatile Task& task = bar.tasks.task[rt.stage];
+      if (!task.valid) break;
+      const int b = task.b, i0 = task.i0, i1 = task.i1;
+      const bool works = warp * 32 < p.R - task.at * 128;        // a warp without rows only keeps step
+      float m = -INFINITY, l = 0.f;               // the maximum the accumulator is relative to, and the sum
+      int2 next = live_block(p, b, i0);
+      for (int i = i0; i < i1; ++i, ++it) {
+        const int2 blk = next;
+        if (i + 1 < i1) next = live_block(p, b, i + 1);
+        const float2* tb = tab + (it & 1) * 128;
+        if (blk.y) {
+          // A wait for V is one for the turn after the last that is known to be over: with one stage the block before has to have left it.
+          if (kS == 1 && i > i0) ok = ok && warp_ready(&bar.pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);
+          const float2 k = key_entry(p, b, blk.x * kKeys + t, task.base);
+          tab[(it & 1) * 128 + t] = k;
           if (p.mask && k.y == -INFINITY && ok) {        // an absent key's values meet a probability of zero
-            ok = mbar_wait(&v_full[it % L::kStages], (it / L::kStages) & 1, abort_flag, p.status, kStatusWaitFull);
-            if (ok) zero_row<kD>(sV + (it % L::kStages) * L::kTile, 128, e);
+            ok = mbar_wait(&bar.v_full[rv.stage], rv.parity, abort_flag, p.status, kStatusWaitFull);
+            if (ok) zero_row<kD>(sV + rv.stage * L::kTile, 128, t);
           }
+          ok = __all_sync(0xffffffffu, ok);
+          fence_proxy_async_smem();
+          asm volatile("bar.sync 1, 128;" ::: "memory");
         }
-        ok = __all_sync(0xffffffffu, ok);
-        fence_proxy_async_smem();
-        asm volatile("bar.sync 1, %0;" ::"r"(warps * 32) : "memory");
-      }
-      ok = ok && warp_ready(s_full, it & 1, abort_flag, p.status, kStatusWaitAccum);
-      if (ok) {
+        rv.next();
+        ok = ok && warp_ready(&bar.s_full, it & 1, abort_flag, p.status, kStatusWaitAccum);
+        if (!ok) continue;
         tc_fence_after_sync();
-        if (kind != 2) apply_table<4>(tmem + L::S + lanes, tb);        // from here on all blocks are alike
+        if (!works) {
+          if (kD == 64) arrive_warp(&bar.s_free, lane);
+          if (i > i0) ok = warp_ready(&bar.pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);
+          arrive_warp(&bar.p_ready, lane);
+          continue;
+        }
+        if (blk.y) apply_table<4>(tmem + L::S + lanes, tb);        // from here on all blocks are alike
         uint32_t s[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(tmem + L::S + lanes + 32 * c, s[c]);
@@ -378,23 +661,26 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(s[c][i]));
+          for (int e = 0; e < 32; ++e) asm volatile("" : "+r"(s[c][e]));
         if (kD == 64) {
           tc_fence_before_sync();
-          arrive_warp(s_free, lane);
+          arrive_warp(&bar.s_free, lane);
         }
-        const float mul = kind == 2 ? sc : 1.f, below = kind == 2 ? base : 0.f;        // a key with nothing added is `base` below the largest
+        const float mul = blk.y ? 1.f : sc, below = blk.y ? 0.f : task.base;        // a key with nothing added is `base` below the largest
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) mx[(i >> 1) & 3] = max3(mx[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+          for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
         const float m_new = fmaxf(m, fmaf(mul, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), -below));
-        if (it > 0) {        // P may be overwritten, O touched
-          ok = warp_ready(pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);
+        if (i == i0) {
+          m = m_new;
+        } else {
+          ok = warp_ready(&bar.pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);        // P may be overwritten, O touched
+          if (!ok) continue;
           tc_fence_after_sync();
           // (m is -inf where no key has been seen: its sums are zeros, and stay so whatever they are scaled by)
-          if (ok && __any_sync(0xffffffffu, m_new > m + kSlack)) {
+          if (__any_sync(0xffffffffu, m_new > m + kSlack)) {
             const float alpha = m_new == -INFINITY ? 1.f : ex2_approx(m - m_new);
             m = m_new;
             l *= alpha;
@@ -404,89 +690,95 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
               tmem_ld16(tmem + L::O + lanes + c, v);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+              for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha);
               tmem_st16(tmem + L::O + lanes + c, v);
             }
           }
         }
-        if (ok) {
-          if (it == 0) m = m_new;
-          const float neg_m = m == -INFINITY ? 0.f : -m - below;
-          F2 sum[2] = {f2_splat(0.f), f2_splat(0.f)};
+        const F2 mul2 = f2_splat(mul), neg_m = f2_splat(m == -INFINITY ? 0.f : -m - below);
+        F2 sum[2] = {f2_splat(0.f), f2_splat(0.f)};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t pk[16];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float lo, hi;
-              f2_get(f2_fma(f2_make(__uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1])), f2_splat(mul), f2_splat(neg_m)), lo, hi);
-              lo = ex2_approx(lo);
-              hi = ex2_approx(hi);
-              sum[(i >> 1) & 1] = f2_add(sum[(i >> 1) & 1], f2_make(lo, hi));
-              pk[i >> 1] = pack2(lo, hi);
-            }
-            tmem_st16(tmem + L::P + lanes + 16 * c, pk);
+          for (int e = 0; e < 32; e += 2) {
+            float lo, hi;
+            f2_get(f2_fma(f2_make(__uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1])), mul2, neg_m), lo, hi);
+            lo = ex2_approx(lo);
+            hi = ex2_approx(hi);
+            sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], f2_make(lo, hi));
+            pk[e >> 1] = pack2(lo, hi);
           }
-          float a0, a1, b0, b1;
-          f2_get(sum[0], a0, a1);
-          f2_get(sum[1], b0, b1);
-          l += (a0 + a1) + (b0 + b1);
-          tmem_st_wait();
-          tc_fence_before_sync();
-          arrive_warp(p_ready, lane);
+          tmem_st16(tmem + L::P + lanes + 16 * c, pk);
         }
+        float a0, a1, b0, b1;
+        f2_get(f2_add(sum[0], sum[1]), a0, a1);
+        l += a0 + a1;
+        tmem_st_wait();
+        tc_fence_before_sync();
+        arrive_warp(&bar.p_ready, lane);
       }
-      ++it;
-    }
-    ok = __all_sync(0xffffffffu, ok && (it > 0 ? mbar_wait(pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum)
-                                               : mbar_wait(q_full, 0, abort_flag, p.status, kStatusWaitFull)));        // Q's place is written below
-    if (ok) {
-      tc_fence_after_sync();
-      const long long at = (static_cast<long long>(b) * p.Hq + h) * p.R + r;
-      const bool split = out.parts > 1;
-      const float inv = split ? 1.f : l == 0.f ? 0.f : 1.f / l;
-      if (t < rows) {
-        const long long pat = static_cast<long long>(part) * p.B * p.Hq * p.R + at;
-        if (split) out.part_ml[pat] = make_float2(m, l);
+      // ---- the run's rows
+      const bool whole = task.whole;
+      const int h = task.h, row0 = task.at * 128, rows = min(128, p.R - row0);
+      ok = ok && warp_ready(&bar.pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);
+      if (!whole && t == 0) bar.left[task.slot] = Left{1, task.ends, b, task.tile};
+      if (ok && works) {
+        tc_fence_after_sync();
+        const long long row = (static_cast<long long>(b) * p.Hq + h) * p.R + row0 + t, slot = blockIdx.x * 2ll + task.slot;
+        const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        if (!whole) out.part_ml[slot * 128 + t] = make_float2(m, l);
         // a row that no key takes part in: +inf, which makes every probability 2^-inf = 0
-        else if (out.stats) out.stats[at] = l == 0.f ? INFINITY : m + log2f(l);
-      }
-      float* po = split ? out.part_o + (static_cast<long long>(part) * p.B * p.Hq * p.R + at) * kD : nullptr;
+        else if (out.stats && t < rows) out.stats[row] = l == 0.f ? INFINITY : m + log2f(l);
+        float* po = whole ? nullptr : out.part_o + (slot * 128 + t) * kD;
 #pragma unroll
-      for (int c0 = 0; c0 < kD; c0 += 32) {
-        uint32_t v[32];
-        if (it > 0) {
+        for (int c0 = 0; c0 < kD; c0 += 32) {
+          uint32_t v[32];
           tmem_ld32_sync(tmem + L::O + lanes + c0, v);
-        } else {
+          float f[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0u;
-        }
-        float f[32];
+          for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(v[e]) * inv;
+          if (whole) {       // through the warp's 4 KB of each of Q's panels, which every product has read
+            stage_half(sQ + (c0 >> 6) * 16384 + warp * 4096, lane, c0 & 32, f);
+          } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]) * inv;
-        if (split) {
-          if (t < rows)
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(po + c0 + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
-        } else {       // through the warp's 4 KB of each of Q's panels, which every product has read
-          stage_half(sQ + (c0 >> 6) * 16384 + warp * 4096, lane, c0 & 32, f);
-        }
-      }
-      if (!split) {
-        __syncwarp();
-        const int sub = lane >> 3, ch = lane & 7;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int rr = k * 4 + sub;
-          if (warp * 32 + rr < rows) {
-            __nv_bfloat16* dst = out_row(p, out.o, out.osb, out.oss, out.osh, b, h, row0 + warp * 32 + rr) + ch * 8;
-#pragma unroll
-            for (int c = 0; c < kD / 64; ++c)
-              *reinterpret_cast<uint4*>(dst + c * 64) = ld_shared_v4(sQ + c * 16384 + warp * 4096 + rr * 128 + ((ch ^ (rr & 7)) << 4));
+            for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(po + c0 + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
           }
         }
+        if (whole) {
+          __syncwarp();
+          const int sub = lane >> 3, ch = lane & 7;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int rr = k * 4 + sub;
+            if (warp * 32 + rr < rows) {
+              __nv_bfloat16* dst = out_row(p, out.o, out.osb, out.oss, out.osh, b, h, row0 + warp * 32 + rr) + ch * 8;
+#pragma unroll
+              for (int c = 0; c < kD / 64; ++c)
+                *reinterpret_cast<uint4*>(dst + c * 64) = ld_shared_v4(sQ + c * 16384 + warp * 4096 + rr * 128 + ((ch ^ (rr & 7)) << 4));
+            }
+          }
+          fence_proxy_async_smem();        // the next Q comes to the same place
+        }
+        tc_fence_before_sync();
       }
+      arrive_warp(&bar.q_empty, lane);
+      arrive_warp(&bar.tasks.empty[rt.stage], lane);
+      rt.next();
     }
+    if (t == 0 && !out.whole) {
+      out.left[blockIdx.x * 2] = bar.left[0];
+      out.left[blockIdx.x * 2 + 1] = bar.left[1];
+    }
+    // batch rows without a key: zeros
+    if (counts)
+      for (int b = blockIdx.x; b < p.B; b += gridDim.x)
+        if (live_of(p, counts, b) == 0)
+          for (long long e = t; e < static_cast<long long>(p.Hq) * p.R * (kD / 8); e += 128) {
+            const int c = static_cast<int>(e % (kD / 8)), row = static_cast<int>(e / (kD / 8) % p.R), h = static_cast<int>(e / (kD / 8) / p.R);
+            *reinterpret_cast<uint4*>(out_row(p, out.o, out.osb, out.oss, out.osh, b, h, row) + c * 8) = make_uint4(0u, 0u, 0u, 0u);
+            if (out.stats && c == 0) out.stats[(static_cast<long long>(b) * p.Hq + h) * p.R + row] = INFINITY;
+          }
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -496,51 +788,77 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
 }
 
-// The parts of a row joined: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i. A warp takes 128 / kD rows at a time, four values a lane.
+// The CTAs that share the tile which `cta` began and did not end, in their order, into `with`; returns how many. By a whole block; at most kWith.
+constexpr int kWith = 512;        // more than there are CTAs of a kernel
+__device__ __forceinline__ int sharers(const Left* left, int cta, int stop, short* with, int* count) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    int n = 1;
+    if (lane == 0) with[0] = static_cast<short>(cta);
+    for (int k0 = cta + 1; k0 < stop; k0 += 32) {
+      const Left l = k0 + lane < stop ? left[(k0 + lane) * 2] : Left{0, 0, 0, 0};        // (a stretch may be empty where blocks are masked)
+      const unsigned ends = __ballot_sync(0xffffffffu, l.ends), upto = ends ? (2u << (__ffs(ends) - 1)) - 1 : 0xffffffffu;
+      const unsigned used = __ballot_sync(0xffffffffu, l.used) & upto;
+      if (used >> lane & 1) with[n + __popc(used & ((1u << lane) - 1))] = static_cast<short>(k0 + lane);
+      n += __popc(used);
+      if (ends) break;
+    }
+    if (lane == 0) *count = n;
+  }
+  __syncthreads();
+  return *count;
+}
+
+// The stretches' shares of a tile joined, by the block of the CTA that began it: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i, four values a thread.
 template <int kD>
-__global__ void __launch_bounds__(256) cross_join_kernel(const CrossParams p, const FwdOut out) {
+__global__ void __launch_bounds__(256) cross_join_kernel(const CrossParams p, const FwdOut out, const int ctas) {
+  __shared__ short with[kWith];
+  __shared__ int count;
   pdl_entry();
   constexpr int kLanes = kD / 4;
-  const long long rows = static_cast<long long>(p.B) * p.Hq * p.R;
-  const int c = (threadIdx.x % kLanes) * 4;
-  for (long long row = (blockIdx.x * 256ll + threadIdx.x) / kLanes; row < rows; row += gridDim.x * 256ll / kLanes) {
-    float m = -INFINITY, l = 0.f;
-    for (int i = 0; i < out.parts; ++i) m = fmaxf(m, out.part_ml[i * rows + row].x);
-    const float ref = m == -INFINITY ? 0.f : m;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < out.parts; ++i) {
-      const float2 ml = out.part_ml[i * rows + row];
-      const float4 v = *reinterpret_cast<const float4*>(out.part_o + (i * rows + row) * kD + c);
-      const float w = ex2_approx(ml.x - ref);
-      l += w * ml.y;
-      acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int r = static_cast<int>(row % p.R);
-    const long long bh = row / p.R;
-    __nv_bfloat16* dst = out_row(p, out.o, out.osb, out.oss, out.osh, static_cast<int>(bh / p.Hq), static_cast<int>(bh % p.Hq), r) + c;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
-    if (out.stats && c == 0) out.stats[row] = l == 0.f ? INFINITY : m + log2f(l);
+  const Left first = out.left[blockIdx.x * 2 + 1];
+  if (!first.used) return;
+  const int n = sharers(out.left, blockIdx.x, ctas, with, &count);
+  const int h = first.tile / p.row_tiles, row0 = (first.tile - h * p.row_tiles) * 128, rows = min(128, p.R - row0);
+  const int c = (threadIdx.x % kLanes) * 4, t = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes;
+  if (t >= rows) return;
+  const auto at = [&](int k) { return (with[k] * 2ll + (k == 0)) * 128 + t; };
+  float m = -INFINITY;
+#pragma unroll 8
+  for (int k = 0; k < n; ++k) m = fmaxf(m, out.part_ml[at(k)].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+  for (int k = 0; k < n; ++k) {
+    const float2 ml = out.part_ml[at(k)];
+    const float4 v = *reinterpret_cast<const float4*>(out.part_o + at(k) * kD + c);
+    const float w = ex2_approx(ml.x - ref);
+    l += w * ml.y;
+    acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
   }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  __nv_bfloat16* dst = out_row(p, out.o, out.osb, out.oss, out.osh, first.b, h, row0 + t) + c;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
+  if (out.stats && c == 0) out.stats[(static_cast<long long>(first.b) * p.Hq + h) * p.R + row0 + t] = l == 0.f ? INFINITY : m + log2f(l);
 }
 
 // ==================================================================================== backward
-// Two kinds of work item, in one launch. Both keep a tile of 128 rows of two tensors in shared memory and stream tiles of 128 rows of the other two:
+// Two kinds of CTAs, in one launch, one an SM. Both keep a tile of 128 rows of two tensors in shared memory and stream tiles of 128 rows of the other two:
 //   keys:  K, V stay; Q, dO stream.   S^T = K Q^T, dP^T = V dO^T;   dV += P^T dO,  dK += dS^T Q
 //   rows:  Q, dO stay; K, V stream.   S = Q K^T,   dP = dO V^T;     dQ += dS K
 // Scores are so worked out twice, but P and dS reach their products in TMEM, in the place of the scores and the dP that they are made from, and never through shared memory,
-// and every gradient is summed by one CTA in the order of the tiles: two calls give the same bits, with no atomics and no pass over a scratch. Sixteen softmax
+// and every gradient is summed in the order of the tiles, with no atomics. Sixteen softmax
 // warps: a thread is a row of the tile that stays and 32 of the streamed tile's columns. (With eight, 64 columns each, a warp's exponentials alone took 1050 cycles where the
 // unit needs 512: two warps a scheduler do not hide the latencies.) Products of one CTA run in the order in which they are issued, so that what overwrites a place may be
 // issued right behind what reads it: S(j+1) behind dV(j) (ahead of time, where there is a second buffer), dP(j+1) behind dK(j) or dQ(j).
 // Tiles of 128 columns, not two of 64: with both operands in shared memory a product of 128 x 64 x 16 takes the 64 cycles of one of 128 x 128 x 16.
-// Where there are few items, the streamed tiles are cut into parts, whose fp32 sums are added in their order by a second launch.
 constexpr int kBwdSoftmaxWarps = 16;
 constexpr int kBwdThreads = 32 * (kBwdSoftmaxWarps + 3);        // ... one that issues products, one that loads, one that fills tables
 
 template <int kD>
 struct Bwd {
-  // Streamed tiles that are there at a time: of Q or K (A), of dO or V (B). A block of V has done its work with dP, Q, K and dO are read again by the products behind.
+  // Streamed tiles that are there at a time: of Q or K (A), of dO or V (B). A block of V has done its work with dP; Q, K and dO are read again by the products behind.
   static constexpr int stages_a(bool keys) { return kD == 64 ? 3 : keys ? 2 : 3; }
   static constexpr int stages_b(bool keys) { return kD == 64 ? 3 : keys ? 2 : 1; }
   static constexpr int kTile = 128 * kD * 2;
@@ -548,7 +866,8 @@ struct Bwd {
   static constexpr int RING = 2 * kTile;                           // A's tiles, then B's
   static constexpr int TAB = RING + (kD == 64 ? 6 : 4) * kTile;    // 3 x 256 floats
   static constexpr int BARS = TAB + 3 * 1024;
-  static constexpr int TOTAL = BARS + 256;
+  static constexpr int COUNTS = BARS + 512;
+  static constexpr int TOTAL = COUNTS + kCounts * 4;
   // Columns of TMEM: one more buffer of scores where the accumulators leave room for it.
   static constexpr uint32_t S = 0, DP = 128, ACC0 = 256, ACC1 = 256 + kD;
   static constexpr uint32_t S2_KEYS = 384, S2_ROWS = kD == 64 ? 384 : 256;
@@ -559,13 +878,11 @@ static_assert(Bwd<128>::TOTAL + 1024 <= 227 * 1024, "shared memory budget");
 struct BwdOut {
   const float* stats;              // of the forward pass
   const float* D;                  // [B, Hq, R]
-  const uint8_t* state;            // [B, blocks] of a mask; null without one
   __nv_bfloat16 *dq, *dk, *dv;
   long long qsb, qss, qsh, ksb, kss, ksh;
-  float *part_q, *part_k, *part_v; // [parts][B, Hq, R][D]; [parts][B, Hk, Sk][D]
-  int parts_q, parts_k;            // parts of an item of rows, of keys
-  int row_tiles, key_blocks;       // items of a row of heads, of a key head
-  int key_items;                   // the first of all
+  Left* left;                      // [CTAs][2]
+  float* part;                     // [CTAs][2][128][D], of the CTAs of keys twice that: dK, then dV
+  int key_ctas, whole_keys, whole_rows;
 };
 
 // P of 32 columns of a thread's scores, as fp32 in `pr` and, for keys, as bf16 in TMEM: P = 2^(mul s - l), with l of the thread's row or, where the columns are rows, -l of `tb`.
@@ -621,186 +938,208 @@ __device__ __forceinline__ void make_ds(uint32_t tDP, const float* tb, float neg
 }
 
 struct BwdBars {
-  uint64_t f_full;
+  uint64_t f_full, f_empty;           // the tiles that stay
   uint64_t a_full[3], a_empty[3];     // a streamed tile of Q or K has landed; every product that reads it has retired
   uint64_t b_full[3], b_empty[3];     // ... of dO or V
   uint64_t tab_full[3];               // A's table is written
   uint64_t s_full[2], dp_full;        // scores and dP are in TMEM
   uint64_t p_ready, ds_ready;         // ... and P and dS in their place
-  uint64_t acc_done;                  // every product has retired
+  uint64_t acc_done;                  // every product of a run has retired
+  TaskRing tasks;
+  Left left[2];
   uint32_t tmem_slot;
   int abort_flag;
 };
 
 template <int kD, bool kKeys>
-__device__ __forceinline__ void bwd_products(BwdBars& bar, int* status, uint32_t tmem, uint32_t smem, int n) {
+__device__ __forceinline__ void bwd_products(BwdBars& bar, const CrossParams& p, uint32_t tmem, uint32_t smem) {
   using L = Bwd<kD>;
+  int* status = p.status;
   volatile int* abort_flag = &bar.abort_flag;
   constexpr bool kTwo = !kKeys || L::kTwoForKeys;
   constexpr int kA = L::stages_a(kKeys), kB = L::stages_b(kKeys);
   const uint32_t idesc_s = make_idesc_bf16(128, 128, 0, 0), idesc_acc = make_idesc_bf16(128, kD, 0, 1);
-  const auto s_at = [&](int it) { return tmem + (kTwo && (it & 1) ? (kKeys ? L::S2_KEYS : L::S2_ROWS) : L::S); };
-  const auto a_at = [&](int it) { return smem + L::RING + it % kA * L::kTile; };
-  const auto b_at = [&](int it) { return smem + L::RING + (kA + it % kB) * L::kTile; };
-  const auto scores = [&](int it) {
-    if (!warp_ready(&bar.a_full[it % kA], (it / kA) & 1, abort_flag, status, kStatusWaitFull)) return false;
+  Ring<kA> ra, fa;        // of the scores, and of the products that read the tile again
+  Ring<kB> rb, fb;
+  int it = 0;
+  const auto s_at = [&](int n) { return tmem + (kTwo && (n & 1) ? (kKeys ? L::S2_KEYS : L::S2_ROWS) : L::S); };
+  const auto a_at = [&](int stage) { return smem + L::RING + stage * L::kTile; };
+  const auto b_at = [&](int stage) { return smem + L::RING + (kA + stage) * L::kTile; };
+  const auto scores = [&](int n) {
+    if (!warp_ready(&bar.a_full[ra.stage], ra.parity, abort_flag, status, kStatusWaitFull)) return false;
     tc_fence_after_sync();
     if (elect_one()) {
 #pragma unroll
       for (int k = 0; k < kD / 16; ++k)
-        umma_bf16<1>(s_at(it), k_desc(smem + L::F0, (k >> 2) * 16384 + (k & 3) * 32), k_desc(a_at(it), (k >> 2) * 16384 + (k & 3) * 32), idesc_s, k > 0);
-      umma_commit(&bar.s_full[kTwo ? it & 1 : 0]);
+        umma_bf16<1>(s_at(n), k_desc(smem + L::F0, (k >> 2) * 16384 + (k & 3) * 32), k_desc(a_at(ra.stage), (k >> 2) * 16384 + (k & 3) * 32), idesc_s, k > 0);
+      umma_commit(&bar.s_full[kTwo ? n & 1 : 0]);
     }
     __syncwarp();
+    ra.next();
     return true;
   };
-  const auto dp = [&](int it) {
-    if (!warp_ready(&bar.b_full[it % kB], (it / kB) & 1, abort_flag, status, kStatusWaitFull)) return false;
+  const auto dp = [&](bool last) {
+    if (!warp_ready(&bar.b_full[rb.stage], rb.parity, abort_flag, status, kStatusWaitFull)) return false;
     tc_fence_after_sync();
     if (elect_one()) {
 #pragma unroll
       for (int k = 0; k < kD / 16; ++k)
-        umma_bf16<1>(tmem + L::DP, k_desc(smem + L::F1, (k >> 2) * 16384 + (k & 3) * 32), k_desc(b_at(it), (k >> 2) * 16384 + (k & 3) * 32), idesc_s, k > 0);
+        umma_bf16<1>(tmem + L::DP, k_desc(smem + L::F1, (k >> 2) * 16384 + (k & 3) * 32), k_desc(b_at(rb.stage), (k >> 2) * 16384 + (k & 3) * 32), idesc_s, k > 0);
       umma_commit(&bar.dp_full);
-      if (!kKeys) umma_commit(&bar.b_empty[it % kB]);
+      if (!kKeys) umma_commit(&bar.b_empty[rb.stage]);
+      if (last) umma_commit(&bar.f_empty);
     }
     __syncwarp();
+    rb.next();
     return true;
   };
   // acc += (the 128 columns, each 32 left as bf16 in the first half of their place) x (the 128 rows of a streamed tile)
-  const auto accumulate = [&](uint32_t acc, uint32_t from, uint32_t tile, int it, uint64_t* ready, uint64_t* empty) {
+  const auto accumulate = [&](uint32_t acc, uint32_t from, uint32_t tile, bool first, uint64_t* ready, uint64_t* empty, bool done) {
     if (!warp_ready(ready, it & 1, abort_flag, status, kStatusWaitEpi)) return false;
     tc_fence_after_sync();
     if (elect_one()) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) umma_bf16_ts(tmem + acc, from + (k >> 1) * 32 + (k & 1) * 8, mn_desc(tile, k * 2048, 16384), idesc_acc, it > 0 || k > 0);
+      for (int k = 0; k < 8; ++k) umma_bf16_ts(tmem + acc, from + (k >> 1) * 32 + (k & 1) * 8, mn_desc(tile, k * 2048, 16384), idesc_acc, !first || k > 0);
       umma_commit(empty);
+      if (done) umma_commit(&bar.acc_done);
     }
     __syncwarp();
     return true;
   };
-  bool ok = n > 0 && warp_ready(&bar.f_full, 0, abort_flag, status, kStatusWaitFull) && scores(0) && dp(0);
-  for (int it = 0; it < n && ok; ++it) {
-    const bool more = it + 1 < n;
-    if (kTwo && more) ok = scores(it + 1);
-    if (kKeys) {
-      ok = ok && accumulate(L::ACC0, s_at(it), b_at(it), it, &bar.p_ready, &bar.b_empty[it % kB]);
-      if (!kTwo && more) ok = ok && scores(it + 1);
-    }
-    ok = ok && accumulate(L::ACC1, tmem + L::DP, a_at(it), it, &bar.ds_ready, &bar.a_empty[it % kA]);
-    if (more) ok = ok && dp(it + 1);
-  }
-  if (ok && elect_one()) umma_commit(&bar.acc_done);
-  __syncwarp();
-}
-
-// What the roles of a work item share.
-struct BwdItem {
-  int tile, h, b;              // the 128 keys or rows that stay; a key head or a row of heads
-  int i0, i1;                  // the streamed tiles: rows of the key head's rows of heads one after the other, or blocks of keys
-  int key_state;               // of the keys that stay
-  float mask_base;
-  const uint8_t* state;        // of the batch row's blocks; null without a mask
-};
-template <bool kKeys>
-__device__ __forceinline__ int kind_of(const CrossParams& p, const BwdItem& x, int i) {
-  return kKeys ? x.key_state : x.state ? __ldg(x.state + i) : block_state_unmasked(p, i);
-}
-// A place in a ring of kN stages, and the parity of its turn.
-template <int kN>
-struct Ring {
-  int stage = 0;
-  uint32_t parity = 0;
-  __device__ void next() {
-    if (++stage == kN) {
-      stage = 0;
-      parity ^= 1;
+  Ring<2> rt;
+  bool ok = true;
+  for (int runs = 0; ok && warp_ready(&bar.tasks.full[rt.stage], rt.parity, abort_flag, status, kStatusWaitFull) && bar.tasks.task[rt.stage].valid; ++runs) {
+    const int n = bar.tasks.task[rt.stage].i1 - bar.tasks.task[rt.stage].i0;
+    arrive_warp(&bar.tasks.empty[rt.stage], static_cast<int>(threadIdx.x & 31));
+    rt.next();
+    ok = warp_ready(&bar.f_full, runs & 1, abort_flag, status, kStatusWaitFull) && scores(it) && dp(n == 1);
+    for (int i = 0; i < n && ok; ++i, ++it) {
+      const bool more = i + 1 < n, first = i == 0;
+      if (kTwo && more) ok = scores(it + 1);
+      if (kKeys) {
+        ok = ok && accumulate(L::ACC0, s_at(it), b_at(fb.stage), first, &bar.p_ready, &bar.b_empty[fb.stage], false);
+        fb.next();
+        if (!kTwo && more) ok = ok && scores(it + 1);
+      }
+      ok = ok && accumulate(L::ACC1, tmem + L::DP, a_at(fa.stage), first, &bar.ds_ready, &bar.a_empty[fa.stage], !more);
+      fa.next();
+      if (more) ok = ok && dp(i + 2 == n);
     }
   }
-};
+}
 
 template <int kD, bool kKeys>
-__device__ __forceinline__ void bwd_loads(BwdBars& bar, const CrossParams& p, const BwdItem& x, uint32_t smem, int row_tiles, const void* f0, const void* f1, const void* a, const void* b) {
+__device__ __forceinline__ void bwd_loads(BwdBars& bar, const CrossParams& p, const int* counts, int key_ctas, bool whole, uint32_t smem, const void* f0, const void* f1, const void* a, const void* b) {
   using L = Bwd<kD>;
   constexpr int kA = L::stages_a(kKeys), kB = L::stages_b(kKeys);
   volatile int* abort_flag = &bar.abort_flag;
-  if (elect_one()) {
-    const int at = kKeys ? x.tile * 128 : (x.tile * 128) >> p.pack_log2;
-    mbar_expect_tx(&bar.f_full, 2 * L::kTile);
-    load_tile<kD>(smem + L::F0, f0, &bar.f_full, 128, at, x.h, x.b);
-    load_tile<kD>(smem + L::F1, f1, &bar.f_full, 128, at, x.h, x.b);
-  }
-  __syncwarp();
   Ring<kA> ra;
   Ring<kB> rb;
-  int as = 0, bs = 0;
-  int head = kKeys ? x.h * p.per_kv + x.i0 / row_tiles : x.h / p.per_kv, row = kKeys ? x.i0 % row_tiles : 0;
-  for (int i = x.i0; i < x.i1; ++i) {
-    if (!kind_of<kKeys>(p, x, i)) continue;
-    const int seq = kKeys ? (row * 128) >> p.pack_log2 : i * 128;
-    if (!warp_ready(&bar.a_empty[ra.stage], ra.parity ^ 1, abort_flag, p.status, kStatusWaitEmpty)) break;
+  int as = 0, bs = 0, runs = 0;
+  const int first = kKeys ? blockIdx.x : blockIdx.x - key_ctas, ctas = kKeys ? key_ctas : gridDim.x - key_ctas;
+  const Share share = share_of<kKeys>(p, counts, first, ctas, whole, threadIdx.x & 31);
+  Walk<kKeys> walk(counts, share, first, ctas);
+  const Place end = share.end;
+  Run r;
+  Ring<2> rt;
+  const int lane = threadIdx.x & 31;
+  bool ok = true;
+  while (ok) {
+    Task task = {};
+    if (walk.next(p, end, r)) task = task_of<kKeys>(p, counts, r);
+    ok = hand_out(bar.tasks, rt.stage, rt.parity, task, abort_flag, p.status, lane);
+    rt.next();
+    if (!ok || !task.valid) break;
+    // keys: the tile is a live block of a key head, whose rows of heads' rows stream; rows: 128 rows of a row of heads, and its key head's blocks stream
+    const int h = task.h, at0 = kKeys ? task.at * 128 : (task.at * 128) >> p.pack_log2;
+    int head = kKeys ? h * p.per_kv + r.i0 / p.row_tiles : h / p.per_kv, row = kKeys ? r.i0 % p.row_tiles : 0;
+    ok = warp_ready(&bar.f_empty, (runs & 1) ^ 1, abort_flag, p.status, kStatusWaitEmpty);
+    if (!ok) break;
     if (elect_one()) {
-      mbar_expect_tx(&bar.a_full[ra.stage], L::kTile);
-      load_tile<kD>(smem + L::RING + ra.stage * L::kTile, a, &bar.a_full[ra.stage], 128, seq, head, x.b);
+      mbar_expect_tx(&bar.f_full, 2 * L::kTile);
+      load_tile<kD>(smem + L::F0, f0, &bar.f_full, 128, at0, h, r.b);
+      load_tile<kD>(smem + L::F1, f1, &bar.f_full, 128, at0, h, r.b);
     }
     __syncwarp();
-    ++as;
-    if (!warp_ready(&bar.b_empty[rb.stage], rb.parity ^ 1, abort_flag, p.status, kStatusWaitEmpty)) break;
-    if (elect_one()) {
-      mbar_expect_tx(&bar.b_full[rb.stage], L::kTile);
-      load_tile<kD>(smem + L::RING + (kA + rb.stage) * L::kTile, b, &bar.b_full[rb.stage], 128, seq, head, x.b);
-    }
-    __syncwarp();
-    ++bs;
-    ra.next();
-    rb.next();
-    if (kKeys && ++row == row_tiles) {
-      row = 0;
-      ++head;
+    ++runs;
+    int2 next = make_int2(0, 0);
+    if (!kKeys) next = live_block(p, r.b, r.i0);
+    for (int i = r.i0; i < r.i1; ++i) {
+      const int seq = kKeys ? (row * 128) >> p.pack_log2 : next.x * 128;
+      if (!kKeys && i + 1 < r.i1) next = live_block(p, r.b, i + 1);
+      ok = warp_ready(&bar.a_empty[ra.stage], ra.parity ^ 1, abort_flag, p.status, kStatusWaitEmpty);
+      if (!ok) break;
+      if (elect_one()) {
+        mbar_expect_tx(&bar.a_full[ra.stage], L::kTile);
+        load_tile<kD>(smem + L::RING + ra.stage * L::kTile, a, &bar.a_full[ra.stage], 128, seq, head, r.b);
+      }
+      __syncwarp();
+      ++as;
+      ok = warp_ready(&bar.b_empty[rb.stage], rb.parity ^ 1, abort_flag, p.status, kStatusWaitEmpty);
+      if (!ok) break;
+      if (elect_one()) {
+        mbar_expect_tx(&bar.b_full[rb.stage], L::kTile);
+        load_tile<kD>(smem + L::RING + (kA + rb.stage) * L::kTile, b, &bar.b_full[rb.stage], 128, seq, head, r.b);
+      }
+      __syncwarp();
+      ++bs;
+      ra.next();
+      rb.next();
+      if (kKeys && ++row == p.row_tiles) {
+        row = 0;
+        ++head;
+      }
     }
   }
-  drain(&bar.f_full, 0);
+  if (runs > 0) drain(&bar.f_full, (runs - 1) & 1);
   for (int u = max(0, as - kA); u < as; ++u) drain(&bar.a_full[u % kA], (u / kA) & 1);
   for (int u = max(0, bs - kB); u < bs; ++u) drain(&bar.b_full[u % kB], (u / kB) & 1);
 }
 
 // The table of a streamed tile: {-l[128], -D[128]} of its rows, or its keys' entries.
 template <int kD, bool kKeys>
-__device__ __forceinline__ void bwd_tables(BwdBars& bar, const CrossParams& p, const BwdItem& x, float* tab, const float* stats, const float* D, int row_tiles, int lane) {
+__device__ __forceinline__ void bwd_tables(BwdBars& bar, const CrossParams& p, float* tab, const float* stats, const float* D, int lane) {
   Ring<Bwd<kD>::stages_a(kKeys)> ra;
-  int head = kKeys ? x.h * p.per_kv + x.i0 / row_tiles : 0, row = kKeys ? x.i0 % row_tiles : 0;
-  for (int i = x.i0; i < x.i1; ++i) {
-    const int kind = kind_of<kKeys>(p, x, i);
-    if (!kind) continue;
-    float* tb = tab + ra.stage * 256;
-    float2 v[4];
+  Ring<2> rt;
+  while (warp_ready(&bar.tasks.full[rt.stage], rt.parity, &bar.abort_flag, p.status, kStatusWaitFull)) {
+    const Task r = bar.tasks.task[rt.stage];
+    arrive_warp(&bar.tasks.empty[rt.stage], lane);
+    rt.next();
+    if (!r.valid) return;
+    const float base = r.base, shift = kKeys && !r.masked ? base : 0.f;        // keys with nothing added are `base` below the largest
+    int head = kKeys ? r.h * p.per_kv + r.i0 / p.row_tiles : 0, row = kKeys ? r.i0 % p.row_tiles : 0;
+    for (int i = r.i0; i < r.i1; ++i) {
+      float* tb = tab + ra.stage * 256;
+      float2 v[4];
+      const int2 blk = kKeys ? make_int2(0, 1) : live_block(p, r.b, i);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (kKeys) {
-        const int r = row * 128 + e * 32 + lane;
-        const long long at = (static_cast<long long>(x.b) * p.Hq + head) * p.R + r;
-        v[e] = make_float2(-INFINITY, 0.f);
-        if (r < p.R) v[e] = make_float2(-__ldg(stats + at) - (x.key_state == 2 ? x.mask_base : 0.f), -__ldcg(D + at));
-      } else {
-        v[e] = kind == 1 ? key_entry(p, x.b, i * 128 + e * 32 + lane, x.mask_base) : make_float2(0.f, 0.f);
+      for (int e = 0; e < 4; ++e) {
+        if (kKeys) {
+          const int n = row * 128 + e * 32 + lane;
+          const long long line = (static_cast<long long>(r.b) * p.Hq + head) * p.R + n;
+          v[e] = make_float2(-INFINITY, 0.f);
+          if (n < p.R) v[e] = make_float2(-__ldcg(stats + line) - shift, -__ldcg(D + line));
+        } else if (blk.y) {
+          v[e] = key_entry(p, r.b, blk.x * 128 + e * 32 + lane, base);
+        }
       }
-    }
-    if (!warp_ready(&bar.a_empty[ra.stage], ra.parity ^ 1, &bar.abort_flag, p.status, kStatusWaitEmpty)) break;
+      if (!warp_ready(&bar.a_empty[ra.stage], ra.parity ^ 1, &bar.abort_flag, p.status, kStatusWaitEmpty)) return;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int at = e * 32 + lane;
-      if (kKeys) {
-        tb[at] = v[e].x;
-        tb[128 + at] = v[e].y;
-      } else if (kind == 1) {
-        reinterpret_cast<float2*>(tb)[at] = v[e];
+      for (int e = 0; e < 4; ++e) {
+        const int n = e * 32 + lane;
+        if (kKeys) {
+          tb[n] = v[e].x;
+          tb[128 + n] = v[e].y;
+        } else if (blk.y) {
+          reinterpret_cast<float2*>(tb)[n] = v[e];
+        }
       }
-    }
-    arrive_warp(&bar.tab_full[ra.stage], lane);
-    ra.next();
-    if (kKeys && ++row == row_tiles) {
-      row = 0;
-      ++head;
+      arrive_warp(&bar.tab_full[ra.stage], lane);
+      ra.next();
+      if (kKeys && ++row == p.row_tiles) {
+        row = 0;
+        ++head;
+      }
     }
   }
 }
@@ -841,63 +1180,110 @@ __device__ __noinline__ void masked_dp(uint32_t tDP, float2 entry, const float2*
   tmem_st_wait();
 }
 
-// P and dS, tile by tile; returns the number of tiles, or -1 after a wait that gave up.
 template <int kD, bool kKeys>
-__device__ __forceinline__ int bwd_softmax(BwdBars& bar, const CrossParams& p, const BwdItem& x, uint32_t tmem, uint32_t smem, const float* tab, const float* stats, const float* D, int warp,
-                                           int lane) {
+__device__ __forceinline__ void bwd_softmax(BwdBars& bar, const CrossParams& p, const BwdOut& out, uint32_t tmem, uint32_t smem, const float* tab, int warp, int lane) {
   using L = Bwd<kD>;
   constexpr bool kTwo = !kKeys || L::kTwoForKeys;
   const int w = warp >> 2, quarter = warp & 3, t = quarter * 32 + lane;
-  const uint32_t at = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + w * 32;
+  const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16, mine = tmem + lanes + w * 32;
   volatile int* abort_flag = &bar.abort_flag;
-  // of the row: an entry of the mask, or statistics
-  float2 entry = make_float2(0.f, 0.f);
-  float neg_l = 0.f, neg_d = 0.f;
-  if (kKeys) {
-    if (x.key_state == 1) entry = key_entry(p, x.b, x.tile * 128 + t, x.mask_base);
-  } else if (x.tile * 128 + t < p.R) {
-    const long long row = (static_cast<long long>(x.b) * p.Hq + x.h) * p.R + x.tile * 128 + t;
-    neg_l = -__ldg(stats + row);
-    neg_d = -__ldcg(D + row);
-  }
   Ring<L::stages_a(kKeys)> ra;
   Ring<kTwo ? 2 : 1> rs;
-  int it = 0;
-  for (int i = x.i0; i < x.i1; ++i) {
-    const int kind = kind_of<kKeys>(p, x, i);
-    if (!kind) continue;
-    const float* tb = tab + ra.stage * 256 + (kKeys ? w * 32 : w * 64);
-    const uint32_t tS = at + (rs.stage ? (kKeys ? L::S2_KEYS : L::S2_ROWS) : L::S), tDP = at + L::DP;
-    if (kKeys || kind != 2)
-      if (!warp_ready(&bar.tab_full[ra.stage], ra.parity, abort_flag, p.status, kStatusWaitFull)) return -1;
-    if (!warp_ready(&bar.s_full[rs.stage], rs.parity, abort_flag, p.status, kStatusWaitAccum)) return -1;
-    tc_fence_after_sync();
-    if (kind != 2) masked_scores<kKeys>(tS, entry, reinterpret_cast<const float2*>(tb));
-    uint32_t pr[32];
-    make_p<kKeys>(tS, kind == 2 ? p.scale * kLog2e : 1.f, tb, kind == 2 ? neg_l - x.mask_base : neg_l, pr);
+  int it = 0, runs = 0;
+  Ring<2> rt;
+  for (; warp_ready(&bar.tasks.full[rt.stage], rt.parity, abort_flag, p.status, kStatusWaitFull); ++runs) {
+    const volatile Task& task = bar.tasks.task[rt.stage];
+    if (!task.valid) break;
+    const int b = task.b, i0 = task.i0, i1 = task.i1;
+    const bool stays_masked = kKeys && task.masked;
+    // of the row: an entry of the mask, or statistics
+    float2 entry = make_float2(0.f, 0.f);
+    float neg_l = 0.f, neg_d = 0.f;
     if (kKeys) {
+      if (stays_masked) entry = key_entry(p, b, task.at * 128 + t, task.base);
+    } else if (task.at * 128 + t < p.R) {
+      const long long row = (static_cast<long long>(b) * p.Hq + task.h) * p.R + task.at * 128 + t;
+      neg_l = -__ldcg(out.stats + row);
+      neg_d = -__ldcg(out.D + row);
+    }
+    bool next = stays_masked;
+    if (!kKeys) next = live_block(p, b, i0).y;
+    for (int i = i0; i < i1; ++i) {
+      const bool masked = next;
+      if (!kKeys && i + 1 < i1) next = live_block(p, b, i + 1).y;
+      const float* tb = tab + ra.stage * 256 + (kKeys ? w * 32 : w * 64);
+      const uint32_t tS = mine + (rs.stage ? (kKeys ? L::S2_KEYS : L::S2_ROWS) : L::S), tDP = mine + L::DP;
+      if (!warp_ready(&bar.tab_full[ra.stage], ra.parity, abort_flag, p.status, kStatusWaitFull)) return;        // every turn: a parity tells only the last two apart
+      if (!warp_ready(&bar.s_full[rs.stage], rs.parity, abort_flag, p.status, kStatusWaitAccum)) return;
+      tc_fence_after_sync();
+      if (masked) masked_scores<kKeys>(tS, entry, reinterpret_cast<const float2*>(tb));
+      uint32_t pr[32];
+      make_p<kKeys>(tS, masked ? 1.f : p.scale * kLog2e, tb, masked || kKeys ? neg_l : neg_l - task.base, pr);
+      if (kKeys) {
+        tmem_st_wait();
+        tc_fence_before_sync();
+        arrive_warp(&bar.p_ready, lane);
+      }
+      if (!warp_ready(&bar.dp_full, it & 1, abort_flag, p.status, kStatusWaitAccum)) return;
+      tc_fence_after_sync();
+      if (masked) {
+        masked_dp<kKeys>(tDP, entry, reinterpret_cast<const float2*>(tb));
+        if (!kKeys && p.mask) {        // nor of an absent key's K, which its dS of zero meets: S and dP have been read from it
+          if (w == 0 && reinterpret_cast<const float2*>(tb)[t].y == -INFINITY) zero_row<kD>(smem + L::RING + ra.stage * L::kTile, 128, t);
+          fence_proxy_async_smem();
+        }
+      }
+      make_ds<kKeys>(tDP, tb + 128, neg_d, pr);
       tmem_st_wait();
       tc_fence_before_sync();
-      arrive_warp(&bar.p_ready, lane);
+      arrive_warp(&bar.ds_ready, lane);
+      ++it;
+      ra.next();
+      rs.next();
     }
-    if (!warp_ready(&bar.dp_full, it & 1, abort_flag, p.status, kStatusWaitAccum)) return -1;
+    // ---- the run's sums. Keys: half of the warps write dK, the others dV; rows: all of them dQ
+    if (!warp_ready(&bar.acc_done, runs & 1, abort_flag, p.status, kStatusWaitAccum)) return;
     tc_fence_after_sync();
-    if (kind != 2) {
-      masked_dp<kKeys>(tDP, entry, reinterpret_cast<const float2*>(tb));
-      if (!kKeys && p.mask) {        // nor of an absent key's K, which its dS of zero meets: S and dP have been read from it
-        if (w == 0 && reinterpret_cast<const float2*>(tb)[t].y == -INFINITY) zero_row<kD>(smem + L::RING + ra.stage * L::kTile, 128, t);
-        fence_proxy_async_smem();
+    const int n = task.at * 128 + t, h = task.h;        // this thread's key or row
+    const bool whole = task.whole, inside = kKeys ? n < p.Sk : n < p.R, is_v = kKeys && w >= 2;
+    constexpr int kStep = kKeys ? kD / 2 : kD / 4;
+    const int c0 = (kKeys ? w & 1 : w) * kStep;
+    const uint32_t acc = tmem + (is_v ? L::ACC0 : L::ACC1) + lanes + c0;
+    const float mul = is_v ? 1.f : p.scale;
+    float* part = nullptr;
+    __nv_bfloat16* to = nullptr;
+    if (!whole) {
+      if (warp == 0 && lane == 0) bar.left[task.slot] = Left{1, task.ends, b, task.tile};
+      const long long slot = kKeys ? (blockIdx.x * 2ll + task.slot) * 2 + is_v : (out.key_ctas + blockIdx.x) * 2ll + task.slot;
+      part = out.part + (slot * 128 + t) * kD + c0;
+    } else if (kKeys) {
+      to = (is_v ? out.dv : out.dk) + b * out.ksb + n * out.kss + h * out.ksh + c0;
+    } else {
+      to = out_row(p, out.dq, out.qsb, out.qss, out.qsh, b, h, n) + c0;
+    }
+#pragma unroll 1
+    for (int c = 0; c < kStep; c += 16) {
+      uint32_t v[16];
+      tmem_ld16(acc + c, v);
+      tmem_ld_wait();
+      float f[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        asm volatile("" : "+r"(v[e]));
+        f[e] = __uint_as_float(v[e]) * mul;
+      }
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(part + c + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+      } else if (inside) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 8) *reinterpret_cast<uint4*>(to + c + e) = pack8(f + e);
       }
     }
-    make_ds<kKeys>(tDP, tb + 128, neg_d, pr);
-    tmem_st_wait();
     tc_fence_before_sync();
-    arrive_warp(&bar.ds_ready, lane);
-    ++it;
-    ra.next();
-    rs.next();
+    arrive_warp(&bar.tasks.empty[rt.stage], lane);
+    rt.next();
   }
-  return it;
 }
 
 template <int kD>
@@ -907,28 +1293,15 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using L = Bwd<kD>;
-  static_assert(sizeof(BwdBars) <= 256, "barriers");
+  static_assert(sizeof(BwdBars) <= 512, "barriers");
   BwdBars& bar = *reinterpret_cast<BwdBars*>(smem + L::BARS);
   float* tab = reinterpret_cast<float*>(smem + L::TAB);
-
   const int warp = uniform_warp(), lane = threadIdx.x & 31;
-  const bool keys = static_cast<int>(blockIdx.x) < out.key_items;
-  int lin = keys ? blockIdx.x : blockIdx.x - out.key_items;
-  const int parts = keys ? out.parts_k : out.parts_q, per = keys ? out.key_blocks : out.row_tiles, heads = keys ? p.Hk : p.Hq;
-  const int part = lin % parts;
-  lin /= parts;
-  BwdItem x;
-  x.tile = lin % per;
-  lin /= per;
-  x.h = lin % heads;
-  x.b = lin / heads;
-  x.state = out.state ? out.state + static_cast<long long>(x.b) * out.key_blocks : nullptr;
-  const int n_all = keys ? p.per_kv * out.row_tiles : out.key_blocks, per_part = (n_all + parts - 1) / parts;
-  x.i0 = part * per_part;
-  x.i1 = min(n_all, x.i0 + per_part);
+  const bool keys = static_cast<int>(blockIdx.x) < out.key_ctas;
 
   if (threadIdx.x == 0) {
     mbar_init(&bar.f_full, 1);
+    mbar_init(&bar.f_empty, 1);
     for (int s = 0; s < 3; ++s) {
       mbar_init(&bar.a_full[s], 1);
       mbar_init(&bar.a_empty[s], 1);
@@ -942,6 +1315,8 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     mbar_init(&bar.p_ready, kBwdSoftmaxWarps);
     mbar_init(&bar.ds_ready, kBwdSoftmaxWarps);
     mbar_init(&bar.acc_done, 1);
+    for (int i = 0; i < 2; ++i) { mbar_init(&bar.tasks.full[i], 1); mbar_init(&bar.tasks.empty[i], kBwdSoftmaxWarps + 2); }
+    bar.left[0] = bar.left[1] = Left{0, 0, 0, 0};
     bar.abort_flag = 0;
     mbar_fence_init();
   }
@@ -949,69 +1324,55 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     tmem_alloc<1>(&bar.tmem_slot, 512);
     tmem_relinquish<1>();
   }
+  if (warp == kBwdSoftmaxWarps + 1 && elect_one()) {
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tmDO);
+  }
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = bar.tmem_slot;
   pdl_entry();
+  const int* counts = counts_of(p, reinterpret_cast<int*>(smem + L::COUNTS));
+  if (counts) __syncthreads();
   const uint32_t base = smem_u32(smem);
-  x.key_state = !keys ? 0 : x.state ? __ldg(x.state + x.tile) : block_state_unmasked(p, x.tile);
-  x.mask_base = p.base ? __ldg(p.base + x.b) : 0.f;
-  if (keys && x.key_state == 0) x.i1 = x.i0;                // no key of the block takes part
 
   if (warp == kBwdSoftmaxWarps + 1) {
-    if (keys) bwd_loads<kD, true>(bar, p, x, base, out.row_tiles, &tmK, &tmV, &tmQ, &tmDO);
-    else bwd_loads<kD, false>(bar, p, x, base, out.row_tiles, &tmQ, &tmDO, &tmK, &tmV);
+    if (keys) bwd_loads<kD, true>(bar, p, counts, out.key_ctas, out.whole_keys, base, &tmK, &tmV, &tmQ, &tmDO);
+    else bwd_loads<kD, false>(bar, p, counts, out.key_ctas, out.whole_rows, base, &tmQ, &tmDO, &tmK, &tmV);
   } else if (warp == kBwdSoftmaxWarps + 2) {
-    if (keys) bwd_tables<kD, true>(bar, p, x, tab, out.stats, out.D, out.row_tiles, lane);
-    else bwd_tables<kD, false>(bar, p, x, tab, out.stats, out.D, out.row_tiles, lane);
+    if (keys) bwd_tables<kD, true>(bar, p, tab, out.stats, out.D, lane);
+    else bwd_tables<kD, false>(bar, p, tab, out.stats, out.D, lane);
   } else if (warp == kBwdSoftmaxWarps) {
-    int n = x.i1 - x.i0;
-    if (keys) {
-      bwd_products<kD, true>(bar, p.status, tmem, base, n);
-    } else {
-      for (int i = x.i0; i < x.i1; ++i) n -= kind_of<false>(p, x, i) == 0;
-      bwd_products<kD, false>(bar, p.status, tmem, base, n);
-    }
+    if (keys) bwd_products<kD, true>(bar, p, tmem, base);
+    else bwd_products<kD, false>(bar, p, tmem, base);
   } else {
-    const int n = keys ? bwd_softmax<kD, true>(bar, p, x, tmem, base, tab, out.stats, out.D, warp, lane) : bwd_softmax<kD, false>(bar, p, x, tmem, base, tab, out.stats, out.D, warp, lane);
-    if (n == 0 || (n > 0 && warp_ready(&bar.acc_done, 0, &bar.abort_flag, p.status, kStatusWaitAccum))) {
-      tc_fence_after_sync();
-      // keys: half of the warps write dK, the others dV; rows: all of them dQ
-      const int w = warp >> 2, quarter = warp & 3, r = x.tile * 128 + quarter * 32 + lane;
-      const bool inside = keys ? r < p.Sk : r < p.R, is_v = keys && w >= 2;
-      const int step = keys ? kD / 2 : kD / 4, c0 = (keys ? w & 1 : w) * step, c1 = c0 + step;
-      const uint32_t acc = tmem + (is_v ? L::ACC0 : L::ACC1) + (static_cast<uint32_t>(quarter * 32) << 16);
-      const float mul = is_v ? 1.f : p.scale;
-      const long long line = keys ? (static_cast<long long>(x.b) * p.Hk + x.h) * p.Sk + r : (static_cast<long long>(x.b) * p.Hq + x.h) * p.R + r;
-      const long long lines = keys ? static_cast<long long>(p.B) * p.Hk * p.Sk : static_cast<long long>(p.B) * p.Hq * p.R;
-      float* part_at = nullptr;
-      __nv_bfloat16* at = nullptr;
-      if (parts > 1) part_at = (keys ? (is_v ? out.part_v : out.part_k) : out.part_q) + (part * lines + line) * kD;
-      else if (keys) at = (is_v ? out.dv : out.dk) + x.b * out.ksb + r * out.kss + x.h * out.ksh;
-      else at = out_row(p, out.dq, out.qsb, out.qss, out.qsh, x.b, x.h, r);
-#pragma unroll 1
-      for (int c = c0; c < c1; c += 16) {
-        uint32_t v[16];
-        if (n > 0) {
-          tmem_ld16(acc + c, v);
-          tmem_ld_wait();
+    if (keys) bwd_softmax<kD, true>(bar, p, out, tmem, base, tab, warp, lane);
+    else bwd_softmax<kD, false>(bar, p, out, tmem, base, tab, warp, lane);
+    if (threadIdx.x == 0) {
+      out.left[blockIdx.x * 2] = bar.left[0];
+      out.left[blockIdx.x * 2 + 1] = bar.left[1];
+    }
+    if (counts) {
+      // what nothing streams past: blocks without a key, and the rows of batch rows without one, get zeros
+      constexpr int kThreads = 32 * kBwdSoftmaxWarps, kVecs = kD / 8;
+      for (long long x = blockIdx.x; x < static_cast<long long>(p.B) * p.key_blocks; x += gridDim.x) {
+        const int b = static_cast<int>(x / p.key_blocks), i = static_cast<int>(x % p.key_blocks), n = live_of(p, counts, b);
+        if (i < n) continue;
+        const int key0 = live_block(p, b, i).x * 128;
+        for (int e = threadIdx.x; e < 128 * p.Hk * kVecs; e += kThreads) {
+          const int c = e % kVecs, h = e / kVecs % p.Hk, key = key0 + e / kVecs / p.Hk;
+          if (key >= p.Sk) break;
+          const long long at = b * out.ksb + key * out.kss + h * out.ksh + c * 8;
+          *reinterpret_cast<uint4*>(out.dk + at) = *reinterpret_cast<uint4*>(out.dv + at) = make_uint4(0u, 0u, 0u, 0u);
         }
-        float f[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          if (n > 0) asm volatile("" : "+r"(v[e]));
-          f[e] = n > 0 ? __uint_as_float(v[e]) * mul : 0.f;
-        }
-        if (inside) {
-          if (parts > 1) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(part_at + c + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; e += 8) *reinterpret_cast<uint4*>(at + c + e) = pack8(f + e);
+        if (n == 0 && i == 0)
+          for (long long e = threadIdx.x; e < static_cast<long long>(p.Hq) * p.R * kVecs; e += kThreads) {
+            const int c = static_cast<int>(e % kVecs), row = static_cast<int>(e / kVecs % p.R), h = static_cast<int>(e / kVecs / p.R);
+            *reinterpret_cast<uint4*>(out_row(p, out.dq, out.qsb, out.qss, out.qsh, b, h, row) + c * 8) = make_uint4(0u, 0u, 0u, 0u);
           }
-        }
       }
     }
   }
@@ -1023,26 +1384,18 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
 }
 
-// Before: D = rowsum(dO o), eight values a lane; and, in the blocks behind, what the mask says of each block of keys.
+// Before: D = rowsum(dO o), eight values a lane.
 template <int kD>
-__global__ void __launch_bounds__(256) cross_pre_kernel(const CrossParams p, const __nv_bfloat16* __restrict__ o, const long long osb, const long long oss, const long long osh,
-                                                        const __nv_bfloat16* __restrict__ d_o, const long long gsb, const long long gss, const long long gsh,
-                                                        float* __restrict__ D, uint8_t* __restrict__ state, const int row_blocks) {
+__global__ void __launch_bounds__(256) cross_pre_kernel(const CrossParams p, const __nv_bfloat16* o, const long long osb, const long long oss, const long long osh,
+                                                        const __nv_bfloat16* d_o, const long long gsb, const long long gss, const long long gsh,
+                                                        float* D) {
   pdl_entry();
   const int lane = threadIdx.x & 31;
-  if (static_cast<int>(blockIdx.x) >= row_blocks) {
-    const int nblk = (p.Sk + kKeys - 1) / kKeys;
-    const long long at = (blockIdx.x - row_blocks) * 8ll + (threadIdx.x >> 5);
-    if (at >= static_cast<long long>(p.B) * nblk) return;
-    const int s = block_state(p, static_cast<int>(at / nblk), static_cast<int>(at % nblk), lane);
-    if (lane == 0) state[at] = static_cast<uint8_t>(s);
-    return;
-  }
   constexpr int kLanes = kD / 8;
   const long long rows = static_cast<long long>(p.B) * p.Hq * p.R;
   const int c = (threadIdx.x % kLanes) * 8;
   const unsigned m = kLanes == 16 ? 0xffffu << (lane & 16) : 0xffu << (lane & 24);
-  for (long long row = (blockIdx.x * 256ll + threadIdx.x) / kLanes; row < rows; row += row_blocks * 256ll / kLanes) {
+  for (long long row = (blockIdx.x * 256ll + threadIdx.x) / kLanes; row < rows; row += gridDim.x * 256ll / kLanes) {
     const int r = static_cast<int>(row % p.R), g = r & ((1 << p.pack_log2) - 1);
     const long long bh = row / p.R, b = bh / p.Hq, h = ((bh % p.Hq) << p.pack_log2) + g, s = r >> p.pack_log2;
     const uint4 x = *reinterpret_cast<const uint4*>(o + b * osb + s * oss + h * osh + c), y = *reinterpret_cast<const uint4*>(d_o + b * gsb + s * gss + h * gsh + c);
@@ -1057,35 +1410,39 @@ __global__ void __launch_bounds__(256) cross_pre_kernel(const CrossParams p, con
   }
 }
 
-// After: parts added in their order, rounded to bf16. Rows of [B, heads, n] (rows of heads, or key heads), four values a lane.
+// After: the stretches' shares of a tile added up in their order, by the block of the CTA that began it, four values a thread; keys: dK and dV.
 template <int kD>
-__global__ void __launch_bounds__(256) cross_sum_kernel(const CrossParams p, const BwdOut out) {
+__global__ void __launch_bounds__(256) cross_sum_kernel(const CrossParams p, const BwdOut out, const int ctas) {
+  __shared__ short with[kWith];
+  __shared__ int count;
   pdl_entry();
   constexpr int kLanes = kD / 4;
-  const long long q_rows = out.parts_q > 1 ? static_cast<long long>(p.B) * p.Hq * p.R : 0, k_rows = out.parts_k > 1 ? static_cast<long long>(p.B) * p.Hk * p.Sk : 0;
-  const int c = (threadIdx.x % kLanes) * 4;
-  for (long long row = (blockIdx.x * 256ll + threadIdx.x) / kLanes; row < q_rows + 2 * k_rows; row += gridDim.x * 256ll / kLanes) {
-    const bool q = row < q_rows, v = !q && row >= q_rows + k_rows;
-    const long long at = q ? row : row - q_rows - (v ? k_rows : 0), rows = q ? q_rows : k_rows;
-    const float* src = (q ? out.part_q : v ? out.part_v : out.part_k) + at * kD + c;
+  const int cta = blockIdx.x;
+  const bool keys = cta < out.key_ctas;
+  const Left first = out.left[cta * 2 + 1];
+  if (!first.used) return;
+  const int sharing = sharers(out.left, cta, keys ? out.key_ctas : ctas, with, &count);
+  const int per = keys ? live_of(p, p.live_count, first.b) : p.row_tiles, h = first.tile / per, tile = first.tile - h * per;
+  const int c = (threadIdx.x % kLanes) * 4, t = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes;
+  const int n = (keys ? live_block(p, first.b, tile).x : tile) * 128 + t;
+  if (n >= (keys ? p.Sk : p.R)) return;
+  for (int v = 0; v < (keys ? 2 : 1); ++v) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < (q ? out.parts_q : out.parts_k); ++i) {
-      const float4 x = *reinterpret_cast<const float4*>(src + i * rows * kD);
+#pragma unroll 8
+    for (int k = 0; k < sharing; ++k) {
+      const long long slot = keys ? (with[k] * 2ll + (k == 0)) * 2 + v : (out.key_ctas + with[k]) * 2ll + (k == 0);
+      const float4 x = *reinterpret_cast<const float4*>(out.part + (slot * 128 + t) * kD + c);
       acc.x += x.x; acc.y += x.y; acc.z += x.z; acc.w += x.w;
     }
-    __nv_bfloat16* dst;
-    if (q) {
-      const long long bh = at / p.R;
-      dst = out_row(p, out.dq, out.qsb, out.qss, out.qsh, static_cast<int>(bh / p.Hq), static_cast<int>(bh % p.Hq), static_cast<int>(at % p.R));
-    } else {
-      const long long bh = at / p.Sk;
-      dst = (v ? out.dv : out.dk) + (bh / p.Hk) * out.ksb + (at % p.Sk) * out.kss + (bh % p.Hk) * out.ksh;
-    }
+    __nv_bfloat16* dst = keys ? (v ? out.dv : out.dk) + first.b * out.ksb + n * out.kss + h * out.ksh : out_row(p, out.dq, out.qsb, out.qss, out.qsh, first.b, h, n);
     *reinterpret_cast<uint2*>(dst + c) = make_uint2(pack2(acc.x, acc.y), pack2(acc.z, acc.w));
   }
 }
 
 // ------------------------------------------------------------------------------------------ host
+int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
+long long round_up(long long n, long long m) { return (n + m - 1) / m * m; }
+
 bool make_cross(const fb_cross_args& a, CrossParams& p, int& pack) {
   if (a.D != 64 && a.D != 128) return false;
   if (a.B < 1 || a.H < 1 || a.Hk < 1 || a.H % a.Hk || a.Sq < 1 || a.Sk < 1) return false;
@@ -1100,42 +1457,63 @@ bool make_cross(const fb_cross_args& a, CrossParams& p, int& pack) {
   if (static_cast<long long>(a.Sq) * pack > 0x7fffff00ll || a.Sk > (1 << 30)) return false;
   p.R = a.Sq * pack;
   p.Sk = a.Sk;
+  p.row_tiles = ceil_div(p.R, 128);
+  p.key_blocks = ceil_div(p.Sk, kKeys);
+  // tiles are counted in 32 bits, and so are the units of one for each CTA
+  if (static_cast<long long>(p.B) * p.Hq * p.row_tiles > 0x3fffffffll || static_cast<long long>(p.B) * p.Hk * p.key_blocks > 0x3fffffffll ||
+      static_cast<long long>(p.per_kv) * p.row_tiles > 0x7fffff || p.key_blocks > 0x7fffff)
+    return false;
   p.mask = a.mask;
   p.mask_stride = a.mask_stride;
   p.mask_bool = a.mask_bool;
-  p.base = a.mask && !a.mask_bool && a.stats ? a.stats + static_cast<long long>(a.B) * a.H * a.Sq : nullptr;
   p.scale = a.scale;
   p.table = !(a.scale > 0.f);
   p.status = a.status;
+  if (a.mask) {
+    p.live_count = a.mask_info;
+    p.base = reinterpret_cast<float*>(a.mask_info + a.B);
+    p.live = a.mask_info + 2ll * a.B;
+  }
   return true;
 }
 
-int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
-
-// Parts of the keys in the forward pass: where the tiles leave CTA slots (two an SM) empty, as many as fill them, of two blocks at least. Each costs a tile of fp32 sums
-// to memory and back.
-int fwd_parts(const CrossParams& p) {
-  const long long tiles = static_cast<long long>(ceil_div(p.R, 128)) * p.Hq * p.B, slots = 2ll * sm_count();
-  const int nblk = ceil_div(p.Sk, kKeys);
-  long long parts = 1;
-  if (tiles * 2 <= slots) parts = slots / tiles;
-  if (parts > nblk / 2) parts = nblk / 2;
-  if (parts < 1) parts = 1;
-  const int least = ceil_div(nblk, kMaxBlocks);
-  if (parts < least) parts = least;
-  return ceil_div(nblk, ceil_div(nblk, parts));
+// CTAs for `units` of work over tiles of `length`, at most `most`, and whether their stretches hold whole tiles only. Tiles of up to four units are not cut: what is left of
+// one costs about as much as a unit. Otherwise a stretch is two units at least.
+int stretches(long long units, int length, int most, int& whole) {
+  whole = length <= 4;
+  const long long n = whole ? units / length : (units + 1) / 2;
+  if (most > kWith) most = kWith;
+  return static_cast<int>(n < most ? n : most);
 }
-
-// Parts of an item's streamed tiles in the backward pass: an item longer than its share of all the work holds up the launch's end.
-void bwd_parts(const CrossParams& p, int& parts_q, int& parts_k) {
-  const long long n_q = ceil_div(p.Sk, 128), n_k = static_cast<long long>(p.per_kv) * ceil_div(p.R, 128);
-  const long long items_q = static_cast<long long>(ceil_div(p.R, 128)) * p.Hq * p.B, items_k = static_cast<long long>(ceil_div(p.Sk, 128)) * p.Hk * p.B;
-  const long long share = (n_q * items_q + n_k * items_k) / sm_count();
-  const long long least = share > 4 ? share : 4;
-  parts_q = n_q > least ? ceil_div(n_q, least) : 1;
-  parts_k = n_k > least ? ceil_div(n_k, least) : 1;
-  parts_q = ceil_div(n_q, ceil_div(n_q, parts_q));
-  parts_k = ceil_div(n_k, ceil_div(n_k, parts_k));
+struct FwdPlan {
+  int ctas, whole;
+  long long left, ml, o, total;        // places in the workspace, in floats
+};
+FwdPlan plan_fwd(const CrossParams& p, int D) {
+  FwdPlan f = {};
+  f.ctas = stretches(static_cast<long long>(p.B) * p.Hq * p.row_tiles * p.key_blocks, p.key_blocks, 2 * sm_count(), f.whole);
+  if (f.whole) return f;
+  f.ml = round_up(f.ctas * 2ll * 4, 32);
+  f.o = f.ml + f.ctas * 2ll * 128 * 2;
+  f.total = f.o + f.ctas * 2ll * 128 * D;
+  return f;
+}
+struct BwdPlan {
+  int key_ctas, row_ctas, whole_keys, whole_rows;
+  long long D, left, part, total;
+};
+BwdPlan plan_bwd(const CrossParams& p, int D) {
+  BwdPlan f = {};
+  const long long units = static_cast<long long>(p.B) * p.Hq * p.row_tiles * p.key_blocks;
+  // A unit of keys takes four products and a unit of rows three: 2450 and 2070 cycles (heads of 64), 3400 and 2250 (128).
+  const int most_keys = D == 64 ? sm_count() * 54 / 100 : sm_count() * 60 / 100;
+  f.key_ctas = stretches(units, p.per_kv * p.row_tiles, most_keys, f.whole_keys);
+  f.row_ctas = stretches(units, p.key_blocks, sm_count() - most_keys, f.whole_rows);
+  f.left = round_up(static_cast<long long>(p.B) * p.Hq * p.R, 32);
+  f.part = f.left + round_up((f.key_ctas + f.row_ctas) * 2ll * 4, 32);
+  f.total = f.part + (f.key_ctas * 4ll + f.row_ctas * 2ll) * 128 * D;
+  if (f.whole_keys && f.whole_rows) f.total = f.part;
+  return f;
 }
 
 template <int kD>
@@ -1145,49 +1523,28 @@ int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   if (!e) e = make_tmap_rows(&tk, a.k, kD, 1, a.Sk, a.Hk, a.B, a.k_strides[0], a.k_strides[1], a.k_strides[2]);
   if (!e) e = make_tmap_rows(&tv, a.v, kD, 1, a.Sk, a.Hk, a.B, a.v_strides[0], a.v_strides[1], a.v_strides[2]);
   if (e) return e;
+  const FwdPlan f = plan_fwd(p, kD);
+  if (f.total && !a.workspace) return -3;
   FwdOut out = {};
   out.o = static_cast<__nv_bfloat16*>(a.o);
   out.osb = a.o_strides[0];
   out.oss = a.o_strides[1];
   out.osh = a.o_strides[2];
   out.stats = a.stats;
-  out.parts = fwd_parts(p);
-  out.blocks_per_part = ceil_div(ceil_div(p.Sk, kKeys), out.parts);
-  out.n_tiles = ceil_div(p.R, 128);
-  const long long rows = static_cast<long long>(p.B) * p.Hq * p.R;
-  if (out.parts > 1) {
-    if (!a.workspace) return -3;
-    out.part_ml = reinterpret_cast<float2*>(a.workspace);
-    out.part_o = a.workspace + (out.parts * rows * 2 + 3) / 4 * 4;
+  out.whole = f.whole;
+  if (!f.whole) {
+    out.left = reinterpret_cast<Left*>(a.workspace);
+    out.part_ml = reinterpret_cast<float2*>(a.workspace + f.ml);
+    out.part_o = a.workspace + f.o;
   }
-  const long long ctas = static_cast<long long>(out.n_tiles) * p.Hq * p.B * out.parts;
-  if (ctas > 0x7fffffffll) return -4;
-  const int smem = Fwd<kD>::bytes(out.blocks_per_part);
-  if (const cudaError_t err = allow_smem<cross_fwd_kernel<kD>>(Fwd<kD>::bytes(kMaxBlocks), true)) return static_cast<int>(err);
-  if (const cudaError_t err = launch_pdl(cross_fwd_kernel<kD>, dim3(static_cast<unsigned>(ctas)), dim3(kFwdThreads), static_cast<size_t>(smem), stream, tq, tk, tv, p, out))
-    return static_cast<int>(err);
-  if (out.parts > 1) {
-    const long long blocks = (rows * (kD / 4) + 255) / 256;
-    launch_pdl(cross_join_kernel<kD>, dim3(static_cast<unsigned>(blocks < 16ll * sm_count() ? blocks : 16ll * sm_count())), dim3(256), 0, stream, p, out);
-  }
+  if (p.mask)
+    if (const cudaError_t err = launch_pdl(cross_live_kernel, dim3(p.B), dim3(256), 0, stream, p)) return static_cast<int>(err);
+  constexpr int smem = Fwd<kD>::TOTAL + 1024;
+  if (const cudaError_t err = allow_smem<cross_fwd_kernel<kD>>(smem, true)) return static_cast<int>(err);
+  if (const cudaError_t err = launch_pdl(cross_fwd_kernel<kD>, dim3(f.ctas), dim3(kFwdThreads), static_cast<size_t>(smem), stream, tq, tk, tv, p, out)) return static_cast<int>(err);
+  if (!f.whole)
+    if (const cudaError_t err = launch_pdl(cross_join_kernel<kD>, dim3(f.ctas, ceil_div((p.R < 128 ? p.R : 128) * kD, 1024)), dim3(256), 0, stream, p, out, f.ctas)) return static_cast<int>(err);
   return static_cast<int>(cudaGetLastError());
-}
-
-// Floats of the backward pass's workspace: D, the parts' sums, and bytes of block states.
-struct BwdSpace {
-  long long D, state, part_q, part_k, part_v, total;
-};
-BwdSpace bwd_space(const CrossParams& p, int D, int parts_q, int parts_k) {
-  const auto round = [](long long n) { return (n + 31) / 32 * 32; };
-  const long long q_rows = static_cast<long long>(p.B) * p.Hq * p.R, k_rows = static_cast<long long>(p.B) * p.Hk * p.Sk;
-  BwdSpace s;
-  s.D = 0;
-  s.state = round(q_rows);
-  s.part_q = s.state + (p.mask ? round((static_cast<long long>(p.B) * ceil_div(p.Sk, kKeys) + 3) / 4) : 0);
-  s.part_k = s.part_q + (parts_q > 1 ? parts_q * q_rows * D : 0);
-  s.part_v = s.part_k + (parts_k > 1 ? parts_k * k_rows * D : 0);
-  s.total = s.part_v + (parts_k > 1 ? parts_k * k_rows * D : 0);
-  return s;
 }
 
 template <int kD>
@@ -1198,44 +1555,32 @@ int cross_bwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   if (!e) e = make_tmap_rows(&tv, a.v, kD, 1, a.Sk, a.Hk, a.B, a.v_strides[0], a.v_strides[1], a.v_strides[2]);
   if (!e) e = make_tmap_rows(&tdo, a.d_o, kD, pack, a.Sq, p.Hq, a.B, a.do_strides[0], a.do_strides[1], a.do_strides[2]);
   if (e) return e;
-  BwdOut out = {};
-  bwd_parts(p, out.parts_q, out.parts_k);
-  const BwdSpace space = bwd_space(p, kD, out.parts_q, out.parts_k);
   if (!a.workspace || !a.stats) return -3;
-  float* D = a.workspace + space.D;
-  uint8_t* state = p.mask ? reinterpret_cast<uint8_t*>(a.workspace + space.state) : nullptr;
+  const BwdPlan f = plan_bwd(p, kD);
+  BwdOut out = {};
+  float* D = a.workspace;
   out.stats = a.stats;
   out.D = D;
-  out.state = state;
-  out.part_q = a.workspace + space.part_q;
-  out.part_k = a.workspace + space.part_k;
-  out.part_v = a.workspace + space.part_v;
+  out.left = reinterpret_cast<Left*>(a.workspace + f.left);
+  out.part = a.workspace + f.part;
   out.dq = static_cast<__nv_bfloat16*>(a.dq);
   out.dk = static_cast<__nv_bfloat16*>(a.dk);
   out.dv = static_cast<__nv_bfloat16*>(a.dv);
   out.qsb = a.dq_strides[0]; out.qss = a.dq_strides[1]; out.qsh = a.dq_strides[2];
   out.ksb = a.dk_strides[0]; out.kss = a.dk_strides[1]; out.ksh = a.dk_strides[2];
-  out.row_tiles = ceil_div(p.R, 128);
-  out.key_blocks = ceil_div(p.Sk, 128);
-  const long long rows = static_cast<long long>(p.B) * p.Hq * p.R;
-  const long long key_items = static_cast<long long>(out.key_blocks) * p.Hk * p.B * out.parts_k, items = key_items + static_cast<long long>(out.row_tiles) * p.Hq * p.B * out.parts_q;
-  if (items > 0x7fffffffll) return -4;
-  out.key_items = static_cast<int>(key_items);
-  const long long want = (rows * (kD / 8) + 255) / 256;
-  const int row_blocks = static_cast<int>(want < 16ll * sm_count() ? want : 16ll * sm_count());
-  const long long state_blocks = state ? (static_cast<long long>(p.B) * out.key_blocks + 7) / 8 : 0;
-  if (state_blocks > 0x3fffffffll) return -4;
-  launch_pdl(cross_pre_kernel<kD>, dim3(row_blocks + static_cast<unsigned>(state_blocks)), dim3(256), 0, stream, p, static_cast<const __nv_bfloat16*>(a.o), a.o_strides[0], a.o_strides[1],
-             a.o_strides[2], static_cast<const __nv_bfloat16*>(a.d_o), a.do_strides[0], a.do_strides[1], a.do_strides[2], D, state, row_blocks);
+  out.key_ctas = f.key_ctas;
+  out.whole_keys = f.whole_keys;
+  out.whole_rows = f.whole_rows;
+  const long long want = (static_cast<long long>(p.B) * p.Hq * p.R * (kD / 8) + 255) / 256, most = 16ll * sm_count();
+  if (const cudaError_t err = launch_pdl(cross_pre_kernel<kD>, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(256), 0, stream, p, static_cast<const __nv_bfloat16*>(a.o), a.o_strides[0],
+                                         a.o_strides[1], a.o_strides[2], static_cast<const __nv_bfloat16*>(a.d_o), a.do_strides[0], a.do_strides[1], a.do_strides[2], D))
+    return static_cast<int>(err);
   constexpr int smem = Bwd<kD>::TOTAL + 1024;
   if (const cudaError_t err = allow_smem<cross_bwd_kernel<kD>>(smem)) return static_cast<int>(err);
-  if (const cudaError_t err = launch_pdl(cross_bwd_kernel<kD>, dim3(static_cast<unsigned>(items)), dim3(kBwdThreads), static_cast<size_t>(smem), stream, tq, tk, tv, tdo,
-                                         p, out))
-    return static_cast<int>(err);
-  if (out.parts_q > 1 || out.parts_k > 1) {
-    const long long sum_rows = (out.parts_q > 1 ? rows : 0) + (out.parts_k > 1 ? 2ll * p.B * p.Hk * p.Sk : 0), blocks = (sum_rows * (kD / 4) + 255) / 256;
-    launch_pdl(cross_sum_kernel<kD>, dim3(static_cast<unsigned>(blocks < 16ll * sm_count() ? blocks : 16ll * sm_count())), dim3(256), 0, stream, p, out);
-  }
+  const int ctas = f.key_ctas + f.row_ctas;
+  if (const cudaError_t err = launch_pdl(cross_bwd_kernel<kD>, dim3(ctas), dim3(kBwdThreads), static_cast<size_t>(smem), stream, tq, tk, tv, tdo, p, out)) return static_cast<int>(err);
+  if (!f.whole_keys || !f.whole_rows)
+    if (const cudaError_t err = launch_pdl(cross_sum_kernel<kD>, dim3(ctas, kD / 8), dim3(256), 0, stream, p, out, ctas)) return static_cast<int>(err);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -1249,14 +1594,9 @@ extern "C" long long fb_cross_workspace(const fb_cross_args* args, int backward)
   CrossParams p = {};
   int pack;
   if (!make_cross(*args, p, pack)) return -4;
-  if (backward) {
-    int parts_q, parts_k;
-    bwd_parts(p, parts_q, parts_k);
-    return bwd_space(p, args->D, parts_q, parts_k).total;
-  }
-  const long long parts = fwd_parts(p), rows = static_cast<long long>(p.B) * p.Hq * p.R;
-  return parts > 1 ? (parts * rows * 2 + 3) / 4 * 4 + parts * rows * args->D : 0;
+  return backward ? plan_bwd(p, args->D).total : plan_fwd(p, args->D).total;
 }
+extern "C" long long fb_cross_mask_info(const fb_cross_args* args) { return args->mask ? args->B * (2ll + (args->Sk + 127ll) / 128) : 0; }
 
 extern "C" int fb_cross_attn_fwd(const fb_cross_args* args, void* stream) {
   using namespace fb;
@@ -1264,7 +1604,7 @@ extern "C" int fb_cross_attn_fwd(const fb_cross_args* args, void* stream) {
   CrossParams p = {};
   int pack;
   if (!make_cross(a, p, pack)) return -4;
-  if (!rows_ok(a.q, a.q_strides) || !rows_ok(a.k, a.k_strides) || !rows_ok(a.v, a.v_strides) || !rows_ok(a.o, a.o_strides)) return -3;
+  if (!rows_ok(a.q, a.q_strides) || !rows_ok(a.k, a.k_strides) || !rows_ok(a.v, a.v_strides) || !rows_ok(a.o, a.o_strides) || (a.mask && !a.mask_info)) return -3;
   const auto s = static_cast<cudaStream_t>(stream);
   return a.D == 64 ? cross_fwd<64>(a, p, pack, s) : cross_fwd<128>(a, p, pack, s);
 }
@@ -1276,7 +1616,7 @@ extern "C" int fb_cross_attn_bwd(const fb_cross_args* args, void* stream) {
   int pack;
   if (!make_cross(a, p, pack)) return -4;
   if (!rows_ok(a.q, a.q_strides) || !rows_ok(a.k, a.k_strides) || !rows_ok(a.v, a.v_strides) || !rows_ok(a.o, a.o_strides) || !rows_ok(a.d_o, a.do_strides) ||
-      !rows_ok(a.dq, a.dq_strides) || !rows_ok(a.dk, a.dk_strides) || !rows_ok(a.dv, a.dk_strides))
+      !rows_ok(a.dq, a.dq_strides) || !rows_ok(a.dk, a.dk_strides) || !rows_ok(a.dv, a.dk_strides) || (a.mask && !a.mask_info))
     return -3;
   const auto s = static_cast<cudaStream_t>(stream);
   return a.D == 64 ? cross_bwd<64>(a, p, pack, s) : cross_bwd<128>(a, p, pack, s);

@@ -275,8 +275,9 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const fb_rotary_args p
   }
 }
 
+// (No read-only loads: they may answer from lines that were in L1 before the kernel before this one wrote them.)
 // dw[seg][column] = sum over the blocks' partial sums: 32 columns a block, 32 threads to a column.
-__global__ void __launch_bounds__(1024) rotary_dw_kernel(const float* __restrict__ partial, float* dwq, float* dwk, const int blocks, const int D) {
+__global__ void __launch_bounds__(1024) rotary_dw_kernel(const float* partial, float* dwq, float* dwk, const int blocks, const int D) {
   __shared__ float s[32][33];
   pdl_entry();
   const int col = blockIdx.x * 32 + (threadIdx.x & 31), first = threadIdx.x >> 5;
