@@ -280,7 +280,9 @@ Tensor launch_cross(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, 
     a.stats = stats->data_ptr<float>();
   }
   if (mask.defined()) {
-    *info = at::empty({fb_cross_mask_info(&a)}, at::TensorOptions().dtype(at::kInt).device(q.device()));
+    const long long n = fb_cross_mask_info(&a);
+    TORCH_CHECK(n > 0, "fb_cross_mask_info: rejected arguments");
+    *info = at::empty({n}, at::TensorOptions().dtype(at::kInt).device(q.device()));
     a.mask_info = info->data_ptr<int>();
   }
   const Tensor space = space_for(a, false, q);

@@ -31,10 +31,27 @@ namespace {
 constexpr int kKeys = 128;                  // keys of a block
 constexpr float kHuge = 1.2676506e30f;      // 2^100
 
+// Quotients by a number of the launch, for n < 2^31: n / d = (high word of n m + n) >> l with m = ceil(2^(32 + l) / d) - 2^32, l = ceil(log2 d) (Granlund and Montgomery).
+// A division by a variable is some 35 instructions, which a CTA meets once, out of a cold instruction cache, while nothing else can start.
+struct Div {
+  unsigned m, d;
+  int l;
+  __device__ int operator()(int n) const { return static_cast<int>((__umulhi(static_cast<unsigned>(n), m) + static_cast<unsigned>(n)) >> l); }
+};
+Div div_by(long long d) {
+  Div r;
+  r.d = static_cast<unsigned>(d < 1 ? 1 : d);
+  r.l = 0;
+  while ((1ull << r.l) < r.d) ++r.l;
+  r.m = static_cast<unsigned>((((1ull << r.l) - r.d) << 32) / r.d + 1);
+  return r;
+}
+
 struct CrossParams {
   int B, Hq, Hk, R, Sk;             // Hq = H / pack rows of heads; R = Sq * pack rows each
   int pack_log2, per_kv;            // log2 of pack; rows of heads that share a key head
   int row_tiles, key_blocks;        // of a row of heads; of a key head
+  Div by_row_tiles, by_per_kv, by_key_blocks;
   const void* mask;                 // [B, Sk]: one byte a key (0: absent), or fp32 addends; null: none
   long long mask_stride;
   int mask_bool;
@@ -117,6 +134,199 @@ __device__ __forceinline__ int block_state(const CrossParams& p, int b, int blk,
   return !any ? 0 : all && !p.table ? 2 : 1;
 }
 
+// What an earlier kernel of the stream wrote is read past L1, and never with read-only loads (ld.global.nc), which may answer from a line that was there before.
+__device__ __forceinline__ int live_of(const CrossParams& p, int b) { return p.live_count ? __ldcg(p.live_count + b) : p.key_blocks; }
+// Live block i of a batch row: {block, whether it goes by the table}.
+__device__ __forceinline__ int2 live_block(const CrossParams& p, int b, int i) {
+  if (p.live) {
+    const int v = __ldcg(p.live + static_cast<long long>(b) * p.key_blocks + i);
+    return make_int2(v >> 1, v & 1);
+  }
+  return make_int2(i, p.table || (i + 1) * kKeys > p.Sk);
+}
+
+// Waits, whatever the block's state, until the copies counted by `bar` have landed: shared memory may not be left while one is on its way to it.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+  for (uint32_t it = 0; it < (1u << 20) && !mbar_test(bar, parity); ++it) __nanosleep(20);
+}
+
+// A whole warp's wait. Most find the phase already over, and a plain test says so in a quarter of the time (26 cycles against 98 of the waiting loop).
+// The loop is one function: inlined at every wait it would more than double the code that a CTA fetches.
+__device__ __noinline__ bool warp_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  return warp_wait(bar, parity, abort_flag, status, code);
+}
+__device__ __forceinline__ bool warp_ready(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
+  return warp_wait_long(bar, parity, abort_flag, status, code);
+}
+
+// A place in a ring of kN stages, and the parity of its turn.
+template <int kN>
+struct Ring {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ void next() {
+    if (++stage == kN) {
+      stage = 0;
+      parity ^= 1;
+    }
+  }
+};
+
+// ---- who does what. Tiles go batch row by batch row.
+struct Place {
+  int b, tile, i;
+};
+struct Run {
+  int b, tile, i0, i1, n;        // a tile's units [i0, i1) of n
+};
+// kKeyTiles: a tile is a live block of a key head, and the rows of its rows of heads stream past it; otherwise it is 128 rows of a row of heads, and live blocks do.
+template <bool kKeyTiles>
+__device__ __forceinline__ int tiles_of(const CrossParams& p, int live) { return kKeyTiles ? p.Hk * live : live ? p.Hq * p.row_tiles : 0; }
+template <bool kKeyTiles>
+__device__ __forceinline__ int length_of(const CrossParams& p, int live) { return kKeyTiles ? p.per_kv * p.row_tiles : live; }
+
+// A CTA's share: tiles c, c + CTAs, ... , `waves` of them, then the stretch [begin, end) of the tiles left.
+struct Share {
+  int waves;
+  Place begin, end;
+};
+// The CTAs of one kind. Without a mask the numbers here say each one's share; with one, the batch rows' live blocks do.
+struct Crew {
+  int ctas, whole;               // whole: stretches begin and end with tiles
+  int waves, first, each, more;  // the first tile of the stretches; their units, and how many of them have one more
+  Div by_ctas, by_length, by_tiles;      // (of a tile, and of a batch row, without a mask)
+};
+// The batch row into which u falls, and what of u is left there, where a batch row of n live blocks holds of(n). By a whole warp; {B, 0} past the last.
+struct InRow {
+  int b, live, left;
+};
+template <typename Of>
+__device__ __forceinline__ InRow row_of(const CrossParams& p, unsigned long long u, int lane, Of of) {
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int n = b0 + lane < p.B ? live_of(p, b0 + lane) : 0;
+    const unsigned long long mine = of(n);
+    unsigned long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, u < upto);
+    if (past) {
+      const int k = __ffs(past) - 1;
+      return {b0 + k, __shfl_sync(0xffffffffu, n, k), static_cast<int>(u - __shfl_sync(0xffffffffu, upto - mine, k))};
+    }
+    u -= __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return {p.B, 0, 0};
+}
+template <bool kKeyTiles>
+__device__ __forceinline__ Share share_of(const CrossParams& p, const Crew& crew, int cta, int lane) {
+  Share s;
+  if (!p.live_count) {
+    s.waves = crew.waves;
+    const int len = length_of<kKeyTiles>(p, p.key_blocks), per_b = tiles_of<kKeyTiles>(p, p.key_blocks);
+#pragma unroll 1
+    for (int k = 0; k < 2; ++k) {
+      const int u = crew.each * (cta + k) + min(cta + k, crew.more);
+      int tile = crew.by_length(u), i = u - tile * len;
+      if (crew.whole && i > 0) {
+        ++tile;
+        i = 0;
+      }
+      tile += crew.first;
+      const int b = crew.by_tiles(tile);
+      (k ? s.end : s.begin) = {b, tile - b * per_b, i};
+    }
+    return s;
+  }
+  const unsigned heads = static_cast<unsigned>(p.Hq) * p.row_tiles;        // units of a live block
+  const auto tiles = [&](int n) { return static_cast<unsigned long long>(tiles_of<kKeyTiles>(p, n)); };
+  const auto units = [&](int n) { return static_cast<unsigned long long>(n) * heads; };
+  int live = 0, total = 0;
+  for (int b = lane; b < p.B; b += 32) {
+    const int n = live_of(p, b);
+    live += n;
+    total += tiles_of<kKeyTiles>(p, n);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    live += __shfl_xor_sync(0xffffffffu, live, o);
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+  }
+  s.waves = crew.by_ctas(total);
+  const int first = s.waves * crew.ctas;
+  const unsigned long long all = units(live);
+  unsigned long long from = 0;        // units ahead of the first tile of the stretches
+  if (first > 0) {
+    from = all;
+    const InRow at = row_of(p, first, lane, tiles);
+    if (at.b < p.B) {
+      int before = 0;
+      for (int b = lane; b < at.b; b += 32) before += live_of(p, b);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+      from = units(before) + static_cast<unsigned long long>(at.left) * length_of<kKeyTiles>(p, at.live);
+    }
+  }
+  const int rest = static_cast<int>(all - from), each = crew.by_ctas(rest), more = rest - each * crew.ctas;        // (less than a tile for each CTA)
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    const InRow in = row_of(p, from + static_cast<unsigned>(each * (cta + k) + min(cta + k, more)), lane, units);
+    Place at = {in.b, 0, 0};
+    if (at.b < p.B) {
+      const int len = length_of<kKeyTiles>(p, in.live);
+      at.tile = static_cast<unsigned>(in.left) / static_cast<unsigned>(len);
+      at.i = in.left - at.tile * len;
+      if (crew.whole && at.i > 0) {
+        at.i = 0;
+        if (++at.tile == tiles_of<kKeyTiles>(p, in.live)) {
+          at.tile = 0;
+          do ++at.b;
+          while (at.b < p.B && live_of(p, at.b) == 0);
+        }
+      }
+    }
+    (k ? s.end : s.begin) = at;
+  }
+  return s;
+}
+// The runs of a share, one after the other, by a whole warp.
+template <bool kKeyTiles>
+struct Walk {
+  Place at, end;
+  int waves, tile, step;
+  __device__ Walk(const Share& s, int first, int ctas) : at(s.begin), end(s.end), waves(s.waves), tile(first), step(ctas) {}
+  __device__ bool next(const CrossParams& p, const Crew& crew, Run& r, int lane) {
+    if (waves > 0) {
+      InRow in;
+      if (!p.live_count) {
+        in.b = crew.by_tiles(tile);
+        in.live = p.key_blocks;
+        in.left = tile - in.b * tiles_of<kKeyTiles>(p, p.key_blocks);
+      } else {
+        in = row_of(p, tile, lane, [&](int n) { return static_cast<unsigned long long>(tiles_of<kKeyTiles>(p, n)); });
+      }
+      const int n = length_of<kKeyTiles>(p, in.live);
+      r = {in.b, in.left, 0, n, n};
+      tile += step;
+      --waves;
+      return true;
+    }
+    if (at.b > end.b || (at.b == end.b && (at.tile > end.tile || (at.tile == end.tile && at.i >= end.i)))) return false;
+    const int live = live_of(p, at.b), n = length_of<kKeyTiles>(p, live);
+    r = {at.b, at.tile, at.i, at.b == end.b && at.tile == end.tile ? end.i : n, n};
+    at.i = 0;
+    if (++at.tile == tiles_of<kKeyTiles>(p, live)) {
+      at.tile = 0;
+      do ++at.b;
+      while (at.b < p.B && live_of(p, at.b) == 0);
+    }
+    return true;
+  }
+};
+
 // One block a batch row: its live blocks in their order, then the others, and its largest addend.
 __global__ void __launch_bounds__(256) cross_live_kernel(const CrossParams p) {
   __shared__ int state[256], warp_live[8];
@@ -165,178 +375,6 @@ __global__ void __launch_bounds__(256) cross_live_kernel(const CrossParams p) {
 
 // What an earlier kernel of the stream wrote is read with plain loads or past L1. A read-only load (ld.global.nc) may answer from a line that was in L1 before the earlier
 // kernel wrote it: with programmatic launches that happened about once in 10^4 calls.
-// Live blocks of the batch rows: null without a mask, a copy in shared memory of up to kCounts, p.live_count otherwise.
-constexpr int kCounts = 512;
-__device__ __forceinline__ int live_of(const CrossParams& p, const int* counts, int b) { return counts ? *reinterpret_cast<const volatile int*>(counts + b) : p.key_blocks; }
-__device__ __forceinline__ const int* counts_of(const CrossParams& p, int* copy) {
-  if (!p.live_count || p.B > kCounts) return p.live_count;
-  for (int b = threadIdx.x; b < p.B; b += blockDim.x) copy[b] = __ldcg(p.live_count + b);
-  return copy;
-}
-// Live block i of a batch row: {block, whether it goes by the table}.
-__device__ __forceinline__ int2 live_block(const CrossParams& p, int b, int i) {
-  if (p.live) {
-    const int v = __ldcg(p.live + static_cast<long long>(b) * p.key_blocks + i);
-    return make_int2(v >> 1, v & 1);
-  }
-  return make_int2(i, p.table || (i + 1) * kKeys > p.Sk);
-}
-
-// Waits, whatever the block's state, until the copies counted by `bar` have landed: shared memory may not be left while one is on its way to it.
-__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
-  for (uint32_t it = 0; it < (1u << 20) && !mbar_test(bar, parity); ++it) __nanosleep(20);
-}
-
-// A whole warp's wait. Most find the phase already over, and a plain test says so in a quarter of the time (26 cycles against 98 of the waiting loop).
-__device__ __forceinline__ bool warp_ready(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
-  if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
-  return warp_wait(bar, parity, abort_flag, status, code);
-}
-
-// A place in a ring of kN stages, and the parity of its turn.
-template <int kN>
-struct Ring {
-  int stage = 0;
-  uint32_t parity = 0;
-  __device__ void next() {
-    if (++stage == kN) {
-      stage = 0;
-      parity ^= 1;
-    }
-  }
-};
-
-// ---- who does what. Tiles go batch row by batch row.
-struct Place {
-  int b, tile, i;
-};
-struct Run {
-  int b, tile, i0, i1, n;        // a tile's units [i0, i1) of n
-};
-// kKeyTiles: a tile is a live block of a key head, and the rows of its rows of heads stream past it; otherwise it is 128 rows of a row of heads, and live blocks do.
-template <bool kKeyTiles>
-__device__ __forceinline__ int tiles_of(const CrossParams& p, const int* counts, int b) {
-  const int n = live_of(p, counts, b);
-  return kKeyTiles ? p.Hk * n : n ? p.Hq * p.row_tiles : 0;
-}
-template <bool kKeyTiles>
-__device__ __forceinline__ int length_of(const CrossParams& p, const int* counts, int b) { return kKeyTiles ? p.per_kv * p.row_tiles : live_of(p, counts, b); }
-
-// A CTA's share: tiles `first`, `first` + CTAs, ... , `waves` of them, then the stretch [begin, end).
-struct Share {
-  int waves;
-  Place begin, end;
-};
-// The batch row in which `u` falls, counted in what `of` gives each, from batch row `b` on; u is left as what remains of it there. By a whole warp.
-template <typename Of>
-__device__ __forceinline__ int row_of(const CrossParams& p, int b, unsigned& u, int lane, Of of) {
-  for (; b < p.B; b += 32) {
-    const unsigned mine = b + lane < p.B ? of(b + lane) : 0;
-    unsigned upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += v;
-    }
-    const unsigned past = __ballot_sync(0xffffffffu, u < upto);
-    if (past) {
-      const int k = __ffs(past) - 1;
-      u -= __shfl_sync(0xffffffffu, upto - mine, k);
-      return b + k;
-    }
-    u -= __shfl_sync(0xffffffffu, upto, 31);
-  }
-  return p.B;
-}
-// By a whole warp.
-template <bool kKeyTiles>
-__device__ __forceinline__ Share share_of(const CrossParams& p, const int* counts, int cta, int ctas, bool whole, int lane) {
-  const auto tiles = [&](int b) { return static_cast<unsigned>(tiles_of<kKeyTiles>(p, counts, b)); };
-  const auto units = [&](int b) { return tiles(b) * static_cast<unsigned>(length_of<kKeyTiles>(p, counts, b)); };
-  unsigned total, tile, rest;
-  int b0;
-  if (!counts) {
-    const unsigned per_b = tiles(0);
-    total = p.B * per_b;
-    tile = total / ctas * ctas;
-    b0 = tile / per_b;
-    rest = (total - tile) * static_cast<unsigned>(length_of<kKeyTiles>(p, counts, 0));        // (less than a tile for each CTA: 32 bits hold the units)
-    tile -= b0 * per_b;
-  } else {
-    total = 0;
-    for (int b = lane; b < p.B; b += 32) total += tiles(b);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    tile = total / ctas * ctas;
-    b0 = row_of(p, 0, tile, lane, tiles);
-    rest = 0;
-    for (int b = b0 + lane; b < p.B; b += 32) rest += units(b);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
-    if (b0 < p.B) rest -= tile * length_of<kKeyTiles>(p, counts, b0);
-  }
-  // the place that is so many units behind the start of tile (b0, tile), or at the next start of a tile from there
-  const auto border = [&](int k) -> Place {
-    unsigned u = static_cast<unsigned>(static_cast<unsigned long long>(rest) * k / ctas);
-    int b = b0;
-    if (b >= p.B) return {p.B, 0, 0};
-    u += tile * length_of<kKeyTiles>(p, counts, b);
-    if (!counts) {
-      const unsigned per_b = units(0), n = u / per_b;
-      b += n;
-      u -= n * per_b;
-    } else {
-      b = row_of(p, b, u, lane, units);
-    }
-    if (b >= p.B) return {p.B, 0, 0};
-    const unsigned len = length_of<kKeyTiles>(p, counts, b);
-    Place at = {b, static_cast<int>(u / len), static_cast<int>(u % len)};
-    if (whole && at.i > 0) {
-      at.i = 0;
-      if (++at.tile == static_cast<int>(tiles(b))) {
-        at.tile = 0;
-        do ++at.b;
-        while (at.b < p.B && live_of(p, counts, at.b) == 0);
-      }
-    }
-    return at;
-  };
-  return {static_cast<int>(total / ctas), border(cta), border(cta + 1)};
-}
-// The runs of a share, one after the other.
-template <bool kKeyTiles>
-struct Walk {
-  const int* counts;
-  Place at;
-  int waves, tile, b = 0, step;
-  __device__ Walk(const int* counts, const Share& s, int first, int ctas) : counts(counts), at(s.begin), waves(s.waves), tile(first), step(ctas) {}
-  __device__ bool next(const CrossParams& p, const Place& end, Run& r) {
-    if (waves > 0) {
-      if (!counts) {
-        const int n = tiles_of<kKeyTiles>(p, counts, 0), k = tile / n;
-        b += k;
-        tile -= k * n;
-      } else {
-        for (int n; tile >= (n = tiles_of<kKeyTiles>(p, counts, b)); ++b) tile -= n;
-      }
-      const int n = length_of<kKeyTiles>(p, counts, b);
-      r = {b, tile, 0, n, n};
-      tile += step;
-      --waves;
-      return true;
-    }
-    if (at.b > end.b || (at.b == end.b && (at.tile > end.tile || (at.tile == end.tile && at.i >= end.i)))) return false;
-    const int n = length_of<kKeyTiles>(p, counts, at.b);
-    r = {at.b, at.tile, at.i, at.b == end.b && at.tile == end.tile ? end.i : n, n};
-    at.i = 0;
-    if (++at.tile == tiles_of<kKeyTiles>(p, counts, at.b)) {
-      at.tile = 0;
-      do ++at.b;
-      while (at.b < p.B && live_of(p, counts, at.b) == 0);
-    }
-    return true;
-  }
-};
 // A run as the warp that loads works it out and hands it to the others, two ahead at most: what the others would keep in registers through their loops, or divide for, they
 // read from here when they need it.
 struct Task {
@@ -347,8 +385,19 @@ struct Task {
   float base;                   // of the mask
 };
 template <bool kKeyTiles>
-__device__ __forceinline__ Task task_of(const CrossParams& p, const int* counts, const Run& r) {
-  const int per = kKeyTiles ? live_of(p, counts, r.b) : p.row_tiles, h = r.tile / per, tile = r.tile - h * per;
+__device__ __forceinline__ Task task_of(const CrossParams& p, const Run& r) {
+  int h, per;
+  if (!kKeyTiles) {
+    per = p.row_tiles;
+    h = p.by_row_tiles(r.tile);
+  } else if (!p.live_count) {
+    per = p.key_blocks;
+    h = p.by_key_blocks(r.tile);
+  } else {
+    per = live_of(p, r.b);
+    h = r.tile / per;
+  }
+  const int tile = r.tile - h * per;
   const int2 at = kKeyTiles ? live_block(p, r.b, tile) : make_int2(tile, 0);
   const bool whole = r.i0 == 0 && r.i1 == r.n;
   return {1, r.b, h, at.x, r.i0, r.i1, whole, r.i0 > 0 ? 0 : 1, r.i1 == r.n, r.tile, at.y, p.base ? __ldcg(p.base + r.b) : 0.f};
@@ -437,8 +486,7 @@ struct Fwd {
   static constexpr int V = K + kStages * kTile;
   static constexpr int TAB = V + kStages * kTile;        // 2 x 128 x {scale, addend}
   static constexpr int BARS = TAB + 2 * 128 * 8;
-  static constexpr int COUNTS = BARS + 512;
-  static constexpr int TOTAL = COUNTS + kCounts * 4;
+  static constexpr int TOTAL = BARS + 512;
   // Columns of TMEM. With 128 values a head P takes the place of the scores that it is made from.
   static constexpr uint32_t S = 0, P = kD == 64 ? 128 : 0, O = kD == 64 ? 192 : 128;
 };
@@ -462,7 +510,7 @@ struct FwdOut {
   Left* left;                  // [CTAs][2]
   float* part_o;               // [CTAs][2][128][D] sums relative to the part's maximum
   float2* part_ml;             // ... [128] {maximum, sum}
-  int whole;                   // stretches begin and end with tiles
+  Crew crew;
 };
 
 template <int kD>
@@ -505,15 +553,11 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   tc_fence_after_sync();
   const uint32_t tmem = bar.tmem_slot;
   pdl_entry();       // behind the allocation: the next kernel's may not come before it
-  const int* counts = counts_of(p, reinterpret_cast<int*>(smem + L::COUNTS));
-  if (counts) __syncthreads();
   const uint32_t sQ = smem_u32(smem + L::Q), sK = smem_u32(smem + L::K), sV = smem_u32(smem + L::V);
 
   if (warp == 5) {
     // ------------------------------------------------------------------ loads
-    const Share share = share_of<false>(p, counts, blockIdx.x, gridDim.x, out.whole, lane);
-    Walk<false> walk(counts, share, blockIdx.x, gridDim.x);
-    const Place end = share.end;
+    Walk<false> walk(share_of<false>(p, out.crew, blockIdx.x, lane), blockIdx.x, gridDim.x);
     Run r;
     Ring<2> rt;
     Ring<kS> ring;
@@ -521,11 +565,11 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     bool ok = true;
     while (ok) {
       Task task = {};
-      if (walk.next(p, end, r)) task = task_of<false>(p, counts, r);
+      if (walk.next(p, out.crew, r, lane)) task = task_of<false>(p, r);
       ok = hand_out(bar.tasks, rt.stage, rt.parity, task, abort_flag, p.status, lane);
       rt.next();
       if (!ok || !task.valid) break;
-      const int hk = task.h / p.per_kv;
+      const int hk = p.by_per_kv(task.h);
       ok = warp_ready(&bar.q_empty, (runs & 1) ^ 1, abort_flag, p.status, kStatusWaitEmpty);
       if (!ok) break;
       if (elect_one()) {
@@ -766,14 +810,14 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       arrive_warp(&bar.tasks.empty[rt.stage], lane);
       rt.next();
     }
-    if (t == 0 && !out.whole) {
+    if (t == 0 && !out.crew.whole) {
       out.left[blockIdx.x * 2] = bar.left[0];
       out.left[blockIdx.x * 2 + 1] = bar.left[1];
     }
     // batch rows without a key: zeros
-    if (counts)
+    if (p.live_count)
       for (int b = blockIdx.x; b < p.B; b += gridDim.x)
-        if (live_of(p, counts, b) == 0)
+        if (live_of(p, b) == 0)
           for (long long e = t; e < static_cast<long long>(p.Hq) * p.R * (kD / 8); e += 128) {
             const int c = static_cast<int>(e % (kD / 8)), row = static_cast<int>(e / (kD / 8) % p.R), h = static_cast<int>(e / (kD / 8) / p.R);
             *reinterpret_cast<uint4*>(out_row(p, out.o, out.osb, out.oss, out.osh, b, h, row) + c * 8) = make_uint4(0u, 0u, 0u, 0u);
@@ -866,8 +910,7 @@ struct Bwd {
   static constexpr int RING = 2 * kTile;                           // A's tiles, then B's
   static constexpr int TAB = RING + (kD == 64 ? 6 : 4) * kTile;    // 3 x 256 floats
   static constexpr int BARS = TAB + 3 * 1024;
-  static constexpr int COUNTS = BARS + 512;
-  static constexpr int TOTAL = COUNTS + kCounts * 4;
+  static constexpr int TOTAL = BARS + 512;
   // Columns of TMEM: one more buffer of scores where the accumulators leave room for it.
   static constexpr uint32_t S = 0, DP = 128, ACC0 = 256, ACC1 = 256 + kD;
   static constexpr uint32_t S2_KEYS = 384, S2_ROWS = kD == 64 ? 384 : 256;
@@ -882,7 +925,8 @@ struct BwdOut {
   long long qsb, qss, qsh, ksb, kss, ksh;
   Left* left;                      // [CTAs][2]
   float* part;                     // [CTAs][2][128][D], of the CTAs of keys twice that: dK, then dV
-  int key_ctas, whole_keys, whole_rows;
+  int key_ctas;
+  Crew keys, rows;
 };
 
 // P of 32 columns of a thread's scores, as fp32 in `pr` and, for keys, as bf16 in TMEM: P = 2^(mul s - l), with l of the thread's row or, where the columns are rows, -l of `tb`.
@@ -1029,30 +1073,28 @@ __device__ __forceinline__ void bwd_products(BwdBars& bar, const CrossParams& p,
 }
 
 template <int kD, bool kKeys>
-__device__ __forceinline__ void bwd_loads(BwdBars& bar, const CrossParams& p, const int* counts, int key_ctas, bool whole, uint32_t smem, const void* f0, const void* f1, const void* a, const void* b) {
+__device__ __forceinline__ void bwd_loads(BwdBars& bar, const CrossParams& p, const Crew& crew, int first, uint32_t smem, const void* f0, const void* f1, const void* a, const void* b) {
   using L = Bwd<kD>;
   constexpr int kA = L::stages_a(kKeys), kB = L::stages_b(kKeys);
   volatile int* abort_flag = &bar.abort_flag;
   Ring<kA> ra;
   Ring<kB> rb;
   int as = 0, bs = 0, runs = 0;
-  const int first = kKeys ? blockIdx.x : blockIdx.x - key_ctas, ctas = kKeys ? key_ctas : gridDim.x - key_ctas;
-  const Share share = share_of<kKeys>(p, counts, first, ctas, whole, threadIdx.x & 31);
-  Walk<kKeys> walk(counts, share, first, ctas);
-  const Place end = share.end;
+  const int lane = threadIdx.x & 31;
+  Walk<kKeys> walk(share_of<kKeys>(p, crew, first, lane), first, crew.ctas);
   Run r;
   Ring<2> rt;
-  const int lane = threadIdx.x & 31;
   bool ok = true;
   while (ok) {
     Task task = {};
-    if (walk.next(p, end, r)) task = task_of<kKeys>(p, counts, r);
+    if (walk.next(p, crew, r, lane)) task = task_of<kKeys>(p, r);
     ok = hand_out(bar.tasks, rt.stage, rt.parity, task, abort_flag, p.status, lane);
     rt.next();
     if (!ok || !task.valid) break;
     // keys: the tile is a live block of a key head, whose rows of heads' rows stream; rows: 128 rows of a row of heads, and its key head's blocks stream
     const int h = task.h, at0 = kKeys ? task.at * 128 : (task.at * 128) >> p.pack_log2;
-    int head = kKeys ? h * p.per_kv + r.i0 / p.row_tiles : h / p.per_kv, row = kKeys ? r.i0 % p.row_tiles : 0;
+    const int past = kKeys ? p.by_row_tiles(r.i0) : 0;
+    int head = kKeys ? h * p.per_kv + past : p.by_per_kv(h), row = kKeys ? r.i0 - past * p.row_tiles : 0;
     ok = warp_ready(&bar.f_empty, (runs & 1) ^ 1, abort_flag, p.status, kStatusWaitEmpty);
     if (!ok) break;
     if (elect_one()) {
@@ -1107,7 +1149,8 @@ __device__ __forceinline__ void bwd_tables(BwdBars& bar, const CrossParams& p, f
     rt.next();
     if (!r.valid) return;
     const float base = r.base, shift = kKeys && !r.masked ? base : 0.f;        // keys with nothing added are `base` below the largest
-    int head = kKeys ? r.h * p.per_kv + r.i0 / p.row_tiles : 0, row = kKeys ? r.i0 % p.row_tiles : 0;
+    const int past = kKeys ? p.by_row_tiles(r.i0) : 0;
+    int head = kKeys ? r.h * p.per_kv + past : 0, row = kKeys ? r.i0 - past * p.row_tiles : 0;
     for (int i = r.i0; i < r.i1; ++i) {
       float* tb = tab + ra.stage * 256;
       float2 v[4];
@@ -1335,13 +1378,11 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   tc_fence_after_sync();
   const uint32_t tmem = bar.tmem_slot;
   pdl_entry();
-  const int* counts = counts_of(p, reinterpret_cast<int*>(smem + L::COUNTS));
-  if (counts) __syncthreads();
   const uint32_t base = smem_u32(smem);
 
   if (warp == kBwdSoftmaxWarps + 1) {
-    if (keys) bwd_loads<kD, true>(bar, p, counts, out.key_ctas, out.whole_keys, base, &tmK, &tmV, &tmQ, &tmDO);
-    else bwd_loads<kD, false>(bar, p, counts, out.key_ctas, out.whole_rows, base, &tmQ, &tmDO, &tmK, &tmV);
+    if (keys) bwd_loads<kD, true>(bar, p, out.keys, blockIdx.x, base, &tmK, &tmV, &tmQ, &tmDO);
+    else bwd_loads<kD, false>(bar, p, out.rows, blockIdx.x - out.key_ctas, base, &tmQ, &tmDO, &tmK, &tmV);
   } else if (warp == kBwdSoftmaxWarps + 2) {
     if (keys) bwd_tables<kD, true>(bar, p, tab, out.stats, out.D, lane);
     else bwd_tables<kD, false>(bar, p, tab, out.stats, out.D, lane);
@@ -1355,11 +1396,11 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       out.left[blockIdx.x * 2] = bar.left[0];
       out.left[blockIdx.x * 2 + 1] = bar.left[1];
     }
-    if (counts) {
+    if (p.live_count) {
       // what nothing streams past: blocks without a key, and the rows of batch rows without one, get zeros
       constexpr int kThreads = 32 * kBwdSoftmaxWarps, kVecs = kD / 8;
       for (long long x = blockIdx.x; x < static_cast<long long>(p.B) * p.key_blocks; x += gridDim.x) {
-        const int b = static_cast<int>(x / p.key_blocks), i = static_cast<int>(x % p.key_blocks), n = live_of(p, counts, b);
+        const int b = static_cast<int>(x / p.key_blocks), i = static_cast<int>(x % p.key_blocks), n = live_of(p, b);
         if (i < n) continue;
         const int key0 = live_block(p, b, i).x * 128;
         for (int e = threadIdx.x; e < 128 * p.Hk * kVecs; e += kThreads) {
@@ -1422,7 +1463,7 @@ __global__ void __launch_bounds__(256) cross_sum_kernel(const CrossParams p, con
   const Left first = out.left[cta * 2 + 1];
   if (!first.used) return;
   const int sharing = sharers(out.left, cta, keys ? out.key_ctas : ctas, with, &count);
-  const int per = keys ? live_of(p, p.live_count, first.b) : p.row_tiles, h = first.tile / per, tile = first.tile - h * per;
+  const int per = keys ? live_of(p, first.b) : p.row_tiles, h = first.tile / per, tile = first.tile - h * per;
   const int c = (threadIdx.x % kLanes) * 4, t = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes;
   const int n = (keys ? live_block(p, first.b, tile).x : tile) * 128 + t;
   if (n >= (keys ? p.Sk : p.R)) return;
@@ -1459,6 +1500,9 @@ bool make_cross(const fb_cross_args& a, CrossParams& p, int& pack) {
   p.Sk = a.Sk;
   p.row_tiles = ceil_div(p.R, 128);
   p.key_blocks = ceil_div(p.Sk, kKeys);
+  p.by_row_tiles = div_by(p.row_tiles);
+  p.by_per_kv = div_by(p.per_kv);
+  p.by_key_blocks = div_by(p.key_blocks);
   // tiles are counted in 32 bits, and so are the units of one for each CTA
   if (static_cast<long long>(p.B) * p.Hq * p.row_tiles > 0x3fffffffll || static_cast<long long>(p.B) * p.Hk * p.key_blocks > 0x3fffffffll ||
       static_cast<long long>(p.per_kv) * p.row_tiles > 0x7fffff || p.key_blocks > 0x7fffff)
@@ -1479,40 +1523,50 @@ bool make_cross(const fb_cross_args& a, CrossParams& p, int& pack) {
 
 // CTAs for `units` of work over tiles of `length`, at most `most`, and whether their stretches hold whole tiles only. Tiles of up to four units are not cut: what is left of
 // one costs about as much as a unit. Otherwise a stretch is two units at least.
-int stretches(long long units, int length, int most, int& whole) {
-  whole = length <= 4;
-  const long long n = whole ? units / length : (units + 1) / 2;
+Crew crew_of(const CrossParams& p, int tiles, int length, int most) {        // tiles of all batch rows, without a mask
+  Crew c = {};
   if (most > kWith) most = kWith;
-  return static_cast<int>(n < most ? n : most);
+  c.whole = length <= 4;
+  const long long units = static_cast<long long>(tiles) * length, n = c.whole ? tiles : (units + 1) / 2;
+  c.ctas = static_cast<int>(n < most ? n : most);
+  c.waves = tiles / c.ctas;
+  c.first = c.waves * c.ctas;
+  const long long rest = static_cast<long long>(tiles - c.first) * length;
+  c.each = static_cast<int>(rest / c.ctas);
+  c.more = static_cast<int>(rest % c.ctas);
+  c.by_ctas = div_by(c.ctas);
+  c.by_length = div_by(length);
+  c.by_tiles = div_by(tiles / p.B);
+  return c;
 }
-struct FwdPlan {
-  int ctas, whole;
-  long long left, ml, o, total;        // places in the workspace, in floats
+// A unit of keys takes four products and a unit of rows three: 2450 and 2070 cycles (heads of 64), 3400 and 2250 (128).
+struct Crews {
+  Crew rows, bwd_keys, bwd_rows;
 };
-FwdPlan plan_fwd(const CrossParams& p, int D) {
-  FwdPlan f = {};
-  f.ctas = stretches(static_cast<long long>(p.B) * p.Hq * p.row_tiles * p.key_blocks, p.key_blocks, 2 * sm_count(), f.whole);
-  if (f.whole) return f;
-  f.ml = round_up(f.ctas * 2ll * 4, 32);
-  f.o = f.ml + f.ctas * 2ll * 128 * 2;
-  f.total = f.o + f.ctas * 2ll * 128 * D;
+Crews crews_of(const CrossParams& p, int D) {
+  const int row_tiles = p.B * p.Hq * p.row_tiles, sms = sm_count(), most_keys = D == 64 ? sms * 54 / 100 : sms * 60 / 100;
+  return {crew_of(p, row_tiles, p.key_blocks, 2 * sms), crew_of(p, p.B * p.Hk * p.key_blocks, p.per_kv * p.row_tiles, most_keys), crew_of(p, row_tiles, p.key_blocks, sms - most_keys)};
+}
+// The forward pass's places in its workspace, in floats.
+struct FwdSpace {
+  long long ml, o, total;
+};
+FwdSpace space_fwd(const Crew& c, int D) {
+  FwdSpace f = {};
+  if (c.whole) return f;
+  f.ml = round_up(c.ctas * 2ll * 4, 32);
+  f.o = f.ml + c.ctas * 2ll * 128 * 2;
+  f.total = f.o + c.ctas * 2ll * 128 * D;
   return f;
 }
-struct BwdPlan {
-  int key_ctas, row_ctas, whole_keys, whole_rows;
-  long long D, left, part, total;
+struct BwdSpace {
+  long long left, part, total;
 };
-BwdPlan plan_bwd(const CrossParams& p, int D) {
-  BwdPlan f = {};
-  const long long units = static_cast<long long>(p.B) * p.Hq * p.row_tiles * p.key_blocks;
-  // A unit of keys takes four products and a unit of rows three: 2450 and 2070 cycles (heads of 64), 3400 and 2250 (128).
-  const int most_keys = D == 64 ? sm_count() * 54 / 100 : sm_count() * 60 / 100;
-  f.key_ctas = stretches(units, p.per_kv * p.row_tiles, most_keys, f.whole_keys);
-  f.row_ctas = stretches(units, p.key_blocks, sm_count() - most_keys, f.whole_rows);
+BwdSpace space_bwd(const CrossParams& p, const Crews& c, int D) {
+  BwdSpace f = {};
   f.left = round_up(static_cast<long long>(p.B) * p.Hq * p.R, 32);
-  f.part = f.left + round_up((f.key_ctas + f.row_ctas) * 2ll * 4, 32);
-  f.total = f.part + (f.key_ctas * 4ll + f.row_ctas * 2ll) * 128 * D;
-  if (f.whole_keys && f.whole_rows) f.total = f.part;
+  f.part = f.left + round_up((c.bwd_keys.ctas + c.bwd_rows.ctas) * 2ll * 4, 32);
+  f.total = f.part + (c.bwd_keys.whole && c.bwd_rows.whole ? 0 : (c.bwd_keys.ctas * 4ll + c.bwd_rows.ctas * 2ll) * 128 * D);
   return f;
 }
 
@@ -1523,7 +1577,8 @@ int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   if (!e) e = make_tmap_rows(&tk, a.k, kD, 1, a.Sk, a.Hk, a.B, a.k_strides[0], a.k_strides[1], a.k_strides[2]);
   if (!e) e = make_tmap_rows(&tv, a.v, kD, 1, a.Sk, a.Hk, a.B, a.v_strides[0], a.v_strides[1], a.v_strides[2]);
   if (e) return e;
-  const FwdPlan f = plan_fwd(p, kD);
+  const Crews crews = crews_of(p, kD);
+  const FwdSpace f = space_fwd(crews.rows, kD);
   if (f.total && !a.workspace) return -3;
   FwdOut out = {};
   out.o = static_cast<__nv_bfloat16*>(a.o);
@@ -1531,8 +1586,8 @@ int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   out.oss = a.o_strides[1];
   out.osh = a.o_strides[2];
   out.stats = a.stats;
-  out.whole = f.whole;
-  if (!f.whole) {
+  out.crew = crews.rows;
+  if (!out.crew.whole) {
     out.left = reinterpret_cast<Left*>(a.workspace);
     out.part_ml = reinterpret_cast<float2*>(a.workspace + f.ml);
     out.part_o = a.workspace + f.o;
@@ -1541,9 +1596,9 @@ int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
     if (const cudaError_t err = launch_pdl(cross_live_kernel, dim3(p.B), dim3(256), 0, stream, p)) return static_cast<int>(err);
   constexpr int smem = Fwd<kD>::TOTAL + 1024;
   if (const cudaError_t err = allow_smem<cross_fwd_kernel<kD>>(smem, true)) return static_cast<int>(err);
-  if (const cudaError_t err = launch_pdl(cross_fwd_kernel<kD>, dim3(f.ctas), dim3(kFwdThreads), static_cast<size_t>(smem), stream, tq, tk, tv, p, out)) return static_cast<int>(err);
-  if (!f.whole)
-    if (const cudaError_t err = launch_pdl(cross_join_kernel<kD>, dim3(f.ctas, ceil_div((p.R < 128 ? p.R : 128) * kD, 1024)), dim3(256), 0, stream, p, out, f.ctas)) return static_cast<int>(err);
+  if (const cudaError_t err = launch_pdl(cross_fwd_kernel<kD>, dim3(out.crew.ctas), dim3(kFwdThreads), static_cast<size_t>(smem), stream, tq, tk, tv, p, out)) return static_cast<int>(err);
+  if (!out.crew.whole)
+    if (const cudaError_t err = launch_pdl(cross_join_kernel<kD>, dim3(out.crew.ctas, ceil_div((p.R < 128 ? p.R : 128) * kD, 1024)), dim3(256), 0, stream, p, out, out.crew.ctas)) return static_cast<int>(err);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -1556,7 +1611,8 @@ int cross_bwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   if (!e) e = make_tmap_rows(&tdo, a.d_o, kD, pack, a.Sq, p.Hq, a.B, a.do_strides[0], a.do_strides[1], a.do_strides[2]);
   if (e) return e;
   if (!a.workspace || !a.stats) return -3;
-  const BwdPlan f = plan_bwd(p, kD);
+  const Crews crews = crews_of(p, kD);
+  const BwdSpace f = space_bwd(p, crews, kD);
   BwdOut out = {};
   float* D = a.workspace;
   out.stats = a.stats;
@@ -1568,18 +1624,18 @@ int cross_bwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   out.dv = static_cast<__nv_bfloat16*>(a.dv);
   out.qsb = a.dq_strides[0]; out.qss = a.dq_strides[1]; out.qsh = a.dq_strides[2];
   out.ksb = a.dk_strides[0]; out.kss = a.dk_strides[1]; out.ksh = a.dk_strides[2];
-  out.key_ctas = f.key_ctas;
-  out.whole_keys = f.whole_keys;
-  out.whole_rows = f.whole_rows;
+  out.keys = crews.bwd_keys;
+  out.rows = crews.bwd_rows;
+  out.key_ctas = out.keys.ctas;
   const long long want = (static_cast<long long>(p.B) * p.Hq * p.R * (kD / 8) + 255) / 256, most = 16ll * sm_count();
   if (const cudaError_t err = launch_pdl(cross_pre_kernel<kD>, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(256), 0, stream, p, static_cast<const __nv_bfloat16*>(a.o), a.o_strides[0],
                                          a.o_strides[1], a.o_strides[2], static_cast<const __nv_bfloat16*>(a.d_o), a.do_strides[0], a.do_strides[1], a.do_strides[2], D))
     return static_cast<int>(err);
   constexpr int smem = Bwd<kD>::TOTAL + 1024;
   if (const cudaError_t err = allow_smem<cross_bwd_kernel<kD>>(smem)) return static_cast<int>(err);
-  const int ctas = f.key_ctas + f.row_ctas;
+  const int ctas = out.keys.ctas + out.rows.ctas;
   if (const cudaError_t err = launch_pdl(cross_bwd_kernel<kD>, dim3(ctas), dim3(kBwdThreads), static_cast<size_t>(smem), stream, tq, tk, tv, tdo, p, out)) return static_cast<int>(err);
-  if (!f.whole_keys || !f.whole_rows)
+  if (!out.keys.whole || !out.rows.whole)
     if (const cudaError_t err = launch_pdl(cross_sum_kernel<kD>, dim3(ctas, kD / 8), dim3(256), 0, stream, p, out, ctas)) return static_cast<int>(err);
   return static_cast<int>(cudaGetLastError());
 }
@@ -1594,9 +1650,17 @@ extern "C" long long fb_cross_workspace(const fb_cross_args* args, int backward)
   CrossParams p = {};
   int pack;
   if (!make_cross(*args, p, pack)) return -4;
-  return backward ? plan_bwd(p, args->D).total : plan_fwd(p, args->D).total;
+  const Crews crews = crews_of(p, args->D);
+  return backward ? space_bwd(p, crews, args->D).total : space_fwd(crews.rows, args->D).total;
 }
-extern "C" long long fb_cross_mask_info(const fb_cross_args* args) { return args->mask ? args->B * (2ll + (args->Sk + 127ll) / 128) : 0; }
+extern "C" long long fb_cross_mask_info(const fb_cross_args* args) {
+  using namespace fb;
+  CrossParams p = {};
+  int pack;
+  if (!make_cross(*args, p, pack)) return -4;
+  if (!p.mask) return 0;
+  return p.B * (2ll + p.key_blocks);
+}
 
 extern "C" int fb_cross_attn_fwd(const fb_cross_args* args, void* stream) {
   using namespace fb;
