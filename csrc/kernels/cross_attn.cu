@@ -14,7 +14,8 @@
 // Work. A unit is a tile of 128 rows that stays with 128 of what streams past it. As many CTAs as fit the GPU take whole tiles as long as there is one for each of them, side by
 // side, so that they stream the same heads out of L2 (with one stretch of all units for each CTA, as long heads of 128 took 287 us against 241). What is left, less
 // than a tile each, is cut into equal stretches of units: no last wave, and few queries over many keys fill the GPU as well. A tile that a stretch's border cuts leaves
-// fp32 sums behind, which a small second launch adds up in the order of the stretches (two calls give the same bits).
+// fp32 sums behind, which a small second launch adds up in the order of the stretches (two calls give the same bits). Where the forward pass has few tiles, the CTAs of a
+// cluster share each of them instead and meet in distributed shared memory, which saves that launch.
 //
 // Statistics, sums and products are fp32; P and dS are rounded to bf16 once, as operands of the tensor cores.
 #include <cuda.h>
@@ -449,6 +450,9 @@ __device__ __forceinline__ void zero_row(uint32_t tile, int rows, int row) {
     for (int g = 0; g < 8; ++g) st_shared_v4(tile + c * rows * 128 + row * 128 + g * 16, make_uint4(0u, 0u, 0u, 0u));
 }
 
+// Operands' descriptors. `base` is an offset into the CTA's own memory (in_own): in a cluster an address carries the CTA's number from bit 24 on, which would fall into the
+// descriptor's other fields.
+__device__ __forceinline__ uint32_t in_own(uint32_t smem) { return smem & 0x3FFFFu; }
 __device__ __forceinline__ uint64_t k_desc(uint32_t base, int bytes) { return desc_of(smem_desc_lo(base, 16) + (bytes >> 4), smem_desc_hi(1024)); }
 __device__ __forceinline__ uint64_t mn_desc(uint32_t base, int bytes, int lbo) { return desc_of(smem_desc_lo(base, lbo) + (bytes >> 4), smem_desc_hi(1024)); }
 
@@ -511,7 +515,62 @@ struct FwdOut {
   float* part_o;               // [CTAs][2][128][D] sums relative to the part's maximum
   float2* part_ml;             // ... [128] {maximum, sum}
   Crew crew;
+  int parts;                   // CTAs of a cluster, which share a tile; 0: no clusters
+  Div by_parts;
 };
+
+// 16-byte chunk c of row t of a tile of fp32 sums in shared memory: a warp's rows, which write the same chunk at a time, meet different banks.
+template <int kD>
+__device__ __forceinline__ uint32_t shared_chunk(int t, int c) { return (t * (kD / 4) + (c ^ (t & 15))) * 16; }
+__device__ __forceinline__ uint32_t in_cta(uint32_t smem, int cta) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem), "r"(cta));
+  return remote;
+}
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_v2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_meet() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The CTAs of a cluster join their parts of a tile, four values a thread, in the order of the parts; each CTA every so manieth group of rows. All threads of all of them,
+// whatever became of the waits before.
+template <int kD>
+__device__ __forceinline__ void join_cluster(const CrossParams& p, const FwdOut& out, const FwdBars& bar, uint32_t sums, uint32_t ml) {
+  cluster_meet();
+  constexpr int kLanes = kD / 4, kRows = kFwdThreads / kLanes;
+  const Task& task = bar.tasks.task[0];
+  const int k0 = blockIdx.x - out.by_parts(blockIdx.x) * out.parts, row0 = task.at * 128, rows = min(128, p.R - row0);
+  const int c = threadIdx.x % kLanes;
+  for (int t = k0 * kRows + threadIdx.x / kLanes; t < rows; t += out.parts * kRows) {
+    float m = -INFINITY;
+#pragma unroll 4
+    for (int k = 0; k < out.parts; ++k) m = fmaxf(m, ld_cluster_v2(in_cta(ml + t * 8, k)).x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = 0; k < out.parts; ++k) {
+      const float2 x = ld_cluster_v2(in_cta(ml + t * 8, k));
+      const float4 v = ld_cluster_v4(in_cta(sums + shared_chunk<kD>(t, c), k));
+      const float w = ex2_approx(x.x - ref);
+      l += w * x.y;
+      acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(out_row(p, out.o, out.osb, out.oss, out.osh, task.b, task.h, row0 + t) + c * 4) = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
+    if (out.stats && c == 0) out.stats[(static_cast<long long>(task.b) * p.Hq + task.h) * p.R + row0 + t] = l == 0.f ? INFINITY : m + log2f(l);
+  }
+  cluster_meet();        // shared memory is there until all have read it
+}
 
 template <int kD>
 __global__ void __launch_bounds__(kFwdThreads, 2)
@@ -557,7 +616,9 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
   if (warp == 5) {
     // ------------------------------------------------------------------ loads
-    Walk<false> walk(share_of<false>(p, out.crew, blockIdx.x, lane), blockIdx.x, gridDim.x);
+    Share share = {};
+    if (!out.parts) share = share_of<false>(p, out.crew, blockIdx.x, lane);
+    Walk<false> walk(share, blockIdx.x, gridDim.x);
     Run r;
     Ring<2> rt;
     Ring<kS> ring;
@@ -565,7 +626,20 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     bool ok = true;
     while (ok) {
       Task task = {};
-      if (walk.next(p, out.crew, r, lane)) task = task_of<false>(p, r);
+      if (out.parts) {
+        if (runs == 0) {
+          const int tile = out.by_parts(blockIdx.x), k = blockIdx.x - tile * out.parts;
+          r.b = out.crew.by_tiles(tile);
+          r.tile = tile - r.b * p.Hq * p.row_tiles;
+          r.n = live_of(p, r.b);
+          r.i0 = out.by_parts(r.n * k);
+          r.i1 = out.by_parts(r.n * (k + 1));
+          task = task_of<false>(p, r);
+          task.whole = 0;
+        }
+      } else if (walk.next(p, out.crew, r, lane)) {
+        task = task_of<false>(p, r);
+      }
       ok = hand_out(bar.tasks, rt.stage, rt.parity, task, abort_flag, p.status, lane);
       rt.next();
       if (!ok || !task.valid) break;
@@ -578,7 +652,8 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       }
       __syncwarp();
       ++runs;
-      int2 next = live_block(p, r.b, r.i0);
+      int2 next = make_int2(0, 0);
+      if (r.i0 < r.i1) next = live_block(p, r.b, r.i0);
       for (int i = r.i0; i < r.i1; ++i) {
         const int key0 = next.x * kKeys;
         if (i + 1 < r.i1) next = live_block(p, r.b, i + 1);
@@ -617,7 +692,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < kD / 16; ++k)
-          umma_bf16<1>(tmem + L::S, k_desc(sQ, (k >> 2) * 16384 + (k & 3) * 32), k_desc(sK + rk.stage * L::kTile, (k >> 2) * 16384 + (k & 3) * 32), idesc_s, k > 0);
+          umma_bf16<1>(tmem + L::S, k_desc(in_own(sQ), (k >> 2) * 16384 + (k & 3) * 32), k_desc(in_own(sK) + rk.stage * L::kTile, (k >> 2) * 16384 + (k & 3) * 32), idesc_s, k > 0);
         umma_commit(&bar.s_full);
         umma_commit(&bar.k_empty[rk.stage]);
       }
@@ -629,7 +704,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const int n = bar.tasks.task[rt.stage].i1 - bar.tasks.task[rt.stage].i0;
       arrive_warp(&bar.tasks.empty[rt.stage], lane);
       rt.next();
-      ok = warp_ready(&bar.q_full, runs & 1, abort_flag, p.status, kStatusWaitFull) && scores();
+      ok = warp_ready(&bar.q_full, runs & 1, abort_flag, p.status, kStatusWaitFull) && (n == 0 || scores());
       ++runs;
       for (int i = 0; i < n && ok; ++i, ++it) {
         // Where P has a place of its own the next scores may come under this block's exponentials, otherwise right behind the product that reads P: a CTA's products
@@ -643,7 +718,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         tc_fence_after_sync();
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 128 / 16; ++k) umma_bf16_ts(tmem + L::O, tmem + L::P + k * 8, mn_desc(sV + rv.stage * L::kTile, k * 2048, 16384), idesc_o, i > 0 || k > 0);
+          for (int k = 0; k < 128 / 16; ++k) umma_bf16_ts(tmem + L::O, tmem + L::P + k * 8, mn_desc(in_own(sV) + rv.stage * L::kTile, k * 2048, 16384), idesc_o, i > 0 || k > 0);
           umma_commit(&bar.pv_done);
           umma_commit(&bar.v_empty[rv.stage]);
         }
@@ -669,7 +744,8 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const int b = task.b, i0 = task.i0, i1 = task.i1;
       const bool works = warp * 32 < p.R - task.at * 128;        // a warp without rows only keeps step
       float m = -INFINITY, l = 0.f;               // the maximum the accumulator is relative to, and the sum
-      int2 next = live_block(p, b, i0);
+      int2 next = make_int2(0, 0);
+      if (i0 < i1) next = live_block(p, b, i0);
       for (int i = i0; i < i1; ++i, ++it) {
         const int2 blk = next;
         if (i + 1 < i1) next = live_block(p, b, i + 1);
@@ -765,24 +841,33 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       // ---- the run's rows
       const bool whole = task.whole;
       const int h = task.h, row0 = task.at * 128, rows = min(128, p.R - row0);
-      ok = ok && warp_ready(&bar.pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);
+      if (i0 < i1) ok = ok && warp_ready(&bar.pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);
       if (!whole && t == 0) bar.left[task.slot] = Left{1, task.ends, b, task.tile};
       if (ok && works) {
         tc_fence_after_sync();
         const long long row = (static_cast<long long>(b) * p.Hq + h) * p.R + row0 + t, slot = blockIdx.x * 2ll + task.slot;
         const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
-        if (!whole) out.part_ml[slot * 128 + t] = make_float2(m, l);
+        if (out.parts) tab[t] = make_float2(m, l);
+        else if (!whole) out.part_ml[slot * 128 + t] = make_float2(m, l);
         // a row that no key takes part in: +inf, which makes every probability 2^-inf = 0
         else if (out.stats && t < rows) out.stats[row] = l == 0.f ? INFINITY : m + log2f(l);
         float* po = whole ? nullptr : out.part_o + (slot * 128 + t) * kD;
 #pragma unroll
         for (int c0 = 0; c0 < kD; c0 += 32) {
           uint32_t v[32];
-          tmem_ld32_sync(tmem + L::O + lanes + c0, v);
+          if (i0 < i1) {
+            tmem_ld32_sync(tmem + L::O + lanes + c0, v);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0u;
+          }
           float f[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(v[e]) * inv;
-          if (whole) {       // through the warp's 4 KB of each of Q's panels, which every product has read
+          if (out.parts) {       // where K and V were, as `shared_chunk` says
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) st_shared_v4(sK + shared_chunk<kD>(t, (c0 + e) / 4), make_uint4(__float_as_uint(f[e]), __float_as_uint(f[e + 1]), __float_as_uint(f[e + 2]), __float_as_uint(f[e + 3])));
+          } else if (whole) {       // through the warp's 4 KB of each of Q's panels, which every product has read
             stage_half(sQ + (c0 >> 6) * 16384 + warp * 4096, lane, c0 & 32, f);
           } else {
 #pragma unroll
@@ -810,7 +895,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       arrive_warp(&bar.tasks.empty[rt.stage], lane);
       rt.next();
     }
-    if (t == 0 && !out.crew.whole) {
+    if (t == 0 && !out.parts && !out.crew.whole) {
       out.left[blockIdx.x * 2] = bar.left[0];
       out.left[blockIdx.x * 2 + 1] = bar.left[1];
     }
@@ -824,6 +909,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (out.stats && c == 0) out.stats[(static_cast<long long>(b) * p.Hq + h) * p.R + row] = INFINITY;
           }
   }
+  if (out.parts) join_cluster<kD>(p, out, bar, sK, smem_u32(tab));
   tc_fence_before_sync();
   __syncthreads();
   if (warp == 4) {
@@ -1551,9 +1637,19 @@ Crews crews_of(const CrossParams& p, int D) {
 struct FwdSpace {
   long long ml, o, total;
 };
-FwdSpace space_fwd(const Crew& c, int D) {
+// CTAs of a cluster to share a tile: as many as there is room for, of two blocks at least; 0 where tiles are short or many, or where a stretch would be so much
+// shorter that it pays for its second launch (about as long as four units).
+int parts_of(const CrossParams& p) {
+  const long long tiles = static_cast<long long>(p.B) * p.Hq * p.row_tiles, slots = 2ll * sm_count();
+  if (p.key_blocks <= 4 || tiles * 2 > slots) return 0;
+  long long c = slots / tiles;
+  if (c > p.key_blocks / 2) c = p.key_blocks / 2;
+  if (c > 8) c = 8;        // (clusters of sixteen find room on few SMs at a time: one token over 32768 keys 94 us against 62 in stretches)
+  return ceil_div(p.key_blocks, c) > tiles * p.key_blocks / slots + 4 ? 0 : static_cast<int>(c);
+}
+FwdSpace space_fwd(const CrossParams& p, const Crew& c, int D) {
   FwdSpace f = {};
-  if (c.whole) return f;
+  if (c.whole || parts_of(p)) return f;
   f.ml = round_up(c.ctas * 2ll * 4, 32);
   f.o = f.ml + c.ctas * 2ll * 128 * 2;
   f.total = f.o + c.ctas * 2ll * 128 * D;
@@ -1570,6 +1666,25 @@ BwdSpace space_bwd(const CrossParams& p, const Crews& c, int D) {
   return f;
 }
 
+// Like launch_pdl, in clusters.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_clusters(void (*kern)(KArgs...), int blocks, int cluster, int threads, size_t smem, cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
 template <int kD>
 int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream_t stream) {
   CUtensorMap tq, tk, tv;
@@ -1578,7 +1693,7 @@ int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   if (!e) e = make_tmap_rows(&tv, a.v, kD, 1, a.Sk, a.Hk, a.B, a.v_strides[0], a.v_strides[1], a.v_strides[2]);
   if (e) return e;
   const Crews crews = crews_of(p, kD);
-  const FwdSpace f = space_fwd(crews.rows, kD);
+  const FwdSpace f = space_fwd(p, crews.rows, kD);
   if (f.total && !a.workspace) return -3;
   FwdOut out = {};
   out.o = static_cast<__nv_bfloat16*>(a.o);
@@ -1587,7 +1702,9 @@ int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   out.osh = a.o_strides[2];
   out.stats = a.stats;
   out.crew = crews.rows;
-  if (!out.crew.whole) {
+  out.parts = parts_of(p);
+  out.by_parts = div_by(out.parts ? out.parts : 1);
+  if (f.total) {
     out.left = reinterpret_cast<Left*>(a.workspace);
     out.part_ml = reinterpret_cast<float2*>(a.workspace + f.ml);
     out.part_o = a.workspace + f.o;
@@ -1596,6 +1713,11 @@ int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
     if (const cudaError_t err = launch_pdl(cross_live_kernel, dim3(p.B), dim3(256), 0, stream, p)) return static_cast<int>(err);
   constexpr int smem = Fwd<kD>::TOTAL + 1024;
   if (const cudaError_t err = allow_smem<cross_fwd_kernel<kD>>(smem, true)) return static_cast<int>(err);
+  if (out.parts) {
+    const int ctas = p.B * p.Hq * p.row_tiles * out.parts;
+    if (const cudaError_t err = launch_clusters(cross_fwd_kernel<kD>, ctas, out.parts, kFwdThreads, smem, stream, tq, tk, tv, p, out)) return static_cast<int>(err);
+    return static_cast<int>(cudaGetLastError());
+  }
   if (const cudaError_t err = launch_pdl(cross_fwd_kernel<kD>, dim3(out.crew.ctas), dim3(kFwdThreads), static_cast<size_t>(smem), stream, tq, tk, tv, p, out)) return static_cast<int>(err);
   if (!out.crew.whole)
     if (const cudaError_t err = launch_pdl(cross_join_kernel<kD>, dim3(out.crew.ctas, ceil_div((p.R < 128 ? p.R : 128) * kD, 1024)), dim3(256), 0, stream, p, out, out.crew.ctas)) return static_cast<int>(err);
@@ -1651,7 +1773,7 @@ extern "C" long long fb_cross_workspace(const fb_cross_args* args, int backward)
   int pack;
   if (!make_cross(*args, p, pack)) return -4;
   const Crews crews = crews_of(p, args->D);
-  return backward ? space_bwd(p, crews, args->D).total : space_fwd(crews.rows, args->D).total;
+  return backward ? space_bwd(p, crews, args->D).total : space_fwd(p, crews.rows, args->D).total;
 }
 extern "C" long long fb_cross_mask_info(const fb_cross_args* args) {
   using namespace fb;

@@ -95,6 +95,9 @@ def case(B, Sq, Sk, H, Hk, D, seed=0, peak=1.0):
 SHAPES = [  # B, Sq, Sk, H, Hk, D
     (1, 1, 1, 1, 1, 64), (1, 1, 129, 2, 2, 64), (2, 3, 64, 4, 4, 128), (2, 128, 128, 2, 2, 64), (1, 129, 127, 3, 3, 64), (2, 77, 1031, 4, 4, 64),
     (1, 300, 257, 4, 2, 128), (2, 33, 190, 6, 2, 64), (1, 5, 700, 32, 1, 64), (1, 70, 65, 12, 3, 128), (3, 1, 500, 16, 4, 128), (1, 640, 384, 2, 1, 64),
+    (1, 1, 1200, 2, 2, 128), (2, 150, 900, 2, 2, 128), (2, 9, 1300, 4, 4, 64),        # few tiles over several blocks of keys: clusters
+    (1, 2, 4100, 8, 8, 64), (1, 2, 4100, 8, 8, 128),                                  # ... of eight
+    (2, 1, 1400, 160, 80, 64),                                                       # more tiles than clusters for them: stretches
 ]
 
 
