@@ -127,7 +127,7 @@ std::vector<Tensor> launch_turn(const Tensor x_in[2], const Tensor dy_in[2], con
   Tensor w32[2], partial;
   for (int i = 0; i < 2; ++i) {
     if (!w[i].defined()) continue;
-    w32[i] = w[i].detach().to(at::kFloat).contiguous();
+    w32[i] = w[i].scalar_type() == at::kFloat && w[i].is_contiguous() ? w[i] : w[i].detach().to(at::kFloat).contiguous();
     a.weight[i] = w32[i].data_ptr<float>();
   }
   if (c.norm && backward) {
@@ -145,16 +145,12 @@ std::vector<Tensor> launch_turn(const Tensor x_in[2], const Tensor dy_in[2], con
   return out;
 }
 
-void keep(AutogradContext* ctx, const Turn& c) {
-  ctx->saved_data["offset"] = c.offset;
-  ctx->saved_data["interleaved"] = c.interleaved;
-  ctx->saved_data["amplitude"] = c.amplitude;
-  ctx->saved_data["norm"] = c.norm;
-  ctx->saved_data["eps"] = c.eps;
+void keep(AutogradContext* ctx, const Turn& c) {       // one entry: each is a look-up by name
+  ctx->saved_data["turn"] = std::vector<double>{static_cast<double>(c.offset), static_cast<double>(c.interleaved), c.amplitude, static_cast<double>(c.norm), c.eps};
 }
 Turn kept(AutogradContext* ctx) {
-  return {ctx->saved_data["offset"].toInt(), ctx->saved_data["interleaved"].toBool(), ctx->saved_data["amplitude"].toDouble(), ctx->saved_data["norm"].toBool(),
-          ctx->saved_data["eps"].toDouble()};
+  const auto v = ctx->saved_data["turn"].toDoubleVector();
+  return {static_cast<int64_t>(v[0]), v[1] != 0, v[2], v[3] != 0, v[4]};
 }
 
 struct TurnFn : public torch::autograd::Function<TurnFn> {
@@ -218,6 +214,7 @@ Found turn(const Tensor& q, const OptTensor& k_in, const Tensor& freqs_in, const
   for (const Tensor* w : {&wq, &wk})
     if (w->defined() && (w->dim() != 1 || w->size(0) != D || w->device() != q.device() || !w->is_floating_point())) return std::nullopt;
   if (wk.defined() && !packed && !k.defined()) return std::nullopt;
+  if (offset > (1ll << 52) || offset < -(1ll << 52)) return std::nullopt;       // kept as a double
   const Turn c = {offset, interleaved, amplitude, norm, eps};
   const Tensor freqs = freqs_in.contiguous();
   if (records({&q, &k, &wq, &wk})) return TurnFn::apply(q, given(k), given(wq), given(wk), freqs, given(positions), c);

@@ -273,6 +273,23 @@ __device__ __forceinline__ bool fb_index_ok(long long i, long long n, int site) 
   extern "C" int fb_bounds_attach_##name(int*) { return 0; }
 #endif
 
+// ---- division by a number of the launch ----------------------------------------------------------------
+// Quotients by a number of the launch, for n < 2^31: n / d = (high word of n m + n) >> l with m = ceil(2^(32 + l) / d) - 2^32, l = ceil(log2 d) (Granlund and Montgomery).
+// A division by a variable is some 35 instructions, which a block often meets once, out of a cold instruction cache, before anything else can start.
+struct Div {
+  unsigned m, d;
+  int l;
+  __device__ int operator()(int n) const { return static_cast<int>((__umulhi(static_cast<unsigned>(n), m) + static_cast<unsigned>(n)) >> l); }
+};
+inline Div div_by(long long d) {
+  Div r;
+  r.d = static_cast<unsigned>(d < 1 ? 1 : d);
+  r.l = 0;
+  while ((1ull << r.l) < r.d) ++r.l;
+  r.m = static_cast<unsigned>((((1ull << r.l) - r.d) << 32) / r.d + 1);
+  return r;
+}
+
 // ---- programmatic dependent launch -----------------------------------------------------------------
 // A kernel launched with the programmatic-serialization attribute may start while its predecessor
 // in the stream is still running. `pdl_wait()` blocks until the predecessor grid has completed and

@@ -32,22 +32,6 @@ namespace {
 constexpr int kKeys = 128;                  // keys of a block
 constexpr float kHuge = 1.2676506e30f;      // 2^100
 
-// Quotients by a number of the launch, for n < 2^31: n / d = (high word of n m + n) >> l with m = ceil(2^(32 + l) / d) - 2^32, l = ceil(log2 d) (Granlund and Montgomery).
-// A division by a variable is some 35 instructions, which a CTA meets once, out of a cold instruction cache, while nothing else can start.
-struct Div {
-  unsigned m, d;
-  int l;
-  __device__ int operator()(int n) const { return static_cast<int>((__umulhi(static_cast<unsigned>(n), m) + static_cast<unsigned>(n)) >> l); }
-};
-Div div_by(long long d) {
-  Div r;
-  r.d = static_cast<unsigned>(d < 1 ? 1 : d);
-  r.l = 0;
-  while ((1ull << r.l) < r.d) ++r.l;
-  r.m = static_cast<unsigned>((((1ull << r.l) - r.d) << 32) / r.d + 1);
-  return r;
-}
-
 struct CrossParams {
   int B, Hq, Hk, R, Sk;             // Hq = H / pack rows of heads; R = Sq * pack rows each
   int pack_log2, per_kv;            // log2 of pack; rows of heads that share a key head

@@ -10,11 +10,14 @@
 // rounding a pair and token, which the heads share. Several heads are one row each of the same launch: q, k and, of a packed projection, v, which is copied.
 // With the norm a row's items lie in neighbouring lanes, so that its sums are shuffles, and a thread always holds the same columns, so that dw stays in registers;
 // blocks then walk over the tokens, and their partial sums are added up in their order by a second launch (two calls give the same bits).
-// What bounds it: HBM. Every value is read once and written once.
+// What bounds it: without the norm HBM, every value is read once and written once: 34 us for fp32 queries and keys [2, 8191, 12, 64], 5.9 TB/s. With the norm the
+// instructions of an item, some 10 for each value forward and 20 backward, at the warps that its registers leave room for: 2.6 TB/s over both passes at
+// [2, 4096, 32 + 8, 128]. So they come two a piece (packed fp32), weights, sines and cosines in 16-byte loads, and the backward pass's two sums in one round of shuffles.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "../include/flodl_b200.h"
 #include "common.cuh"
@@ -23,7 +26,6 @@ namespace fb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kItems = 4;                 // items a thread has in flight
 constexpr int kMaxTokens = 64;            // of a tile
 
 template <int kBytes> struct RawOf;
@@ -52,82 +54,194 @@ __device__ __forceinline__ void load(Pack<T, kVec>& p, const T* at) { p.raw = *r
 template <typename T, int kVec>
 __device__ __forceinline__ void store(const Pack<T, kVec>& p, T* at) { *reinterpret_cast<decltype(p.raw)*>(at) = p.raw; }
 
-// The two accesses of item i: where they start in the head, and the first of its pairs.
+// The two accesses of item i: where they start in the head, and the first of its pairs. What does not turn is pairs that do not.
 struct ItemAt {
   int a, b, pair;
   bool turns;
 };
-template <int kVec>
-__device__ __forceinline__ ItemAt item_at(int i, int rot, bool interleaved) {
-  const int turning = rot / (2 * kVec);
+template <int kVec, bool kSide>
+__device__ __forceinline__ ItemAt item_at(int i, int rot) {
   ItemAt w;
-  w.turns = i < turning;
+  w.turns = i * 2 * kVec < rot;
   w.pair = i * kVec;
-  const bool side = interleaved || !w.turns;        // neighbours
-  w.a = side ? i * 2 * kVec : i * kVec;
-  w.b = side ? w.a + kVec : w.a + rot / 2;
+  w.a = kSide || !w.turns ? i * 2 * kVec : i * kVec;
+  w.b = kSide || !w.turns ? w.a + kVec : w.a + rot / 2;
   return w;
 }
 
-// The values of an item as pairs (lo[j], hi[j]), and back.
-template <typename T, int kVec>
-__device__ __forceinline__ void unpack(const Pack<T, kVec>& a, const Pack<T, kVec>& b, bool side, float (&lo)[kVec], float (&hi)[kVec]) {
+// The values of an item as pairs (lo[j], hi[j]), and back. kSide: neighbours, pair j is values 2j and 2j + 1 of a and b one after the other.
+template <typename T, int kVec, bool kSide>
+__device__ __forceinline__ void unpack(const Pack<T, kVec>& a, const Pack<T, kVec>& b, float (&lo)[kVec], float (&hi)[kVec]) {
 #pragma unroll
   for (int j = 0; j < kVec; ++j) {
-    // neighbours: pair j is values 2j and 2j + 1 of a and b one after the other
-    const float sl = to_float(2 * j < kVec ? a.v[(2 * j) % kVec] : b.v[(2 * j) % kVec]);
-    const float sh = to_float(2 * j + 1 < kVec ? a.v[(2 * j + 1) % kVec] : b.v[(2 * j + 1) % kVec]);
-    lo[j] = side ? sl : to_float(a.v[j]);
-    hi[j] = side ? sh : to_float(b.v[j]);
+    lo[j] = to_float(!kSide ? a.v[j] : 2 * j < kVec ? a.v[(2 * j) % kVec] : b.v[(2 * j) % kVec]);
+    hi[j] = to_float(!kSide ? b.v[j] : 2 * j + 1 < kVec ? a.v[(2 * j + 1) % kVec] : b.v[(2 * j + 1) % kVec]);
   }
 }
-template <typename T, int kVec>
-__device__ __forceinline__ void pack(Pack<T, kVec>& a, Pack<T, kVec>& b, bool side, const float (&lo)[kVec], const float (&hi)[kVec]) {
+template <typename T, int kVec, bool kSide>
+__device__ __forceinline__ void pack(Pack<T, kVec>& a, Pack<T, kVec>& b, const float (&lo)[kVec], const float (&hi)[kVec]) {
 #pragma unroll
   for (int j = 0; j < kVec; ++j) {
-    a.v[j] = from_float<T>(side ? (j % 2 ? hi[j / 2] : lo[j / 2]) : lo[j]);
-    b.v[j] = from_float<T>(side ? ((kVec + j) % 2 ? hi[(kVec + j) / 2] : lo[(kVec + j) / 2]) : hi[j]);
+    a.v[j] = from_float<T>(!kSide ? lo[j] : j % 2 ? hi[j / 2] : lo[j / 2]);
+    b.v[j] = from_float<T>(!kSide ? hi[j] : (kVec + j) % 2 ? hi[(kVec + j) / 2] : lo[(kVec + j) / 2]);
   }
+}
+// Columns of the values lo[j] and hi[j].
+template <int kVec, bool kSide>
+__device__ __forceinline__ int lo_at(const ItemAt& w, int j) { return kSide ? w.a + 2 * j : w.a + j; }
+template <int kVec, bool kSide>
+__device__ __forceinline__ int hi_at(const ItemAt& w, int j) { return kSide ? w.a + 2 * j + 1 : w.b + j; }
+
+// kN fp32 values in a row of shared memory, in the widest loads.
+template <int kN>
+__device__ __forceinline__ void load_row(const float* at, float (&v)[kN]) {
+  if constexpr (kN % 4 == 0) {
+#pragma unroll
+    for (int j = 0; j < kN; j += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(at + j);
+      v[j] = x.x; v[j + 1] = x.y; v[j + 2] = x.z; v[j + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kN; ++j) v[j] = at[j];
+  }
+}
+// An item's weights, as pairs.
+template <int kVec, bool kSide>
+__device__ __forceinline__ void load_weights(const float* w, const ItemAt& at, float (&lo)[kVec], float (&hi)[kVec]) {
+  float a[kVec], b[kVec];
+  load_row(w + at.a, a);
+  load_row(w + at.b, b);
+#pragma unroll
+  for (int j = 0; j < kVec; ++j) {
+    lo[j] = !kSide ? a[j] : 2 * j < kVec ? a[(2 * j) % kVec] : b[(2 * j) % kVec];
+    hi[j] = !kSide ? b[j] : 2 * j + 1 < kVec ? a[(2 * j + 1) % kVec] : b[(2 * j + 1) % kVec];
+  }
+}
+
+// o = a b + c for kN values, two an instruction.
+template <int kN>
+__device__ __forceinline__ void v_fma(float (&o)[kN], const float (&a)[kN], const float (&b)[kN], const float (&c)[kN]) {
+  if constexpr (kN == 1) {
+    o[0] = fmaf(a[0], b[0], c[0]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kN; j += 2) f2_get(f2_fma(f2_make(a[j], a[j + 1]), f2_make(b[j], b[j + 1]), f2_make(c[j], c[j + 1])), o[j], o[j + 1]);
+  }
+}
+template <int kN>
+__device__ __forceinline__ void v_mul(float (&o)[kN], const float (&a)[kN], const float (&b)[kN]) {
+  if constexpr (kN == 1) {
+    o[0] = a[0] * b[0];
+  } else {
+#pragma unroll
+    for (int j = 0; j < kN; j += 2) f2_get(f2_mul(f2_make(a[j], a[j + 1]), f2_make(b[j], b[j + 1])), o[j], o[j + 1]);
+  }
+}
+template <int kN>
+__device__ __forceinline__ void v_scale(float (&o)[kN], const float (&a)[kN], float s) {
+  if constexpr (kN == 1) {
+    o[0] = a[0] * s;
+  } else {
+#pragma unroll
+    for (int j = 0; j < kN; j += 2) f2_get(f2_mul(f2_make(a[j], a[j + 1]), f2_splat(s)), o[j], o[j + 1]);
+  }
+}
+template <int kN>
+__device__ __forceinline__ float v_sum(const float (&a)[kN]) {
+  float r = a[0];
+#pragma unroll
+  for (int j = 1; j < kN; ++j) r += a[j];
+  return r;
+}
+// Pairs (lo, hi) turned: lo cos - hi sin, hi cos + lo sin.
+template <int kN>
+__device__ __forceinline__ void v_turn(float (&lo)[kN], float (&hi)[kN], const float* cos_at, const float* sin_at) {
+  float c[kN], s[kN], minus[kN], a[kN], b[kN];
+  load_row(cos_at, c);
+  load_row(sin_at, s);
+#pragma unroll
+  for (int j = 0; j < kN; ++j) minus[j] = -s[j];
+  v_mul(a, hi, minus);
+  v_mul(b, lo, s);
+  v_fma(lo, lo, c, a);
+  v_fma(hi, hi, c, b);
+}
+// The sum over a group of neighbouring lanes, a power of two of them.
+__device__ __forceinline__ float group_sum(float v, int group) {
+  if (group > 1) v += __shfl_xor_sync(0xffffffffu, v, 1);
+  if (group > 2) v += __shfl_xor_sync(0xffffffffu, v, 2);
+  if (group > 4) v += __shfl_xor_sync(0xffffffffu, v, 4);
+  if (group > 8) v += __shfl_xor_sync(0xffffffffu, v, 8);
+  if (group > 16) v += __shfl_xor_sync(0xffffffffu, v, 16);
+  return v;
 }
 
 // One item in flight.
 template <typename T, int kVec, bool kBoth>
 struct Item {
-  Pack<T, kVec> xa, xb, da, db;
+  Pack<T, kVec> xa, xb;
+  Pack<T, kBoth ? kVec : 1> da, db;
   T* y;                     // the head's row of the result; null where there is none to do
   short tok, seg;
 };
 
-template <typename T, int kVec, bool kNorm, bool kBwd>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const fb_rotary_args p, const int tokens, const int tile, const int group, const int items) {
-  extern __shared__ float2 turn[];              // [tile][rot / 2] cos and sin, amplitude included
+struct Geometry {
+  Div by_group, by_heads, by_seq, by_pairs;
+  int tokens, tile, group, items, heads;
+  int row;                  // of a token's cosines in shared memory, then its sines: the pairs, rounded up to whole 16-byte accesses
+  float inv_d;
+};
+
+// Items a thread has in flight. With the norm two: its sums and weights take the registers.
+constexpr int items_of(bool norm) { return norm ? 2 : 4; }
+// Times that a block's threads are filled by a tile: a block's start (weights, the barrier behind the angles) is shared by as many, but nothing of
+// the next tile's is in flight meanwhile. With norms, forward and backward of bf16 queries [2, 4096, 32, 128] and keys [2, 4096, 8, 128] took 174, 132, 129 and
+// 143 us with 1, 2, 4 and 8, of a packed [4, 1024, 3, 8, 64] 24.4, 26.1, 21.2 and 21.1. Without, a packed [32, 256, 3, 8, 64] took 27.9, 27.2, 32.7 and 32.7, and the
+// forward pass of fp32 queries and keys [2, 8191, 12, 64] 34.9, 34.2, 36.8 and 40.6.
+constexpr int passes_of(bool norm) { return norm ? 4 : 2; }
+
+template <typename T, int kVec, bool kSide, bool kNorm, bool kBwd>
+__global__ void __launch_bounds__(kThreads, kNorm ? 2 : 3) rotary_kernel(const fb_rotary_args p, const Geometry g) {
+  extern __shared__ __align__(16) float turn[];              // [tile][2][row] cos and sin, amplitude included; with the norm, both weights behind them
   constexpr bool kSums = kNorm && kBwd;
-  const int pairs = p.rot / 2, heads = p.heads[0] + p.heads[1] + p.heads[2];
-  float acc[kSums ? 2 : 1][2 * kVec];
+  constexpr int kItems = items_of(kNorm);
+  const int pairs = p.rot / 2;
+  float* weights = turn + g.tile * 2 * g.row;        // [2][D rounded up to 4]
+  const int w_row = (p.D + 3) / 4 * 4;
+  // with the norm a group is a power of two that divides the threads: the item is the thread's own
+  const int own = kNorm ? threadIdx.x & (g.group - 1) : 0;
+  float acc[kSums ? 4 : 1][kVec];        // dw of queries and of keys: of lo and of hi
   if constexpr (kSums) {
 #pragma unroll
-    for (int j = 0; j < 2 * kVec; ++j) acc[0][j] = acc[1][j] = 0.f;
+    for (int j = 0; j < kVec; ++j) acc[0][j] = acc[1][j] = acc[2][j] = acc[3][j] = 0.f;
   }
   pdl_entry();
-  const int n_tiles = (tokens + tile - 1) / tile;
+  if constexpr (kNorm) {
+    for (int e = threadIdx.x; e < 2 * p.D; e += kThreads) {
+      const float* w = p.weight[e >= p.D];
+      weights[e >= p.D ? w_row + e - p.D : e] = w ? w[e >= p.D ? e - p.D : e] : 1.f;
+    }
+  }
+  const int n_tiles = (g.tokens + g.tile - 1) / g.tile;
   for (int at = blockIdx.x; at < n_tiles; at += gridDim.x) {
-    const int tok0 = at * tile, n_tok = min(tile, tokens - tok0), n = n_tok * heads * group;
+    const int tok0 = at * g.tile, n_tok = min(g.tile, g.tokens - tok0), n = n_tok * g.heads * g.group;
     for (int base = 0; base < n; base += kThreads * kItems) {
       Item<T, kVec, kSums> it[kItems];
 #pragma unroll
       for (int u = 0; u < kItems; ++u) {
-        const int idx = base + u * kThreads + threadIdx.x, row = idx / group, i = idx - row * group;
+        const int idx = base + u * kThreads + threadIdx.x, row = g.by_group(idx), i = kNorm ? own : idx - row * g.group;
         it[u].y = nullptr;
         it[u].seg = 2;
-        if (idx < n && i < items) {
-          const int t = row / heads;
-          int h = row - t * heads;
+        if (idx < n && i < g.items) {
+          const int t = g.by_heads(row);
+          int h = row - t * g.heads;
           int seg = 0;
           if (h >= p.heads[0]) { h -= p.heads[0]; seg = 1; }
           if (seg == 1 && h >= p.heads[1]) { h -= p.heads[1]; seg = 2; }
-          const int b = (tok0 + t) / p.S, s = tok0 + t - b * p.S;
+          const int b = g.by_seq(tok0 + t), s = tok0 + t - b * p.S;
           const long long *xs = p.x_strides[seg], *ds = p.dy_strides[seg], *ys = p.y_strides[seg];
-          const ItemAt w = item_at<kVec>(i, p.rot, p.interleaved != 0);
+          const ItemAt w = item_at<kVec, kSide>(i, p.rot);
           if (!kBwd || (kNorm && seg < 2)) {
             const T* x = static_cast<const T*>(p.x[seg]) + b * xs[0] + s * xs[1] + h * xs[2];
             load(it[u].xa, x + w.a);
@@ -135,8 +249,13 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const fb_rotary_args p
           }
           if constexpr (kBwd) {
             const T* d = static_cast<const T*>(p.dy[seg]) + b * ds[0] + s * ds[1] + h * ds[2];
-            load(it[u].da, d + w.a);
-            load(it[u].db, d + w.b);
+            if constexpr (kNorm) {
+              load(it[u].da, d + w.a);
+              load(it[u].db, d + w.b);
+            } else {
+              load(it[u].xa, d + w.a);
+              load(it[u].xb, d + w.b);
+            }
           }
           it[u].y = static_cast<T*>(p.y[seg]) + b * ys[0] + s * ys[1] + h * ys[2];
           it[u].tok = static_cast<short>(t);
@@ -146,99 +265,96 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const fb_rotary_args p
       if (base == 0) {
         if (at != static_cast<int>(blockIdx.x)) __syncthreads();       // the last tile's have been read
         for (int e = threadIdx.x; e < n_tok * pairs; e += kThreads) {
-          const int t = e / pairs, b = (tok0 + t) / p.S, s = tok0 + t - b * p.S;
+          const int t = g.by_pairs(e), b = g.by_seq(tok0 + t), s = tok0 + t - b * p.S;
           const long long pos = p.positions ? p.positions[b * p.pos_strides[0] + s * p.pos_strides[1]] : s;
           const double turns = static_cast<double>(pos + p.offset) * (p.freqs[e - t * pairs] * 0.15915494309189533577);      // 1 / (2 pi)
           float sn, cs;
           sincospif(2.f * static_cast<float>(turns - rint(turns)), &sn, &cs);
-          turn[e] = make_float2(cs * p.amplitude, (kBwd ? -sn : sn) * p.amplitude);
+          float* to = turn + t * 2 * g.row + e - t * pairs;
+          to[0] = cs * p.amplitude;
+          to[g.row] = (kBwd ? -sn : sn) * p.amplitude;
         }
         __syncthreads();
       }
 #pragma unroll
       for (int u = 0; u < kItems; ++u) {
-        const int idx = base + u * kThreads + threadIdx.x, i = idx % group, seg = it[u].seg;
-        const ItemAt w = item_at<kVec>(i, p.rot, p.interleaved != 0);
-        const bool side = p.interleaved != 0 || !w.turns;
+        const int idx = base + u * kThreads + threadIdx.x, i = kNorm ? own : idx - g.by_group(idx) * g.group, seg = it[u].seg;
+        const ItemAt w = item_at<kVec, kSide>(i, p.rot);
         float lo[kVec], hi[kVec];
+        const float* cos_at = turn + it[u].tok * 2 * g.row + w.pair;
         if constexpr (!kNorm) {
           if (!it[u].y) continue;
-          Pack<T, kVec>&ra = kBwd ? it[u].da : it[u].xa, &rb = kBwd ? it[u].db : it[u].xb;
           if (seg < 2 && w.turns) {
-            unpack(ra, rb, side, lo, hi);
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-              const float2 c = turn[it[u].tok * pairs + w.pair + j];
-              const float a = lo[j];
-              lo[j] = a * c.x - hi[j] * c.y;
-              hi[j] = hi[j] * c.x + a * c.y;
-            }
-            pack(ra, rb, side, lo, hi);
+            unpack<T, kVec, kSide>(it[u].xa, it[u].xb, lo, hi);
+            v_turn(lo, hi, cos_at, cos_at + g.row);
+            pack<T, kVec, kSide>(it[u].xa, it[u].xb, lo, hi);
           }
-          store(ra, it[u].y + w.a);
-          store(rb, it[u].y + w.b);
+          store(it[u].xa, it[u].y + w.a);
+          store(it[u].xb, it[u].y + w.b);
         } else {
           const bool here = it[u].y != nullptr, normed = here && seg < 2;
-          float n_lo[kVec], n_hi[kVec], g_lo[kVec], g_hi[kVec], w_lo[kVec], w_hi[kVec];
+          float x_lo[kVec], x_hi[kVec], w_lo[kVec], w_hi[kVec], t_lo[kVec], t_hi[kVec];
           float sq = 0.f;
           if (normed) {
-            unpack(it[u].xa, it[u].xb, side, n_lo, n_hi);
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) sq += n_lo[j] * n_lo[j] + n_hi[j] * n_hi[j];
-            const float* wt = p.weight[seg];
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-              w_lo[j] = wt ? wt[side ? w.a + 2 * j : w.a + j] : 1.f;
-              w_hi[j] = wt ? wt[side ? w.a + 2 * j + 1 : w.b + j] : 1.f;
-            }
+            unpack<T, kVec, kSide>(it[u].xa, it[u].xb, x_lo, x_hi);
+            v_mul(t_lo, x_lo, x_lo);
+            v_fma(t_lo, x_hi, x_hi, t_lo);
+            sq = v_sum(t_lo);
+            load_weights<kVec, kSide>(weights + (seg == 1 ? w_row : 0), w, w_lo, w_hi);
           }
-          for (int o = group >> 1; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
-          const float r = rsqrtf(sq / p.D + p.eps);
-          float dot = 0.f;
-          if (normed) {
-            if constexpr (kBwd) unpack(it[u].da, it[u].db, side, g_lo, g_hi);
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-              float2 c = make_float2(1.f, 0.f);
-              if (w.turns) c = turn[it[u].tok * pairs + w.pair + j];
-              n_lo[j] *= r;
-              n_hi[j] *= r;
-              if constexpr (!kBwd) {
-                const float a = n_lo[j] * w_lo[j], b = n_hi[j] * w_hi[j];
-                lo[j] = a * c.x - b * c.y;
-                hi[j] = b * c.x + a * c.y;
-              } else {
-                const float a = g_lo[j] * c.x - g_hi[j] * c.y, b = g_hi[j] * c.x + g_lo[j] * c.y;
-                const float da = a * n_lo[j], db = b * n_hi[j];
-                if (seg == 0) {
-                  acc[0][2 * j] += da;
-                  acc[0][2 * j + 1] += db;
-                } else {
-                  acc[1][2 * j] += da;
-                  acc[1][2 * j + 1] += db;
-                }
-                g_lo[j] = a * w_lo[j];
-                g_hi[j] = b * w_hi[j];
-                dot += da * w_lo[j] + db * w_hi[j];
-              }
-            }
-          }
-          if constexpr (kBwd) {
-            for (int o = group >> 1; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-            dot /= p.D;
+          if constexpr (!kBwd) {
+            const float r = rsqrtf(group_sum(sq, g.group) * g.inv_d + p.eps);
             if (normed) {
+              v_scale(lo, x_lo, r);
+              v_scale(hi, x_hi, r);
+              v_mul(lo, lo, w_lo);
+              v_mul(hi, hi, w_hi);
+              if (w.turns) v_turn(lo, hi, cos_at, cos_at + g.row);
+            }
+          } else {
+            // with S = sum of w g x: mean(w g n) n = x r^2 S / D, so both sums are taken at once, before r is known
+            float s = 0.f, e_lo[kVec], e_hi[kVec];
+            if (normed) {
+              unpack<T, kVec, kSide>(it[u].da, it[u].db, e_lo, e_hi);
+              if (w.turns) v_turn(e_lo, e_hi, cos_at, cos_at + g.row);
+              v_mul(lo, e_lo, w_lo);
+              v_mul(hi, e_hi, w_hi);
+              v_mul(t_lo, lo, x_lo);
+              v_fma(t_lo, hi, x_hi, t_lo);
+              s = v_sum(t_lo);
+            }
+            sq = group_sum(sq, g.group);
+            s = group_sum(s, g.group);
+            const float r = rsqrtf(sq * g.inv_d + p.eps), k = -(r * s) * (r * g.inv_d);
+            if (normed) {
+              v_scale(t_lo, x_lo, r);
+              v_scale(t_hi, x_hi, r);
+              if (seg == 0) {
+                v_fma(acc[0], e_lo, t_lo, acc[0]);
+                v_fma(acc[1], e_hi, t_hi, acc[1]);
+              } else {
+                v_fma(acc[2], e_lo, t_lo, acc[2]);
+                v_fma(acc[3], e_hi, t_hi, acc[3]);
+              }
+              v_scale(x_lo, x_lo, k);
+              v_scale(x_hi, x_hi, k);
 #pragma unroll
               for (int j = 0; j < kVec; ++j) {
-                lo[j] = r * (g_lo[j] - n_lo[j] * dot);
-                hi[j] = r * (g_hi[j] - n_hi[j] * dot);
+                lo[j] = r * (lo[j] + x_lo[j]);
+                hi[j] = r * (hi[j] + x_hi[j]);
               }
             }
           }
           if (here) {
-            Pack<T, kVec>&ra = kBwd ? it[u].da : it[u].xa, &rb = kBwd ? it[u].db : it[u].xb;
-            if (normed) pack(ra, rb, side, lo, hi);
-            store(ra, it[u].y + w.a);
-            store(rb, it[u].y + w.b);
+            if constexpr (kBwd) {
+              if (normed) pack<T, kVec, kSide>(it[u].da, it[u].db, lo, hi);
+              store(it[u].da, it[u].y + w.a);
+              store(it[u].db, it[u].y + w.b);
+            } else {
+              if (normed) pack<T, kVec, kSide>(it[u].xa, it[u].xb, lo, hi);
+              store(it[u].xa, it[u].y + w.a);
+              store(it[u].xb, it[u].y + w.b);
+            }
           }
         }
       }
@@ -246,24 +362,23 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const fb_rotary_args p
   }
   if constexpr (kSums) {
     // this block's share of dw: over the groups of a warp, then over the warps, in their order
-    float* part = reinterpret_cast<float*>(turn);        // [warps][2][D]
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, i = lane % group;
+    float* part = turn;        // [warps][2][D]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     __syncthreads();
 #pragma unroll
-    for (int seg = 0; seg < 2; ++seg)
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
-      for (int j = 0; j < 2 * kVec; ++j)
-        for (int o = 16; o >= group; o >>= 1) acc[seg][j] += __shfl_xor_sync(0xffffffffu, acc[seg][j], o);
-    if (lane < group && i < items) {
-      const ItemAt w = item_at<kVec>(i, p.rot, p.interleaved != 0);
-      const bool side = p.interleaved != 0 || !w.turns;
+      for (int j = 0; j < kVec; ++j)
+        for (int o = 16; o >= g.group; o >>= 1) acc[k][j] += __shfl_xor_sync(0xffffffffu, acc[k][j], o);
+    if (lane < g.group && own < g.items) {
+      const ItemAt w = item_at<kVec, kSide>(own, p.rot);
 #pragma unroll
       for (int seg = 0; seg < 2; ++seg)
 #pragma unroll
         for (int j = 0; j < kVec; ++j) {
           float* row = part + (warp * 2 + seg) * p.D;
-          row[side ? w.a + 2 * j : w.a + j] = acc[seg][2 * j];
-          row[side ? w.a + 2 * j + 1 : w.b + j] = acc[seg][2 * j + 1];
+          row[lo_at<kVec, kSide>(w, j)] = acc[2 * seg][j];
+          row[hi_at<kVec, kSide>(w, j)] = acc[2 * seg + 1][j];
         }
     }
     __syncthreads();
@@ -317,24 +432,27 @@ int widest(const fb_rotary_args& a, int size) {
   return 1;
 }
 
-template <typename T, int kVec, bool kNorm, bool kBwd>
-int launch(const fb_rotary_args& a, int grid, int tokens, int tile, int group, int items, size_t smem, cudaStream_t stream) {
-  constexpr auto kern = rotary_kernel<T, kVec, kNorm, kBwd>;
-  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kThreads), smem, stream, a, tokens, tile, group, items);
+template <typename T, int kVec, bool kSide, bool kNorm, bool kBwd>
+int launch(const fb_rotary_args& a, const Geometry& g, int grid, size_t smem, cudaStream_t stream) {
+  constexpr auto kern = rotary_kernel<T, kVec, kSide, kNorm, kBwd>;
+  const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(kThreads), smem, stream, a, g);
   if (e != cudaSuccess) return static_cast<int>(e);
   if constexpr (kNorm && kBwd) {
-    if (a.dw[0] || a.dw[1])
-      launch_pdl(rotary_dw_kernel, dim3((2 * a.D + 31) / 32), dim3(1024), 0, stream, a.partial, a.dw[0], a.dw[1], grid, a.D);
+    if (a.dw[0] || a.dw[1]) launch_pdl(rotary_dw_kernel, dim3((2 * a.D + 31) / 32), dim3(1024), 0, stream, a.partial, a.dw[0], a.dw[1], grid, a.D);
   }
   return static_cast<int>(cudaGetLastError());
 }
 template <typename T, int kVec>
-int pick(const fb_rotary_args& a, int grid, int tokens, int tile, int group, int items, size_t smem, cudaStream_t s) {
-  if (a.norm) return a.backward ? launch<T, kVec, true, true>(a, grid, tokens, tile, group, items, smem, s) : launch<T, kVec, true, false>(a, grid, tokens, tile, group, items, smem, s);
-  return a.backward ? launch<T, kVec, false, true>(a, grid, tokens, tile, group, items, smem, s) : launch<T, kVec, false, false>(a, grid, tokens, tile, group, items, smem, s);
+int pick(const fb_rotary_args& a, const Geometry& g, int grid, size_t smem, cudaStream_t s) {
+  const auto by_side = [&](auto side) {
+    constexpr bool kSide = decltype(side)::value;
+    if (a.norm) return a.backward ? launch<T, kVec, kSide, true, true>(a, g, grid, smem, s) : launch<T, kVec, kSide, true, false>(a, g, grid, smem, s);
+    return a.backward ? launch<T, kVec, kSide, false, true>(a, g, grid, smem, s) : launch<T, kVec, kSide, false, false>(a, g, grid, smem, s);
+  };
+  return a.interleaved ? by_side(std::true_type()) : by_side(std::false_type());
 }
 
-int rotary_blocks() { return 4 * sm_count(); }       // of the backward pass with the norm: those that are resident together
+int rotary_blocks() { return 2 * sm_count(); }       // of the backward pass with the norm: those that are resident together
 
 }  // namespace
 }  // namespace fb
@@ -358,30 +476,42 @@ extern "C" int fb_rotary(const fb_rotary_args* args, void* stream) {
   }
   if (heads * group > 0x7fffffffll / kMaxTokens) return -4;
   // A tile: as many tokens as the threads have items for, fewer where that would leave SMs without a block.
-  long long tile = kThreads * kItems / (heads * group);
+  long long tile = kThreads * items_of(a.norm) * passes_of(a.norm) / (heads * group);
   const long long spread = (tokens + 2 * sm_count() - 1) / (2 * sm_count());
   tile = tile < 1 ? 1 : tile > kMaxTokens ? kMaxTokens : tile;
   if (tile > spread) tile = spread;
-  if (a.rot > 0 && tile * a.rot * 4 > 32768) tile = 32768 / (a.rot * 4) > 0 ? 32768 / (a.rot * 4) : 1;
+  const int row = (a.rot / 2 + 3) / 4 * 4;
+  if (row > 0 && tile * row * 8 > 32768) tile = 32768 / (row * 8) > 0 ? 32768 / (row * 8) : 1;
   const long long n_tiles = (tokens + tile - 1) / tile;
   const bool sums = a.norm && a.backward;
   const int grid = static_cast<int>(sums && n_tiles > rotary_blocks() ? rotary_blocks() : n_tiles);
-  size_t smem = static_cast<size_t>(tile) * a.rot * 4;
+  size_t smem = static_cast<size_t>(tile) * row * 8 + (a.norm ? static_cast<size_t>(a.D + 3) / 4 * 32 : 0);
   if (sums && smem < static_cast<size_t>(kThreads / 32) * 2 * a.D * 4) smem = static_cast<size_t>(kThreads / 32) * 2 * a.D * 4;
   if (smem > 48 * 1024) return -4;
   const auto s = static_cast<cudaStream_t>(stream);
-  const int ntok = static_cast<int>(tokens), nt = static_cast<int>(tile);
+  Geometry g;
+  g.tokens = static_cast<int>(tokens);
+  g.tile = static_cast<int>(tile);
+  g.group = group;
+  g.items = items;
+  g.heads = static_cast<int>(heads);
+  g.row = row;
+  g.inv_d = 1.f / static_cast<float>(a.D);
+  g.by_group = div_by(group);
+  g.by_heads = div_by(heads);
+  g.by_seq = div_by(a.S);
+  g.by_pairs = div_by(a.rot / 2);
   if (a.dtype == FLODL_FLOAT32) {
-    if (v == 4) return pick<float, 4>(a, grid, ntok, nt, group, items, smem, s);
-    if (v == 2) return pick<float, 2>(a, grid, ntok, nt, group, items, smem, s);
-    return pick<float, 1>(a, grid, ntok, nt, group, items, smem, s);
+    if (v == 4) return pick<float, 4>(a, g, grid, smem, s);
+    if (v == 2) return pick<float, 2>(a, g, grid, smem, s);
+    return pick<float, 1>(a, g, grid, smem, s);
   }
   const auto by_width = [&](auto t) {
     using T = decltype(t);
-    if (v == 8) return pick<T, 8>(a, grid, ntok, nt, group, items, smem, s);
-    if (v == 4) return pick<T, 4>(a, grid, ntok, nt, group, items, smem, s);
-    if (v == 2) return pick<T, 2>(a, grid, ntok, nt, group, items, smem, s);
-    return pick<T, 1>(a, grid, ntok, nt, group, items, smem, s);
+    if (v == 8) return pick<T, 8>(a, g, grid, smem, s);
+    if (v == 4) return pick<T, 4>(a, g, grid, smem, s);
+    if (v == 2) return pick<T, 2>(a, g, grid, smem, s);
+    return pick<T, 1>(a, g, grid, smem, s);
   };
   return a.dtype == FLODL_BFLOAT16 ? by_width(__nv_bfloat16()) : by_width(__half());
 }
