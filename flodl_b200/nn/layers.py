@@ -571,7 +571,9 @@ class MultiheadAttention(Module):
     """Four xavier-uniform projections with zero bias around scaled dot-product attention
     (flodl/src/nn/attention.rs:20-160). Parameter names: q_proj.weight, q_proj.bias, k_proj..., out_proj....
     `mask` marks positions to exclude (non-zero = masked); a strictly upper-triangular [S, S] mask is
-    recognised as causal and, like an absent mask, runs on the fused attention kernel."""
+    recognised as causal and, like an absent mask, runs on the fused attention kernel. Keys of another length than the
+    queries go through `ops.cross_attention` in bf16 with heads of 64 and 128 on a GPU, where no mask or one of keys ([1, Sk],
+    [B, 1, 1, Sk]) is given; a query none of whose keys are left gets zeros there."""
 
     def __init__(self, embed_dim: int, num_heads: int, device=None):
         if embed_dim % num_heads:
@@ -598,6 +600,12 @@ class MultiheadAttention(Module):
         w, b = self.proj[nm]
         return _ops.linear(x, w.t, b.t)
 
+    @staticmethod
+    def _of_keys(mask: torch.Tensor, B: int, Sk: int) -> bool:
+        """Whether every query and head of a batch row has the same mask."""
+        shape = (1,) * (4 - mask.dim()) + tuple(mask.shape)
+        return len(shape) == 4 and shape[0] in (1, B) and shape[1:] == (1, 1, Sk) and Sk > 0
+
     def forward_ext(self, query, key, value, mask: Optional[torch.Tensor] = None):
         q, k, v = query.t, key.t, value.t
         B, Sq, Sk = q.shape[0], q.shape[1], k.shape[1]
@@ -615,6 +623,8 @@ class MultiheadAttention(Module):
                 add_mask = torch.zeros(mb.shape, dtype=torch.float32, device=q.device).masked_fill(mb, float("-inf"))
         if Sq == Sk:
             o = _ops.attention(q=qp, k=kp, v=vp, mask=add_mask, causal=causal, scale=self.scale)
+        elif _ops.FLAGS.native and qp.is_cuda and qp.dtype == torch.bfloat16 and D in (64, 128) and (mask is None or self._of_keys(mask, B, Sk)):
+            o = _ops.cross_attention(qp, kp, vp, None if mask is None else (mask == 0).reshape(-1, Sk), scale=self.scale)
         else:
             qh, kh, vh = (t.transpose(1, 2) for t in (qp, kp, vp))
             s = (qh @ kh.transpose(-1, -2)) * self.scale
