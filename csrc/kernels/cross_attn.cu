@@ -145,6 +145,24 @@ __device__ __forceinline__ bool warp_ready(uint64_t* bar, uint32_t parity, volat
   return warp_wait_long(bar, parity, abort_flag, status, code);
 }
 
+// The loop in place, for waits with registers full: a call would have them moved out of its way (8 x 12 x 1024 x 4096 of 128 columns 214 us against 207).
+__device__ __forceinline__ bool warp_ready_here(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
+  return warp_wait(bar, parity, abort_flag, status, code);
+}
+// One arrival for a warp whose lanes are all done, by a predicate in place of a branch.
+__device__ __forceinline__ void arrive_together(uint64_t* bar, int lane) {
+  __syncwarp();
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.eq.s32 p, %1, 0;\n\t"
+      "@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t"
+      "}\n" ::"r"(smem_u32(bar)),
+      "r"(lane)
+      : "memory");
+}
+
 // A place in a ring of kN stages, and the parity of its turn.
 template <int kN>
 struct Ring {
@@ -484,7 +502,7 @@ struct FwdBars {
   uint64_t s_full;             // the scores of a block are in TMEM
   uint64_t s_free;             // ... and in the softmax warps' registers
   uint64_t p_ready;            // the probabilities are in TMEM and O has been rescaled where it had to be
-  uint64_t pv_done;            // P V has been added to O
+  uint64_t pv_done;            // P V has been added to O: of every block where P has a place of its own, else of a run's last (the next scores tell of the others)
   TaskRing tasks;
   Left left[2];
   uint32_t tmem_slot;
@@ -563,6 +581,8 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   using L = Fwd<kD>;
   constexpr int kS = L::kStages;
+  constexpr bool kOwnP = L::P != L::S;
+  static_assert(kOwnP || kS == 1, "waits for V");
   static_assert(sizeof(FwdBars) <= 512, "barriers");
   FwdBars& bar = *reinterpret_cast<FwdBars*>(smem + L::BARS);
   volatile int* abort_flag = &bar.abort_flag;
@@ -693,7 +713,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       for (int i = 0; i < n && ok; ++i, ++it) {
         // Where P has a place of its own the next scores may come under this block's exponentials, otherwise right behind the product that reads P: a CTA's products
         // run in the order in which they are issued.
-        if (kD == 64 && i + 1 < n) {
+        if (kOwnP && i + 1 < n) {
           ok = warp_ready(&bar.s_free, it & 1, abort_flag, p.status, kStatusWaitEpi) && scores();
           if (!ok) break;
         }
@@ -703,12 +723,12 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < 128 / 16; ++k) umma_bf16_ts(tmem + L::O, tmem + L::P + k * 8, mn_desc(in_own(sV) + rv.stage * L::kTile, k * 2048, 16384), idesc_o, i > 0 || k > 0);
-          umma_commit(&bar.pv_done);
+          if (kOwnP || i + 1 == n) umma_commit(&bar.pv_done);
           umma_commit(&bar.v_empty[rv.stage]);
         }
         __syncwarp();
         rv.next();
-        if (kD != 64 && i + 1 < n) ok = scores();
+        if (!kOwnP && i + 1 < n) ok = scores();
       }
     }
   } else {
@@ -718,7 +738,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const float sc = p.scale * kLog2e;
     Ring<2> rt;
     Ring<kS> rv;
-    int it = 0;
+    int it = 0, runs = 0;        // blocks, and runs with any
     bool ok = true;
     // After a wait that gave up the loop over a run's blocks runs out without work, and the four warps go on to the next run or leave together, so that none is missed at
     // the barriers.
@@ -728,16 +748,17 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const int b = task.b, i0 = task.i0, i1 = task.i1;
       const bool works = warp * 32 < p.R - task.at * 128;        // a warp without rows only keeps step
       float m = -INFINITY, l = 0.f;               // the maximum the accumulator is relative to, and the sum
-      int2 next = make_int2(0, 0);
-      if (i0 < i1) next = live_block(p, b, i0);
+      const float base = task.base;
+      const int ragged = p.table ? i0 : p.Sk / kKeys;        // without a list, the first block that goes by the table
+      int next = p.live ? i0 < i1 ? __ldcg(p.live + static_cast<long long>(b) * p.key_blocks + i0) : 0 : i0 >= ragged;
       for (int i = i0; i < i1; ++i, ++it) {
-        const int2 blk = next;
-        if (i + 1 < i1) next = live_block(p, b, i + 1);
+        const bool tabled = next & 1;
         const float2* tb = tab + (it & 1) * 128;
-        if (blk.y) {
-          // A wait for V is one for the turn after the last that is known to be over: with one stage the block before has to have left it.
-          if (kS == 1 && i > i0) ok = ok && warp_ready(&bar.pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);
-          const float2 k = key_entry(p, b, blk.x * kKeys + t, task.base);
+        if (tabled) {
+          const int block = p.live ? next >> 1 : i;
+          // A wait for V is one for the turn after the last that is known to be over: with one stage the block before has to have left it, as it has once the scores are there.
+          if (kS == 1) ok = ok && warp_ready(&bar.s_full, it & 1, abort_flag, p.status, kStatusWaitAccum);
+          const float2 k = key_entry(p, b, block * kKeys + t, base);
           tab[(it & 1) * 128 + t] = k;
           if (p.mask && k.y == -INFINITY && ok) {        // an absent key's values meet a probability of zero
             ok = mbar_wait(&bar.v_full[rv.stage], rv.parity, abort_flag, p.status, kStatusWaitFull);
@@ -747,17 +768,18 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           fence_proxy_async_smem();
           asm volatile("bar.sync 1, 128;" ::: "memory");
         }
+        next = !p.live ? i + 1 >= ragged : i + 1 < i1 ? __ldcg(p.live + static_cast<long long>(b) * p.key_blocks + i + 1) : 0;
         rv.next();
-        ok = ok && warp_ready(&bar.s_full, it & 1, abort_flag, p.status, kStatusWaitAccum);
+        ok = ok && warp_ready_here(&bar.s_full, it & 1, abort_flag, p.status, kStatusWaitAccum);
         if (!ok) continue;
         tc_fence_after_sync();
         if (!works) {
-          if (kD == 64) arrive_warp(&bar.s_free, lane);
-          if (i > i0) ok = warp_ready(&bar.pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);
+          if (kOwnP) arrive_warp(&bar.s_free, lane);
+          if (kOwnP && i > i0) ok = warp_ready(&bar.pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);
           arrive_warp(&bar.p_ready, lane);
           continue;
         }
-        if (blk.y) apply_table<4>(tmem + L::S + lanes, tb);        // from here on all blocks are alike
+        if (tabled) apply_table<4>(tmem + L::S + lanes, tb);        // from here on all blocks are alike
         uint32_t s[4][32];
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld32(tmem + L::S + lanes + 32 * c, s[c]);
@@ -766,25 +788,30 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int e = 0; e < 32; ++e) asm volatile("" : "+r"(s[c][e]));
-        if (kD == 64) {
+        if (kOwnP) {
           tc_fence_before_sync();
-          arrive_warp(&bar.s_free, lane);
+          arrive_together(&bar.s_free, lane);
         }
-        const float mul = blk.y ? 1.f : sc, below = blk.y ? 0.f : task.base;        // a key with nothing added is `base` below the largest
+        const float mul = tabled ? 1.f : sc, below = tabled ? 0.f : base;        // a key with nothing added is `base` below the largest
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], __uint_as_float(s[c][e]), __uint_as_float(s[c][e + 1]));
         const float m_new = fmaxf(m, fmaf(mul, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), -below));
+        // Until the product of the block before is over, O is not touched and P not overwritten. Where P takes the place of the scores, these came behind that product.
+        bool over = i == i0 || !kOwnP;
         if (i == i0) {
           m = m_new;
         } else {
-          ok = warp_ready(&bar.pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);        // P may be overwritten, O touched
-          if (!ok) continue;
-          tc_fence_after_sync();
           // (m is -inf where no key has been seen: its sums are zeros, and stay so whatever they are scaled by)
           if (__any_sync(0xffffffffu, m_new > m + kSlack)) {
+            if (!over) {
+              ok = warp_ready(&bar.pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);
+              if (!ok) continue;
+              tc_fence_after_sync();
+              over = true;
+            }
             const float alpha = m_new == -INFINITY ? 1.f : ex2_approx(m - m_new);
             m = m_new;
             l *= alpha;
@@ -813,19 +840,24 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             sum[(e >> 1) & 1] = f2_add(sum[(e >> 1) & 1], f2_make(lo, hi));
             pk[e >> 1] = pack2(lo, hi);
           }
+          if (c == 0 && !over) {        // (behind 64, 96 or all 128 exponentials, with P in registers meanwhile, 8 x 12 x 1024 x 4096 took 169, 177 and 180 us, behind 32 of them 168)
+            ok = warp_ready_here(&bar.pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);
+            tc_fence_after_sync();
+          }
           tmem_st16(tmem + L::P + lanes + 16 * c, pk);
         }
+        if (!ok) continue;
         float a0, a1, b0, b1;
         f2_get(f2_add(sum[0], sum[1]), a0, a1);
         l += a0 + a1;
         tmem_st_wait();
         tc_fence_before_sync();
-        arrive_warp(&bar.p_ready, lane);
+        arrive_together(&bar.p_ready, lane);
       }
       // ---- the run's rows
       const bool whole = task.whole;
       const int h = task.h, row0 = task.at * 128, rows = min(128, p.R - row0);
-      if (i0 < i1) ok = ok && warp_ready(&bar.pv_done, (it - 1) & 1, abort_flag, p.status, kStatusWaitAccum);
+      if (i0 < i1) ok = ok && warp_ready(&bar.pv_done, kOwnP ? (it - 1) & 1 : runs++ & 1, abort_flag, p.status, kStatusWaitAccum);
       if (!whole && t == 0) bar.left[task.slot] = Left{1, task.ends, b, task.tile};
       if (ok && works) {
         tc_fence_after_sync();
@@ -1327,7 +1359,7 @@ __device__ __forceinline__ void bwd_softmax(BwdBars& bar, const CrossParams& p, 
       const float* tb = tab + ra.stage * 256 + (kKeys ? w * 32 : w * 64);
       const uint32_t tS = mine + (rs.stage ? (kKeys ? L::S2_KEYS : L::S2_ROWS) : L::S), tDP = mine + L::DP;
       if (!warp_ready(&bar.tab_full[ra.stage], ra.parity, abort_flag, p.status, kStatusWaitFull)) return;        // every turn: a parity tells only the last two apart
-      if (!warp_ready(&bar.s_full[rs.stage], rs.parity, abort_flag, p.status, kStatusWaitAccum)) return;
+      if (!warp_ready_here(&bar.s_full[rs.stage], rs.parity, abort_flag, p.status, kStatusWaitAccum)) return;
       tc_fence_after_sync();
       if (masked) masked_scores<kKeys>(tS, entry, reinterpret_cast<const float2*>(tb));
       uint32_t pr[32];
@@ -1335,9 +1367,9 @@ __device__ __forceinline__ void bwd_softmax(BwdBars& bar, const CrossParams& p, 
       if (kKeys) {
         tmem_st_wait();
         tc_fence_before_sync();
-        arrive_warp(&bar.p_ready, lane);
+        arrive_together(&bar.p_ready, lane);
       }
-      if (!warp_ready(&bar.dp_full, it & 1, abort_flag, p.status, kStatusWaitAccum)) return;
+      if (!warp_ready_here(&bar.dp_full, it & 1, abort_flag, p.status, kStatusWaitAccum)) return;
       tc_fence_after_sync();
       if (masked) {
         masked_dp<kKeys>(tDP, entry, reinterpret_cast<const float2*>(tb));
@@ -1349,7 +1381,7 @@ __device__ __forceinline__ void bwd_softmax(BwdBars& bar, const CrossParams& p, 
       make_ds<kKeys>(tDP, tb + 128, neg_d, pr);
       tmem_st_wait();
       tc_fence_before_sync();
-      arrive_warp(&bar.ds_ready, lane);
+      arrive_together(&bar.ds_ready, lane);
       ++it;
       ra.next();
       rs.next();
