@@ -3,8 +3,10 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_runtime.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
+#include <cfloat>
 #include <cmath>
 #include <optional>
 #include <vector>
@@ -35,6 +37,17 @@ bool records(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+// Whether a tensor is its memory and nothing else: no transform's wrapper, subclass, tangent or sign that a reader has to apply. The plain forms take the others.
+bool plain_memory(const Tensor& t) {
+  constexpr c10::DispatchKeySet wrapped({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper});
+  return t.has_storage() && !t.key_set().has_any(wrapped) && !t.is_neg() && !t._fw_grad(/*level=*/0).defined();
+}
+// ... of all that are there; and no trace, which would keep a result of these functions as a constant.
+bool plain_call(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && !plain_memory(*t)) return false;
+  return !torch::jit::tracer::isTracing();
 }
 void first_derivative_only() { TORCH_CHECK(!at::GradMode::is_enabled(), "the native kernels have no second derivative: use ops.set_native(False)"); }
 
@@ -198,15 +211,17 @@ Found turn(const Tensor& q, const OptTensor& k_in, const Tensor& freqs_in, const
   const int64_t B = q.size(0), S = q.size(1), D = q.size(-1);
   if (k.defined() && (k.dim() != 4 || k.size(0) != B || k.size(1) != S || k.size(3) != D || k.scalar_type() != kind || k.device() != q.device())) return std::nullopt;
   if (freqs_in.dim() != 1 || freqs_in.scalar_type() != at::kDouble || freqs_in.device() != q.device()) return std::nullopt;
+  if (!plain_call({&q, &k, &freqs_in, &wq, &wk}) || records({&freqs_in})) return std::nullopt;       // the kernel knows no gradient of frequencies
   const int64_t pairs = freqs_in.numel();
   if (D < 2 || D % 2 || 2 * pairs > D || B >= 1 << 30 || S >= 1 << 30 || B * S >= 1ll << 31 || q.size(-2) < 1 || q.size(-2) >= 1 << 14) return std::nullopt;
   if (k.defined() && (k.size(2) < 1 || k.size(2) >= 1 << 14)) return std::nullopt;
   if (!std::isfinite(amplitude) || !(eps >= 0)) return std::nullopt;
   if (norm && (D > 64 * width(q, pairs) || D > 512)) return std::nullopt;
+  if (D > 8192 || (q.size(-2) * (packed ? 3 : 1) + (k.defined() ? k.size(2) : 0)) * D > 1 << 24) return std::nullopt;       // of a tile's items and its angles
   Tensor positions;
   if (positions_in.has_value()) {
     positions = *positions_in;
-    if (!c10::isIntegralType(positions.scalar_type(), false) || positions.device() != q.device()) return std::nullopt;
+    if (!c10::isIntegralType(positions.scalar_type(), false) || !plain_memory(positions) || positions.device() != q.device()) return std::nullopt;
     if ((positions.dim() != 1 && positions.dim() != 2) || positions.size(-1) != S || (positions.dim() == 2 && positions.size(0) != 1 && positions.size(0) != B)) return std::nullopt;
     if (positions.scalar_type() != at::kLong) positions = positions.to(at::kLong);
     positions = positions.expand({B, S});
@@ -330,12 +345,15 @@ std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Te
   if ((D != 64 && D != 128) || k.sizes() != v.sizes() || k.size(0) != B || k.size(3) != D || !std::isfinite(scale)) return std::nullopt;
   if (B < 1 || H < 1 || Hk < 1 || H % Hk || q.size(1) < 1 || Sk < 1 || q.size(1) > 1 << 26 || Sk > 1 << 28 || B > 1 << 20 || H > 1 << 16) return std::nullopt;
   Tensor mask;
+  if (!plain_call({&q, &k, &v})) return std::nullopt;
   if (mask_in.has_value()) {
     mask = *mask_in;
+    if (!plain_memory(mask)) return std::nullopt;
     if (mask.requires_grad() && at::GradMode::is_enabled()) return std::nullopt;
     if (mask.device() != q.device() || (mask.scalar_type() != at::kBool && !mask.is_floating_point())) return std::nullopt;
     if (mask.dim() == 4 && mask.size(1) == 1 && mask.size(2) == 1) mask = mask.select(1, 0).select(1, 0);
     if (mask.dim() != 2 || mask.size(1) != Sk || (mask.size(0) != 1 && mask.size(0) != B)) return std::nullopt;
+    if (mask.scalar_type() == at::kDouble) mask = at::where(mask.isinf(), mask, mask.clamp(-FLT_MAX, FLT_MAX));       // finite values stay finite
     if (mask.scalar_type() != at::kBool) mask = mask.to(at::kFloat);
     if (Sk > 1 && mask.stride(1) != 1) mask = mask.contiguous();
   }

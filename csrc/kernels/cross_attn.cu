@@ -1778,7 +1778,7 @@ int cross_bwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   return static_cast<int>(cudaGetLastError());
 }
 
-bool rows_ok(const void* p, const long long* st) { return strides_ok(p, st[0], st[1], st[2]); }
+bool rows_ok(const void* p, const long long* st) { return p && strides_ok(p, st[0], st[1], st[2]); }
 
 }  // namespace
 }  // namespace fb

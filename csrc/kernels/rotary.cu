@@ -468,6 +468,10 @@ extern "C" int fb_rotary(const fb_rotary_args* args, void* stream) {
   if (a.B < 0 || a.S < 0 || a.D < 2 || a.D % 2 || a.rot < 0 || a.rot % 2 || a.rot > a.D || a.heads[0] < 1 || a.heads[1] < 0 || a.heads[2] < 0) return -4;
   if (tokens > 0x7fffffffll) return -4;
   if (tokens == 0) return 0;
+  const bool reads_x = !a.backward || a.norm;
+  for (int s = 0; s < 3; ++s)
+    if (a.heads[s] && (!a.y[s] || (reads_x && !a.x[s]) || (a.backward && !a.dy[s]))) return -3;
+  if ((a.rot && !a.freqs) || (a.norm && a.backward && !a.partial)) return -3;
   const int v = widest(a, size), items = a.D / (2 * v);
   int group = items;
   if (a.norm) {

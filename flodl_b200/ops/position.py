@@ -145,7 +145,9 @@ def qk_norm_rotary(x, q_weight: Optional[torch.Tensor] = None, k_weight: Optiona
     """Queries and keys normalised per head, `x / sqrt(mean(x^2) + eps) * weight` over the head's values, then turned as `rotary` does (not at all
     without `freqs`), in one pass. The weights are [D], shared by the heads; None is ones. Statistics are taken in 32 bits."""
     if freqs is None:
-        lead = x if torch.is_tensor(x) else x[0]
+        lead = x if torch.is_tensor(x) else next(iter(x), None)
+        if not torch.is_tensor(lead):
+            raise TensorError("x must be a tensor or a pair of them")
         freqs = torch.empty(0, dtype=torch.float64, device=lead.device)
     out = _native(x, freqs, positions, offset, interleaved, amplitude, True, q_weight, k_weight, eps)
     if out is not None:

@@ -283,3 +283,27 @@ def test_queries_and_keys_in_turn_over_a_source(C):
     for a, b in zip(got, want):
         assert (a.double() - b.double()).norm() <= 4 * H_ * b.double().norm()
     assert (got[2][1, 100:] == 0).all()
+
+
+def test_calls_that_look_at_more_than_memory():
+    """Tangents and vmap go by the plain form, which knows them; both sides round their results to bf16 once."""
+    g = torch.Generator().manual_seed(9)
+    q, k, v, dv = (torch.randn(2, s, 2, 64, generator=g).bfloat16().cuda() for s in (3, 40, 40, 40))
+    want, turn = ops.cross_attention(q, k, v), ops.cross_attention(q, k, dv)
+    o, do = torch.func.jvp(lambda t: ops.cross_attention(q, k, t), (v,), (dv,))
+    # P <= 1 rounded once by the kernel, the results once by either side, of sums that are at most the largest |v|
+    assert (o - want).abs().max() <= 3 * H_ * v.abs().max() and (do - turn).abs().max() <= 3 * H_ * dv.abs().max()
+    both = torch.func.vmap(lambda t: ops.cross_attention(q, k, t))(torch.stack((v, dv)))
+    assert (both[1] - turn).abs().max() <= 3 * H_ * dv.abs().max()
+
+
+@pytest.mark.parametrize("low", [-1e300, torch.finfo(torch.float64).min])
+def test_lowest_values_of_a_64_bit_mask_stay_finite(low):
+    """A row of them is a row of equal scores, not one without keys."""
+    g = torch.Generator().manual_seed(10)
+    q, k, v = (torch.randn(1, s, 1, 64, generator=g).bfloat16().cuda() for s in (3, 40, 40))
+    mask = torch.full((1, 40), low, dtype=torch.float64, device="cuda")
+    mask[0, 30:] = float("-inf")
+    got = ops.cross_attention(q, k, v, mask)
+    want = v[0, :30, 0].double().mean(0)
+    assert ((got[0, :, 0].double() - want).abs() <= (H_ + T_) * v.abs().max().item() + H_ * want.abs()).all()

@@ -117,3 +117,11 @@ def test_refusals():
     for call in bad:
         with pytest.raises(TensorError):
             call()
+
+
+def test_norm_of_nothing_is_refused():
+    for x in ((), [1], (None, None)):
+        with pytest.raises(TensorError, match="must be a tensor or a pair"):
+            ops.qk_norm_rotary(x)
+        with pytest.raises(TensorError, match="must be a tensor or a pair"):
+            ops.rotary(x, ops.rotary_frequencies(2))
