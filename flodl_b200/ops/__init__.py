@@ -8,6 +8,9 @@ Every function here has two paths:
   libtorch's engine does in the reference (flodl/src/autograd/variable.rs:199-204).
 * anything else (CPU, fp64, odd shapes)          -> the plain PyTorch op with the same semantics.
 
+Positions and attention: `rotary`, `qk_norm_rotary` (with frequencies of `rotary_frequencies`) between a projection and `attention`,
+`cross_attention` over another sequence.
+
 On a CUDA device the native library is mandatory: if it cannot be loaded these functions raise
 instead of silently running the PyTorch path.
 """
