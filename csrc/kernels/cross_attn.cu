@@ -1089,7 +1089,7 @@ struct BwdBars {
   uint64_t b_full[3], b_empty[3];     // ... of dO or V
   uint64_t tab_full[3];               // A's table is written
   uint64_t s_full[2], dp_full;        // scores and dP are in TMEM
-  uint64_t p_ready, ds_ready;         // ... and P and dS in their place
+  uint64_t p_ready[2], ds_ready;      // ... and P (one for each place of scores: a warp may be a turn ahead of another there) and dS in their place
   uint64_t acc_done;                  // every product of a run has retired
   TaskRing tasks;
   Left left[2];
@@ -1140,8 +1140,8 @@ __device__ __forceinline__ void bwd_products(BwdBars& bar, const CrossParams& p,
     return true;
   };
   // acc += (the 128 columns, each 32 left as bf16 in the first half of their place) x (the 128 rows of a streamed tile)
-  const auto accumulate = [&](uint32_t acc, uint32_t from, uint32_t tile, bool first, uint64_t* ready, uint64_t* empty, bool done) {
-    if (!warp_ready(ready, it & 1, abort_flag, status, kStatusWaitEpi)) return false;
+  const auto accumulate = [&](uint32_t acc, uint32_t from, uint32_t tile, bool first, uint64_t* ready, uint32_t parity, uint64_t* empty, bool done) {
+    if (!warp_ready(ready, parity, abort_flag, status, kStatusWaitEpi)) return false;
     tc_fence_after_sync();
     if (elect_one()) {
 #pragma unroll
@@ -1163,11 +1163,11 @@ __device__ __forceinline__ void bwd_products(BwdBars& bar, const CrossParams& p,
       const bool more = i + 1 < n, first = i == 0;
       if (kTwo && more) ok = scores(it + 1);
       if (kKeys) {
-        ok = ok && accumulate(L::ACC0, s_at(it), b_at(fb.stage), first, &bar.p_ready, &bar.b_empty[fb.stage], false);
+        ok = ok && accumulate(L::ACC0, s_at(it), b_at(fb.stage), first, &bar.p_ready[kTwo ? it & 1 : 0], (kTwo ? it >> 1 : it) & 1, &bar.b_empty[fb.stage], false);
         fb.next();
         if (!kTwo && more) ok = ok && scores(it + 1);
       }
-      ok = ok && accumulate(L::ACC1, tmem + L::DP, a_at(fa.stage), first, &bar.ds_ready, &bar.a_empty[fa.stage], !more);
+      ok = ok && accumulate(L::ACC1, tmem + L::DP, a_at(fa.stage), first, &bar.ds_ready, it & 1, &bar.a_empty[fa.stage], !more);
       fa.next();
       if (more) ok = ok && dp(i + 2 == n);
     }
@@ -1367,7 +1367,7 @@ __device__ __forceinline__ void bwd_softmax(BwdBars& bar, const CrossParams& p, 
       if (kKeys) {
         tmem_st_wait();
         tc_fence_before_sync();
-        arrive_together(&bar.p_ready, lane);
+        arrive_together(&bar.p_ready[rs.stage], lane);
       }
       if (!warp_ready_here(&bar.dp_full, it & 1, abort_flag, p.status, kStatusWaitAccum)) return;
       tc_fence_after_sync();
@@ -1457,7 +1457,7 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     mbar_init(&bar.s_full[0], 1);
     mbar_init(&bar.s_full[1], 1);
     mbar_init(&bar.dp_full, 1);
-    mbar_init(&bar.p_ready, kBwdSoftmaxWarps);
+    for (int i = 0; i < 2; ++i) mbar_init(&bar.p_ready[i], kBwdSoftmaxWarps);
     mbar_init(&bar.ds_ready, kBwdSoftmaxWarps);
     mbar_init(&bar.acc_done, 1);
     for (int i = 0; i < 2; ++i) { mbar_init(&bar.tasks.full[i], 1); mbar_init(&bar.tasks.empty[i], kBwdSoftmaxWarps + 2); }
