@@ -31,6 +31,7 @@ namespace {
 
 constexpr int kKeys = 128;                  // keys of a block
 constexpr float kHuge = 1.2676506e30f;      // 2^100
+constexpr int kWith = 512;                  // more than there are CTAs of a kernel that share a tile
 
 struct CrossParams {
   int B, Hq, Hk, R, Sk;             // Hq = H / pack rows of heads; R = Sq * pack rows each
@@ -462,6 +463,359 @@ __device__ __forceinline__ __nv_bfloat16* out_row(const CrossParams& p, __nv_bfl
   const int g = r & ((1 << p.pack_log2) - 1);
   return base + b * sb + (r >> p.pack_log2) * ss + ((static_cast<long long>(h) << p.pack_log2) + g) * sh;
 }
+__device__ __forceinline__ uint32_t in_cta(uint32_t smem, int cta) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem), "r"(cta));
+  return remote;
+}
+__device__ __forceinline__ float4 ld_cluster_v4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_v2(uint32_t at) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_meet() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// ============================================================================ forward, few rows
+// Tiles of sixteen rows, for a token of each sequence and for whatever is as little work. HBM bounds a token, and how long a block of keys takes: a tcgen05 tile has 128 rows
+// whatever is in them, and its chain of copy, scores, TMEM, probabilities and product took 1.7 us a block with one warp at work. Here each warp is on its own: it streams
+// chunks of keys through a ring of its own with cp.async, two in flight, and multiplies them with mma.sync; warps meet at the end, the CTAs that share a tile in
+// distributed shared memory or, more than eight of them, by a second launch. Chunks go round all warps of a tile, so that padding at its end takes from each the same.
+// Masks are read as the chunks are asked for: absent keys are not copied but filled with zeros, chunks without a key left out.
+// One token of 16 x 8 heads of 64 over up to 1500 keys 10.1 us (37 MB; in 128-row tiles 18.4), of 4 x 32 heads of 128 on 4 key heads over 32768 49.9 (5.4 TB/s; 61.3).
+template <int kD>
+struct Few {
+  static constexpr int kWarps = 4, kStages = 3;
+  static constexpr int kChunk = 2048 / kD;                  // keys
+  static constexpr int kTile = kChunk * kD * 2;             // bytes of K, and of V
+  static constexpr int TAB = 2 * kTile, STAGE = TAB + kChunk * 8, WARP = kStages * STAGE;
+  static constexpr int kRow = kD + 8;                       // floats of a row of sums: rows of a quad's warp meet different banks
+  static constexpr int SUMS = kWarps * 16 * kRow * 4, ML = SUMS + 16 * kRow * 4, ML_JOINED = ML + kWarps * 16 * 8;
+  static constexpr int TOTAL = kWarps * WARP;
+  static_assert(ML_JOINED + 16 * 8 <= TOTAL, "sums take the place of the rings");
+};
+struct FewArgs {
+  const __nv_bfloat16 *q, *k, *v;
+  __nv_bfloat16* o;
+  long long qs[3], ks[3], vs[3], os[3];
+  float* stats;                // as in FwdOut
+  float* part_o;               // [tiles * parts][16][D] sums relative to the part's maximum; null: the CTAs of a tile are a cluster
+  float2* part_ml;             // ... [16] {maximum, sum}
+  int parts;                   // CTAs that share a tile
+  int row_tiles;               // of sixteen rows
+  Div by_parts, by_rows, by_heads;
+};
+// A tile's place: batch row, row of heads, first row, and how many rows.
+struct FewTile {
+  int b, h, row0, rows;
+};
+__device__ __forceinline__ FewTile few_tile(const CrossParams& p, const FewArgs& f, int tile) {
+  const int all = f.by_rows(tile), b = f.by_heads(all), row0 = (tile - all * f.row_tiles) * 16;
+  return {b, all - b * p.Hq, row0, min(16, p.R - row0)};
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory"); }
+template <bool kTransposed>
+__device__ __forceinline__ void ld_matrices(uint32_t at, uint32_t (&m)[4]) {
+  if (kTransposed)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3]) : "r"(at) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(m[0]), "=r"(m[1]), "=r"(m[2]), "=r"(m[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Four columns of a row: the sum of `of` parts' sums, each relative to its own maximum, in their order.
+template <typename Ml, typename Sums>
+__device__ __forceinline__ void few_join(int of, Ml ml_of, Sums sums_of, float4& acc, float& top, float& sum) {
+  top = -INFINITY;
+#pragma unroll 4
+  for (int k = 0; k < of; ++k) top = fmaxf(top, ml_of(k).x);
+  const float ref = top == -INFINITY ? 0.f : top;
+  sum = 0.f;
+  acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = 0; k < of; ++k) {
+    const float2 x = ml_of(k);
+    const float4 v = sums_of(k);
+    const float w = ex2_approx(x.x - ref);
+    sum += w * x.y;
+    acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
+  }
+}
+__device__ __forceinline__ void few_put(const CrossParams& p, const FewArgs& f, const FewTile& at, int row, int col, float4 acc, float top, float sum) {
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (f.stats && col == 0) f.stats[(static_cast<long long>(at.b) * p.Hq + at.h) * p.R + at.row0 + row] = sum == 0.f ? INFINITY : top + log2f(sum);
+  *reinterpret_cast<uint2*>(out_row(p, f.o, f.os[0], f.os[1], f.os[2], at.b, at.h, at.row0 + row) + col * 4) = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
+}
+
+template <int kD>
+__global__ void __launch_bounds__(Few<kD>::kWarps * 32, 2) cross_few_kernel(const CrossParams p, const FewArgs f) {
+  using L = Few<kD>;
+  extern __shared__ __align__(128) uint8_t ring[];
+  constexpr int kChunk = L::kChunk, kStages = L::kStages, kCols = kD / 8;        // 16-byte columns of a row
+  const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int tile = f.by_parts(blockIdx.x), part = blockIdx.x - tile * f.parts;
+  const FewTile at = few_tile(p, f, tile);
+  const int b = at.b, h = at.h;
+  const uint32_t mine = smem_u32(ring) + warp * L::WARP;
+  float2* tab = reinterpret_cast<float2*>(ring + warp * L::WARP + L::TAB);        // of stage 0; others STAGE bytes on
+  pdl_entry();
+
+  // rows g and g + 8 of Q, as the products take them
+  uint32_t q[kD / 16][4];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const bool there = g + r * 8 < at.rows;
+    const __nv_bfloat16* row = out_row(p, const_cast<__nv_bfloat16*>(f.q), f.qs[0], f.qs[1], f.qs[2], b, h, at.row0 + (there ? g + r * 8 : 0)) + t * 2;
+#pragma unroll
+    for (int c = 0; c < kD / 16; ++c)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) q[c][half * 2 + r] = there ? __ldcg(reinterpret_cast<const unsigned*>(row + c * 16 + half * 8)) : 0u;
+  }
+  const int hk = p.by_per_kv(h), chunks = (p.Sk + kChunk - 1) / kChunk, step = f.parts * L::kWarps;
+  const __nv_bfloat16 *k0 = f.k + b * f.ks[0] + hk * f.ks[2], *v0 = f.v + b * f.vs[0] + hk * f.vs[2];
+  const float sc = p.scale * kLog2e, base = p.mask && !p.mask_bool ? __ldcg(p.base + b) : 0.f;
+
+  // The mask is read a chunk ahead of the copies, these two chunks ahead of the products.
+  int c = part * L::kWarps + warp, have = 0;
+  unsigned tabled = 0;         // a bit for each stage
+  const auto entry_of = [&](int c) {
+    const int key = c * kChunk + lane;
+    if (lane >= kChunk || key >= p.Sk) return make_float2(sc, -INFINITY);
+    return p.mask ? key_entry(p, b, key, base) : make_float2(sc, 0.f);
+  };
+  float2 ahead = entry_of(c);
+  const auto ask = [&]() {
+    while (c < chunks) {
+      const float2 e = ahead;
+      const int first = c * kChunk;
+      c += step;
+      ahead = entry_of(c);
+      const unsigned live = __ballot_sync(0xffffffffu, e.y != -INFINITY);
+      if (live == 0) continue;
+      const int stage = have % kStages;
+      const bool plain = __all_sync(0xffffffffu, lane >= kChunk || (e.x == sc && e.y == 0.f));
+      tabled = plain ? tabled & ~(1u << stage) : tabled | 1u << stage;
+      if (!plain && lane < kChunk) *reinterpret_cast<float2*>(reinterpret_cast<uint8_t*>(tab + lane) + stage * L::STAGE) = e;
+#pragma unroll
+      for (int j = 0; j < L::kTile / 512; ++j) {
+        const int row = (j * 32 + lane) / kCols, col = (j * 32 + lane) % kCols;
+        const bool there = live >> row & 1;
+        const uint32_t to = mine + stage * L::STAGE + row * (kD * 2) + ((col ^ (row & 7)) << 4);
+        const long long key = there ? first + row : 0;
+        cp_async16(to, k0 + key * f.ks[1] + col * 8, there);
+        cp_async16(to + L::kTile, v0 + key * f.vs[1] + col * 8, there);
+      }
+      ++have;
+      break;
+    }
+    cp_async_commit();
+  };
+
+  float o[kD / 8][4];
+#pragma unroll
+  for (int n = 0; n < kD / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};        // of rows g and g + 8; l of this thread's columns
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) ask();
+#pragma unroll 1
+  for (int it = 0; it < have; ++it) {
+    ask();
+    cp_async_wait<kStages - 1>();
+    __syncwarp();
+    const int stage = it % kStages;
+    const uint32_t sK = mine + stage * L::STAGE, sV = sK + L::kTile;
+    float s[kChunk / 8][4];
+#pragma unroll
+    for (int n = 0; n < kChunk / 8; ++n) {
+      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      const int row = n * 8 + (lane & 7);
+#pragma unroll
+      for (int kk = 0; kk < kD / 32; ++kk) {
+        uint32_t w[4];
+        ld_matrices<false>(sK + row * (kD * 2) + (((kk * 4 + (lane >> 3)) ^ (lane & 7)) << 4), w);
+        mma16(s[n], q[kk * 2], w[0], w[1]);
+        mma16(s[n], q[kk * 2 + 1], w[2], w[3]);
+      }
+    }
+    float top[2] = {m[0], m[1]};
+    const bool by_table = tabled >> stage & 1;
+#pragma unroll
+    for (int n = 0; n < kChunk / 8; ++n) {
+      float4 e = make_float4(sc, 0.f, sc, 0.f);
+      if (by_table) e = *reinterpret_cast<const float4*>(reinterpret_cast<const uint8_t*>(tab + n * 8 + t * 2) + stage * L::STAGE);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        s[n][2 * r] = e.y == -INFINITY ? -INFINITY : fmaf(s[n][2 * r], e.x, e.y);
+        s[n][2 * r + 1] = e.w == -INFINITY ? -INFINITY : fmaf(s[n][2 * r + 1], e.z, e.w);
+        top[r] = max3(top[r], s[n][2 * r], s[n][2 * r + 1]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+    }
+    if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+      const float a0 = top[0] == -INFINITY ? 1.f : ex2_approx(m[0] - top[0]), a1 = top[1] == -INFINITY ? 1.f : ex2_approx(m[1] - top[1]);
+      m[0] = top[0];
+      m[1] = top[1];
+      l[0] *= a0;
+      l[1] *= a1;
+#pragma unroll
+      for (int n = 0; n < kD / 8; ++n) {
+        o[n][0] *= a0;
+        o[n][1] *= a0;
+        o[n][2] *= a1;
+        o[n][3] *= a1;
+      }
+    }
+    const float ref[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+    for (int n = 0; n < kChunk / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[n][e] = ex2_approx(s[n][e] - ref[e >> 1]);
+        l[e >> 1] += s[n][e];
+      }
+#pragma unroll
+    for (int j = 0; j < kChunk / 16; ++j) {
+      const uint32_t a[4] = {pack2(s[2 * j][0], s[2 * j][1]), pack2(s[2 * j][2], s[2 * j][3]), pack2(s[2 * j + 1][0], s[2 * j + 1][1]), pack2(s[2 * j + 1][2], s[2 * j + 1][3])};
+      const int row = j * 16 + (lane >> 3 & 1) * 8 + (lane & 7);
+#pragma unroll
+      for (int n = 0; n < kD / 16; ++n) {
+        uint32_t w[4];
+        ld_matrices<true>(sV + row * (kD * 2) + (((n * 2 + (lane >> 4)) ^ (lane & 7)) << 4), w);
+        mma16(o[2 * n], a, w[0], w[1]);
+        mma16(o[2 * n + 1], a, w[2], w[3]);
+      }
+    }
+    __syncwarp();        // the stage may be filled again
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+  // ---- the warps' sums, then the CTAs', in their order
+  float* sums = reinterpret_cast<float*>(ring);
+  float2* ml = reinterpret_cast<float2*>(ring + L::ML);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int row = warp * 16 + g + r * 8;
+    if (t == 0) ml[row] = make_float2(m[r], l[r]);
+#pragma unroll
+    for (int n = 0; n < kD / 8; ++n) *reinterpret_cast<float2*>(sums + row * L::kRow + n * 8 + t * 2) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+  }
+  __syncthreads();
+  float4 acc;
+  float top, sum;
+  for (int e = threadIdx.x; e < at.rows * (kD / 4); e += L::kWarps * 32) {
+    const int row = e / (kD / 4), col = e % (kD / 4);
+    few_join(L::kWarps, [&](int k) { return ml[k * 16 + row]; }, [&](int k) { return *reinterpret_cast<const float4*>(sums + (k * 16 + row) * L::kRow + col * 4); }, acc, top, sum);
+    if (f.parts == 1) {
+      few_put(p, f, at, row, col, acc, top, sum);
+    } else if (f.part_o) {
+      const long long to = blockIdx.x * 16ll + row;
+      *reinterpret_cast<float4*>(f.part_o + to * kD + col * 4) = acc;
+      if (col == 0) f.part_ml[to] = make_float2(top, sum);
+    } else {
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(ring + L::SUMS) + row * L::kRow + col * 4) = acc;
+      if (col == 0) *reinterpret_cast<float2*>(ring + L::ML_JOINED + row * 8) = make_float2(top, sum);
+    }
+  }
+  if (f.parts > 1 && !f.part_o) {
+    cluster_meet();
+    const uint32_t all = smem_u32(ring);
+    for (int e = part * (L::kWarps * 32) + threadIdx.x; e < at.rows * (kD / 4); e += f.parts * L::kWarps * 32) {
+      const int row = e / (kD / 4), col = e % (kD / 4);
+      few_join(f.parts, [&](int k) { return ld_cluster_v2(in_cta(all + L::ML_JOINED + row * 8, k)); },
+               [&](int k) { return ld_cluster_v4(in_cta(all + L::SUMS + (row * L::kRow + col * 4) * 4, k)); }, acc, top, sum);
+      few_put(p, f, at, row, col, acc, top, sum);
+    }
+    cluster_meet();        // shared memory is there until all have read it
+  }
+}
+// The parts of a tile that were left in global memory: a block a row, its threads four columns of every so manieth part each, the first of which are on their way before
+// their weights are known.
+template <int kD>
+__global__ void __launch_bounds__(128) cross_few_join_kernel(const CrossParams p, const FewArgs f) {
+  constexpr int kLanes = kD / 4, kGroups = 128 / kLanes, kAhead = 4;
+  __shared__ float weight[kWith], of_warp[8];
+  __shared__ float4 of_group[kGroups][kLanes];
+  pdl_entry();
+  const int tile = blockIdx.x, row = blockIdx.y;
+  const FewTile at = few_tile(p, f, tile);
+  if (row >= at.rows) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = threadIdx.x / kLanes, col = threadIdx.x % kLanes;
+  const long long first = static_cast<long long>(tile) * f.parts * 16 + row;
+  const auto sums = [&](int k) { return k < f.parts ? __ldcg(reinterpret_cast<const float4*>(f.part_o + (first + k * 16) * kD) + col) : make_float4(0.f, 0.f, 0.f, 0.f); };
+  float4 ahead[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) ahead[i] = sums(group + i * kGroups);
+  float2 x[kWith / 128];
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kWith / 128; ++i) {
+    const int k = i * 128 + static_cast<int>(threadIdx.x);
+    x[i] = k < f.parts ? __ldcg(f.part_ml + first + k * 16) : make_float2(-INFINITY, 0.f);
+    top = fmaxf(top, x[i].x);
+  }
+  top = warp_max(top);
+  if (lane == 0) of_warp[warp] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(of_warp[0], of_warp[1]), fmaxf(of_warp[2], of_warp[3]));
+  const float ref = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kWith / 128; ++i) {
+    const float w = ex2_approx(x[i].x - ref);
+    weight[i * 128 + threadIdx.x] = w;
+    sum += w * x[i].y;
+  }
+  sum = warp_sum(sum);
+  if (lane == 0) of_warp[4 + warp] = sum;
+  __syncthreads();
+  sum = of_warp[4] + of_warp[5] + of_warp[6] + of_warp[7];
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = group; k < f.parts; k += kGroups * kAhead) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const float4 v = ahead[i];
+      const float w = k + i * kGroups < f.parts ? weight[k + i * kGroups] : 0.f;
+      acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
+      ahead[i] = sums(k + (kAhead + i) * kGroups);
+    }
+  }
+  of_group[group][col] = acc;
+  __syncthreads();
+  if (group > 0) return;
+#pragma unroll
+  for (int k = 1; k < kGroups; ++k) {
+    const float4 v = of_group[k][col];
+    acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+  }
+  few_put(p, f, at, row, col, acc, top, sum);
+}
+
 // ===================================================================================== forward
 // Two CTAs an SM, so that one's products run under the other's exponentials. Four softmax warps (a thread is a row and all of a block's keys: with two warps to a row, which
 // have to agree on its maximum, 8 x 12 x 1024 x 4096 took 206 us against 176), one that issues products, one that loads. P goes to the second product through TMEM.
@@ -524,25 +878,6 @@ struct FwdOut {
 // 16-byte chunk c of row t of a tile of fp32 sums in shared memory: a warp's rows, which write the same chunk at a time, meet different banks.
 template <int kD>
 __device__ __forceinline__ uint32_t shared_chunk(int t, int c) { return (t * (kD / 4) + (c ^ (t & 15))) * 16; }
-__device__ __forceinline__ uint32_t in_cta(uint32_t smem, int cta) {
-  uint32_t remote;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem), "r"(cta));
-  return remote;
-}
-__device__ __forceinline__ float4 ld_cluster_v4(uint32_t at) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ float2 ld_cluster_v2(uint32_t at) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ void cluster_meet() {
-  __syncwarp();
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // The CTAs of a cluster join their parts of a tile, four values a thread, in the order of the parts; each CTA every so manieth group of rows. All threads of all of them,
 // whatever became of the waits before.
 template <int kD>
@@ -935,7 +1270,6 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 }
 
 // The CTAs that share the tile which `cta` began and did not end, in their order, into `with`; returns how many. By a whole block; at most kWith.
-constexpr int kWith = 512;        // more than there are CTAs of a kernel
 __device__ __forceinline__ int sharers(const Left* left, int cta, int stop, short* with, int* count) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
@@ -1701,8 +2035,71 @@ cudaError_t launch_clusters(void (*kern)(KArgs...), int blocks, int cluster, int
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
+// CTAs to share a tile of sixteen rows, 0 where tiles of 128 are better, and whether as a cluster. Two CTAs are on an SM, and a warp has two chunks at least. A row more than
+// sixteen makes the tensor cores' tile a better bargain as work grows: forward passes of B x H x Sq x Sk, D took, in tiles of sixteen and of 128 rows, with 2 x 12 x 64 x 200, 64
+// (5 chunks an SM) 3.9 and 8.4 us, 3 x 12 x 77 x 1031, 64 (40) 12.0 and 13.0, 32 x 8 x 32 x 509, 64 (55) 13.2 and 17.2, 3 x 12 x 128 x 1031, 64 (64) 12.2 and 13.9, but 3 x 12 x 77 x 1031,
+// 128 (79) 21.3 and 16.2, 32 x 8 x 64 x 509, 64 (111) 23.4 and 17.5. Up to sixteen rows these won at every size: 8 x 32 heads x 4 x 2000 on 8 key heads of 128 15.0 and 16.4,
+// 64 x 32 heads x 1 x 1000 on 8 43.6 and 55.8, 128 x 16 x 1 x 500, 64 44.7 and 68.6, a single 1 x 8 x 1 x 1500, 64 4.8 and 9.2.
+struct FewShape {
+  int parts;
+  bool cluster;
+  long long ml, total;        // floats of workspace
+};
+FewShape few_shape(const CrossParams& p, int D) {
+  FewShape f = {};
+  const int chunks = ceil_div(p.Sk, 2048 / D);
+  const long long tiles = static_cast<long long>(p.B) * p.Hq * ceil_div(p.R, 16);
+  if (p.R > 16 && tiles * chunks > 70ll * sm_count()) return f;
+  long long parts = 2ll * sm_count() / tiles;
+  if (parts > ceil_div(chunks, 8)) parts = ceil_div(chunks, 8);
+  if (parts > kWith) parts = kWith;
+  if (parts < 1) parts = 1;
+  f.cluster = parts <= 8;
+  f.parts = static_cast<int>(parts);
+  if (!f.cluster) {
+    f.ml = round_up(tiles * parts * 16 * D, 32);
+    f.total = f.ml + tiles * parts * 16 * 2;
+  }
+  return f;
+}
+template <int kD>
+int cross_few(const fb_cross_args& a, const CrossParams& p, const FewShape& shape, cudaStream_t stream) {
+  if (shape.total && !a.workspace) return -3;
+  FewArgs f = {};
+  f.q = static_cast<const __nv_bfloat16*>(a.q);
+  f.k = static_cast<const __nv_bfloat16*>(a.k);
+  f.v = static_cast<const __nv_bfloat16*>(a.v);
+  f.o = static_cast<__nv_bfloat16*>(a.o);
+  for (int d = 0; d < 3; ++d) {
+    f.qs[d] = a.q_strides[d];
+    f.ks[d] = a.k_strides[d];
+    f.vs[d] = a.v_strides[d];
+    f.os[d] = a.o_strides[d];
+  }
+  f.stats = a.stats;
+  f.parts = shape.parts;
+  f.by_parts = div_by(f.parts);
+  if (shape.total) {
+    f.part_o = a.workspace;
+    f.part_ml = reinterpret_cast<float2*>(a.workspace + shape.ml);
+  }
+  f.row_tiles = ceil_div(p.R, 16);
+  f.by_rows = div_by(f.row_tiles);
+  f.by_heads = div_by(p.Hq);
+  if (p.mask && (a.stats || !p.mask_bool))        // the largest addends, and the lists for the backward pass
+    if (const cudaError_t err = launch_pdl(cross_live_kernel, dim3(p.B), dim3(256), 0, stream, p)) return static_cast<int>(err);
+  constexpr int smem = Few<kD>::TOTAL, threads = Few<kD>::kWarps * 32;
+  if (const cudaError_t err = allow_smem<cross_few_kernel<kD>>(smem, true)) return static_cast<int>(err);
+  const int tiles = p.B * p.Hq * f.row_tiles, ctas = tiles * f.parts;
+  cudaError_t err = f.parts > 1 && shape.cluster ? launch_clusters(cross_few_kernel<kD>, ctas, f.parts, threads, smem, stream, p, f)
+                                                 : launch_pdl(cross_few_kernel<kD>, dim3(ctas), dim3(threads), static_cast<size_t>(smem), stream, p, f);
+  if (!err && !shape.cluster) err = launch_pdl(cross_few_join_kernel<kD>, dim3(tiles, p.R < 16 ? p.R : 16), dim3(128), 0, stream, p, f);
+  return static_cast<int>(err ? err : cudaGetLastError());
+}
+
 template <int kD>
 int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream_t stream) {
+  if (const FewShape shape = few_shape(p, kD); shape.parts) return cross_few<kD>(a, p, shape, stream);
   CUtensorMap tq, tk, tv;
   int e = make_tmap_rows(&tq, a.q, kD, pack, a.Sq, p.Hq, a.B, a.q_strides[0], a.q_strides[1], a.q_strides[2]);
   if (!e) e = make_tmap_rows(&tk, a.k, kD, 1, a.Sk, a.Hk, a.B, a.k_strides[0], a.k_strides[1], a.k_strides[2]);
@@ -1789,7 +2186,7 @@ extern "C" long long fb_cross_workspace(const fb_cross_args* args, int backward)
   int pack;
   if (!make_cross(*args, p, pack)) return -4;
   const Crews crews = crews_of(p, args->D);
-  return backward ? space_bwd(p, crews, args->D).total : space_fwd(p, crews.rows, args->D).total;
+  return backward ? space_bwd(p, crews, args->D).total : few_shape(p, args->D).parts ? few_shape(p, args->D).total : space_fwd(p, crews.rows, args->D).total;
 }
 extern "C" long long fb_cross_mask_info(const fb_cross_args* args) {
   using namespace fb;
