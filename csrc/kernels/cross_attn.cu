@@ -15,7 +15,13 @@
 // side, so that they stream the same heads out of L2 (with one stretch of all units for each CTA, as long heads of 128 took 287 us against 241). What is left, less
 // than a tile each, is cut into equal stretches of units: no last wave, and few queries over many keys fill the GPU as well. A tile that a stretch's border cuts leaves
 // fp32 sums behind, which a small second launch adds up in the order of the stretches (two calls give the same bits). Where the forward pass has few tiles, the CTAs of a
-// cluster share each of them instead and meet in distributed shared memory, which saves that launch.
+// cluster share each of them instead and meet in distributed shared memory, which saves that launch. Tokens, and whatever else is little work, take a forward kernel of their own
+// in tiles of sixteen rows.
+//
+// What bounds it. Tokens: HBM (5.4 TB/s at 268 MB of keys and values). Forward, heads of 128: the tensor cores' 100 cycles for a step of 16 with both operands in shared memory, and the
+// softmax warps between them (250 us, 1.1 PFLOP/s at 2 x 16 heads x 2048 x 8192). Heads of 64: the softmax warps' chain of loads from TMEM, maximum, exponentials and store, two
+// CTAs an SM (165 us, 0.63 PFLOP/s at 8 x 12 x 1024 x 4096; without its exponentials it would take 121). Backward: seven products in place of five, as keys and rows are
+// worked out apart, so that no sum is added up by atomics (0.8 ms, 0.86 PFLOP/s of the five at 2 x 16 x 2048 x 8192 of 128).
 //
 // Statistics, sums and products are fp32; P and dS are rounded to bf16 once, as operands of the tensor cores.
 #include <cuda.h>
@@ -1994,7 +2000,7 @@ int parts_of(const CrossParams& p) {
   if (p.key_blocks <= 4 || tiles * 2 > slots) return 0;
   long long c = slots / tiles;
   if (c > p.key_blocks / 2) c = p.key_blocks / 2;
-  if (c > 8) c = 8;        // (clusters of sixteen find room on few SMs at a time: one token over 32768 keys 94 us against 62 in stretches)
+  if (c > 8) c = 8;        // (clusters of sixteen find room on few SMs at a time: 16 tiles of 256 blocks took 94 us against 62 in stretches)
   return ceil_div(p.key_blocks, c) > tiles * p.key_blocks / slots + 4 ? 0 : static_cast<int>(c);
 }
 FwdSpace space_fwd(const CrossParams& p, const Crew& c, int D) {
