@@ -492,13 +492,13 @@ __device__ __forceinline__ void cluster_meet() {
 // ============================================================================ forward, few rows
 // Tiles of sixteen rows, for a token of each sequence and for whatever is as little work. HBM bounds a token, and how long a block of keys takes: a tcgen05 tile has 128 rows
 // whatever is in them, and its chain of copy, scores, TMEM, probabilities and product took 1.7 us a block with one warp at work. Here each warp is on its own: it streams
-// chunks of keys through a ring of its own with cp.async, two in flight, and multiplies them with mma.sync; warps meet at the end, the CTAs that share a tile in
+// chunks of keys through a ring of its own with cp.async, one or two in flight, and multiplies them with mma.sync; warps meet at the end, the CTAs that share a tile in
 // distributed shared memory or, more than eight of them, by a second launch. Chunks go round all warps of a tile, so that padding at its end takes from each the same.
 // Masks are read as the chunks are asked for: absent keys are not copied but filled with zeros, chunks without a key left out.
-// One token of 16 x 8 heads of 64 over up to 1500 keys 10.1 us (37 MB; in 128-row tiles 18.4), of 4 x 32 heads of 128 on 4 key heads over 32768 49.9 (5.4 TB/s; 61.3).
-template <int kD>
+// One token of 16 x 8 heads of 64 over up to 1500 keys 9.2 us (37 MB; in 128-row tiles 18.4), of 4 x 32 heads of 128 on 4 key heads over 32768 49.9 (5.4 TB/s; 61.3).
+template <int kD, int kPerSm>
 struct Few {
-  static constexpr int kWarps = 4, kStages = 3;
+  static constexpr int kWarps = 4, kStages = kPerSm == 3 ? 2 : 3;        // CTAs on an SM, and the stages that shared memory has room for then
   static constexpr int kChunk = 2048 / kD;                  // keys
   static constexpr int kTile = kChunk * kD * 2;             // bytes of K, and of V
   static constexpr int TAB = 2 * kTile, STAGE = TAB + kChunk * 8, WARP = kStages * STAGE;
@@ -570,9 +570,9 @@ __device__ __forceinline__ void few_put(const CrossParams& p, const FewArgs& f, 
   *reinterpret_cast<uint2*>(out_row(p, f.o, f.os[0], f.os[1], f.os[2], at.b, at.h, at.row0 + row) + col * 4) = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
 }
 
-template <int kD>
-__global__ void __launch_bounds__(Few<kD>::kWarps * 32, 2) cross_few_kernel(const CrossParams p, const FewArgs f) {
-  using L = Few<kD>;
+template <int kD, int kPerSm>
+__global__ void __launch_bounds__(Few<kD, kPerSm>::kWarps * 32, kPerSm) cross_few_kernel(const CrossParams p, const FewArgs f) {
+  using L = Few<kD, kPerSm>;
   extern __shared__ __align__(128) uint8_t ring[];
   constexpr int kChunk = L::kChunk, kStages = L::kStages, kCols = kD / 8;        // 16-byte columns of a row
   const int warp = uniform_warp(), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -598,7 +598,7 @@ __global__ void __launch_bounds__(Few<kD>::kWarps * 32, 2) cross_few_kernel(cons
   const __nv_bfloat16 *k0 = f.k + b * f.ks[0] + hk * f.ks[2], *v0 = f.v + b * f.vs[0] + hk * f.vs[2];
   const float sc = p.scale * kLog2e, base = p.mask && !p.mask_bool ? __ldcg(p.base + b) : 0.f;
 
-  // The mask is read a chunk ahead of the copies, these two chunks ahead of the products.
+  // The mask is read a chunk ahead of the copies, these one or two chunks ahead of the products.
   int c = part * L::kWarps + warp, have = 0;
   unsigned tabled = 0;         // a bit for each stage
   const auto entry_of = [&](int c) {
@@ -2041,13 +2041,16 @@ cudaError_t launch_clusters(void (*kern)(KArgs...), int blocks, int cluster, int
   return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
-// CTAs to share a tile of sixteen rows, 0 where tiles of 128 are better, and whether as a cluster. Two CTAs are on an SM, and a warp has two chunks at least. A row more than
+// CTAs to share a tile of sixteen rows, 0 where tiles of 128 are better, and whether as a cluster. A warp has two chunks at least. A row more than
 // sixteen makes the tensor cores' tile a better bargain as work grows: forward passes of B x H x Sq x Sk, D took, in tiles of sixteen and of 128 rows, with 2 x 12 x 64 x 200, 64
-// (5 chunks an SM) 3.9 and 8.4 us, 3 x 12 x 77 x 1031, 64 (40) 12.0 and 13.0, 32 x 8 x 32 x 509, 64 (55) 13.2 and 17.2, 3 x 12 x 128 x 1031, 64 (64) 12.2 and 13.9, but 3 x 12 x 77 x 1031,
+// (5 chunks an SM) 3.9 and 8.4 us, 3 x 12 x 77 x 1031, 64 (40) 11.7 and 13.0, 32 x 8 x 32 x 509, 64 (55) 13.2 and 17.2, 3 x 12 x 128 x 1031, 64 (64) 12.2 and 13.9, but 3 x 12 x 77 x 1031,
 // 128 (79) 21.3 and 16.2, 32 x 8 x 64 x 509, 64 (111) 23.4 and 17.5. Up to sixteen rows these won at every size: 8 x 32 heads x 4 x 2000 on 8 key heads of 128 15.0 and 16.4,
-// 64 x 32 heads x 1 x 1000 on 8 43.6 and 55.8, 128 x 16 x 1 x 500, 64 44.7 and 68.6, a single 1 x 8 x 1 x 1500, 64 4.8 and 9.2.
+// 64 x 32 heads x 1 x 1000 on 8 43.7 and 55.8, 128 x 16 x 1 x 500, 64 41.4 and 68.6, a single 1 x 8 x 1 x 1500, 64 4.8 and 9.2.
+//
+// With heads of 64 three CTAs fit an SM, with two stages to a warp's ring in place of three. That is better where there is work for the third (tokens of 16 x 8 over 1500 9.2 us against
+// 10.1, 3 x 12 x 32 x 1031 8.7 and 11.3, 128 x 16 x 1 x 500 41.4 and 44.7), two better where there is not (4 x 8 x 4 x 2000 6.9 and 6.1, 3 x 12 x 128 x 1031 15.3 and 12.2).
 struct FewShape {
-  int parts;
+  int parts, per_sm;
   bool cluster;
   long long ml, total;        // floats of workspace
 };
@@ -2056,10 +2059,14 @@ FewShape few_shape(const CrossParams& p, int D) {
   const int chunks = ceil_div(p.Sk, 2048 / D);
   const long long tiles = static_cast<long long>(p.B) * p.Hq * ceil_div(p.R, 16);
   if (p.R > 16 && tiles * chunks > 70ll * sm_count()) return f;
-  long long parts = 2ll * sm_count() / tiles;
-  if (parts > ceil_div(chunks, 8)) parts = ceil_div(chunks, 8);
-  if (parts > kWith) parts = kWith;
-  if (parts < 1) parts = 1;
+  const auto parts_at = [&](int per_sm) {
+    long long n = static_cast<long long>(per_sm) * sm_count() / tiles;
+    if (n > ceil_div(chunks, 8)) n = ceil_div(chunks, 8);
+    if (n > kWith) n = kWith;
+    return n < 1 ? 1 : n;
+  };
+  f.per_sm = D == 64 && (tiles > 2ll * sm_count() || parts_at(3) > parts_at(2)) ? 3 : 2;
+  const long long parts = parts_at(f.per_sm);
   f.cluster = parts <= 8;
   f.parts = static_cast<int>(parts);
   if (!f.cluster) {
@@ -2068,7 +2075,7 @@ FewShape few_shape(const CrossParams& p, int D) {
   }
   return f;
 }
-template <int kD>
+template <int kD, int kPerSm>
 int cross_few(const fb_cross_args& a, const CrossParams& p, const FewShape& shape, cudaStream_t stream) {
   if (shape.total && !a.workspace) return -3;
   FewArgs f = {};
@@ -2094,18 +2101,23 @@ int cross_few(const fb_cross_args& a, const CrossParams& p, const FewShape& shap
   f.by_heads = div_by(p.Hq);
   if (p.mask && (a.stats || !p.mask_bool))        // the largest addends, and the lists for the backward pass
     if (const cudaError_t err = launch_pdl(cross_live_kernel, dim3(p.B), dim3(256), 0, stream, p)) return static_cast<int>(err);
-  constexpr int smem = Few<kD>::TOTAL, threads = Few<kD>::kWarps * 32;
-  if (const cudaError_t err = allow_smem<cross_few_kernel<kD>>(smem, true)) return static_cast<int>(err);
+  constexpr auto kern = cross_few_kernel<kD, kPerSm>;
+  constexpr int smem = Few<kD, kPerSm>::TOTAL, threads = Few<kD, kPerSm>::kWarps * 32;
+  if (const cudaError_t err = allow_smem<kern>(smem, true)) return static_cast<int>(err);
   const int tiles = p.B * p.Hq * f.row_tiles, ctas = tiles * f.parts;
-  cudaError_t err = f.parts > 1 && shape.cluster ? launch_clusters(cross_few_kernel<kD>, ctas, f.parts, threads, smem, stream, p, f)
-                                                 : launch_pdl(cross_few_kernel<kD>, dim3(ctas), dim3(threads), static_cast<size_t>(smem), stream, p, f);
+  cudaError_t err = f.parts > 1 && shape.cluster ? launch_clusters(kern, ctas, f.parts, threads, smem, stream, p, f)
+                                                 : launch_pdl(kern, dim3(ctas), dim3(threads), static_cast<size_t>(smem), stream, p, f);
   if (!err && !shape.cluster) err = launch_pdl(cross_few_join_kernel<kD>, dim3(tiles, p.R < 16 ? p.R : 16), dim3(128), 0, stream, p, f);
   return static_cast<int>(err ? err : cudaGetLastError());
 }
 
 template <int kD>
 int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream_t stream) {
-  if (const FewShape shape = few_shape(p, kD); shape.parts) return cross_few<kD>(a, p, shape, stream);
+  if (const FewShape shape = few_shape(p, kD); shape.parts) {
+    if constexpr (kD == 64)
+      if (shape.per_sm == 3) return cross_few<64, 3>(a, p, shape, stream);
+    return cross_few<kD, 2>(a, p, shape, stream);
+  }
   CUtensorMap tq, tk, tv;
   int e = make_tmap_rows(&tq, a.q, kD, pack, a.Sq, p.Hq, a.B, a.q_strides[0], a.q_strides[1], a.q_strides[2]);
   if (!e) e = make_tmap_rows(&tk, a.k, kD, 1, a.Sk, a.Hk, a.B, a.k_strides[0], a.k_strides[1], a.k_strides[2]);
