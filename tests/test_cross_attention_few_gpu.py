@@ -106,3 +106,33 @@ def test_several_tiles_of_rows(C, shape):
     mask[0, :Sk // 3] = False
     check(C, q, k, v, do, mask)
     check(C, q, k, v, do, torch.where(mask, torch.randn(B, Sk, device="cuda"), float("-inf")))
+
+
+@pytest.mark.parametrize("shape", [(2, 1, 1500, 8, 8, 64), (1, 1, 9000, 2, 1, 128), (1, 2, 9000, 2, 2, 64), (160, 1, 90, 4, 4, 64)], ids=str)
+def test_captured_tokens_replay_over_new_masks(C, shape):
+    """Two graphs of one pool, in turn on two streams: a tile's parts meet in a cluster, by a second launch, or there is one."""
+    B, Sq, Sk = shape[:3]
+    q, k, v, _ = case(*shape, seed=21)
+    masks = [torch.zeros(B, Sk, dtype=torch.bool, device="cuda"), torch.zeros(B, Sk, device="cuda")]
+    side, pool, made = torch.cuda.Stream(), torch.cuda.graph_pool_handle(), []
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for m in masks:
+            ops.cross_attention(q, k, v, m)
+    torch.cuda.synchronize()
+    for m in masks:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool, stream=side):
+            o = ops.cross_attention(q, k, v, m)
+        made.append((graph, o))
+    g = torch.Generator(device="cuda").manual_seed(22)
+    for i in range(6):
+        masks[0].copy_(torch.rand(B, Sk, generator=g, device="cuda") < 0.2 * i)
+        masks[1].copy_(torch.randn(B, Sk, generator=g, device="cuda").masked_fill_(~masks[0], float("-inf")))
+        q.copy_(torch.randn(q.shape, generator=g, device="cuda"))
+        torch.cuda.synchronize()
+        for (graph, o), m in zip(made, masks):
+            with torch.cuda.stream(side if i % 2 else torch.cuda.current_stream()):
+                graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(o, ops.cross_attention(q, k, v, m))
