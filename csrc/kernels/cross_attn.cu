@@ -38,6 +38,14 @@ namespace {
 constexpr int kKeys = 128;                  // keys of a block
 constexpr float kHuge = 1.2676506e30f;      // 2^100
 constexpr int kWith = 512;                  // more than there are CTAs of a kernel that share a tile
+constexpr float kLowest = -3.402823466e38f;
+
+// A row's maximum is -inf where it has no key, and at least kLowest (`seen`) where it has any, so that the two stay apart when parts are joined. No key: zeros, and a
+// statistic of +inf, which makes every probability 2^-inf = 0. Keys whose scores are all -inf: a sum of zero, 0 / 0, NaN, as their softmax is, and a statistic of -inf, which
+// makes the backward pass's probabilities 2^(-inf + inf).
+__device__ __forceinline__ float seen(float top) { return fmaxf(top, kLowest); }
+__device__ __forceinline__ float inverse_of(float top, float sum) { return top == -INFINITY ? 0.f : 1.f / sum; }
+__device__ __forceinline__ float statistic_of(float top, float sum) { return top == -INFINITY ? INFINITY : top + log2f(sum); }
 
 struct CrossParams {
   int B, Hq, Hk, R, Sk;             // Hq = H / pack rows of heads; R = Sq * pack rows each
@@ -565,8 +573,8 @@ __device__ __forceinline__ void few_join(int of, Ml ml_of, Sums sums_of, float4&
   }
 }
 __device__ __forceinline__ void few_put(const CrossParams& p, const FewArgs& f, const FewTile& at, int row, int col, float4 acc, float top, float sum) {
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (f.stats && col == 0) f.stats[(static_cast<long long>(at.b) * p.Hq + at.h) * p.R + at.row0 + row] = sum == 0.f ? INFINITY : top + log2f(sum);
+  const float inv = inverse_of(top, sum);
+  if (f.stats && col == 0) f.stats[(static_cast<long long>(at.b) * p.Hq + at.h) * p.R + at.row0 + row] = statistic_of(top, sum);
   *reinterpret_cast<uint2*>(out_row(p, f.o, f.os[0], f.os[1], f.os[2], at.b, at.h, at.row0 + row) + col * 4) = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
 }
 
@@ -727,7 +735,7 @@ __global__ void __launch_bounds__(Few<kD, kPerSm>::kWarps * 32, kPerSm) cross_fe
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int row = warp * 16 + g + r * 8;
-    if (t == 0) ml[row] = make_float2(m[r], l[r]);
+    if (t == 0) ml[row] = make_float2(have ? seen(m[r]) : m[r], l[r]);
 #pragma unroll
     for (int n = 0; n < kD / 8; ++n) *reinterpret_cast<float2*>(sums + row * L::kRow + n * 8 + t * 2) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
   }
@@ -908,9 +916,9 @@ __device__ __forceinline__ void join_cluster(const CrossParams& p, const FwdOut&
       l += w * x.y;
       acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = inverse_of(m, l);
     *reinterpret_cast<uint2*>(out_row(p, out.o, out.osb, out.oss, out.osh, task.b, task.h, row0 + t) + c * 4) = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
-    if (out.stats && c == 0) out.stats[(static_cast<long long>(task.b) * p.Hq + task.h) * p.R + row0 + t] = l == 0.f ? INFINITY : m + log2f(l);
+    if (out.stats && c == 0) out.stats[(static_cast<long long>(task.b) * p.Hq + task.h) * p.R + row0 + t] = statistic_of(m, l);
   }
   cluster_meet();        // shared memory is there until all have read it
 }
@@ -1203,11 +1211,11 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (ok && works) {
         tc_fence_after_sync();
         const long long row = (static_cast<long long>(b) * p.Hq + h) * p.R + row0 + t, slot = blockIdx.x * 2ll + task.slot;
-        const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        if (i0 < i1) m = seen(m);
+        const float inv = whole ? inverse_of(m, l) : 1.f;
         if (out.parts) tab[t] = make_float2(m, l);
         else if (!whole) out.part_ml[slot * 128 + t] = make_float2(m, l);
-        // a row that no key takes part in: +inf, which makes every probability 2^-inf = 0
-        else if (out.stats && t < rows) out.stats[row] = l == 0.f ? INFINITY : m + log2f(l);
+        else if (out.stats && t < rows) out.stats[row] = statistic_of(m, l);
         float* po = whole ? nullptr : out.part_o + (slot * 128 + t) * kD;
 #pragma unroll
         for (int c0 = 0; c0 < kD; c0 += 32) {
@@ -1323,10 +1331,10 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const CrossParams p, co
     l += w * ml.y;
     acc.x += w * v.x; acc.y += w * v.y; acc.z += w * v.z; acc.w += w * v.w;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = inverse_of(m, l);
   __nv_bfloat16* dst = out_row(p, out.o, out.osb, out.oss, out.osh, first.b, h, row0 + t) + c;
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack2(acc.x * inv, acc.y * inv), pack2(acc.z * inv, acc.w * inv));
-  if (out.stats && c == 0) out.stats[(static_cast<long long>(first.b) * p.Hq + h) * p.R + row0 + t] = l == 0.f ? INFINITY : m + log2f(l);
+  if (out.stats && c == 0) out.stats[(static_cast<long long>(first.b) * p.Hq + h) * p.R + row0 + t] = statistic_of(m, l);
 }
 
 // ==================================================================================== backward

@@ -15,7 +15,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
 
     `Hk` divides `H`: query head `h` reads key head `h // (H / Hk)`, whose gradient is the sum over them. `scale` is 1 / sqrt(D) unless given. `mask` is of keys, [B, Sk],
     [1, Sk] or [B, 1, 1, Sk]: bool, True for the keys that take part, or floating point, added to the scores. A key at False or -inf is absent, whatever its key and
-    value hold, and gets no gradient; a query without any key gets zeros. bf16 heads of 64 and 128 on a GPU run on the kernel, at any size, others as plain
+    value hold, and gets no gradient; a query without any key gets zeros, one whose keys' scores are all -inf gets NaN. bf16 heads of 64 and 128 on a GPU run on the kernel, at any size, others as plain
     products in 32 bits (64 for fp64)."""
     if FLAGS.native and torch.is_tensor(q) and q.is_cuda and q.dim() == 4:
         o = _C().cross_attention(q, k, v, mask, float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1] or 1))
@@ -66,7 +66,8 @@ def _plain(q, k, v, mask, scale):
         p = s
     else:
         top = s.detach().amax(-1, keepdim=True)
-        p = torch.exp(s - top.masked_fill(top == float("-inf"), 0.0))
+        none = absent.all(-1)[:, None, None, None] if absent is not None else None      # zeros without a key; scores that are all -inf are NaN, as their softmax is
+        p = torch.exp(s - (top if none is None else top.masked_fill(none, 0.0)))
         total = p.sum(-1, keepdim=True)
-        p = p / torch.where(total == 0, torch.ones_like(total), total)
+        p = p / (total if none is None else total.masked_fill(none, 1.0))
     return (p @ vh).reshape(B, H, Sq, D).transpose(1, 2).to(q.dtype)

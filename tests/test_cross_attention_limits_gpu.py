@@ -1,0 +1,41 @@
+"""Attention over another sequence at the limits of what scores, masks and gradients may hold, on every way that a tile's rows take: one CTA, a cluster, parts that a
+second launch joins, in tiles of sixteen and of 128 rows."""
+import pytest
+import torch
+
+from flodl_b200 import ops
+from test_cross_attention_gpu import C, case  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+WAYS = [  # B, Sq, Sk, H, Hk, D
+    (2, 2, 40, 2, 2, 64), (2, 1, 1500, 8, 8, 64), (2, 1, 9000, 2, 1, 128), (160, 1, 90, 4, 4, 64),          # tiles of sixteen rows
+    (24, 130, 300, 16, 16, 64), (2, 120, 1300, 12, 12, 64), (2, 130, 20000, 2, 1, 128), (2, 400, 9000, 2, 1, 64), (2, 100, 1400, 160, 80, 64),
+]
+
+
+@pytest.mark.parametrize("shape", WAYS, ids=str)
+def test_scores_that_are_all_minus_infinity_are_not_rows_without_a_key(C, shape):
+    """Their softmax and its gradients are NaN; a batch row without a key has zeros; one key with a score among them carries the row."""
+    B, Sq, Sk, H, Hk, D = shape
+    q, k, v, do = case(*shape, seed=1)
+    q, group = q.abs(), H // Hk
+    k[0, :, 0] = float("-inf")
+    want = v[0, Sk // 2, 0]
+    mask = torch.ones(B, Sk, dtype=torch.bool, device="cuda")
+    mask[0, :Sk // 3] = False
+    mask[-1] = False
+    for m in (None, mask, torch.zeros(B, Sk, device="cuda").masked_fill(~mask, float("-inf"))):
+        leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+        o = ops.cross_attention(*leaves, m)
+        dq, dk, dv = torch.autograd.grad(o, leaves, do)
+        assert o[0, :, :group].isnan().all() and not o[0, :, group:].isnan().any() and not o[1:].isnan().any()
+        assert dq[0, :, :group].isnan().all() and not dq[0, :, group:].isnan().any() and not dq[1:].isnan().any()
+        there = slice(Sk // 3, None) if m is not None else slice(None)
+        assert dk[0, there, 0].isnan().all() and dv[0, there, 0].isnan().all() and not dk[0, :, 1:].isnan().any() and not dv[1:].isnan().any()
+        if m is not None:
+            assert (o[-1] == 0).all() and (dq[-1] == 0).all() and (dk[-1] == 0).all() and (dv[-1] == 0).all()
+    k[0, Sk // 2, 0] = 1.0
+    for m in (None, mask):
+        assert torch.equal(ops.cross_attention(q, k, v, m)[0, :, :group], want.expand(Sq, group, D))
+    assert C.read_status(0) == 0
