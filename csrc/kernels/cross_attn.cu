@@ -1743,6 +1743,7 @@ __device__ __forceinline__ void bwd_softmax(BwdBars& bar, const CrossParams& p, 
     const int c0 = (kKeys ? w & 1 : w) * kStep;
     const uint32_t acc = tmem + (is_v ? L::ACC0 : L::ACC1) + lanes + c0;
     const float mul = is_v ? 1.f : p.scale;
+    const bool absent = stays_masked && entry.y == -INFINITY;        // no gradient, whatever its probability of zero has met: a row's NaN or infinity is no number times zero
     float* part = nullptr;
     __nv_bfloat16* to = nullptr;
     if (!whole) {
@@ -1763,7 +1764,7 @@ __device__ __forceinline__ void bwd_softmax(BwdBars& bar, const CrossParams& p, 
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         asm volatile("" : "+r"(v[e]));
-        f[e] = __uint_as_float(v[e]) * mul;
+        f[e] = absent ? 0.f : __uint_as_float(v[e]) * mul;
       }
       if (!whole) {
 #pragma unroll

@@ -39,3 +39,20 @@ def test_scores_that_are_all_minus_infinity_are_not_rows_without_a_key(C, shape)
     for m in (None, mask):
         assert torch.equal(ops.cross_attention(q, k, v, m)[0, :, :group], want.expand(Sq, group, D))
     assert C.read_status(0) == 0
+
+
+@pytest.mark.parametrize("shape", WAYS, ids=str)
+def test_absent_keys_get_no_gradient_from_rows_that_are_no_numbers(C, shape):
+    """A NaN in a query, an infinity in a result's gradient: what such rows give a key that takes part is no number, but an absent key still gets zeros."""
+    B, Sq, Sk, H, Hk, D = shape
+    q, k, v, do = case(*shape, seed=2)
+    mask = torch.rand(B, Sk, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) < 0.5
+    mask[:, 0] = True
+    q[0, 0, 0, 3] = float("nan")
+    do[1, Sq - 1, H - 1, 5] = float("inf")
+    for m in (mask, torch.zeros(B, Sk, device="cuda").masked_fill(~mask, float("-inf"))):
+        leaves = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+        dk, dv = torch.autograd.grad(ops.cross_attention(*leaves, m), leaves[1:], do)
+        assert (dk[~mask] == 0).all() and (dv[~mask] == 0).all()
+        assert dk[0, 0, 0].isnan().all() and dv[0, 0, 0].isnan().all() and not dv[1, 0, Hk - 1].isfinite().all()
+    assert C.read_status(0) == 0
