@@ -336,6 +336,14 @@ struct CrossFn : public torch::autograd::Function<CrossFn> {
   }
 };
 
+// A 64-bit mask for the kernel, relative to each row's largest before it is rounded to 32 bits; finite values stay finite. A largest beyond 2^100 leaves nothing of the scores, nor of keys
+// that are any further away: it is told from the others by one that is as large in 32 bits.
+Tensor narrowed(const Tensor& mask) {
+  const Tensor top = mask.amax(-1, true), rest = mask - top.masked_fill(top.isinf(), 0.0);
+  const Tensor far = at::where(rest == 0, top.clamp(-0x1p101, 0x1p101), -FLT_MAX);
+  return at::where(mask.isinf(), mask, at::where(top.abs() >= 0x1p100, far, rest.clamp(-FLT_MAX, FLT_MAX)));
+}
+
 // The rules of a call to `ops.cross_attention`, and the call. `mask`: bool or floating point [B or 1, Sk], or with two dimensions of one between.
 std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask_in, double scale) {
   if (!q.is_cuda() || q.dim() != 4 || k.dim() != 4 || v.dim() != 4) return std::nullopt;
@@ -353,7 +361,7 @@ std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Te
     if (mask.device() != q.device() || (mask.scalar_type() != at::kBool && !mask.is_floating_point())) return std::nullopt;
     if (mask.dim() == 4 && mask.size(1) == 1 && mask.size(2) == 1) mask = mask.select(1, 0).select(1, 0);
     if (mask.dim() != 2 || mask.size(1) != Sk || (mask.size(0) != 1 && mask.size(0) != B)) return std::nullopt;
-    if (mask.scalar_type() == at::kDouble) mask = at::where(mask.isinf(), mask, mask.clamp(-FLT_MAX, FLT_MAX));       // finite values stay finite
+    if (mask.scalar_type() == at::kDouble) mask = narrowed(mask);
     if (mask.scalar_type() != at::kBool) mask = mask.to(at::kFloat);
     if (Sk > 1 && mask.stride(1) != 1) mask = mask.contiguous();
   }

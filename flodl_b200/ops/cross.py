@@ -44,7 +44,7 @@ def _plain(q, k, v, mask, scale):
     wide = torch.float64 if q.dtype == torch.float64 else torch.float32
     qh = q.to(wide).transpose(1, 2).reshape(B, Hk, H // Hk * Sq, D)
     kh, vh = (t.to(wide).transpose(1, 2) for t in (k, v))
-    add = absent = None
+    add = alone = absent = None
     if mask is not None:
         m = mask
         if m.device != q.device or not (m.dtype == torch.bool or m.is_floating_point()):
@@ -54,12 +54,17 @@ def _plain(q, k, v, mask, scale):
         if m.dim() != 2 or m.shape[1] != Sk or m.shape[0] not in (1, B):
             raise TensorError(f"mask must be of keys, [{B}, {Sk}], not {list(mask.shape)}")
         absent = ~m if m.dtype == torch.bool else m == float("-inf")
-        if m.dtype != torch.bool:
-            add = m.to(wide).masked_fill(absent, 0.0)[:, None, None]
+        if m.dtype != torch.bool and Sk > 0:
+            # Relative to the row's largest, before anything is rounded to fewer bits: an addend that a row's keys share costs its scores none. Finite values stay
+            # finite, and one beyond 2^100 leaves nothing of its score, as in 64 bits.
+            m = m.to(torch.promote_types(m.dtype, wide))
+            top = m.detach().amax(-1, keepdim=True)
+            add = (m - top.masked_fill(top.isinf(), 0.0)).masked_fill(absent, 0.0).clamp(min=torch.finfo(wide).min).to(wide)[:, None, None]
+            alone = (m.detach().abs() >= 2.0 ** 100)[:, None, None]
         kh, vh = (t.masked_fill(absent[:, None, :, None], 0.0) for t in (kh, vh))
     s = (qh @ kh.transpose(-1, -2)) * scale
     if add is not None:
-        s = s + add
+        s = torch.where(alone, s - s.detach(), s) + add
     if absent is not None:
         s = s.masked_fill(absent[:, None, None], float("-inf"))
     if Sk == 0:

@@ -56,3 +56,31 @@ def test_absent_keys_get_no_gradient_from_rows_that_are_no_numbers(C, shape):
         assert (dk[~mask] == 0).all() and (dv[~mask] == 0).all()
         assert dk[0, 0, 0].isnan().all() and dv[0, 0, 0].isnan().all() and not dv[1, 0, Hk - 1].isfinite().all()
     assert C.read_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.bfloat16, 80), (torch.float16, 64), (torch.float32, 64)])
+@pytest.mark.parametrize("kind,value", [(torch.float64, -1e300), (torch.float64, -1e9), (torch.float64, 2.0 ** 30), (torch.float32, -1e9), (torch.float16, -60000.0)], ids=str)
+def test_addends_that_a_row_shares(C, dtype, D, kind, value):
+    """By the kernel and by the plain form, which takes the other types and heads: as by the plain form in 64 bits; of a 64-bit mask also what is behind a large one."""
+    q, k, v, _ = (t.to(dtype) for t in case(2, 5, 300, 4, 2, D, seed=4))
+    add = torch.full((2, 300), value, dtype=kind, device="cuda")
+    add[0, 250:] = float("-inf")
+    if kind == torch.float64 and abs(value) < 1e10:
+        add[1] += torch.randn(300, device="cuda", dtype=torch.float64, generator=torch.Generator(device="cuda").manual_seed(5))
+    got = ops.cross_attention(q, k, v, add)
+    with torch.no_grad():
+        ops.set_native(False)
+        try:
+            want = ops.cross_attention(*(t.double() for t in (q, k, v)), add)
+        finally:
+            ops.set_native(True)
+    # bf16: P rounded once by the kernel, and the result; otherwise the result and fp32 sums
+    bound = (2.0 ** -8 + 2.0 ** -12 if dtype == torch.bfloat16 else 2.0 ** -16) * v.double().abs().max() + torch.finfo(dtype).eps / 2 * want.abs()
+    assert ((got.double() - want).abs() <= bound).all()
+    assert C.read_status(0) == 0
+
+
+def test_beyond_all_scores_the_largest_addend_decides(C):
+    q, k, v, _ = case(1, 2, 3, 1, 1, 64, seed=6)
+    for add in ([-2e300, -1e300, -2e300], [1e31, 1.0000001e31, -1e31], [-1e38, 5.0, -1e300]):
+        assert torch.equal(ops.cross_attention(q, k, v, torch.tensor([add], dtype=torch.float64, device="cuda"))[0], v[0, 1].expand(2, 1, 64))
