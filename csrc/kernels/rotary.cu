@@ -6,8 +6,8 @@
 //
 // An item is the pairs of one thread: kVec values of the first half and the kVec they turn with (or 2 kVec neighbours), two 16-byte accesses where the
 // addresses allow. A block takes a few tokens with all their heads: sines and cosines of a token are worked out once, into shared memory, behind the loads of the
-// values. Angles are turns in 64 bits, reduced to half a turn before they become fp32, so any position is as exact as the first; that costs one 64-bit product and one
-// rounding a pair and token, which the heads share. Several heads are one row each of the same launch: q, k and, of a packed projection, v, which is copied.
+// values. Angles are turns, reduced to half a turn before they become fp32, and known to fp32's last bit at any position (turn_of); that costs some ten 64-bit
+// instructions a pair and token, which the heads share. Several heads are one row each of the same launch: q, k and, of a packed projection, v, which is copied.
 // With the norm a row's items lie in neighbouring lanes, so that its sums are shuffles, and a thread always holds the same columns, so that dw stays in registers;
 // blocks then walk over the tokens, and their partial sums are added up in their order by a second launch (two calls give the same bits).
 // What bounds it: without the norm HBM, every value is read once and written once: 34 us for fp32 queries and keys [2, 8191, 12, 64], 5.9 TB/s. With the norm the
@@ -177,6 +177,20 @@ __device__ __forceinline__ float group_sum(float v, int group) {
   return v;
 }
 
+// Cosine and sine of x f, position times radians. The turns x f / (2 pi) are a product whose every factor and rounding is carried as two numbers, so that what is left of
+// them behind the whole turns is exact to 2^-52 for any whole position. sincospif takes its fp32 part; the rest, below 2^-25, turns the result once more, to first order.
+__device__ __forceinline__ void turn_of(double x, double f, float& cs, float& sn) {
+  constexpr double kHi = 0x1.45f306dc9c883p-3, kLo = -0x1.6b01ec5417056p-57;        // 1 / (2 pi)
+  const double c = __dmul_rn(f, kHi), c_lo = fma(f, kHi, -c) + f * kLo;             // turns a position
+  const double t = __dmul_rn(x, c), t_lo = fma(x, c, -t) + x * c_lo;
+  const double half = 2.0 * ((t - rint(t)) + t_lo);
+  const float a = static_cast<float>(half), rest = static_cast<float>(half - a) * 3.14159265f;
+  float s0, c0;
+  sincospif(a, &s0, &c0);
+  cs = fmaf(-rest, s0, c0);
+  sn = fmaf(rest, c0, s0);
+}
+
 // One item in flight.
 template <typename T, int kVec, bool kBoth>
 struct Item {
@@ -267,9 +281,8 @@ __global__ void __launch_bounds__(kThreads, kNorm ? 2 : 3) rotary_kernel(const f
         for (int e = threadIdx.x; e < n_tok * pairs; e += kThreads) {
           const int t = g.by_pairs(e), b = g.by_seq(tok0 + t), s = tok0 + t - b * p.S;
           const long long pos = p.positions ? p.positions[b * p.pos_strides[0] + s * p.pos_strides[1]] : s;
-          const double turns = static_cast<double>(pos + p.offset) * (p.freqs[e - t * pairs] * 0.15915494309189533577);      // 1 / (2 pi)
           float sn, cs;
-          sincospif(2.f * static_cast<float>(turns - rint(turns)), &sn, &cs);
+          turn_of(static_cast<double>(pos + p.offset), p.freqs[e - t * pairs], cs, sn);
           float* to = turn + t * 2 * g.row + e - t * pairs;
           to[0] = cs * p.amplitude;
           to[g.row] = (kBwd ? -sn : sn) * p.amplitude;
