@@ -119,33 +119,41 @@ __device__ __forceinline__ void load_weights(const float* w, const ItemAt& at, f
   }
 }
 
-// o = a b + c for kN values, two an instruction.
+// o = a b + c, a b and a s for kN values, two an instruction. None flushes subnormal values, as the build's own arithmetic does: a turn by nothing gives back what came.
+__device__ __forceinline__ F2 whole_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 whole_mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
 template <int kN>
 __device__ __forceinline__ void v_fma(float (&o)[kN], const float (&a)[kN], const float (&b)[kN], const float (&c)[kN]) {
   if constexpr (kN == 1) {
-    o[0] = fmaf(a[0], b[0], c[0]);
+    asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(o[0]) : "f"(a[0]), "f"(b[0]), "f"(c[0]));
   } else {
 #pragma unroll
-    for (int j = 0; j < kN; j += 2) f2_get(f2_fma(f2_make(a[j], a[j + 1]), f2_make(b[j], b[j + 1]), f2_make(c[j], c[j + 1])), o[j], o[j + 1]);
+    for (int j = 0; j < kN; j += 2) f2_get(whole_fma(f2_make(a[j], a[j + 1]), f2_make(b[j], b[j + 1]), f2_make(c[j], c[j + 1])), o[j], o[j + 1]);
   }
 }
 template <int kN>
 __device__ __forceinline__ void v_mul(float (&o)[kN], const float (&a)[kN], const float (&b)[kN]) {
   if constexpr (kN == 1) {
-    o[0] = a[0] * b[0];
+    asm("mul.rn.f32 %0, %1, %2;" : "=f"(o[0]) : "f"(a[0]), "f"(b[0]));
   } else {
 #pragma unroll
-    for (int j = 0; j < kN; j += 2) f2_get(f2_mul(f2_make(a[j], a[j + 1]), f2_make(b[j], b[j + 1])), o[j], o[j + 1]);
+    for (int j = 0; j < kN; j += 2) f2_get(whole_mul(f2_make(a[j], a[j + 1]), f2_make(b[j], b[j + 1])), o[j], o[j + 1]);
   }
 }
 template <int kN>
 __device__ __forceinline__ void v_scale(float (&o)[kN], const float (&a)[kN], float s) {
-  if constexpr (kN == 1) {
-    o[0] = a[0] * s;
-  } else {
+  float b[kN];
 #pragma unroll
-    for (int j = 0; j < kN; j += 2) f2_get(f2_mul(f2_make(a[j], a[j + 1]), f2_splat(s)), o[j], o[j + 1]);
-  }
+  for (int j = 0; j < kN; ++j) b[j] = s;
+  v_mul(o, a, b);
 }
 template <int kN>
 __device__ __forceinline__ float v_sum(const float (&a)[kN]) {
@@ -349,13 +357,12 @@ __global__ void __launch_bounds__(kThreads, kNorm ? 2 : 3) rotary_kernel(const f
                 v_fma(acc[2], e_lo, t_lo, acc[2]);
                 v_fma(acc[3], e_hi, t_hi, acc[3]);
               }
-              v_scale(x_lo, x_lo, k);
-              v_scale(x_hi, x_hi, k);
 #pragma unroll
-              for (int j = 0; j < kVec; ++j) {
-                lo[j] = r * (lo[j] + x_lo[j]);
-                hi[j] = r * (hi[j] + x_hi[j]);
-              }
+              for (int j = 0; j < kVec; ++j) t_lo[j] = k;
+              v_fma(lo, x_lo, t_lo, lo);
+              v_fma(hi, x_hi, t_lo, hi);
+              v_scale(lo, lo, r);
+              v_scale(hi, hi, r);
             }
           }
           if (here) {

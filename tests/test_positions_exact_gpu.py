@@ -46,3 +46,35 @@ def test_a_far_position_is_as_exact_as_the_first(first):
     # the angle is known to 2^-50, and so is the reference's
     check(x, y, angle[None, :, None].cuda(), 2.0 ** -48)
     assert torch.equal(ops.rotary(x, f.cuda(), offset=first), y)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 64), (torch.float32, 6), (torch.bfloat16, 64), (torch.bfloat16, 10)])
+def test_subnormal_values_stay(dtype, D, interleaved):
+    """A turn by nothing gives back every value; others are rounded once at each product and sum, half a step of 2^-149 (2^-133 in bf16) at the least."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = (torch.randn(1, 3, 2, D, device="cuda", generator=g) * 2.0 ** -130).to(dtype)
+    assert (x != 0).any()
+    f = ops.rotary_frequencies(D, device="cuda")
+    y = ops.rotary(x, f, interleaved=interleaved)
+    assert torch.equal(y[:, 0], x[:, 0])
+    want = ops.rotary(x.double(), f, interleaved=interleaved)
+    step = 2.0 ** (-149 if dtype == torch.float32 else -133)
+    assert ((y.double() - want).abs() <= 2.0 ** -149 + step / 2 + 8 * U * 2.0 ** -127).all()
+    (dx,) = torch.autograd.grad(ops.rotary(x.requires_grad_(), f, interleaved=interleaved), x, x.detach())
+    assert torch.equal(dx[:, 0], x[:, 0])
+
+
+@pytest.mark.parametrize("D", [64, 6])
+def test_norms_of_subnormal_values(D):
+    """x / sqrt(eps) is an ordinary value, and so is the gradient of an ordinary one: dx = w g / sqrt(eps), far from x."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x, dy = (torch.randn(2, 3, 2, D, device="cuda", generator=g) * s for s in (2.0 ** -130, 2.0 ** -130))
+    f = ops.rotary_frequencies(D, device="cuda")
+    x.requires_grad_()
+    y = ops.qk_norm_rotary(x, None, None, f)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    xd = x.detach().double()
+    # an fp32 eps (half a step), a reciprocal root (2 u... 4 u), a product, a turn (8 u), and subnormal steps of 2^-149 that the root raises by 1000
+    for got, want in ((y, ops.rotary(xd * 1000, f)), (dx, ops.rotary(dy.double(), -f) * 1000)):
+        assert ((got.double() - want).abs() <= 24 * U * 2.0 ** -117 + 2000 * 2.0 ** -149).all()
