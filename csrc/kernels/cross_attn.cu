@@ -61,8 +61,10 @@ struct CrossParams {
   int* live_count;
   float* base;
   int* live;
+  int* before;                      // [2][B + 1] live blocks, and batch rows with any, ahead of a batch row; null for up to kScanned of them
   int* status;
 };
+constexpr int kScanned = 64;
 
 // 5-D tensor map over [B, S, H, D] bf16 as (D, pack, S, H / pack, B), one 64-wide panel of 128 rows a box.
 int make_tmap_rows(CUtensorMap* out, const void* base, int D, int pack, long long S, long long Hq, long long B, long long sb, long long ss, long long sh) {
@@ -215,15 +217,29 @@ struct Crew {
   int waves, first, each, more;  // the first tile of the stretches; their units, and how many of them have one more
   Div by_ctas, by_length, by_tiles;      // (of a tile, and of a batch row, without a mask)
 };
-// The batch row into which u falls, and what of u is left there, where a batch row of n live blocks holds of(n). By a whole warp; {B, 0} past the last.
+// The batch row into which u falls, and what of u is left there, where a batch row of n live blocks holds `each` a live block or, `by_rows`, `each` if it has any. By a whole warp; {B, 0}
+// past the last. Few batch rows are looked through 32 at a time, more by a search of 32 parts (8000 x 2 heads x 17 x 33 with a mask took 3.0 ms forward and 12 backward with the look).
 struct InRow {
   int b, live, left;
 };
-template <typename Of>
-__device__ __forceinline__ InRow row_of(const CrossParams& p, unsigned long long u, int lane, Of of) {
+__device__ __forceinline__ InRow row_of(const CrossParams& p, unsigned long long u, int lane, unsigned each, bool by_rows) {
+  if (p.before) {
+    const int* before = p.before + (by_rows ? p.B + 1 : 0);
+    const long long q = static_cast<long long>(u / each);
+    int b = 0, n = p.B + 1, ahead = 0;        // before[b] <= q, and the last such is in [b, b + n)
+    while (n > 1) {
+      const int step = (n + 31) / 32, at = lane * step, v = at < n ? __ldcg(before + b + at) : 0;
+      const int k = __popc(__ballot_sync(0xffffffffu, at < n && v <= q)) - 1;
+      ahead = __shfl_sync(0xffffffffu, v, k);
+      b += k * step;
+      n = min(step, n - k * step);
+    }
+    if (b == p.B) return {p.B, 0, 0};
+    return {b, live_of(p, b), static_cast<int>(u - static_cast<unsigned long long>(ahead) * each)};
+  }
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int n = b0 + lane < p.B ? live_of(p, b0 + lane) : 0;
-    const unsigned long long mine = of(n);
+    const unsigned long long mine = static_cast<unsigned long long>(by_rows ? n > 0 : n) * each;
     unsigned long long upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -238,6 +254,18 @@ __device__ __forceinline__ InRow row_of(const CrossParams& p, unsigned long long
     u -= __shfl_sync(0xffffffffu, upto, 31);
   }
   return {p.B, 0, 0};
+}
+// The next batch row with a key, B past the last. By a whole warp.
+__device__ __forceinline__ int next_row(const CrossParams& p, int b, int lane) {
+  if (p.before) return row_of(p, __ldcg(p.before + p.B + 1 + b) + 1u, lane, 1, true).b;
+  do ++b;
+  while (b < p.B && live_of(p, b) == 0);
+  return b;
+}
+// Tiles of a batch row: so many a live block (kKeyTiles), or so many if it has any.
+template <bool kKeyTiles>
+__device__ __forceinline__ InRow row_of_tile(const CrossParams& p, int tile, int lane) {
+  return row_of(p, static_cast<unsigned>(tile), lane, static_cast<unsigned>(kKeyTiles ? p.Hk : p.Hq * p.row_tiles), !kKeyTiles);
 }
 template <bool kKeyTiles>
 __device__ __forceinline__ Share share_of(const CrossParams& p, const Crew& crew, int cta, int lane) {
@@ -260,38 +288,38 @@ __device__ __forceinline__ Share share_of(const CrossParams& p, const Crew& crew
     return s;
   }
   const unsigned heads = static_cast<unsigned>(p.Hq) * p.row_tiles;        // units of a live block
-  const auto tiles = [&](int n) { return static_cast<unsigned long long>(tiles_of<kKeyTiles>(p, n)); };
-  const auto units = [&](int n) { return static_cast<unsigned long long>(n) * heads; };
-  int live = 0, total = 0;
-  for (int b = lane; b < p.B; b += 32) {
-    const int n = live_of(p, b);
-    live += n;
-    total += tiles_of<kKeyTiles>(p, n);
-  }
+  const auto live_ahead = [&](int end) {
+    if (p.before) return __ldcg(p.before + end);
+    int n = 0;
+    for (int b = lane; b < end; b += 32) n += live_of(p, b);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    live += __shfl_xor_sync(0xffffffffu, live, o);
-    total += __shfl_xor_sync(0xffffffffu, total, o);
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n;
+  };
+  const int live = live_ahead(p.B);
+  int total = live * p.Hk;
+  if (!kKeyTiles) {
+    int rows = 0;
+    if (p.before) {
+      rows = __ldcg(p.before + 2 * p.B + 1);
+    } else {
+      for (int b0 = 0; b0 < p.B; b0 += 32) rows += __popc(__ballot_sync(0xffffffffu, b0 + lane < p.B && live_of(p, b0 + lane) > 0));
+    }
+    total = rows * p.Hq * p.row_tiles;
   }
   s.waves = crew.by_ctas(total);
   const int first = s.waves * crew.ctas;
-  const unsigned long long all = units(live);
+  const unsigned long long all = static_cast<unsigned long long>(live) * heads;
   unsigned long long from = 0;        // units ahead of the first tile of the stretches
   if (first > 0) {
     from = all;
-    const InRow at = row_of(p, first, lane, tiles);
-    if (at.b < p.B) {
-      int before = 0;
-      for (int b = lane; b < at.b; b += 32) before += live_of(p, b);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-      from = units(before) + static_cast<unsigned long long>(at.left) * length_of<kKeyTiles>(p, at.live);
-    }
+    const InRow at = row_of_tile<kKeyTiles>(p, first, lane);
+    if (at.b < p.B) from = static_cast<unsigned long long>(live_ahead(at.b)) * heads + static_cast<unsigned long long>(at.left) * length_of<kKeyTiles>(p, at.live);
   }
   const int rest = static_cast<int>(all - from), each = crew.by_ctas(rest), more = rest - each * crew.ctas;        // (less than a tile for each CTA)
 #pragma unroll 1
   for (int k = 0; k < 2; ++k) {
-    const InRow in = row_of(p, from + static_cast<unsigned>(each * (cta + k) + min(cta + k, more)), lane, units);
+    const InRow in = row_of(p, from + static_cast<unsigned>(each * (cta + k) + min(cta + k, more)), lane, heads, false);
     Place at = {in.b, 0, 0};
     if (at.b < p.B) {
       const int len = length_of<kKeyTiles>(p, in.live);
@@ -301,8 +329,7 @@ __device__ __forceinline__ Share share_of(const CrossParams& p, const Crew& crew
         at.i = 0;
         if (++at.tile == tiles_of<kKeyTiles>(p, in.live)) {
           at.tile = 0;
-          do ++at.b;
-          while (at.b < p.B && live_of(p, at.b) == 0);
+          at.b = next_row(p, at.b, lane);
         }
       }
     }
@@ -324,7 +351,7 @@ struct Walk {
         in.live = p.key_blocks;
         in.left = tile - in.b * tiles_of<kKeyTiles>(p, p.key_blocks);
       } else {
-        in = row_of(p, tile, lane, [&](int n) { return static_cast<unsigned long long>(tiles_of<kKeyTiles>(p, n)); });
+        in = row_of_tile<kKeyTiles>(p, tile, lane);
       }
       const int n = length_of<kKeyTiles>(p, in.live);
       r = {in.b, in.left, 0, n, n};
@@ -338,8 +365,7 @@ struct Walk {
     at.i = 0;
     if (++at.tile == tiles_of<kKeyTiles>(p, live)) {
       at.tile = 0;
-      do ++at.b;
-      while (at.b < p.B && live_of(p, at.b) == 0);
+      at.b = next_row(p, at.b, lane);
     }
     return true;
   }
@@ -388,6 +414,40 @@ __global__ void __launch_bounds__(256) cross_live_kernel(const CrossParams p) {
     for (int k = 1; k < 8; ++k) a = fmaxf(a, largest[k]);
     p.base[b] = isinf(a) ? 0.f : a;
     p.live_count[b] = n_live;
+  }
+}
+
+// One block: `before`, for many batch rows.
+__global__ void __launch_bounds__(1024) cross_before_kernel(const CrossParams p) {
+  __shared__ int2 of_warp[32];
+  pdl_entry();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int2 sum = make_int2(0, 0);        // ahead of this turn's batch rows
+  for (int b0 = 0; b0 <= p.B; b0 += 1024) {
+    const int b = b0 + static_cast<int>(threadIdx.x), n = b < p.B ? live_of(p, b) : 0;
+    int2 upto = make_int2(n, n > 0);
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto.x, o), y = __shfl_up_sync(0xffffffffu, upto.y, o);
+      if (lane >= o) {
+        upto.x += x;
+        upto.y += y;
+      }
+    }
+    if (lane == 31) of_warp[warp] = upto;
+    __syncthreads();
+    int2 all = sum;
+    for (int k = 0; k < 32; ++k) {
+      if (k == warp) sum = all;
+      all.x += of_warp[k].x;
+      all.y += of_warp[k].y;
+    }
+    if (b <= p.B) {
+      p.before[b] = sum.x + upto.x - n;
+      p.before[p.B + 1 + b] = sum.y + upto.y - (n > 0);
+    }
+    sum = all;
+    __syncthreads();        // all have read the warps' sums
   }
 }
 
@@ -1968,6 +2028,7 @@ bool make_cross(const fb_cross_args& a, CrossParams& p, int& pack) {
     p.live_count = a.mask_info;
     p.base = reinterpret_cast<float*>(a.mask_info + a.B);
     p.live = a.mask_info + 2ll * a.B;
+    if (a.B > kScanned) p.before = p.live + static_cast<long long>(a.B) * p.key_blocks;
   }
   return true;
 }
@@ -2029,6 +2090,13 @@ BwdSpace space_bwd(const CrossParams& p, const Crews& c, int D) {
   f.part = f.left + round_up((c.bwd_keys.ctas + c.bwd_rows.ctas) * 2ll * 4, 32);
   f.total = f.part + (c.bwd_keys.whole && c.bwd_rows.whole ? 0 : (c.bwd_keys.ctas * 4ll + c.bwd_rows.ctas * 2ll) * 128 * D);
   return f;
+}
+
+// What a mask comes to, for the 128-row kernels (`lists`), or its largest addends only.
+cudaError_t look_through(const CrossParams& p, bool lists, cudaStream_t stream) {
+  cudaError_t err = launch_pdl(cross_live_kernel, dim3(p.B), dim3(256), 0, stream, p);
+  if (!err && lists && p.before) err = launch_pdl(cross_before_kernel, dim3(1), dim3(1024), 0, stream, p);
+  return err;
 }
 
 // Like launch_pdl, in clusters.
@@ -2109,7 +2177,7 @@ int cross_few(const fb_cross_args& a, const CrossParams& p, const FewShape& shap
   f.by_rows = div_by(f.row_tiles);
   f.by_heads = div_by(p.Hq);
   if (p.mask && (a.stats || !p.mask_bool))        // the largest addends, and the lists for the backward pass
-    if (const cudaError_t err = launch_pdl(cross_live_kernel, dim3(p.B), dim3(256), 0, stream, p)) return static_cast<int>(err);
+    if (const cudaError_t err = look_through(p, a.stats != nullptr, stream)) return static_cast<int>(err);
   constexpr auto kern = cross_few_kernel<kD, kPerSm>;
   constexpr int smem = Few<kD, kPerSm>::TOTAL, threads = Few<kD, kPerSm>::kWarps * 32;
   if (const cudaError_t err = allow_smem<kern>(smem, true)) return static_cast<int>(err);
@@ -2150,7 +2218,7 @@ int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
     out.part_o = a.workspace + f.o;
   }
   if (p.mask)
-    if (const cudaError_t err = launch_pdl(cross_live_kernel, dim3(p.B), dim3(256), 0, stream, p)) return static_cast<int>(err);
+    if (const cudaError_t err = look_through(p, true, stream)) return static_cast<int>(err);
   constexpr int smem = Fwd<kD>::TOTAL + 1024;
   if (const cudaError_t err = allow_smem<cross_fwd_kernel<kD>>(smem, true)) return static_cast<int>(err);
   if (out.parts) {
@@ -2221,7 +2289,7 @@ extern "C" long long fb_cross_mask_info(const fb_cross_args* args) {
   int pack;
   if (!make_cross(*args, p, pack)) return -4;
   if (!p.mask) return 0;
-  return p.B * (2ll + p.key_blocks);
+  return p.B * (2ll + p.key_blocks) + (p.B > kScanned ? 2 * (p.B + 1ll) : 0);
 }
 
 extern "C" int fb_cross_attn_fwd(const fb_cross_args* args, void* stream) {
