@@ -1169,7 +1169,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           if (kS == 1) ok = ok && warp_ready(&bar.s_full, it & 1, abort_flag, p.status, kStatusWaitAccum);
           const float2 k = key_entry(p, b, block * kKeys + t, base);
           tab[(it & 1) * 128 + t] = k;
-          if (p.mask && k.y == -INFINITY && ok) {        // an absent key's values meet a probability of zero
+          if (p.mask && k.y == -INFINITY && block * kKeys + t < p.Sk && ok) {        // an absent key's values meet a probability of zero (what is behind the last key is zeros)
             ok = mbar_wait(&bar.v_full[rv.stage], rv.parity, abort_flag, p.status, kStatusWaitFull);
             if (ok) zero_row<kD>(sV + rv.stage * L::kTile, 128, t);
           }
@@ -1759,11 +1759,12 @@ __device__ __forceinline__ void bwd_softmax(BwdBars& bar, const CrossParams& p, 
       neg_l = -__ldcg(out.stats + row);
       neg_d = -__ldcg(out.D + row);
     }
-    bool next = stays_masked;
-    if (!kKeys) next = live_block(p, b, i0).y;
+    int2 next = make_int2(0, stays_masked);
+    if (!kKeys) next = live_block(p, b, i0);
     for (int i = i0; i < i1; ++i) {
-      const bool masked = next;
-      if (!kKeys && i + 1 < i1) next = live_block(p, b, i + 1).y;
+      const bool masked = next.y;
+      const int here = p.Sk - next.x * kKeys;        // keys of the block
+      if (!kKeys && i + 1 < i1) next = live_block(p, b, i + 1);
       const float* tb = tab + ra.stage * 256 + (kKeys ? w * 32 : w * 64);
       const uint32_t tS = mine + (rs.stage ? (kKeys ? L::S2_KEYS : L::S2_ROWS) : L::S), tDP = mine + L::DP;
       if (!warp_ready(&bar.tab_full[ra.stage], ra.parity, abort_flag, p.status, kStatusWaitFull)) return;        // every turn: a parity tells only the last two apart
@@ -1782,7 +1783,7 @@ __device__ __forceinline__ void bwd_softmax(BwdBars& bar, const CrossParams& p, 
       if (masked) {
         masked_dp<kKeys>(tDP, entry, reinterpret_cast<const float2*>(tb));
         if (!kKeys && p.mask) {        // nor of an absent key's K, which its dS of zero meets: S and dP have been read from it
-          if (w == 0 && reinterpret_cast<const float2*>(tb)[t].y == -INFINITY) zero_row<kD>(smem + L::RING + ra.stage * L::kTile, 128, t);
+          if (w == 0 && t < here && reinterpret_cast<const float2*>(tb)[t].y == -INFINITY) zero_row<kD>(smem + L::RING + ra.stage * L::kTile, 128, t);
           fence_proxy_async_smem();
         }
       }
