@@ -218,12 +218,14 @@ struct Crew {
   Div by_ctas, by_length, by_tiles;      // (of a tile, and of a batch row, without a mask)
 };
 // The batch row into which u falls, and what of u is left there, where a batch row of n live blocks holds `each` a live block or, `by_rows`, `each` if it has any. By a whole warp; {B, 0}
-// past the last. Few batch rows are looked through 32 at a time, more by a search of 32 parts (8000 x 2 heads x 17 x 33 with a mask took 3.0 ms forward and 12 backward with the look).
+// past the last. Few batch rows are looked through 32 at a time, more (kMany) by a search in 32 parts: 8000 x 2 heads x 17 x 33 with a mask took 3.0 ms forward and 12 backward with the
+// look. A kernel has one or the other: with both 32 x 8 heads x 256 x 509 both ways took 121.5 us against 119, as a CTA fetches more code at its start.
 struct InRow {
   int b, live, left;
 };
+template <bool kMany>
 __device__ __forceinline__ InRow row_of(const CrossParams& p, unsigned long long u, int lane, unsigned each, bool by_rows) {
-  if (p.before) {
+  if constexpr (kMany) {
     const int* before = p.before + (by_rows ? p.B + 1 : 0);
     const long long q = static_cast<long long>(u / each);
     int b = 0, n = p.B + 1, ahead = 0;        // before[b] <= q, and the last such is in [b, b + n)
@@ -256,18 +258,19 @@ __device__ __forceinline__ InRow row_of(const CrossParams& p, unsigned long long
   return {p.B, 0, 0};
 }
 // The next batch row with a key, B past the last. By a whole warp.
+template <bool kMany>
 __device__ __forceinline__ int next_row(const CrossParams& p, int b, int lane) {
-  if (p.before) return row_of(p, __ldcg(p.before + p.B + 1 + b) + 1u, lane, 1, true).b;
+  if constexpr (kMany) return row_of<true>(p, __ldcg(p.before + p.B + 1 + b) + 1u, lane, 1, true).b;
   do ++b;
   while (b < p.B && live_of(p, b) == 0);
   return b;
 }
 // Tiles of a batch row: so many a live block (kKeyTiles), or so many if it has any.
-template <bool kKeyTiles>
+template <bool kKeyTiles, bool kMany>
 __device__ __forceinline__ InRow row_of_tile(const CrossParams& p, int tile, int lane) {
-  return row_of(p, static_cast<unsigned>(tile), lane, static_cast<unsigned>(kKeyTiles ? p.Hk : p.Hq * p.row_tiles), !kKeyTiles);
+  return row_of<kMany>(p, static_cast<unsigned>(tile), lane, static_cast<unsigned>(kKeyTiles ? p.Hk : p.Hq * p.row_tiles), !kKeyTiles);
 }
-template <bool kKeyTiles>
+template <bool kKeyTiles, bool kMany>
 __device__ __forceinline__ Share share_of(const CrossParams& p, const Crew& crew, int cta, int lane) {
   Share s;
   if (!p.live_count) {
@@ -289,7 +292,7 @@ __device__ __forceinline__ Share share_of(const CrossParams& p, const Crew& crew
   }
   const unsigned heads = static_cast<unsigned>(p.Hq) * p.row_tiles;        // units of a live block
   const auto live_ahead = [&](int end) {
-    if (p.before) return __ldcg(p.before + end);
+    if constexpr (kMany) return __ldcg(p.before + end);
     int n = 0;
     for (int b = lane; b < end; b += 32) n += live_of(p, b);
 #pragma unroll
@@ -300,7 +303,7 @@ __device__ __forceinline__ Share share_of(const CrossParams& p, const Crew& crew
   int total = live * p.Hk;
   if (!kKeyTiles) {
     int rows = 0;
-    if (p.before) {
+    if constexpr (kMany) {
       rows = __ldcg(p.before + 2 * p.B + 1);
     } else {
       for (int b0 = 0; b0 < p.B; b0 += 32) rows += __popc(__ballot_sync(0xffffffffu, b0 + lane < p.B && live_of(p, b0 + lane) > 0));
@@ -313,13 +316,13 @@ __device__ __forceinline__ Share share_of(const CrossParams& p, const Crew& crew
   unsigned long long from = 0;        // units ahead of the first tile of the stretches
   if (first > 0) {
     from = all;
-    const InRow at = row_of_tile<kKeyTiles>(p, first, lane);
+    const InRow at = row_of_tile<kKeyTiles, kMany>(p, first, lane);
     if (at.b < p.B) from = static_cast<unsigned long long>(live_ahead(at.b)) * heads + static_cast<unsigned long long>(at.left) * length_of<kKeyTiles>(p, at.live);
   }
   const int rest = static_cast<int>(all - from), each = crew.by_ctas(rest), more = rest - each * crew.ctas;        // (less than a tile for each CTA)
 #pragma unroll 1
   for (int k = 0; k < 2; ++k) {
-    const InRow in = row_of(p, from + static_cast<unsigned>(each * (cta + k) + min(cta + k, more)), lane, heads, false);
+    const InRow in = row_of<kMany>(p, from + static_cast<unsigned>(each * (cta + k) + min(cta + k, more)), lane, heads, false);
     Place at = {in.b, 0, 0};
     if (at.b < p.B) {
       const int len = length_of<kKeyTiles>(p, in.live);
@@ -329,7 +332,7 @@ __device__ __forceinline__ Share share_of(const CrossParams& p, const Crew& crew
         at.i = 0;
         if (++at.tile == tiles_of<kKeyTiles>(p, in.live)) {
           at.tile = 0;
-          at.b = next_row(p, at.b, lane);
+          at.b = next_row<kMany>(p, at.b, lane);
         }
       }
     }
@@ -338,7 +341,7 @@ __device__ __forceinline__ Share share_of(const CrossParams& p, const Crew& crew
   return s;
 }
 // The runs of a share, one after the other, by a whole warp.
-template <bool kKeyTiles>
+template <bool kKeyTiles, bool kMany>
 struct Walk {
   Place at, end;
   int waves, tile, step;
@@ -351,7 +354,7 @@ struct Walk {
         in.live = p.key_blocks;
         in.left = tile - in.b * tiles_of<kKeyTiles>(p, p.key_blocks);
       } else {
-        in = row_of_tile<kKeyTiles>(p, tile, lane);
+        in = row_of_tile<kKeyTiles, kMany>(p, tile, lane);
       }
       const int n = length_of<kKeyTiles>(p, in.live);
       r = {in.b, in.left, 0, n, n};
@@ -365,7 +368,7 @@ struct Walk {
     at.i = 0;
     if (++at.tile == tiles_of<kKeyTiles>(p, live)) {
       at.tile = 0;
-      at.b = next_row(p, at.b, lane);
+      at.b = next_row<kMany>(p, at.b, lane);
     }
     return true;
   }
@@ -983,7 +986,7 @@ __device__ __forceinline__ void join_cluster(const CrossParams& p, const FwdOut&
   cluster_meet();        // shared memory is there until all have read it
 }
 
-template <int kD>
+template <int kD, bool kMany>
 __global__ void __launch_bounds__(kFwdThreads, 2)
 cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const CrossParams p, const FwdOut out) {
   extern __shared__ uint8_t smem_raw[];
@@ -1030,8 +1033,8 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   if (warp == 5) {
     // ------------------------------------------------------------------ loads
     Share share = {};
-    if (!out.parts) share = share_of<false>(p, out.crew, blockIdx.x, lane);
-    Walk<false> walk(share, blockIdx.x, gridDim.x);
+    if (!out.parts) share = share_of<false, kMany>(p, out.crew, blockIdx.x, lane);
+    Walk<false, kMany> walk(share, blockIdx.x, gridDim.x);
     Run r;
     Ring<2> rt;
     Ring<kS> ring;
@@ -1256,7 +1259,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           tmem_st16(tmem + L::P + lanes + 16 * c, pk);
         }
         if (!ok) continue;
-        float a0, a1, b0, b1;
+        float a0, a1;
         f2_get(f2_add(sum[0], sum[1]), a0, a1);
         l += a0 + a1;
         tmem_st_wait();
@@ -1582,7 +1585,7 @@ __device__ __forceinline__ void bwd_products(BwdBars& bar, const CrossParams& p,
   }
 }
 
-template <int kD, bool kKeys>
+template <int kD, bool kKeys, bool kMany>
 __device__ __forceinline__ void bwd_loads(BwdBars& bar, const CrossParams& p, const Crew& crew, int first, uint32_t smem, const void* f0, const void* f1, const void* a, const void* b) {
   using L = Bwd<kD>;
   constexpr int kA = L::stages_a(kKeys), kB = L::stages_b(kKeys);
@@ -1591,7 +1594,7 @@ __device__ __forceinline__ void bwd_loads(BwdBars& bar, const CrossParams& p, co
   Ring<kB> rb;
   int as = 0, bs = 0, runs = 0;
   const int lane = threadIdx.x & 31;
-  Walk<kKeys> walk(share_of<kKeys>(p, crew, first, lane), first, crew.ctas);
+  Walk<kKeys, kMany> walk(share_of<kKeys, kMany>(p, crew, first, lane), first, crew.ctas);
   Run r;
   Ring<2> rt;
   bool ok = true;
@@ -1841,7 +1844,7 @@ __device__ __forceinline__ void bwd_softmax(BwdBars& bar, const CrossParams& p, 
   }
 }
 
-template <int kD>
+template <int kD, bool kMany>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
                  const CrossParams p, const BwdOut out) {
@@ -1893,8 +1896,8 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const uint32_t base = smem_u32(smem);
 
   if (warp == kBwdSoftmaxWarps + 1) {
-    if (keys) bwd_loads<kD, true>(bar, p, out.keys, blockIdx.x, base, &tmK, &tmV, &tmQ, &tmDO);
-    else bwd_loads<kD, false>(bar, p, out.rows, blockIdx.x - out.key_ctas, base, &tmQ, &tmDO, &tmK, &tmV);
+    if (keys) bwd_loads<kD, true, kMany>(bar, p, out.keys, blockIdx.x, base, &tmK, &tmV, &tmQ, &tmDO);
+    else bwd_loads<kD, false, kMany>(bar, p, out.rows, blockIdx.x - out.key_ctas, base, &tmQ, &tmDO, &tmK, &tmV);
   } else if (warp == kBwdSoftmaxWarps + 2) {
     if (keys) bwd_tables<kD, true>(bar, p, tab, out.stats, out.D, lane);
     else bwd_tables<kD, false>(bar, p, tab, out.stats, out.D, lane);
@@ -2189,6 +2192,26 @@ int cross_few(const fb_cross_args& a, const CrossParams& p, const FewShape& shap
   return static_cast<int>(err ? err : cudaGetLastError());
 }
 
+template <int kD, bool kMany>
+int cross_fwd_tiles(const FwdOut& out, const CrossParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, cudaStream_t stream) {
+  constexpr auto kern = cross_fwd_kernel<kD, kMany>;
+  constexpr int smem = Fwd<kD>::TOTAL + 1024;
+  if (const cudaError_t err = allow_smem<kern>(smem, true)) return static_cast<int>(err);
+  if (out.parts) {
+    const int ctas = p.B * p.Hq * p.row_tiles * out.parts;
+    if (const cudaError_t err = launch_clusters(kern, ctas, out.parts, kFwdThreads, smem, stream, tq, tk, tv, p, out)) return static_cast<int>(err);
+    return static_cast<int>(cudaGetLastError());
+  }
+  return static_cast<int>(launch_pdl(kern, dim3(out.crew.ctas), dim3(kFwdThreads), static_cast<size_t>(smem), stream, tq, tk, tv, p, out));
+}
+template <int kD, bool kMany>
+int cross_bwd_tiles(const BwdOut& out, const CrossParams& p, const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo, cudaStream_t stream) {
+  constexpr auto kern = cross_bwd_kernel<kD, kMany>;
+  constexpr int smem = Bwd<kD>::TOTAL + 1024;
+  if (const cudaError_t err = allow_smem<kern>(smem)) return static_cast<int>(err);
+  return static_cast<int>(launch_pdl(kern, dim3(out.keys.ctas + out.rows.ctas), dim3(kBwdThreads), static_cast<size_t>(smem), stream, tq, tk, tv, tdo, p, out));
+}
+
 template <int kD>
 int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream_t stream) {
   if (const FewShape shape = few_shape(p, kD); shape.parts) {
@@ -2220,15 +2243,8 @@ int cross_fwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   }
   if (p.mask)
     if (const cudaError_t err = look_through(p, true, stream)) return static_cast<int>(err);
-  constexpr int smem = Fwd<kD>::TOTAL + 1024;
-  if (const cudaError_t err = allow_smem<cross_fwd_kernel<kD>>(smem, true)) return static_cast<int>(err);
-  if (out.parts) {
-    const int ctas = p.B * p.Hq * p.row_tiles * out.parts;
-    if (const cudaError_t err = launch_clusters(cross_fwd_kernel<kD>, ctas, out.parts, kFwdThreads, smem, stream, tq, tk, tv, p, out)) return static_cast<int>(err);
-    return static_cast<int>(cudaGetLastError());
-  }
-  if (const cudaError_t err = launch_pdl(cross_fwd_kernel<kD>, dim3(out.crew.ctas), dim3(kFwdThreads), static_cast<size_t>(smem), stream, tq, tk, tv, p, out)) return static_cast<int>(err);
-  if (!out.crew.whole)
+  if (const int rc = p.before ? cross_fwd_tiles<kD, true>(out, p, tq, tk, tv, stream) : cross_fwd_tiles<kD, false>(out, p, tq, tk, tv, stream)) return rc;
+  if (!out.parts && !out.crew.whole)
     if (const cudaError_t err = launch_pdl(cross_join_kernel<kD>, dim3(out.crew.ctas, ceil_div((p.R < 128 ? p.R : 128) * kD, 1024)), dim3(256), 0, stream, p, out, out.crew.ctas)) return static_cast<int>(err);
   return static_cast<int>(cudaGetLastError());
 }
@@ -2262,10 +2278,8 @@ int cross_bwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   if (const cudaError_t err = launch_pdl(cross_pre_kernel<kD>, dim3(static_cast<unsigned>(want < most ? want : most)), dim3(256), 0, stream, p, static_cast<const __nv_bfloat16*>(a.o), a.o_strides[0],
                                          a.o_strides[1], a.o_strides[2], static_cast<const __nv_bfloat16*>(a.d_o), a.do_strides[0], a.do_strides[1], a.do_strides[2], D))
     return static_cast<int>(err);
-  constexpr int smem = Bwd<kD>::TOTAL + 1024;
-  if (const cudaError_t err = allow_smem<cross_bwd_kernel<kD>>(smem)) return static_cast<int>(err);
   const int ctas = out.keys.ctas + out.rows.ctas;
-  if (const cudaError_t err = launch_pdl(cross_bwd_kernel<kD>, dim3(ctas), dim3(kBwdThreads), static_cast<size_t>(smem), stream, tq, tk, tv, tdo, p, out)) return static_cast<int>(err);
+  if (const int rc = p.before ? cross_bwd_tiles<kD, true>(out, p, tq, tk, tv, tdo, stream) : cross_bwd_tiles<kD, false>(out, p, tq, tk, tv, tdo, stream)) return rc;
   if (!out.keys.whole || !out.rows.whole)
     if (const cudaError_t err = launch_pdl(cross_sum_kernel<kD>, dim3(ctas, kD / 8), dim3(256), 0, stream, p, out, ctas)) return static_cast<int>(err);
   return static_cast<int>(cudaGetLastError());
