@@ -302,17 +302,41 @@ Tensor launch_cross(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, 
   return o;
 }
 
+// The gradients by way of the plain form, for those that are differentiated again or are more than memory themselves (a batch of them).
+variable_list plain_gradients(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& mask, const Tensor& d_o, double scale) {
+  const bool again = at::GradMode::is_enabled();
+  at::AutoGradMode record(true);
+  Tensor o;
+  {
+    py::gil_scoped_acquire gil;
+    o = py::module_::import("flodl_b200.ops.cross").attr("_plain")(q, k, v, mask.defined() ? py::cast(mask) : py::none(), scale).cast<Tensor>();
+  }
+  variable_list of, out(6);
+  for (const Tensor* t : {&q, &k, &v})
+    if (t->requires_grad()) of.push_back(*t);
+  const auto grads = torch::autograd::grad({o}, of, {d_o}, /*retain_graph=*/again, /*create_graph=*/again);
+  size_t i = 0, at = 0;
+  for (const Tensor* t : {&q, &k, &v}) {
+    if (t->requires_grad()) out[i] = grads[at++];
+    ++i;
+  }
+  return out;
+}
+
 struct CrossFn : public torch::autograd::Function<CrossFn> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask_in, double scale) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask_in, double scale, bool twice) {
     const Tensor mask = value(mask_in);
     Tensor stats, info, o = launch_cross(q, k, v, mask, scale, &stats, &info);
     ctx->save_for_backward({q, k, v, mask, o, stats, info});
     ctx->saved_data["scale"] = scale;
+    ctx->saved_data["twice"] = twice;
     return o;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    first_derivative_only();
+    if (!ctx->saved_data["twice"].toBool()) first_derivative_only();
     const auto saved = ctx->get_saved_variables();
+    if (at::GradMode::is_enabled() || !plain_memory(grads[0]))
+      return plain_gradients(saved[0], saved[1], saved[2], saved[3], grads[0], ctx->saved_data["scale"].toDouble());
     const Tensor q = mapped(saved[0]), k = mapped(saved[1]), v = mapped(saved[2]), d_o = mapped(grads[0]);
     const Tensor &mask = saved[3], &o = saved[4], &stats = saved[5];
     c10::cuda::CUDAGuard guard(q.device());
@@ -332,7 +356,7 @@ struct CrossFn : public torch::autograd::Function<CrossFn> {
     if (mask.defined()) a.mask_info = saved[6].data_ptr<int>();
     const Tensor space = space_for(a, true, q);
     check(fb_cross_attn_bwd(&a, stream_of(q)), "fb_cross_attn_bwd");
-    return {dq, dk, dv, Tensor(), Tensor()};
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -344,8 +368,8 @@ Tensor narrowed(const Tensor& mask) {
   return at::where(mask.isinf(), mask, at::where(top.abs() >= 0x1p100, far, rest.clamp(-FLT_MAX, FLT_MAX)));
 }
 
-// The rules of a call to `ops.cross_attention`, and the call. `mask`: bool or floating point [B or 1, Sk], or with two dimensions of one between.
-std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask_in, double scale) {
+// The rules of a call to `ops.cross_attention`, and the call; with `twice` its gradients can be differentiated again. `mask`: bool or floating point [B or 1, Sk], or with two dimensions of one between.
+std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& mask_in, double scale, bool twice) {
   if (!q.is_cuda() || q.dim() != 4 || k.dim() != 4 || v.dim() != 4) return std::nullopt;
   for (const Tensor* t : {&q, &k, &v})
     if (t->scalar_type() != at::kBFloat16 || t->device() != q.device()) return std::nullopt;
@@ -365,7 +389,7 @@ std::optional<Tensor> cross_attention(const Tensor& q, const Tensor& k, const Te
     if (mask.scalar_type() != at::kBool) mask = mask.to(at::kFloat);
     if (Sk > 1 && mask.stride(1) != 1) mask = mask.contiguous();
   }
-  if (records({&q, &k, &v})) return CrossFn::apply(q, k, v, given(mask), scale);
+  if (records({&q, &k, &v})) return CrossFn::apply(q, k, v, given(mask), scale, twice);
   Tensor info;
   return launch_cross(q, k, v, mask, scale, nullptr, &info);
 }

@@ -16,6 +16,7 @@ import torch.nn.functional as F
 from .. import ops as _ops
 from ..autograd import Variable
 from ..autograd import ops as A
+from ..ops.cross import attend as _attend
 from ..tensor import Device, TensorError
 from . import init
 from .module import Buffer, Module, Parameter
@@ -572,8 +573,8 @@ class MultiheadAttention(Module):
     (flodl/src/nn/attention.rs:20-160). Parameter names: q_proj.weight, q_proj.bias, k_proj..., out_proj....
     `mask` marks positions to exclude (non-zero = masked); a strictly upper-triangular [S, S] mask is
     recognised as causal and, like an absent mask, runs on the fused attention kernel. Keys of another length than the
-    queries go through `ops.cross_attention` in bf16 with heads of 64 and 128 on a GPU, where no mask or one of keys ([1, Sk],
-    [B, 1, 1, Sk]) is given; a query none of whose keys are left gets zeros there."""
+    queries go through the kernel of `ops.cross_attention` in bf16 with heads of 64 and 128 on a GPU, where no mask or one of keys
+    ([1, Sk], [B, 1, 1, Sk]) is given. A query none of whose keys are left gets zeros there."""
 
     def __init__(self, embed_dim: int, num_heads: int, device=None):
         if embed_dim % num_heads:
@@ -624,7 +625,8 @@ class MultiheadAttention(Module):
         if Sq == Sk:
             o = _ops.attention(q=qp, k=kp, v=vp, mask=add_mask, causal=causal, scale=self.scale)
         elif _ops.FLAGS.native and qp.is_cuda and qp.dtype == torch.bfloat16 and D in (64, 128) and (mask is None or self._of_keys(mask, B, Sk)):
-            o = _ops.cross_attention(qp, kp, vp, None if mask is None else (mask == 0).reshape(-1, Sk), scale=self.scale)
+            keys = None if mask is None else (mask == 0).reshape(-1, Sk)
+            o = _attend(qp, kp, vp, keys, self.scale, True)
         else:
             qh, kh, vh = (t.transpose(1, 2) for t in (qp, kp, vp))
             s = (qh @ kh.transpose(-1, -2)) * self.scale
