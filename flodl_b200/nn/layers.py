@@ -574,7 +574,7 @@ class MultiheadAttention(Module):
     `mask` marks positions to exclude (non-zero = masked); a strictly upper-triangular [S, S] mask is
     recognised as causal and, like an absent mask, runs on the fused attention kernel. Keys of another length than the
     queries go through the kernel of `ops.cross_attention` in bf16 with heads of 64 and 128 on a GPU, where no mask or one of keys
-    ([1, Sk], [B, 1, 1, Sk]) is given. A query none of whose keys are left gets zeros there."""
+    ([1, Sk], [B, 1, 1, Sk]) is given. A query none of whose keys are left gets NaN over another length."""
 
     def __init__(self, embed_dim: int, num_heads: int, device=None):
         if embed_dim % num_heads:
@@ -625,7 +625,9 @@ class MultiheadAttention(Module):
         if Sq == Sk:
             o = _ops.attention(q=qp, k=kp, v=vp, mask=add_mask, causal=causal, scale=self.scale)
         elif _ops.FLAGS.native and qp.is_cuda and qp.dtype == torch.bfloat16 and D in (64, 128) and (mask is None or self._of_keys(mask, B, Sk)):
-            keys = None if mask is None else (mask == 0).reshape(-1, Sk)
+            keys = None
+            if add_mask is not None:        # less its largest: 0 and -inf as they were, and NaN where every key is masked
+                keys = (add_mask - add_mask.amax(-1, keepdim=True)).reshape(-1, Sk)
             o = _attend(qp, kp, vp, keys, self.scale, True)
         else:
             qh, kh, vh = (t.transpose(1, 2) for t in (qp, kp, vp))

@@ -1,5 +1,5 @@
 """`nn.MultiheadAttention` over keys of another length answers on the kernel what it answers as separate operators: gradients that are differentiated again, batches of
-gradients."""
+gradients, queries whose keys are all masked."""
 import pytest
 import torch
 
@@ -68,6 +68,19 @@ def test_a_batch_of_gradients():
         for a, b in zip(got, torch.autograd.grad(o, (q, s), do[i], retain_graph=True)):
             # the kernel's roundings of P and dS on one side, the projections' on both
             assert (a[i].double() - b.double()).norm() <= 4 * 2.0 ** -8 * b.double().norm()
+
+
+def test_queries_without_a_key_are_as_in_separate_operators():
+    m, q, s, mask = layer()
+    mask[1] = 1
+    o = call(m, q, s, mask)
+    (dw,) = torch.autograd.grad(o.sum(), m.proj["v_proj"][0].t)
+    qw, sw = wide(m, q, s)
+    want = call(m, qw, sw, mask, kernel=False)
+    assert torch.equal(o.isnan(), want.isnan()) and o[1].isnan().all() and not o[[0, 2]].isnan().any()
+    assert dw.isnan().all()
+    # one mask for the batch
+    assert call(m, q, s, torch.ones(1, 70, device="cuda")).isnan().all()
 
 
 def test_the_operator_itself_refuses_a_second_derivative():
