@@ -181,21 +181,30 @@ struct TurnFn : public torch::autograd::Function<TurnFn> {
     first_derivative_only();
     const Turn c = kept(ctx);
     const auto saved = ctx->get_saved_variables();
-    const Tensor dy[2] = {dys[0], dys.size() > 1 ? dys[1] : Tensor()};
     variable_list grads(7);
-    if (!c.norm) {
-      const Tensor none[2];
-      auto out = launch_turn(nullptr, dy, saved[0], saved[1], c, none, false);
-      for (size_t i = 0; i < out.size(); ++i) grads[i] = out[i];
-      return grads;
+    const bool pair = dys.size() > 1;
+    bool want_w[2] = {false, false};
+    for (int i = 0, at = pair ? 2 : 1; c.norm && i < 2; ++i)
+      if (saved[4 + i].defined()) want_w[i] = ctx->needs_input_grad(at++);
+    // of a pair, the one or both that anything is wanted of
+    int of[2] = {0, 1}, n = 0;
+    for (int i = 0; i < (pair ? 2 : 1); ++i)
+      if (ctx->needs_input_grad(i) || want_w[i] || (!pair && want_w[1])) of[n++] = i;
+    if (n == 0) return grads;
+    Tensor dy[2], x[2], w[2];
+    for (int i = 0; i < n; ++i) {
+      dy[i] = dys[of[i]];
+      if (c.norm) x[i] = saved[2 + of[i]];
     }
-    const Tensor x[2] = {saved[2], saved[3]}, w[2] = {saved[4], saved[5]};
-    const bool want[2] = {w[0].defined() && w[0].requires_grad(), w[1].defined() && w[1].requires_grad()};
-    auto out = launch_turn(x, dy, saved[0], saved[1], c, w, want[0] || want[1]);
-    const size_t n = dys.size();
-    for (size_t i = 0; i < n; ++i) grads[i] = out[i];
-    for (size_t i = 0; i < 2; ++i)
-      if (want[i]) grads[2 + i] = out[n + i].to(w[i].scalar_type());
+    if (c.norm)
+      for (int i = 0; i < (pair ? n : 2); ++i) w[i] = saved[4 + (pair ? of[i] : i)];
+    const bool want_dw = want_w[0] || want_w[1];
+    auto out = launch_turn(c.norm ? x : nullptr, dy, saved[0], saved[1], c, w, want_dw);
+    for (int i = 0; i < n; ++i) grads[of[i]] = out[i];
+    for (int i = 0; want_dw && i < (pair ? n : 2); ++i) {
+      const int j = pair ? of[i] : i;
+      if (want_w[j]) grads[2 + j] = out[n + i].to(w[i].scalar_type());
+    }
     return grads;
   }
 };
@@ -341,22 +350,30 @@ struct CrossFn : public torch::autograd::Function<CrossFn> {
     const Tensor &mask = saved[3], &o = saved[4], &stats = saved[5];
     c10::cuda::CUDAGuard guard(q.device());
     const auto bf16 = at::TensorOptions().dtype(at::kBFloat16).device(q.device());
-    Tensor dq = at::empty(q.sizes(), bf16), dk = at::empty(k.sizes(), bf16), dv = at::empty(v.sizes(), bf16);
+    const bool for_k = ctx->needs_input_grad(1), for_v = ctx->needs_input_grad(2);
+    Tensor dq, dk, dv;
+    if (ctx->needs_input_grad(0)) dq = at::empty(q.sizes(), bf16);
+    if (for_k || for_v) dk = at::empty(k.sizes(), bf16), dv = at::empty(v.sizes(), bf16);       // one pass gives both
+    if (!dq.defined() && !dk.defined()) return variable_list(6);
     fb_cross_args a = cross_args(q, k, v, mask, ctx->saved_data["scale"].toDouble());
     a.o = o.data_ptr();
     strides_of(o, a.o_strides);
     a.d_o = d_o.data_ptr();
     strides_of(d_o, a.do_strides);
-    a.dq = dq.data_ptr();
-    strides_of(dq, a.dq_strides);
-    a.dk = dk.data_ptr();
-    a.dv = dv.data_ptr();
-    strides_of(dk, a.dk_strides);
+    if (dq.defined()) {
+      a.dq = dq.data_ptr();
+      strides_of(dq, a.dq_strides);
+    }
+    if (dk.defined()) {
+      a.dk = dk.data_ptr();
+      a.dv = dv.data_ptr();
+      strides_of(dk, a.dk_strides);
+    }
     a.stats = stats.data_ptr<float>();
     if (mask.defined()) a.mask_info = saved[6].data_ptr<int>();
     const Tensor space = space_for(a, true, q);
     check(fb_cross_attn_bwd(&a, stream_of(q)), "fb_cross_attn_bwd");
-    return {dq, dk, dv, Tensor(), Tensor(), Tensor()};
+    return {dq, for_k ? dk : Tensor(), for_v ? dv : Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 

@@ -122,7 +122,8 @@ int fb_rotary_partial_rows(void);
 
 /* ---- attention over another sequence ------------------------------------------------------------ */
 /* q, o, d_o, dq: bf16 [B, Sq, H, D], k, v, dk, dv: bf16 [B, Sk, Hk, D] with a unit inner stride, the others in elements {batch, seq, head} (multiples of 8, not 0 where the
- * dimension is more than one; 16-byte aligned bases). D is 64 or 128; Hk divides H, query head h reads key head h / (H / Hk). dk and dv share dk_strides.
+ * dimension is more than one; 16-byte aligned bases). D is 64 or 128; Hk divides H, query head h reads key head h / (H / Hk). dk and dv share dk_strides;
+ * dq, or dk and dv together, may be NULL where they are not wanted.
  * mask: [B, Sk] with a unit inner stride, one byte a key (mask_bool; 0: the key is absent) or fp32 addends (-inf: absent). stats: fp32, B * H * Sq
  * floats, written by the forward pass (or NULL) and read by the backward pass, like mask_info, fb_cross_mask_info ints (with a mask; a forward pass without stats
  * may leave them as they are). workspace: fb_cross_workspace

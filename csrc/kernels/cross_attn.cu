@@ -1918,13 +1918,13 @@ cross_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const int b = static_cast<int>(x / p.key_blocks), i = static_cast<int>(x % p.key_blocks), n = live_of(p, b);
         if (i < n) continue;
         const int key0 = live_block(p, b, i).x * 128;
-        for (int e = threadIdx.x; e < 128 * p.Hk * kVecs; e += kThreads) {
+        for (int e = threadIdx.x; out.dk && e < 128 * p.Hk * kVecs; e += kThreads) {
           const int c = e % kVecs, h = e / kVecs % p.Hk, key = key0 + e / kVecs / p.Hk;
           if (key >= p.Sk) break;
           const long long at = b * out.ksb + key * out.kss + h * out.ksh + c * 8;
           *reinterpret_cast<uint4*>(out.dk + at) = *reinterpret_cast<uint4*>(out.dv + at) = make_uint4(0u, 0u, 0u, 0u);
         }
-        if (n == 0 && i == 0)
+        if (n == 0 && i == 0 && out.dq)
           for (long long e = threadIdx.x; e < static_cast<long long>(p.Hq) * p.R * kVecs; e += kThreads) {
             const int c = static_cast<int>(e % kVecs), row = static_cast<int>(e / kVecs % p.R), h = static_cast<int>(e / kVecs / p.R);
             *reinterpret_cast<uint4*>(out_row(p, out.dq, out.qsb, out.qss, out.qsh, b, h, row) + c * 8) = make_uint4(0u, 0u, 0u, 0u);
@@ -2042,7 +2042,8 @@ bool make_cross(const fb_cross_args& a, CrossParams& p, int& pack) {
 Crew crew_of(const CrossParams& p, int tiles, int length, int most) {        // tiles of all batch rows, without a mask
   Crew c = {};
   if (most > kWith) most = kWith;
-  c.whole = length <= 4;
+  c.whole = length <= 4 || most == 0;
+  if (most == 0) return c;        // not wanted
   const long long units = static_cast<long long>(tiles) * length, n = c.whole ? tiles : (units + 1) / 2;
   c.ctas = static_cast<int>(n < most ? n : most);
   c.waves = tiles / c.ctas;
@@ -2059,8 +2060,11 @@ Crew crew_of(const CrossParams& p, int tiles, int length, int most) {        // 
 struct Crews {
   Crew rows, bwd_keys, bwd_rows;
 };
-Crews crews_of(const CrossParams& p, int D) {
-  const int row_tiles = p.B * p.Hq * p.row_tiles, sms = sm_count(), most_keys = D == 64 ? sms * 54 / 100 : sms * 60 / 100;
+// Whichever of the backward pass's gradients are not wanted leave the GPU to the others.
+enum Wanted { kBoth, kRowsOnly, kKeysOnly };
+Crews crews_of(const CrossParams& p, int D, Wanted wanted = kBoth) {
+  const int row_tiles = p.B * p.Hq * p.row_tiles, sms = sm_count();
+  const int most_keys = wanted == kRowsOnly ? 0 : wanted == kKeysOnly ? sms : D == 64 ? sms * 54 / 100 : sms * 60 / 100;
   return {crew_of(p, row_tiles, p.key_blocks, 2 * sms), crew_of(p, p.B * p.Hk * p.key_blocks, p.per_kv * p.row_tiles, most_keys), crew_of(p, row_tiles, p.key_blocks, sms - most_keys)};
 }
 // The forward pass's places in its workspace, in floats.
@@ -2258,7 +2262,7 @@ int cross_bwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   if (!e) e = make_tmap_rows(&tdo, a.d_o, kD, pack, a.Sq, p.Hq, a.B, a.do_strides[0], a.do_strides[1], a.do_strides[2]);
   if (e) return e;
   if (!a.workspace || !a.stats) return -3;
-  const Crews crews = crews_of(p, kD);
+  const Crews crews = crews_of(p, kD, !a.dk ? kRowsOnly : !a.dq ? kKeysOnly : kBoth);
   const BwdSpace f = space_bwd(p, crews, kD);
   BwdOut out = {};
   float* D = a.workspace;
@@ -2296,7 +2300,13 @@ extern "C" long long fb_cross_workspace(const fb_cross_args* args, int backward)
   int pack;
   if (!make_cross(*args, p, pack)) return -4;
   const Crews crews = crews_of(p, args->D);
-  return backward ? space_bwd(p, crews, args->D).total : few_shape(p, args->D).parts ? few_shape(p, args->D).total : space_fwd(p, crews.rows, args->D).total;
+  if (backward) {        // of whichever gradients the call will want
+    long long most = 0;
+    for (const Wanted w : {kBoth, kRowsOnly, kKeysOnly})
+      if (const long long n = space_bwd(p, crews_of(p, args->D, w), args->D).total; n > most) most = n;
+    return most;
+  }
+  return few_shape(p, args->D).parts ? few_shape(p, args->D).total : space_fwd(p, crews.rows, args->D).total;
 }
 extern "C" long long fb_cross_mask_info(const fb_cross_args* args) {
   using namespace fb;
@@ -2325,8 +2335,9 @@ extern "C" int fb_cross_attn_bwd(const fb_cross_args* args, void* stream) {
   int pack;
   if (!make_cross(a, p, pack)) return -4;
   if (!rows_ok(a.q, a.q_strides) || !rows_ok(a.k, a.k_strides) || !rows_ok(a.v, a.v_strides) || !rows_ok(a.o, a.o_strides) || !rows_ok(a.d_o, a.do_strides) ||
-      !rows_ok(a.dq, a.dq_strides) || !rows_ok(a.dk, a.dk_strides) || !rows_ok(a.dv, a.dk_strides) || (a.mask && !a.mask_info))
+      (a.dq && !rows_ok(a.dq, a.dq_strides)) || (a.dk && !rows_ok(a.dk, a.dk_strides)) || (a.dv && !rows_ok(a.dv, a.dk_strides)) || (a.mask && !a.mask_info))
     return -3;
+  if (!a.dk != !a.dv || (!a.dq && !a.dk)) return -3;
   const auto s = static_cast<cudaStream_t>(stream);
   return a.D == 64 ? cross_bwd<64>(a, p, pack, s) : cross_bwd<128>(a, p, pack, s);
 }
