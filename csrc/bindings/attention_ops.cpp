@@ -224,7 +224,7 @@ Found turn(const Tensor& q, const OptTensor& k_in, const Tensor& freqs_in, const
   const int64_t pairs = freqs_in.numel();
   if (D < 2 || D % 2 || 2 * pairs > D || B >= 1 << 30 || S >= 1 << 30 || B * S >= 1ll << 31 || q.size(-2) < 1 || q.size(-2) >= 1 << 14) return std::nullopt;
   if (k.defined() && (k.size(2) < 1 || k.size(2) >= 1 << 14)) return std::nullopt;
-  if (!std::isfinite(amplitude) || !(eps >= 0)) return std::nullopt;
+  if (!std::isfinite(amplitude) || !std::isfinite(eps) || eps < 0) return std::nullopt;
   if (norm && (D > 64 * width(q, pairs) || D > 512)) return std::nullopt;
   if (D > 8192 || (q.size(-2) * (packed ? 3 : 1) + (k.defined() ? k.size(2) : 0)) * D > 1 << 24) return std::nullopt;       // of a tile's items and its angles
   Tensor positions;

@@ -8,6 +8,7 @@ import torch
 
 from ..tensor import TensorError
 from .core import FLAGS, _C, _launched
+from .position import is_number
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
@@ -23,7 +24,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
 def attend(q, k, v, mask, scale, twice: bool) -> torch.Tensor:
     """`cross_attention`; with `twice` its gradients may be differentiated again, which goes by the plain form."""
     if FLAGS.native and torch.is_tensor(q) and q.is_cuda and q.dim() == 4:
-        o = _C().cross_attention(q, k, v, mask, float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1] or 1), twice)
+        try:
+            o = _C().cross_attention(q, k, v, mask, scale if scale is not None else 1.0 / math.sqrt(q.shape[-1] or 1), twice)
+        except TypeError:         # an argument that is of none of the kinds it may be: the checks say which
+            o = None
         if o is not None:
             _launched()
             return o
@@ -43,15 +47,17 @@ def _plain(q, k, v, mask, scale):
         raise TensorError("queries, keys and values must be floating point, of one type and on one device")
     if D == 0:
         raise TensorError("heads of no values")
+    if scale is not None and not is_number(scale):
+        raise TensorError(f"scale ({scale}) must be a finite number")
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(D)
-    if not math.isfinite(scale):
-        raise TensorError(f"scale ({scale}) must be finite")
     wide = torch.float64 if q.dtype == torch.float64 else torch.float32
     qh = q.to(wide).transpose(1, 2).reshape(B, Hk, H // Hk * Sq, D)
     kh, vh = (t.to(wide).transpose(1, 2) for t in (k, v))
     add = alone = absent = None
     if mask is not None:
         m = mask
+        if not torch.is_tensor(m):
+            raise TensorError(f"mask must be a tensor, not {type(m).__name__}")
         if m.device != q.device or not (m.dtype == torch.bool or m.is_floating_point()):
             raise TensorError("mask must be bool or floating point on the device of the rows")
         if m.dim() == 4 and m.shape[1] == 1 and m.shape[2] == 1:

@@ -44,6 +44,22 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Optional
 
 
 # ------------------------------------------------------------------------------------------- arguments
+def _given(x):
+    """The tensors in `x`, or a TensorError."""
+    given = (x,) if torch.is_tensor(x) else tuple(x) if isinstance(x, (tuple, list)) else ()
+    if not given or len(given) > 2 or not all(torch.is_tensor(t) for t in given):
+        raise TensorError("x must be a tensor or a pair of them")
+    return given
+
+
+def is_number(v) -> bool:
+    """Whether it is one number, and finite."""
+    try:
+        return math.isfinite(v)
+    except (TypeError, ValueError, RuntimeError, OverflowError):
+        return False
+
+
 def _parts(x):
     """The queries and keys in `x`."""
     if torch.is_tensor(x):
@@ -53,13 +69,11 @@ def _parts(x):
 
 def _check(x, freqs, positions, offset, amplitude):
     """(tensors given, positions as [B, S] int64 or None), or a TensorError."""
-    given = (x,) if torch.is_tensor(x) else tuple(x)
-    if not given or len(given) > 2 or not all(torch.is_tensor(t) for t in given):
-        raise TensorError("x must be a tensor or a pair of them")
+    given = _given(x)
     lead = given[0]
     packed = lead.dim() == 5
-    if packed and (len(given) != 1 or lead.shape[2] != 3):
-        raise TensorError(f"a packed projection is [B, S, 3, H, D], not {list(lead.shape)}")
+    if packed and (not torch.is_tensor(x) or lead.shape[2] != 3):
+        raise TensorError(f"a packed projection is one tensor [B, S, 3, H, D], not {list(lead.shape)}")
     for t in given:
         if not packed and t.dim() != 4:
             raise TensorError(f"queries and keys are [B, S, H, D], not {list(t.shape)}")
@@ -67,16 +81,19 @@ def _check(x, freqs, positions, offset, amplitude):
             raise TensorError("queries and keys must share batch, length, head dim, type and device")
         if not t.is_floating_point():
             raise TensorError(f"queries and keys must be floating point, not {t.dtype}")
-    if freqs is not None:
-        if freqs.dim() != 1 or freqs.dtype != torch.float64 or freqs.device != lead.device:
-            raise TensorError("freqs must be fp64 [rotary_dim / 2] on the device of the rows (rotary_frequencies makes them)")
-        if 2 * freqs.numel() > lead.shape[-1]:
-            raise TensorError(f"{freqs.numel()} pairs do not fit a head of {lead.shape[-1]}")
-    if not math.isfinite(amplitude):
-        raise TensorError(f"amplitude ({amplitude}) must be finite")
-    if int(offset) != offset:
-        raise TensorError(f"offset ({offset}) must be a whole number")
+    if not torch.is_tensor(freqs):
+        raise TensorError(f"freqs must be a tensor (rotary_frequencies makes it), not {type(freqs).__name__}")
+    if freqs.dim() != 1 or freqs.dtype != torch.float64 or freqs.device != lead.device:
+        raise TensorError("freqs must be fp64 [rotary_dim / 2] on the device of the rows (rotary_frequencies makes them)")
+    if 2 * freqs.numel() > lead.shape[-1]:
+        raise TensorError(f"{freqs.numel()} pairs do not fit a head of {lead.shape[-1]}")
+    if not is_number(amplitude):
+        raise TensorError(f"amplitude ({amplitude}) must be a finite number")
+    if not is_number(offset) or int(offset) != offset or not abs(offset) < 2 ** 62:
+        raise TensorError(f"offset ({offset}) must be a whole number, below 2^62")
     if positions is not None:
+        if not torch.is_tensor(positions):
+            raise TensorError(f"positions must be a tensor, not {type(positions).__name__}")
         if positions.is_floating_point() or positions.is_complex() or positions.dtype == torch.bool:
             raise TensorError(f"positions must be whole numbers, not {positions.dtype}")
         B, S = lead.shape[:2]
@@ -90,12 +107,15 @@ def _native(x, freqs, positions, offset, interleaved, amplitude, norm=False, wq=
     """The kernel's results, or None for a call that it does not take: another device or type, or arguments that the checks explain. At any size: the
     plain form is a dozen launches."""
     pair = isinstance(x, (tuple, list))
-    if pair and len(x) not in (1, 2):
+    if pair and (len(x) not in (1, 2) or torch.is_tensor(x[0]) and x[0].dim() == 5):
         return None
     q, k = (x if len(x) == 2 else (x[0], None)) if pair else (x, None)
     if not (FLAGS.native and torch.is_tensor(q) and q.is_cuda and (k is None or torch.is_tensor(k)) and type(offset) is int):
         return None
-    out = _C().turn(q, k, freqs, positions, offset, interleaved, amplitude, norm, wq, wk, eps)
+    try:
+        out = _C().turn(q, k, freqs, positions, offset, interleaved, amplitude, norm, wq, wk, eps)
+    except TypeError:         # an argument that is of none of the kinds it may be: the checks say which
+        return None
     if out is None:
         return None
     _launched()
@@ -145,21 +165,18 @@ def qk_norm_rotary(x, q_weight: Optional[torch.Tensor] = None, k_weight: Optiona
     """Queries and keys normalised per head, `x / sqrt(mean(x^2) + eps) * weight` over the head's values, then turned as `rotary` does (not at all
     without `freqs`), in one pass. The weights are [D], shared by the heads; None is ones. Statistics are taken in 32 bits."""
     if freqs is None:
-        lead = x if torch.is_tensor(x) else next(iter(x), None)
-        if not torch.is_tensor(lead):
-            raise TensorError("x must be a tensor or a pair of them")
-        freqs = torch.empty(0, dtype=torch.float64, device=lead.device)
+        freqs = torch.empty(0, dtype=torch.float64, device=_given(x)[0].device)
     out = _native(x, freqs, positions, offset, interleaved, amplitude, True, q_weight, k_weight, eps)
     if out is not None:
         return out
     given, positions = _check(x, freqs, positions, offset, amplitude)
     D = given[0].shape[-1]
     for w in (q_weight, k_weight):
-        if w is not None and (tuple(w.shape) != (D,) or w.device != given[0].device or not w.is_floating_point()):
+        if w is not None and (not torch.is_tensor(w) or tuple(w.shape) != (D,) or w.device != given[0].device or not w.is_floating_point()):
             raise TensorError(f"weights must be [{D}] on the device of the rows")
     if k_weight is not None and len(_parts(x)) < 2:
         raise TensorError("k_weight without keys")
-    if not eps >= 0:
+    if not is_number(eps) or eps < 0:
         raise TensorError(f"eps ({eps}) must not be negative")
     out = []
     for t, w in zip(_parts(x), (q_weight, k_weight)):
