@@ -98,7 +98,7 @@ int fb_attn_bwd(const void* q, const void* k, const void* v, const void* o, cons
  * positions[b, s] + offset (strides in elements), or s + offset where `positions` is NULL. `norm`: RMS norm of the first two over D with `weight`
  * (fp32 [D] or NULL) before the turn. `backward`: dy -> y = dx; x is read with `norm` alone, whose weight gradients go to `dw`
  * (fp32 [D] or NULL) by way of `partial`, fb_rotary_partial_rows() x 2 x D floats. rot <= D, both even; with `norm` D / 64
- * values have to fit one access (16 bytes where all addresses and halves are so aligned). */
+ * values have to fit one access (16 bytes where all addresses and halves are so aligned). Pointers off their type's alignment are refused, as null ones are (-3). */
 typedef struct fb_rotary_args {
   const void* x[3];
   const void* dy[3];
@@ -127,7 +127,7 @@ int fb_rotary_partial_rows(void);
  * mask: [B, Sk] with a unit inner stride, one byte a key (mask_bool; 0: the key is absent) or fp32 addends (-inf: absent). stats: fp32, B * H * Sq
  * floats, written by the forward pass (or NULL) and read by the backward pass, like mask_info, fb_cross_mask_info ints (with a mask; a forward pass without stats
  * may leave them as they are). workspace: fb_cross_workspace
- * floats, 16-byte aligned. */
+ * floats, 16-byte aligned. Pointers off these alignments, or their type's, are refused, as null ones are (-3). */
 typedef struct fb_cross_args {
   const void *q, *k, *v, *d_o;
   void *o, *dq, *dk, *dv;

@@ -306,6 +306,9 @@ __device__ __forceinline__ void pdl_entry() {
   pdl_launch_dependents();
 }
 
+// Whether a pointer is a multiple of n bytes (null is).
+inline bool aligned(const void* p, unsigned n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
 // A number per device of the process, made on first use there. A device's properties and a kernel's attributes are its own: worker threads with a
 // device each share these functions. `make` returns a positive number; anything else (a failed call) is not kept.
 class PerDevice {

@@ -2261,7 +2261,6 @@ int cross_bwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
   if (!e) e = make_tmap_rows(&tv, a.v, kD, 1, a.Sk, a.Hk, a.B, a.v_strides[0], a.v_strides[1], a.v_strides[2]);
   if (!e) e = make_tmap_rows(&tdo, a.d_o, kD, pack, a.Sq, p.Hq, a.B, a.do_strides[0], a.do_strides[1], a.do_strides[2]);
   if (e) return e;
-  if (!a.workspace || !a.stats) return -3;
   const Crews crews = crews_of(p, kD, !a.dk ? kRowsOnly : !a.dq ? kKeysOnly : kBoth);
   const BwdSpace f = space_bwd(p, crews, kD);
   BwdOut out = {};
@@ -2290,12 +2289,16 @@ int cross_bwd(const fb_cross_args& a, const CrossParams& p, int pack, cudaStream
 }
 
 bool rows_ok(const void* p, const long long* st) { return p && strides_ok(p, st[0], st[1], st[2]); }
+bool aside_ok(const fb_cross_args& a) {
+  return (!a.mask || (a.mask_info && (a.mask_bool || aligned(a.mask, 4)))) && aligned(a.mask_info, 4) && aligned(a.stats, 4) && aligned(a.workspace, 16) && aligned(a.status, 4);
+}
 
 }  // namespace
 }  // namespace fb
 
 extern "C" long long fb_cross_workspace(const fb_cross_args* args, int backward) {
   using namespace fb;
+  if (!args) return -3;
   CrossParams p = {};
   int pack;
   if (!make_cross(*args, p, pack)) return -4;
@@ -2310,6 +2313,7 @@ extern "C" long long fb_cross_workspace(const fb_cross_args* args, int backward)
 }
 extern "C" long long fb_cross_mask_info(const fb_cross_args* args) {
   using namespace fb;
+  if (!args) return -3;
   CrossParams p = {};
   int pack;
   if (!make_cross(*args, p, pack)) return -4;
@@ -2319,23 +2323,26 @@ extern "C" long long fb_cross_mask_info(const fb_cross_args* args) {
 
 extern "C" int fb_cross_attn_fwd(const fb_cross_args* args, void* stream) {
   using namespace fb;
+  if (!args) return -3;
   const fb_cross_args& a = *args;
   CrossParams p = {};
   int pack;
   if (!make_cross(a, p, pack)) return -4;
-  if (!rows_ok(a.q, a.q_strides) || !rows_ok(a.k, a.k_strides) || !rows_ok(a.v, a.v_strides) || !rows_ok(a.o, a.o_strides) || (a.mask && !a.mask_info)) return -3;
+  if (!rows_ok(a.q, a.q_strides) || !rows_ok(a.k, a.k_strides) || !rows_ok(a.v, a.v_strides) || !rows_ok(a.o, a.o_strides) || !aside_ok(a)) return -3;
   const auto s = static_cast<cudaStream_t>(stream);
   return a.D == 64 ? cross_fwd<64>(a, p, pack, s) : cross_fwd<128>(a, p, pack, s);
 }
 
 extern "C" int fb_cross_attn_bwd(const fb_cross_args* args, void* stream) {
   using namespace fb;
+  if (!args) return -3;
   const fb_cross_args& a = *args;
   CrossParams p = {};
   int pack;
   if (!make_cross(a, p, pack)) return -4;
   if (!rows_ok(a.q, a.q_strides) || !rows_ok(a.k, a.k_strides) || !rows_ok(a.v, a.v_strides) || !rows_ok(a.o, a.o_strides) || !rows_ok(a.d_o, a.do_strides) ||
-      (a.dq && !rows_ok(a.dq, a.dq_strides)) || (a.dk && !rows_ok(a.dk, a.dk_strides)) || (a.dv && !rows_ok(a.dv, a.dk_strides)) || (a.mask && !a.mask_info))
+      (a.dq && !rows_ok(a.dq, a.dq_strides)) || (a.dk && !rows_ok(a.dk, a.dk_strides)) || (a.dv && !rows_ok(a.dv, a.dk_strides)) || !aside_ok(a) || !a.stats ||
+      !a.workspace)
     return -3;
   if (!a.dk != !a.dv || (!a.dq && !a.dk)) return -3;
   const auto s = static_cast<cudaStream_t>(stream);

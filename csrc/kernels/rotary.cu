@@ -481,6 +481,7 @@ extern "C" int fb_rotary_partial_rows(void) { return fb::rotary_blocks(); }
 
 extern "C" int fb_rotary(const fb_rotary_args* args, void* stream) {
   using namespace fb;
+  if (!args) return -3;
   const fb_rotary_args& a = *args;
   const int size = a.dtype == FLODL_FLOAT32 ? 4 : 2;
   if (a.dtype != FLODL_FLOAT32 && a.dtype != FLODL_BFLOAT16 && a.dtype != FLODL_FLOAT16) return -2;
@@ -492,6 +493,11 @@ extern "C" int fb_rotary(const fb_rotary_args* args, void* stream) {
   for (int s = 0; s < 3; ++s)
     if (a.heads[s] && (!a.y[s] || (reads_x && !a.x[s]) || (a.backward && !a.dy[s]))) return -3;
   if ((a.rot && !a.freqs) || (a.norm && a.backward && !a.partial)) return -3;
+  for (int s = 0; s < 3; ++s)
+    if (a.heads[s] && (!aligned(a.x[s], size) || !aligned(a.dy[s], size) || !aligned(a.y[s], size))) return -3;
+  if (!aligned(a.freqs, 8) || !aligned(a.positions, 8) || !aligned(a.partial, 4)) return -3;
+  for (int s = 0; s < 2; ++s)
+    if (!aligned(a.weight[s], 4) || !aligned(a.dw[s], 4)) return -3;
   const int v = widest(a, size), items = a.D / (2 * v);
   int group = items;
   if (a.norm) {
