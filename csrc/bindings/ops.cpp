@@ -190,6 +190,7 @@ int* bounds_word(bool create) {
     check(fb_bounds_attach_elementwise(dev), "fb_bounds_attach_elementwise");
     check(fb_bounds_attach_gemm(dev), "fb_bounds_attach_gemm");
     check(fb_bounds_attach_softmax_ce(dev), "fb_bounds_attach_softmax_ce");
+    check(fb_bounds_attach_cross_attn(dev), "fb_bounds_attach_cross_attn");
   }
   return host;
 }

@@ -285,6 +285,7 @@ long long fb_grad_norm_noalloc_max(void);
 int fb_bounds_attach_elementwise(int* dev_word);
 int fb_bounds_attach_gemm(int* dev_word);
 int fb_bounds_attach_softmax_ce(int* dev_word);
+int fb_bounds_attach_cross_attn(int* dev_word);
 
 /* ---- collectives over peer-mapped buffers ---------------------------------------------------- */
 int fb_allreduce(const fb_symm_ctx* ctx, long long byte_off, long long n, int is_bf16, const float* weights,

@@ -137,11 +137,20 @@ __device__ __forceinline__ int block_state(const CrossParams& p, int b, int blk,
 }
 
 // What an earlier kernel of the stream wrote is read past L1, and never with read-only loads (ld.global.nc), which may answer from a line that was there before.
-__device__ __forceinline__ int live_of(const CrossParams& p, int b) { return p.live_count ? __ldcg(p.live_count + b) : p.key_blocks; }
+__device__ __forceinline__ int live_of(const CrossParams& p, int b) {
+  if (!p.live_count) return p.key_blocks;
+  const int n = __ldcg(p.live_count + b);
+  return FB_INDEX_OK(n, p.key_blocks + 1ll, 301) ? n : 0;
+}
+// Entry i of a batch row's list; in place of one that is no block, a block behind the last key.
+__device__ __forceinline__ int listed(const CrossParams& p, int b, int i) {
+  const int v = __ldcg(p.live + static_cast<long long>(b) * p.key_blocks + i);
+  return FB_INDEX_OK(v >> 1, p.key_blocks, 302) ? v : p.key_blocks << 1 | 1;
+}
 // Live block i of a batch row: {block, whether it goes by the table}.
 __device__ __forceinline__ int2 live_block(const CrossParams& p, int b, int i) {
   if (p.live) {
-    const int v = __ldcg(p.live + static_cast<long long>(b) * p.key_blocks + i);
+    const int v = listed(p, b, i);
     return make_int2(v >> 1, v & 1);
   }
   return make_int2(i, p.table || (i + 1) * kKeys > p.Sk);
@@ -237,7 +246,8 @@ __device__ __forceinline__ InRow row_of(const CrossParams& p, unsigned long long
       n = min(step, n - k * step);
     }
     if (b == p.B) return {p.B, 0, 0};
-    return {b, live_of(p, b), static_cast<int>(u - static_cast<unsigned long long>(ahead) * each)};
+    const int live = live_of(p, b), left = static_cast<int>(u - static_cast<unsigned long long>(ahead) * each);
+    return {b, live, FB_INDEX_OK(left, static_cast<long long>(each) * (by_rows ? 1 : live), 303) ? left : 0};
   }
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int n = b0 + lane < p.B ? live_of(p, b0 + lane) : 0;
@@ -1162,7 +1172,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       float m = -INFINITY, l = 0.f;               // the maximum the accumulator is relative to, and the sum
       const float base = task.base;
       const int ragged = p.table ? i0 : p.Sk / kKeys;        // without a list, the first block that goes by the table
-      int next = p.live ? i0 < i1 ? __ldcg(p.live + static_cast<long long>(b) * p.key_blocks + i0) : 0 : i0 >= ragged;
+      int next = p.live ? i0 < i1 ? listed(p, b, i0) : 0 : i0 >= ragged;
       for (int i = i0; i < i1; ++i, ++it) {
         const bool tabled = next & 1;
         const float2* tb = tab + (it & 1) * 128;
@@ -1180,7 +1190,7 @@ cross_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           fence_proxy_async_smem();
           asm volatile("bar.sync 1, 128;" ::: "memory");
         }
-        next = !p.live ? i + 1 >= ragged : i + 1 < i1 ? __ldcg(p.live + static_cast<long long>(b) * p.key_blocks + i + 1) : 0;
+        next = !p.live ? i + 1 >= ragged : i + 1 < i1 ? listed(p, b, i + 1) : 0;
         rv.next();
         ok = ok && warp_ready_here(&bar.s_full, it & 1, abort_flag, p.status, kStatusWaitAccum);
         if (!ok) continue;
@@ -1374,7 +1384,7 @@ __global__ void __launch_bounds__(256) cross_join_kernel(const CrossParams p, co
   pdl_entry();
   constexpr int kLanes = kD / 4;
   const Left first = out.left[blockIdx.x * 2 + 1];
-  if (!first.used) return;
+  if (!first.used || !FB_INDEX_OK(first.b, p.B, 304) || !FB_INDEX_OK(first.tile, static_cast<long long>(p.Hq) * p.row_tiles, 305)) return;
   const int n = sharers(out.left, blockIdx.x, ctas, with, &count);
   const int h = first.tile / p.row_tiles, row0 = (first.tile - h * p.row_tiles) * 128, rows = min(128, p.R - row0);
   const int c = (threadIdx.x % kLanes) * 4, t = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes;
@@ -1976,7 +1986,8 @@ __global__ void __launch_bounds__(256) cross_sum_kernel(const CrossParams p, con
   const int cta = blockIdx.x;
   const bool keys = cta < out.key_ctas;
   const Left first = out.left[cta * 2 + 1];
-  if (!first.used) return;
+  if (!first.used || !FB_INDEX_OK(first.b, p.B, 304)) return;
+  if (!FB_INDEX_OK(first.tile, keys ? static_cast<long long>(p.Hk) * live_of(p, first.b) : static_cast<long long>(p.Hq) * p.row_tiles, 305)) return;
   const int sharing = sharers(out.left, cta, keys ? out.key_ctas : ctas, with, &count);
   const int per = keys ? live_of(p, first.b) : p.row_tiles, h = first.tile / per, tile = first.tile - h * per;
   const int c = (threadIdx.x % kLanes) * 4, t = blockIdx.y * (256 / kLanes) + threadIdx.x / kLanes;
@@ -2348,3 +2359,5 @@ extern "C" int fb_cross_attn_bwd(const fb_cross_args* args, void* stream) {
   const auto s = static_cast<cudaStream_t>(stream);
   return a.D == 64 ? cross_bwd<64>(a, p, pack, s) : cross_bwd<128>(a, p, pack, s);
 }
+
+FB_BOUNDS_ATTACH(cross_attn)
