@@ -296,6 +296,9 @@ inline Div div_by(long long d) {
 // its writes are visible; it must precede the first access to anything the predecessor produced
 // (and any write the predecessor might still read). `pdl_launch_dependents()` tells the scheduler
 // that the successor may begin its own preamble. Both are no-ops for ordinary launches.
+// A kernel so launched runs while data that it will read is being written, so that data may not be read by read-only loads (ld.global.nc: __ldg, or a `const` parameter
+// with `__restrict__`, which the compiler may take for one): they may answer from lines that were in L1 before the predecessor wrote them, as happened about once in 10^4
+// calls. Plain loads and loads past L1 (__ldcg) are ordered behind `pdl_wait()`.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -264,8 +264,8 @@ template <bool kShort>
 __global__ void __launch_bounds__(kAttnThreads, 2)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                 const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmDO,
-                const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ d_o,
-                const float* __restrict__ lse, __nv_bfloat16* __restrict__ dq, __nv_bfloat16* __restrict__ dk,
+                const __nv_bfloat16* o, const __nv_bfloat16* d_o,
+                const float* lse, __nv_bfloat16* __restrict__ dq, __nv_bfloat16* __restrict__ dk,
                 __nv_bfloat16* __restrict__ dv, const AttnParams p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // The layout leaves no room for alignment slack (two CTAs must fit in one SM): it relies on the 1024-byte alignment
@@ -380,8 +380,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__
     // The mask and the row statistics are in flight together: the LSE of a query row and D = rowsum(dO * O) (eight lanes per row, coalesced). The four
     // warps start them at once, behind the tensor loads: 256 x 12 heads x 128 tokens 111 us, without the barrier 132.
     asm volatile("bar.sync 1, 128;");
-    const float mraw = (t < p.S && p.mask) ? __ldg(p.mask + static_cast<long long>(b) * p.S + t) : 0.f;
-    const float lse_q = q_ok ? __ldg(lse + (static_cast<long long>(b) * p.H + h) * p.S + q) * kLog2e : 0.f;
+    const float mraw = (t < p.S && p.mask) ? __ldcg(p.mask + static_cast<long long>(b) * p.S + t) : 0.f;
+    const float lse_q = q_ok ? __ldcg(lse + (static_cast<long long>(b) * p.H + h) * p.S + q) * kLog2e : 0.f;
     const float Dq = row_dot64(o + static_cast<long long>(b) * p.osb + static_cast<long long>(h) * p.osh,
                                d_o + static_cast<long long>(b) * p.osb + static_cast<long long>(h) * p.osh, p.oss, warp * 32, p.S, lane);
     mask_s[t] = (t < p.S) ? mraw * kLog2e : -INFINITY;

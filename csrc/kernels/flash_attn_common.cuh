@@ -122,8 +122,8 @@ __device__ __forceinline__ float row_dot64(const __nv_bfloat16* a, const __nv_bf
       const int r = (half * 4 + k) * 4 + sub;
       xa[k] = xb[k] = make_uint4(0u, 0u, 0u, 0u);
       if (row0 + r < row_limit) {
-        xa[k] = __ldg(reinterpret_cast<const uint4*>(a + static_cast<long long>(row0 + r) * row_stride + ch * 8));
-        xb[k] = __ldg(reinterpret_cast<const uint4*>(b + static_cast<long long>(row0 + r) * row_stride + ch * 8));
+        xa[k] = __ldcg(reinterpret_cast<const uint4*>(a + static_cast<long long>(row0 + r) * row_stride + ch * 8));
+        xb[k] = __ldcg(reinterpret_cast<const uint4*>(b + static_cast<long long>(row0 + r) * row_stride + ch * 8));
       }
     }
 #pragma unroll

@@ -102,7 +102,7 @@ __device__ __forceinline__ bool wait_added(const unsigned int* added, unsigned i
 
 // Per query row: the first words of the row's dQ slot (overwritten by attn_dq_kernel at the end) take D = dot(dO, O) and two zeroed
 // counters (DqSlot), and the row's share of the dQ scratch is zeroed. Eight lanes per row, rows of one (batch, head) consecutive.
-__global__ void __launch_bounds__(256) attn_bwd_pre_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ d_o,
+__global__ void __launch_bounds__(256) attn_bwd_pre_kernel(const __nv_bfloat16* o, const __nv_bfloat16* d_o,
                                                            __nv_bfloat16* __restrict__ dq, float* __restrict__ dq_accum, const AttnParams p) {
   pdl_entry();
   const long long rows = static_cast<long long>(p.B) * p.H * p.S;
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(256) attn_bwd_pre_kernel(const __nv_bfloat16* 
     const long long bh = r / p.S;
     const int h = static_cast<int>(bh % p.H), b = static_cast<int>(bh / p.H);
     const long long off = b * p.osb + h * p.osh + s * p.oss + ch * 8;
-    const uint4 xa = __ldg(reinterpret_cast<const uint4*>(o + off)), xb = __ldg(reinterpret_cast<const uint4*>(d_o + off));
+    const uint4 xa = __ldcg(reinterpret_cast<const uint4*>(o + off)), xb = __ldcg(reinterpret_cast<const uint4*>(d_o + off));
     const __nv_bfloat162* ha = reinterpret_cast<const __nv_bfloat162*>(&xa);
     const __nv_bfloat162* hb = reinterpret_cast<const __nv_bfloat162*>(&xb);
     float d = 0.f;
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(256) attn_bwd_pre_kernel(const __nv_bfloat16* 
 }
 
 // dQ scratch (layout above) -> bf16 rows. Eight lanes per row.
-__global__ void __launch_bounds__(256) attn_dq_kernel(const float* __restrict__ dq_accum, __nv_bfloat16* __restrict__ dq, const AttnParams p) {
+__global__ void __launch_bounds__(256) attn_dq_kernel(const float* dq_accum, __nv_bfloat16* __restrict__ dq, const AttnParams p) {
   pdl_entry();
   const long long rows = static_cast<long long>(p.B) * p.H * p.S;
   const int ch = threadIdx.x & 7;
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(256) attn_dq_kernel(const float* __restrict__ 
 
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_long_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                     const __grid_constant__ CUtensorMap tmDO, const float* __restrict__ lse, __nv_bfloat16* dq,
+                     const __grid_constant__ CUtensorMap tmDO, const float* lse, __nv_bfloat16* dq,
                      __nv_bfloat16* __restrict__ dk, __nv_bfloat16* __restrict__ dv, float* __restrict__ dq_accum, const AttnParams p) {
   // No room for alignment slack: the kernel relies on the 1024-byte alignment of the dynamic shared-memory window and reports instead of
   // computing if that does not hold.
@@ -256,7 +256,7 @@ attn_bwd_long_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         const int q = query_block(it) * kBlk + i * 32 + lane;
         ahead[i] = make_float2(-INFINITY, 0.f);
         if (q < p.S) {
-          ahead[i].x = __ldg(lse + bh * p.S + q);
+          ahead[i].x = __ldcg(lse + bh * p.S + q);
           ahead[i].y = __ldcg(&reinterpret_cast<const DqSlot*>(dq + b * p.gsb + h * p.gsh + q * p.gss)->D);
         }
       }
@@ -376,7 +376,7 @@ attn_bwd_long_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const int kv0 = item[0] * kBlk;
     if (threadIdx.x < kBlk) {      // the additive mask (mask * log2e; -inf beyond S)
       const int kv = kv0 + threadIdx.x;
-      mask_s[threadIdx.x] = kv < p.S ? (p.mask ? __ldg(p.mask + static_cast<long long>(item[2]) * p.S + kv) * kLog2e : 0.f) : -INFINITY;
+      mask_s[threadIdx.x] = kv < p.S ? (p.mask ? __ldcg(p.mask + static_cast<long long>(item[2]) * p.S + kv) * kLog2e : 0.f) : -INFINITY;
     }
     asm volatile("bar.sync 1, 512;" ::: "memory");
     const bool masked = p.mask != nullptr || kv0 + kBlk > p.S;
@@ -663,7 +663,7 @@ attn_fwd_long_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       if constexpr (kMask) {       // additive mask of this key block (mask * log2e; -inf beyond S); the other buffer may still be in use
         if (half == 0) {
           const int kv = kv0 + t;
-          mask_s[(j & 1) * kBlk + t] = kv < p.S ? __ldg(p.mask + static_cast<long long>(b) * p.S + kv) * kLog2e : -INFINITY;
+          mask_s[(j & 1) * kBlk + t] = kv < p.S ? __ldcg(p.mask + static_cast<long long>(b) * p.S + kv) * kLog2e : -INFINITY;
         }
         asm volatile("bar.sync 1, 256;" ::: "memory");
       }
