@@ -56,7 +56,7 @@ __device__ __forceinline__ bool bn_aligned(const void* p) {
 // grid (C, kBnSplits)
 template <typename T>
 __global__ void __launch_bounds__(kBnThreads)
-bn_stats_kernel(const T* __restrict__ x, float* __restrict__ partial, int N, int C, int HW) {
+bn_stats_kernel(const T* x, float* __restrict__ partial, int N, int C, int HW) {
   pdl_entry();
   constexpr int V = VecIO<T>::kVec;
   __shared__ float scratch[32];
@@ -92,8 +92,8 @@ bn_stats_kernel(const T* __restrict__ x, float* __restrict__ partial, int N, int
 // grid (C, kBnSplits)
 template <typename T>
 __global__ void __launch_bounds__(kBnThreads)
-bn_apply_kernel(const T* __restrict__ x, const T* __restrict__ residual, const float* __restrict__ gamma,
-                const float* __restrict__ beta, const float* __restrict__ partial, float* __restrict__ running_mean,
+bn_apply_kernel(const T* x, const T* residual, const float* gamma,
+                const float* beta, const float* partial, float* __restrict__ running_mean,
                 float* __restrict__ running_var, float* __restrict__ save_mean, float* __restrict__ save_rstd,
                 T* __restrict__ y, int N, int C, int HW, float eps, float momentum, int relu, int training) {
   pdl_entry();
@@ -151,8 +151,8 @@ bn_apply_kernel(const T* __restrict__ x, const T* __restrict__ residual, const f
 
 template <typename T>
 __global__ void __launch_bounds__(kBnThreads)
-bn_bwd_reduce_kernel(const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ y,
-                     const float* __restrict__ save_mean, const float* __restrict__ save_rstd, float* __restrict__ partial,
+bn_bwd_reduce_kernel(const T* dy, const T* x, const T* y,
+                     const float* save_mean, const float* save_rstd, float* __restrict__ partial,
                      int N, int C, int HW, int relu) {
   pdl_entry();
   constexpr int V = VecIO<T>::kVec;
@@ -194,8 +194,8 @@ bn_bwd_reduce_kernel(const T* __restrict__ dy, const T* __restrict__ x, const T*
 
 template <typename T>
 __global__ void __launch_bounds__(kBnThreads)
-bn_bwd_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ y, const float* __restrict__ gamma,
-                    const float* __restrict__ save_mean, const float* __restrict__ save_rstd, const float* __restrict__ partial,
+bn_bwd_apply_kernel(const T* dy, const T* x, const T* y, const float* gamma,
+                    const float* save_mean, const float* save_rstd, const float* partial,
                     T* __restrict__ dx, T* __restrict__ dres, float* __restrict__ dgamma, float* __restrict__ dbeta,
                     int accumulate, int N, int C, int HW, int relu) {
   pdl_entry();
@@ -320,7 +320,7 @@ __device__ __forceinline__ bool nhwc_publish(const NhwcMap<T>& m, int C, const f
 // slices are then folded through shared memory. Results land in sm[0 .. 2C): plane 0 then plane 1.
 // The backward's reduction over a ResNet-20 step, us per launch, with one column and four rows in flight against this: batch 1000
 // 21.8 -> 17.5, batch 128 9.1 -> 8.0.
-__device__ __forceinline__ void nhwc_fold(const float* __restrict__ partial, int nrows, int C, float* sm) {
+__device__ __forceinline__ void nhwc_fold(const float* partial, int nrows, int C, float* sm) {
   constexpr int kRows = 8;
   const int four = C / 2, slices = kBnThreads / four;       // C is a multiple of 4 and at most kBnThreads
   const int c4 = (threadIdx.x % four) * 4, sl = threadIdx.x / four;
@@ -367,7 +367,7 @@ constexpr int kBnStatsPerSm = 4, kBnApplyPerSm = 3, kBnBwdPerSm = 2;
 
 template <typename T>
 __global__ void __launch_bounds__(kBnThreads, kBnStatsPerSm)
-bn_nhwc_stats_kernel(const T* __restrict__ x, float* __restrict__ partial, unsigned int* __restrict__ counter,
+bn_nhwc_stats_kernel(const T* x, float* __restrict__ partial, unsigned int* __restrict__ counter,
                      float* __restrict__ running_mean, float* __restrict__ running_var, float* __restrict__ save_mean,
                      float* __restrict__ save_rstd, long long P, int C, float eps, float momentum) {
   pdl_entry();
@@ -406,9 +406,9 @@ bn_nhwc_stats_kernel(const T* __restrict__ x, float* __restrict__ partial, unsig
 // statistics pass over x.
 template <typename T, bool kFromSums>
 __global__ void __launch_bounds__(kBnThreads, kBnApplyPerSm)
-bn_nhwc_apply_kernel(const T* __restrict__ x, const T* __restrict__ residual, const float* __restrict__ gamma,
-                     const float* __restrict__ beta, const float* __restrict__ mean, const float* __restrict__ rstd,
-                     T* __restrict__ y, long long P, int C, int relu, const float* __restrict__ sums, float* __restrict__ save_mean,
+bn_nhwc_apply_kernel(const T* x, const T* residual, const float* gamma,
+                     const float* beta, const float* mean, const float* rstd,
+                     T* __restrict__ y, long long P, int C, int relu, const float* sums, float* __restrict__ save_mean,
                      float* __restrict__ save_rstd, float* __restrict__ running_mean, float* __restrict__ running_var, float eps,
                      float momentum) {
   pdl_entry();
@@ -470,8 +470,8 @@ bn_nhwc_apply_kernel(const T* __restrict__ x, const T* __restrict__ residual, co
 // fold[0..C) = mean of dy', fold[C..2C) = mean of dy' * xhat
 template <typename T>
 __global__ void __launch_bounds__(kBnThreads, kBnBwdPerSm)
-bn_nhwc_bwd_reduce_kernel(const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ y, const float* __restrict__ mean,
-                          const float* __restrict__ rstd, float* __restrict__ partial, unsigned int* __restrict__ counter,
+bn_nhwc_bwd_reduce_kernel(const T* dy, const T* x, const T* y, const float* mean,
+                          const float* rstd, float* __restrict__ partial, unsigned int* __restrict__ counter,
                           float* __restrict__ fold, float* __restrict__ dgamma, float* __restrict__ dbeta, int accumulate,
                           long long P, int C, int relu) {
   pdl_entry();
@@ -528,8 +528,8 @@ bn_nhwc_bwd_reduce_kernel(const T* __restrict__ dy, const T* __restrict__ x, con
 
 template <typename T>
 __global__ void __launch_bounds__(kBnThreads, kBnBwdPerSm)
-bn_nhwc_bwd_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x, const T* __restrict__ y, const float* __restrict__ gamma,
-                         const float* __restrict__ mean, const float* __restrict__ rstd, const float* __restrict__ fold,
+bn_nhwc_bwd_apply_kernel(const T* dy, const T* x, const T* y, const float* gamma,
+                         const float* mean, const float* rstd, const float* fold,
                          T* __restrict__ dx, T* __restrict__ dres, long long P, int C, int relu) {
   pdl_entry();
   constexpr int V = VecIO<T>::kVec;

@@ -302,6 +302,9 @@ inline Div div_by(long long d) {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+template <typename T>
+__device__ __forceinline__ T plain_load(const T* p) { return *p; }
+
 // First statements of every kernel launched through `launch_pdl`: wait for the predecessor, then let the
 // successor's blocks be scheduled as this grid's blocks retire.
 __device__ __forceinline__ void pdl_entry() {

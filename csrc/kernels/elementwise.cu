@@ -35,7 +35,7 @@ __device__ __forceinline__ float gelu_bwd_f(float x, int tanh_approx) {
 }
 
 template <typename T>
-__global__ void gelu_fwd_kernel(const T* __restrict__ x, T* __restrict__ y, long long n, int tanh_approx) {
+__global__ void gelu_fwd_kernel(const T* x, T* __restrict__ y, long long n, int tanh_approx) {
   pdl_entry();
   constexpr int V = VecIO<T>::kVec;
   const long long stride = static_cast<long long>(gridDim.x) * blockDim.x * V;
@@ -53,7 +53,7 @@ __global__ void gelu_fwd_kernel(const T* __restrict__ x, T* __restrict__ y, long
 }
 
 template <typename T>
-__global__ void gelu_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, T* __restrict__ dx,
+__global__ void gelu_bwd_kernel(const T* dy, const T* x, T* __restrict__ dx,
                                 long long n, int tanh_approx) {
   pdl_entry();
   constexpr int V = VecIO<T>::kVec;
@@ -75,8 +75,8 @@ __global__ void gelu_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ 
 
 // y = x * mask(seed, idx) / (1 - p); used for forward and (with dy as x) for backward.
 template <typename T>
-__global__ void dropout_kernel(const T* __restrict__ x, T* __restrict__ y, long long n, float p,
-                               unsigned long long seed_in, const unsigned long long* __restrict__ seed_dev) {
+__global__ void dropout_kernel(const T* x, T* __restrict__ y, long long n, float p,
+                               unsigned long long seed_in, const unsigned long long* seed_dev) {
   pdl_entry();
   constexpr int V = VecIO<T>::kVec;
   const unsigned long long seed = seed_in + (seed_dev ? *seed_dev : 0ull);
@@ -103,8 +103,8 @@ __global__ void dropout_kernel(const T* __restrict__ x, T* __restrict__ y, long 
 
 // out[c] (+)= sum_r x[r][c]; a 32x32 tile per block so reads stay coalesced.
 template <typename T>
-__global__ void colsum_kernel(const T* __restrict__ x, float* __restrict__ out, int rows, int cols,
-                              long long ld, int rows_per_block, const int* __restrict__ rows_dyn) {
+__global__ void colsum_kernel(const T* x, float* __restrict__ out, int rows, int cols,
+                              long long ld, int rows_per_block, const int* rows_dyn) {
   pdl_entry();
   if (rows_dyn) rows = min(rows, *rows_dyn);
   __shared__ float tile[32][33];
@@ -128,8 +128,8 @@ __global__ void colsum_kernel(const T* __restrict__ x, float* __restrict__ out, 
 // a block different rows; partials meet in shared memory, one atomicAdd per column per block.
 template <typename T>
 __global__ void __launch_bounds__(256)
-colsum_vec_kernel(const T* __restrict__ x, float* __restrict__ out, int rows, int cols, long long ld, int rows_per_block,
-                  const int* __restrict__ rows_dyn) {
+colsum_vec_kernel(const T* x, float* __restrict__ out, int rows, int cols, long long ld, int rows_per_block,
+                  const int* rows_dyn) {
   pdl_entry();
   if (rows_dyn) rows = min(rows, *rows_dyn);
   constexpr int V = VecIO<T>::kVec;
@@ -176,7 +176,7 @@ colsum_vec_kernel(const T* __restrict__ x, float* __restrict__ out, int rows, in
 // Counts stay on the device, buffers keep their full static size: the sequence is graph-capturable.
 // ---------------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(1024)
-compact_targets_kernel(const long long* __restrict__ targets, int rows, long long ignore_index, int* __restrict__ idx,
+compact_targets_kernel(const long long* targets, int rows, long long ignore_index, int* __restrict__ idx,
                        long long* __restrict__ targets_c, int* __restrict__ counts) {
   pdl_entry();
   __shared__ int warp_tot[32];
@@ -223,7 +223,7 @@ compact_targets_kernel(const long long* __restrict__ targets, int rows, long lon
 
 template <typename T>
 __global__ void __launch_bounds__(128)
-gather_rows_kernel(const T* __restrict__ x, long long ld, const int* __restrict__ idx, const int* __restrict__ counts,
+gather_rows_kernel(const T* x, long long ld, const int* idx, const int* counts,
                    T* __restrict__ xc, long long ldc, int cols) {
   pdl_entry();
   const int i = blockIdx.x;
@@ -250,7 +250,7 @@ gather_rows_kernel(const T* __restrict__ x, long long ld, const int* __restrict_
 
 template <typename T>
 __global__ void __launch_bounds__(128)
-scatter_rows_kernel(const T* __restrict__ dxc, long long ldc, const int* __restrict__ idx, const int* __restrict__ counts,
+scatter_rows_kernel(const T* dxc, long long ldc, const int* idx, const int* counts,
                     T* __restrict__ dx, long long ld, int cols) {
   pdl_entry();
   const int i = blockIdx.x;
@@ -287,7 +287,7 @@ struct Vec4<__nv_bfloat16> {
 
 // dW[ids[t]][:] += dy[t][:] for an embedding table (fp32 accumulation, rows equal to padding_idx skipped).
 template <typename T>
-__global__ void embedding_bwd_kernel(const T* __restrict__ dy, const long long* __restrict__ ids, float* __restrict__ dw,
+__global__ void embedding_bwd_kernel(const T* dy, const long long* ids, float* __restrict__ dw,
                                      long long tokens, int dim, long long vocab, long long padding_idx) {
   pdl_entry();
   const long long t = static_cast<long long>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
@@ -309,7 +309,7 @@ __global__ void embedding_bwd_kernel(const T* __restrict__ dy, const long long* 
 // 4.2 (4.3); 32768 tokens of one id 21 (288), of random ids 22 (22); fp32 35 (35).
 template <typename T, int kEmbRows>
 __global__ void __launch_bounds__(256)
-embedding_bwd_vec_kernel(const T* __restrict__ dy, const long long* __restrict__ ids, float* __restrict__ dw, long long tokens, int dim,
+embedding_bwd_vec_kernel(const T* dy, const long long* ids, float* __restrict__ dw, long long tokens, int dim,
                          long long vocab, long long padding_idx, int per_block) {
   pdl_entry();
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 4;
@@ -348,7 +348,7 @@ embedding_bwd_vec_kernel(const T* __restrict__ dy, const long long* __restrict__
 }
 
 template <typename TI, typename TO>
-__global__ void cast_kernel(const TI* __restrict__ x, TO* __restrict__ y, long long n, float scale) {
+__global__ void cast_kernel(const TI* x, TO* __restrict__ y, long long n, float scale) {
   pdl_entry();
   const long long stride = static_cast<long long>(gridDim.x) * blockDim.x;
   for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < n; i += stride)

@@ -185,9 +185,9 @@ gemm_small_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant
       const int bc = col - grp * p.group;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        bias[j] = p.bias_fp32 ? __ldg(static_cast<const float*>(bias_of) + bc + j) : __bfloat162float(static_cast<const __nv_bfloat16*>(bias_of)[bc + j]);
+        bias[j] = p.bias_fp32 ? plain_load(static_cast<const float*>(bias_of) + bc + j) : __bfloat162float(static_cast<const __nv_bfloat16*>(bias_of)[bc + j]);
     }
-    const float alpha = p.alpha ? __ldg(p.alpha) : 1.f;
+    const float alpha = p.alpha ? plain_load(p.alpha) : 1.f;
     for (int r = rank * per + (threadIdx.x >> 4); r < min(rows, (rank + 1) * per); r += kThreads / 16) {
       const uint32_t at = smem_u32(part + r * kPitch + (threadIdx.x & 15) * 4);
       float v[4] = {0.f, 0.f, 0.f, 0.f};

@@ -149,20 +149,20 @@ __device__ __forceinline__ void add_bias32(const GemmParams& p, int col0, int nv
     if (nvalid == 32 && (reinterpret_cast<uintptr_t>(b) & 15) == 0) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float4 q = __ldg(reinterpret_cast<const float4*>(b) + j);
+        const float4 q = plain_load(reinterpret_cast<const float4*>(b) + j);
         v[4 * j] += q.x; v[4 * j + 1] += q.y; v[4 * j + 2] += q.z; v[4 * j + 3] += q.w;
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (i < nvalid) v[i] += __ldg(b + i);
+        if (i < nvalid) v[i] += plain_load(b + i);
     }
   } else {
     const __nv_bfloat16* b = static_cast<const __nv_bfloat16*>(p.bias) + col0;
     if (nvalid == 32 && (reinterpret_cast<uintptr_t>(b) & 15) == 0) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(b) + j);
+        const uint4 q = plain_load(reinterpret_cast<const uint4*>(b) + j);
         float h[8];
         unpack_bf16x2(q.x, h[0], h[1]); unpack_bf16x2(q.y, h[2], h[3]);
         unpack_bf16x2(q.z, h[4], h[5]); unpack_bf16x2(q.w, h[6], h[7]);
@@ -187,7 +187,7 @@ __device__ __forceinline__ void add_bias32(const GemmParams& p, int col0, int nv
 __device__ __forceinline__ void epilogue_compute32(const GemmParams& p, const uint32_t (&acc)[32], int row, int col0,
                                                    bool add_bias, float (&v)[32], float (&pre)[32]) {
   if (p.alpha) {
-    const float alpha = __ldg(p.alpha);
+    const float alpha = plain_load(p.alpha);
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(acc[i]) * alpha;
   } else {
@@ -301,7 +301,7 @@ __device__ __forceinline__ void epilogue_tile_f32(const GemmParams& p, const CUt
     tmem_ld32_sync(taddr + c, acc);
     if (c + 32 >= cols) hand_back();
     if (p.alpha) {
-      const float alpha = __ldg(p.alpha);
+      const float alpha = plain_load(p.alpha);
 #pragma unroll
       for (int i = 0; i < 32; ++i) acc[i] = __float_as_uint(__uint_as_float(acc[i]) * alpha);
     }
@@ -351,7 +351,7 @@ __device__ __forceinline__ bool epilogue_tile(const GemmParams& p, const CUtenso
       }
     }
     if (p.alpha) {
-      const F2 alpha = f2_splat(__ldg(p.alpha));
+      const F2 alpha = f2_splat(plain_load(p.alpha));
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = f2_mul(v[i], alpha);
     }
@@ -424,7 +424,7 @@ __device__ __forceinline__ void epilogue_store32(const GemmParams& p, const uint
   if (row >= p.M || col0 >= p.N) return;
   float v[32];
   if (p.alpha) {
-    const float alpha = __ldg(p.alpha);
+    const float alpha = plain_load(p.alpha);
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(acc[i]) * alpha;
   } else {
@@ -665,7 +665,7 @@ __device__ __forceinline__ void column_sums(const GemmLaunch<kProblems>& g, int 
     for (int r = r0; r < r1; r += 8) {
       uint4 q[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = r + i < r1 ? __ldg(reinterpret_cast<const uint4*>(x + static_cast<long long>(r + i) * g.sum_ld)) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < 8; ++i) q[i] = r + i < r1 ? plain_load(reinterpret_cast<const uint4*>(x + static_cast<long long>(r + i) * g.sum_ld)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
@@ -680,7 +680,7 @@ __device__ __forceinline__ void column_sums(const GemmLaunch<kProblems>& g, int 
     float v[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      if (g.p[0].alpha) acc[j] = f2_mul(acc[j], f2_splat(__ldg(g.p[0].alpha)));
+      if (g.p[0].alpha) acc[j] = f2_mul(acc[j], f2_splat(plain_load(g.p[0].alpha)));
       f2_get(acc[j], v[2 * j], v[2 * j + 1]);
     }
     red_add_v4(g.sum_out + col, v[0], v[1], v[2], v[3]);
@@ -924,7 +924,7 @@ gemm_bf16_kernel(const __grid_constant__ GemmLaunch<kProblems> g) {
       tile_of(u / work.parts(), work.num_m, work.num_n, p.band, tm, tn);
       const int c = q * 32 + lane, col = tn * kBN + half * kSplit + c;
       if (c >= cols || col >= p.N) return 0.f;
-      return p.bias_fp32 ? __ldg(static_cast<const float*>(p.bias) + col) : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col]);
+      return p.bias_fp32 ? plain_load(static_cast<const float*>(p.bias) + col) : __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[col]);
     };
     float next_bias = staged_bias ? bias_of(group) : 0.f;
     int it = 0;
@@ -1640,8 +1640,8 @@ long long part_rows(int M, int N, int K, bool counted, int groups) {
 // A chain of latencies: the grid is what two waves hold, so that many rows are walked and few are shared. The whole of fb_gemm_parts, us, a block for every
 // 64 quads instead: 2048 x 768 x 8200 26.5 (45.5), 4096 x 768 x 30522 with 614 rows 38.0 (63.3); without the four lanes 64 x 768 x 50257 20.6 (27.8).
 constexpr int kSumThreads = 256, kSumLanes = 4, kSumBlocks = 8;
-__global__ void __launch_bounds__(kSumThreads, 4) sum_parts_kernel(const float* __restrict__ parts, int rows, int cols, int num_kb, int groups,
-                                                                            const int* __restrict__ idx, const int* __restrict__ counts,
+__global__ void __launch_bounds__(kSumThreads, 4) sum_parts_kernel(const float* parts, int rows, int cols, int num_kb, int groups,
+                                                                            const int* idx, const int* counts,
                                                                             __nv_bfloat16* __restrict__ dx, long long ld) {
   __shared__ float4 meet[kSumLanes - 1][kSumThreads / kSumLanes];
   pdl_entry();

@@ -20,7 +20,7 @@ constexpr int kLnWarps = 4;
 // N consecutive fp32 values p[off .. off+N) as 16-byte loads (N is 4 or 8, off a multiple of N, the
 // array 16-byte aligned as every parameter slot is); `fill` when p is null.
 template <int N>
-__device__ __forceinline__ void load_f32_vec(const float* __restrict__ p, int off, float fill, float (&out)[N]) {
+__device__ __forceinline__ void load_f32_vec(const float* p, int off, float fill, float (&out)[N]) {
   if (!p) {
 #pragma unroll
     for (int j = 0; j < N; ++j) out[j] = fill;
@@ -29,12 +29,12 @@ __device__ __forceinline__ void load_f32_vec(const float* __restrict__ p, int of
   if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
 #pragma unroll
     for (int j = 0; j < N; j += 4) {
-      const float4 q = __ldg(reinterpret_cast<const float4*>(p + off + j));
+      const float4 q = plain_load(reinterpret_cast<const float4*>(p + off + j));
       out[j] = q.x; out[j + 1] = q.y; out[j + 2] = q.z; out[j + 3] = q.w;
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) out[j] = __ldg(p + off + j);
+    for (int j = 0; j < N; ++j) out[j] = plain_load(p + off + j);
   }
 }
 
@@ -45,29 +45,29 @@ struct Param;
 template <int N>
 struct Param<float, N> {
   float v[N];
-  __device__ __forceinline__ void load(const float* __restrict__ p, int off, float fill) { load_f32_vec<N>(p, off, fill, v); }
+  __device__ __forceinline__ void load(const float* p, int off, float fill) { load_f32_vec<N>(p, off, fill, v); }
   __device__ __forceinline__ float get(int j) const { return v[j]; }
 };
 template <int N>
 struct Param<__nv_bfloat16, N> {
   static_assert(N == 4 || N == 8, "");
   uint32_t h[N / 2];
-  __device__ __forceinline__ void load(const __nv_bfloat16* __restrict__ p, int off, float fill) {
+  __device__ __forceinline__ void load(const __nv_bfloat16* p, int off, float fill) {
     if (!p) {
 #pragma unroll
       for (int j = 0; j < N / 2; ++j) h[j] = __float_as_uint(fill) >> 16 | (__float_as_uint(fill) & 0xffff0000u);
     } else if ((reinterpret_cast<uintptr_t>(p) & (2 * N - 1)) == 0) {
       if constexpr (N == 8) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(p + off));
+        const uint4 q = plain_load(reinterpret_cast<const uint4*>(p + off));
         h[0] = q.x; h[1] = q.y; h[2] = q.z; h[3] = q.w;
       } else {
-        const uint2 q = __ldg(reinterpret_cast<const uint2*>(p + off));
+        const uint2 q = plain_load(reinterpret_cast<const uint2*>(p + off));
         h[0] = q.x; h[1] = q.y;
       }
     } else {
       const uint16_t* u = reinterpret_cast<const uint16_t*>(p + off);
 #pragma unroll
-      for (int j = 0; j < N / 2; ++j) h[j] = static_cast<uint32_t>(__ldg(u + 2 * j)) | static_cast<uint32_t>(__ldg(u + 2 * j + 1)) << 16;
+      for (int j = 0; j < N / 2; ++j) h[j] = static_cast<uint32_t>(plain_load(u + 2 * j)) | static_cast<uint32_t>(plain_load(u + 2 * j + 1)) << 16;
     }
   }
   __device__ __forceinline__ float get(int j) const { return __uint_as_float(j & 1 ? h[j / 2] & 0xffff0000u : h[j / 2] << 16); }
@@ -89,10 +89,10 @@ constexpr int ln_bwd_blocks(int values) { return values <= 16 ? 4 : values <= 24
 // which half is the parameters' conversion, which had made each of six loads wait for the one before.
 template <typename T, int VPL, typename P, bool kFew>
 __global__ void __launch_bounds__(kLnWarps * 32, kFew ? 2 : ln_fwd_blocks(sizeof(T)))
-ln_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const P* __restrict__ gamma,
-              const P* __restrict__ beta, T* __restrict__ y, T* __restrict__ pre_out,
+ln_fwd_kernel(const T* x, const T* residual, const P* gamma,
+              const P* beta, T* __restrict__ y, T* __restrict__ pre_out,
               float* __restrict__ mean_out, float* __restrict__ rstd_out, int rows, int cols, float eps,
-              float p_drop, uint64_t seed_in, const unsigned long long* __restrict__ seed_dev) {
+              float p_drop, uint64_t seed_in, const unsigned long long* seed_dev) {
   if constexpr (kFew) {
     const int at = threadIdx.x * (128 / static_cast<int>(sizeof(P)));
     if (at < cols) {
@@ -204,10 +204,10 @@ ln_fwd_kernel(const T* __restrict__ x, const T* __restrict__ residual, const P* 
 // 54 us (5.5 TB/s) against 104, 65536 x 1024, where two blocks fit an SM, 133 against 245; fp32 32768 x 768 60 against 97.
 template <typename T, int VPL>
 __global__ void __launch_bounds__(kLnWarps * 32, ln_bwd_blocks(VPL * VecIO<T>::kVec))
-ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ pre, const float* __restrict__ mean,
-              const float* __restrict__ rstd, const float* __restrict__ gamma, T* __restrict__ dpre,
+ln_bwd_kernel(const T* dy, const T* pre, const float* mean,
+              const float* rstd, const float* gamma, T* __restrict__ dpre,
               T* __restrict__ dx_drop, float* __restrict__ partial, float* __restrict__ dgamma, float* __restrict__ dbeta,
-              int rows, int cols, float p_drop, uint64_t seed_in, const unsigned long long* __restrict__ seed_dev) {
+              int rows, int cols, float p_drop, uint64_t seed_in, const unsigned long long* seed_dev) {
   pdl_entry();
   constexpr int V = VecIO<T>::kVec;
   const uint64_t seed = seed_in + (seed_dev ? *seed_dev : 0ull);
@@ -346,7 +346,7 @@ ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ pre, const float* 
 
 // dgamma / dbeta = the column sums of the partial rows: 32 columns x 32 row groups per block, four rows in flight per thread.
 __global__ void __launch_bounds__(1024)
-ln_bwd_finalize_kernel(const float* __restrict__ partial, float* __restrict__ dgamma, float* __restrict__ dbeta, int nblocks, int cols) {
+ln_bwd_finalize_kernel(const float* partial, float* __restrict__ dgamma, float* __restrict__ dbeta, int nblocks, int cols) {
   pdl_entry();
   __shared__ float rg[32][33], rb[32][33];
   const int lane = threadIdx.x & 31, grp = threadIdx.x >> 5;

@@ -24,13 +24,13 @@ namespace fb {
 // hyper = {lr, 1-b1^t, 1-b2^t, weight_decay}
 template <typename TG>
 __global__ void __launch_bounds__(256)
-adam_kernel(float* __restrict__ p, const TG* __restrict__ g, float* __restrict__ m, float* __restrict__ v,
-            __nv_bfloat16* __restrict__ p16, long long n, const float* __restrict__ hyper, float b1, float b2,
-            float eps, const float* __restrict__ grad_scale, const int* __restrict__ skip, float4 hv) {
+adam_kernel(float* __restrict__ p, const TG* g, float* __restrict__ m, float* __restrict__ v,
+            __nv_bfloat16* __restrict__ p16, long long n, const float* hyper, float b1, float b2,
+            float eps, const float* grad_scale, const int* skip, float4 hv) {
   pdl_entry();
   // `skip`: a device-visible word that a collective sets when it gave up; the update is then left out
   // and the parameters stay as they were, so the host can raise before anything diverged.
-  if (skip && __ldg(skip) != 0) return;
+  if (skip && plain_load(skip) != 0) return;
   // hyper-parameters from device memory (a captured graph replays with fresh values) or, when `hyper` is null, by value
   const float lr = hyper ? hyper[0] : hv.x, bc1 = hyper ? hyper[1] : hv.y, bc2 = hyper ? hyper[2] : hv.z, wd = hyper ? hyper[3] : hv.w;
   const float gs = grad_scale ? *grad_scale : 1.f;
@@ -88,10 +88,10 @@ adam_kernel(float* __restrict__ p, const TG* __restrict__ g, float* __restrict__
 // hyper = {lr, momentum, weight_decay, first_step (0/1)}
 template <typename TG>
 __global__ void __launch_bounds__(256)
-sgd_kernel(float* __restrict__ p, const TG* __restrict__ g, float* __restrict__ buf, __nv_bfloat16* __restrict__ p16,
-           long long n, const float* __restrict__ hyper, const float* __restrict__ grad_scale, const int* __restrict__ skip) {
+sgd_kernel(float* __restrict__ p, const TG* g, float* __restrict__ buf, __nv_bfloat16* __restrict__ p16,
+           long long n, const float* hyper, const float* grad_scale, const int* skip) {
   pdl_entry();
-  if (skip && __ldg(skip) != 0) return;
+  if (skip && plain_load(skip) != 0) return;
   const float lr = hyper[0], mu = hyper[1], wd = hyper[2];
   const bool first = hyper[3] != 0.f;
   const float gs = grad_scale ? *grad_scale : 1.f;
@@ -112,7 +112,7 @@ sgd_kernel(float* __restrict__ p, const TG* __restrict__ g, float* __restrict__ 
 
 template <typename T>
 __global__ void __launch_bounds__(256)
-sumsq_partial_kernel(const T* __restrict__ x, long long n, float* __restrict__ partial) {
+sumsq_partial_kernel(const T* x, long long n, float* __restrict__ partial) {
   pdl_entry();
   __shared__ float scratch[32];
   constexpr int V = VecIO<T>::kVec;
@@ -149,7 +149,7 @@ sumsq_partial_kernel(const T* __restrict__ x, long long n, float* __restrict__ p
 }
 
 // out = {norm, clip coefficient = min(1, max_norm / (norm + 1e-6)) or 1 when max_norm <= 0}
-__global__ void sumsq_finalize_kernel(const float* __restrict__ partial, int nparts, float max_norm,
+__global__ void sumsq_finalize_kernel(const float* partial, int nparts, float max_norm,
                                       float extra_scale, float* __restrict__ out) {
   pdl_entry();
   __shared__ float scratch[32];

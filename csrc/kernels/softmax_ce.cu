@@ -12,7 +12,7 @@
 
 namespace fb {
 
-__global__ void ce_count_kernel(const long long* __restrict__ targets, int rows, long long ignore_index,
+__global__ void ce_count_kernel(const long long* targets, int rows, long long ignore_index,
                                 float* __restrict__ count_inv /* [0]=count, [1]=1/max(count,1) */) {
   pdl_entry();
   __shared__ float scratch[32];
@@ -89,9 +89,9 @@ __device__ __forceinline__ float sum_rebased(float s, float m, float to) { retur
 // kUnroll vectors in flight per thread, kBlocks blocks of kThreads on an SM.
 template <typename T, bool kWarpRow, int kThreads, int kBlocks, int kUnroll>
 __global__ void __launch_bounds__(kThreads, kBlocks)
-ce_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* __restrict__ targets, int rows,
+ce_fwd_kernel(const T* logits, long long ld, const long long* targets, int rows,
               int V, long long ignore_index, T* __restrict__ dlogits, long long ldd,
-              const float* __restrict__ count_inv, float* __restrict__ row_loss, const int* __restrict__ counts) {
+              const float* count_inv, float* __restrict__ row_loss, const int* counts) {
   pdl_entry();
   constexpr int VEC = VecIO<T>::kVec;
   constexpr int kWarps = kThreads / 32;
@@ -197,7 +197,7 @@ ce_fwd_kernel(const T* __restrict__ logits, long long ld, const long long* __res
 }
 
 // loss = sum(row_loss) / max(count, 1), in a fixed order (deterministic).
-__global__ void ce_finalize_kernel(const float* __restrict__ row_loss, int rows, const float* __restrict__ count_inv,
+__global__ void ce_finalize_kernel(const float* row_loss, int rows, const float* count_inv,
                                    float* __restrict__ loss) {
   pdl_entry();
   __shared__ float scratch[32];
@@ -210,7 +210,7 @@ __global__ void ce_finalize_kernel(const float* __restrict__ row_loss, int rows,
 // x[r][c] *= *scalar (device scalar); rows of length `cols` with leading dimension `ld`. A factor of one, which is what the
 // gradient of a loss that is differentiated itself arrives with, leaves x as it is and costs the launch only.
 template <typename T>
-__global__ void __launch_bounds__(256) scale_rows_kernel(T* __restrict__ x, long long ld, int rows, int cols, const float* __restrict__ scalar) {
+__global__ void __launch_bounds__(256) scale_rows_kernel(T* __restrict__ x, long long ld, int rows, int cols, const float* scalar) {
   pdl_entry();
   constexpr int VEC = VecIO<T>::kVec;
   const float a = *scalar;

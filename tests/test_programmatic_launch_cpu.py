@@ -5,12 +5,12 @@ import re
 
 import pytest
 
-KERNELS = pathlib.Path(__file__).resolve().parent.parent / "csrc" / "kernels"
-FILES = ["flash_attn.cu", "flash_attn_long.cu", "flash_attn_common.cuh", "cross_attn.cu", "rotary.cu"]
+CSRC = pathlib.Path(__file__).resolve().parent.parent / "csrc"
+FILES = sorted(str(p.relative_to(CSRC)) for folder in ("kernels", "comm") for p in (CSRC / folder).glob("*.cu*"))
 
 
 def code(name):
-    return re.sub(r"//[^\n]*", "", (KERNELS / name).read_text())
+    return re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
 
 
 @pytest.mark.parametrize("name", FILES)
@@ -19,6 +19,10 @@ def test_no_read_only_loads(name):
     assert not re.findall(r"__ldg\s*\(|ld\.global(?:\.\w+)*\.nc", text)
     # a read-only parameter that nothing else may point at
     assert not re.findall(r"const\s+[\w:]+(?:\s+[\w:]+)?\s*\*\s*__restrict__\s+\w+", text)
+
+
+def test_all_kernels_are_looked_at():
+    assert len(FILES) >= 16 and "kernels/flash_attn_long.cu" in FILES
 
 
 def test_the_patterns_find_what_they_look_for():
