@@ -25,7 +25,7 @@ def masks(B, Sk):
     yield torch.where(some, torch.randn(B, Sk, generator=g, device="cuda"), float("-inf"))
 
 
-@pytest.mark.parametrize("shape", [(64, 40, 700, 8, 8, 64), (65, 40, 700, 8, 8, 64), (66, 130, 300, 4, 2, 128), (300, 17, 600, 8, 8, 64), (1025, 20, 130, 8, 4, 64), (1500, 3, 30, 2, 2, 64),
+@pytest.mark.parametrize("shape", [(64, 40, 700, 8, 8, 64), (65, 40, 700, 8, 8, 64), (66, 130, 300, 4, 2, 128), (70, 40, 3000, 1, 1, 64), (300, 17, 600, 8, 8, 64), (1025, 20, 130, 8, 4, 64), (1500, 3, 30, 2, 2, 64),
                                    (2047, 17, 33, 6, 6, 64)], ids=str)
 def test_masks_of_many_batch_rows(C, shape):
     q, k, v, do = case(*shape, seed=1)
