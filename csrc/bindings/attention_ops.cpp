@@ -312,23 +312,21 @@ Tensor launch_cross(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, 
 }
 
 // The gradients by way of the plain form, for those that are differentiated again or are more than memory themselves (a batch of them).
-variable_list plain_gradients(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& mask, const Tensor& d_o, double scale) {
+variable_list plain_gradients(const Tensor (&given)[3], const Tensor& mask, const Tensor& d_o, double scale) {
   const bool again = at::GradMode::is_enabled();
   at::AutoGradMode record(true);
-  Tensor o;
+  Tensor x[3], o;        // each by a name of its own: one tensor may be queries, keys and values
+  for (int i = 0; i < 3; ++i) x[i] = given[i].view_as(given[i]);
   {
     py::gil_scoped_acquire gil;
-    o = py::module_::import("flodl_b200.ops.cross").attr("_plain")(q, k, v, mask.defined() ? py::cast(mask) : py::none(), scale).cast<Tensor>();
+    o = py::module_::import("flodl_b200.ops.cross").attr("_plain")(x[0], x[1], x[2], mask.defined() ? py::cast(mask) : py::none(), scale).cast<Tensor>();
   }
   variable_list of, out(6);
-  for (const Tensor* t : {&q, &k, &v})
-    if (t->requires_grad()) of.push_back(*t);
+  for (const Tensor& t : x)
+    if (t.requires_grad()) of.push_back(t);
   const auto grads = torch::autograd::grad({o}, of, {d_o}, /*retain_graph=*/again, /*create_graph=*/again);
-  size_t i = 0, at = 0;
-  for (const Tensor* t : {&q, &k, &v}) {
-    if (t->requires_grad()) out[i] = grads[at++];
-    ++i;
-  }
+  for (size_t i = 0, at = 0; i < 3; ++i)
+    if (x[i].requires_grad()) out[i] = grads[at++];
   return out;
 }
 
@@ -345,7 +343,7 @@ struct CrossFn : public torch::autograd::Function<CrossFn> {
     if (!ctx->saved_data["twice"].toBool()) first_derivative_only();
     const auto saved = ctx->get_saved_variables();
     if (at::GradMode::is_enabled() || !plain_memory(grads[0]))
-      return plain_gradients(saved[0], saved[1], saved[2], saved[3], grads[0], ctx->saved_data["scale"].toDouble());
+      return plain_gradients({saved[0], saved[1], saved[2]}, saved[3], grads[0], ctx->saved_data["scale"].toDouble());
     const Tensor q = mapped(saved[0]), k = mapped(saved[1]), v = mapped(saved[2]), d_o = mapped(grads[0]);
     const Tensor &mask = saved[3], &o = saved[4], &stats = saved[5];
     c10::cuda::CUDAGuard guard(q.device());

@@ -73,3 +73,13 @@ def test_gradients_of_masks_with_shared_addends():
     add = torch.tensor([[100.0, 101.0, 99.5, float("-inf"), 100.25]], dtype=torch.float64)
     keep = add > float("-inf")
     assert torch.autograd.gradcheck(lambda m: ops.cross_attention(q, k, v, torch.where(keep, m, float("-inf"))), add.masked_fill(~keep, 0.0).requires_grad_())
+
+
+def test_absent_keys_get_no_gradient_from_rows_that_are_no_numbers():
+    q, k, v, do = (normal(2, n, 2, 8, seed=n + i) for i, n in enumerate((4, 6, 6, 4)))
+    mask = torch.tensor([[True, False, True, True, False, True], [True, True, False, True, True, True]])
+    q[0, 0, 0, 3], do[1, 2, 1, 5] = float("nan"), float("inf")
+    for m in (mask, torch.zeros(2, 6).masked_fill(~mask, float("-inf"))):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        dk, dv = torch.autograd.grad(ops.cross_attention(*leaves, m), leaves[1:], do)
+        assert (dk[~mask] == 0).all() and (dv[~mask] == 0).all() and dk[0, 0, 0].isnan().all()

@@ -71,3 +71,19 @@ def test_positions(packed, norm):
     for count in range(1, n):
         for which in itertools.combinations(range(n), count):
             assert all(torch.equal(a, every[i]) for a, i in zip(grads(which), which))
+
+
+def test_one_tensor_for_all_inputs():
+    """Its gradient is the sum of three, one by one and in a batch, which goes by the plain form."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x, do = torch.randn(2, 9, 2, 64, device="cuda", generator=g).bfloat16(), torch.randn(3, 2, 9, 2, 64, device="cuda", generator=g).bfloat16()
+    for leaf in (True, False):
+        t = x.clone().requires_grad_()
+        used = t if leaf else t * 1
+        o = ops.cross_attention(used, used, used)
+        one = [torch.autograd.grad(o, t, d, retain_graph=True)[0] for d in do]
+        every = torch.autograd.grad(o, t, do, is_grads_batched=True)[0]
+        for d, a, b in zip(do, one, every):
+            want = torch.autograd.grad(ops.cross_attention(*[(w := x.double().requires_grad_())] * 3), w, d.double())[0]
+            # three gradients of bf16 with P, dS and D rounded before them, or rounded only themselves
+            assert (a.double() - want).norm() <= 6 * 2.0 ** -8 * want.norm() and (b.double() - want).norm() <= 3 * 2.0 ** -8 * want.norm()
