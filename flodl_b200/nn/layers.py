@@ -574,7 +574,7 @@ class MultiheadAttention(Module):
     `mask` marks positions to exclude (non-zero = masked); a strictly upper-triangular [S, S] mask is
     recognised as causal and, like an absent mask, runs on the fused attention kernel. Keys of another length than the
     queries go through the kernel of `ops.cross_attention` in bf16 with heads of 64 and 128 on a GPU, where no mask or one of keys
-    ([1, Sk], [B, 1, 1, Sk]) is given. A query none of whose keys are left gets NaN over another length."""
+    ([1, Sk], [B, 1, 1, Sk]) is given and it is faster there than separate operators. A query none of whose keys are left gets NaN over another length."""
 
     def __init__(self, embed_dim: int, num_heads: int, device=None):
         if embed_dim % num_heads:
@@ -607,6 +607,24 @@ class MultiheadAttention(Module):
         shape = (1,) * (4 - mask.dim()) + tuple(mask.shape)
         return len(shape) == 4 and shape[0] in (1, B) and shape[1:] == (1, 1, Sk) and Sk > 0
 
+    @staticmethod
+    def _kernel_is_faster(B: int, H: int, Sq: int, Sk: int, trained: bool, masked: bool) -> bool:
+        """Whether the kernel, whose time goes by tiles of 128 queries by 128 keys, beats separate operators, whose time goes by the values and by the launches.
+
+        With two tiles for each SM at most it is the launches (2 heads of 2 batch rows: 936 us a call forward and backward, 560 on the kernel). Beyond that the backward pass takes 0.06 to 0.09 us a
+        tile, and the operators 0.001 us for each query and key, which they copy: 80 of them a tile pay for it. With one head they copy nothing, and 4096 pairs a tile do. Forward and backward, replayed,
+        us of B x H x Sq x Sk, heads of 64, separate operators and kernel: 1412 x 16 x 2 x 1 393 and 1484, 2848 x 16 x 42 x 2 2664 and 3511, 2171 x 16 x 64 x 2 2714 and 3073, 1024 x 8 x 48 x 200 4545 and
+        2217, 1140 x 1 x 25 x 112 107 and 137. The forward pass loses where a mask is looked through for one to four keys (930 x 8 x 21 x 2 117 and 148), and with one head where many queries see few
+        keys (409 x 1 x 240 x 1 30 and 55, 1237 x 1 x 89 x 20 39 and 49). Over 1700 sizes drawn from 1 x 1 x 1 x 1 to 6000 x 16 x 600 x 3000 this is
+        at most 7 % slower than separate operators in all but 3, which take 37 to 55 us.
+        Sizes alone decide, so that a capture goes the way of its warm-up."""
+        tiles = -(-Sq // 128) * -(-Sk // 128)
+        if B * H * tiles <= 2 * 148:
+            return True
+        if trained:
+            return Sq + Sk >= 80 * tiles if H > 1 else Sq * Sk >= 4096 * tiles
+        return not (masked and Sk <= 4) and (H > 1 or Sk >= 48 or Sq <= 16)
+
     def forward_ext(self, query, key, value, mask: Optional[torch.Tensor] = None):
         q, k, v = query.t, key.t, value.t
         B, Sq, Sk = q.shape[0], q.shape[1], k.shape[1]
@@ -624,7 +642,8 @@ class MultiheadAttention(Module):
                 add_mask = torch.zeros(mb.shape, dtype=torch.float32, device=q.device).masked_fill(mb, float("-inf"))
         if Sq == Sk:
             o = _ops.attention(q=qp, k=kp, v=vp, mask=add_mask, causal=causal, scale=self.scale)
-        elif _ops.FLAGS.native and qp.is_cuda and qp.dtype == torch.bfloat16 and D in (64, 128) and (mask is None or self._of_keys(mask, B, Sk)):
+        elif (_ops.FLAGS.native and qp.is_cuda and qp.dtype == torch.bfloat16 and D in (64, 128) and (mask is None or self._of_keys(mask, B, Sk))
+              and self._kernel_is_faster(B, H, Sq, Sk, torch.is_grad_enabled() and any(t.requires_grad for t in (qp, kp, vp)), mask is not None)):
             keys = None
             if add_mask is not None:        # less its largest: 0 and -inf as they were, and NaN where every key is masked
                 keys = (add_mask - add_mask.amax(-1, keepdim=True)).reshape(-1, Sk)
