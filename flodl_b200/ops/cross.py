@@ -16,8 +16,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, mask: Opt
 
     `Hk` divides `H`: query head `h` reads key head `h // (H / Hk)`, whose gradient is the sum over them. `scale` is 1 / sqrt(D) unless given. `mask` is of keys, [B, Sk],
     [1, Sk] or [B, 1, 1, Sk]: bool, True for the keys that take part, or floating point, added to the scores. A key at False or -inf is absent, whatever its key and
-    value hold, and gets no gradient; a query without any key gets zeros, one whose keys' scores are all -inf gets NaN. bf16 heads of 64 and 128 on a GPU run on the kernel, at any size, others as plain
-    products in 32 bits (64 for fp64). The kernel's gradients have no second derivative."""
+    value hold, and gets no gradient; a query without any key gets zeros, one whose keys' scores are all -inf gets NaN. bf16 heads of 64 and 128 on a GPU run on the kernel, at any
+    size, others as plain products in 32 bits (64 for fp64). The kernel adds up before it divides, so that values beyond 2^119 / Sk overflow, and its gradients have no second derivative."""
     return attend(q, k, v, mask, scale, False)
 
 
